@@ -475,6 +475,113 @@ int vx_fused_rms_swiglu(vx_ctx *ctx, const vx_model *model, const vx_buf *hidden
                         const vx_fused_swiglu_args *a);
 
 /* ------------------------------------------------------------------------- */
+/* KV cache held in 4 bits, its attention, and eviction from it (no reference */
+/* counterpart: the reference's caches are f16 and end at VX_ERR_CONTEXT_FULL). */
+/*                                                                            */
+/* A cache holds slots 0..context-1 for every layer, sequence and KV head; one */
+/* vx_buf for K and one for V, of vx_kv4_cache_bytes each. A row of head_dim   */
+/* values is cut into groups of 32. With x clamped to +-61440 and lo, hi a     */
+/* group's least and greatest value, every operation in f32 rounded once:      */
+/*   d = f16((hi - lo) / 15), o = f16(lo),                                     */
+/*   c = clamp(rint((x - o) / d), 0, 15), ties to even, 0 where d is 0;        */
+/* the group stands for the f16 values o + d * c (rounded once). A group with  */
+/* a NaN among its values is all NaN. 5 bits a value in all.                   */
+/* Planes [layer][sequence][kv_head] of ceil(context / 32) blocks; a block is  */
+/* 32 slots in 20 * head_dim bytes:                                            */
+/*   K: [slot 32][head_dim / 8] dwords of 8 dimensions, then                   */
+/*      [slot 32][group] f16 pairs (d, o);                                     */
+/*   V: [octet 4][dimension % 32][group] dwords of the octet's 8 slots, then   */
+/*      [octet 4][group] f16 d[8], o[8] of the octet's slots;                  */
+/* element e of a dword's eight is bits 4 (e / 2) + 16 (e % 2) and the three   */
+/* above. (V is transposed for the matrix products that read it.)              */
+/*                                                                            */
+/* `slots` is u32[sequences] on the device: the slots a sequence has filled    */
+/* before the call. Token t of sequence s has slot slots[s] + t: vx_kv4_store  */
+/* fills it and vx_kv4_attention's row attends to slots 0..slots[s] + t, so a  */
+/* step stores, attends, and after the last layer advances. A sequence with    */
+/* VX_KV4_NO_SLOT takes no part (nothing stored, rows of zeros), nor does a    */
+/* token whose slot is not below context. Nothing outside the cache is read or */
+/* written for any content of a device buffer. Calls on one context are in     */
+/* order; two calls that overlap (other contexts, replayed graphs) need caches */
+/* and scratch of their own.                                                   */
+/* ------------------------------------------------------------------------- */
+#define VX_KV4_NO_SLOT 4294967295u
+typedef struct vx_kv4_geom {
+    uint32_t layers, sequences, kv_heads;
+    uint32_t head_dim;              /* 64, 128 or 256 */
+    uint32_t context;               /* slots a sequence, at most 2^28 */
+} vx_kv4_geom;
+/* Bytes of the K cache, and of the V cache; 0 for a geometry that is not valid. */
+uint64_t vx_kv4_cache_bytes(const vx_kv4_geom *geom);
+
+typedef struct vx_kv4_rows_push {
+    vx_kv4_geom geom;
+    uint32_t layer, first_sequence, n_sequences;   /* the call's sequences */
+    uint32_t tokens;                /* rows of each; row of (i, t): i * tokens + t */
+    uint32_t k_stride, v_stride, k_base, v_base;   /* floats */
+} vx_kv4_rows_push;
+/* Rows k, v (f32, kv_heads * head_dim wide) into their slots. slot_positions
+ * (nullable) u32 [layer][sequence][kv_head][context] receives each slot's
+ * position: positions[s] + t, or the slot itself where positions (u32[sequences])
+ * is null. */
+int vx_kv4_store(vx_ctx *ctx, const vx_buf *k, const vx_buf *v, vx_buf *k_cache, vx_buf *v_cache,
+                 const vx_buf *slots, const vx_buf *positions, vx_buf *slot_positions,
+                 const vx_kv4_rows_push *pc);
+/* The values that slots stand for, as f32 rows: what vx_kv4_store with the same
+ * push has written. k or v may be null. Rows without a slot are left as they were. */
+int vx_kv4_load(vx_ctx *ctx, const vx_buf *k_cache, const vx_buf *v_cache, vx_buf *k, vx_buf *v,
+                const vx_buf *slots, const vx_kv4_rows_push *pc);
+/* slots[s] += tokens and positions[s] += tokens (positions nullable) for sequences
+ * that take part; slots stops at context. */
+int vx_kv4_advance(vx_ctx *ctx, vx_buf *slots, vx_buf *positions, uint32_t first_sequence,
+                   uint32_t n_sequences, uint32_t tokens, uint32_t context);
+
+typedef struct vx_kv4_attention_push {
+    vx_kv4_geom geom;
+    uint32_t layer, first_sequence, n_sequences, tokens;
+    uint32_t q_heads;               /* a multiple of kv_heads */
+    uint32_t q_stride, out_stride, q_base, out_base;   /* floats */
+    float decay;                    /* of the accumulated weights, 0..1 */
+} vx_kv4_attention_push;
+/* Scratch of one call; 0 for a push that is not valid. */
+uint64_t vx_kv4_attention_scratch_bytes(const vx_kv4_attention_push *pc, uint32_t with_weights);
+/* out = softmax(q . K / sqrt(head_dim)) . V over the slots each row attends to, in
+ * f32 (products on the matrix cores, q and the weights as two f16 terms each, sums
+ * in f32). One token a sequence, a few (drafts) or a prompt's many. weights
+ * (nullable) f32 [layer][sequence][kv_head][context]: for every slot that a row of
+ * the call may attend to, w = decay * w + the sum of the softmax weights it got
+ * from the call's rows and the KV head's query heads (decay 0, or a slot the
+ * call's own tokens fill: the sum alone). Other entries are left as they were. A
+ * NaN stored by the call's own tokens reaches every row of the call. */
+int vx_kv4_attention(vx_ctx *ctx, const vx_buf *q, const vx_buf *k_cache, const vx_buf *v_cache, vx_buf *out,
+                     vx_buf *weights, const vx_buf *slots, vx_buf *scratch, const vx_kv4_attention_push *pc);
+
+typedef struct vx_kv4_evict_push {
+    vx_kv4_geom geom;
+    uint32_t first_sequence, n_sequences;
+    uint32_t keep;                  /* slots that stay, 1..context - 1 */
+    uint32_t sinks;                 /* positions below this stay */
+    uint32_t recent;                /* and the last so many positions */
+} vx_kv4_evict_push;
+/* Bytes of a plan: u32 pairs (from, to) [layers][n_sequences][kv_heads][moves],
+ * moves = min(keep, context - keep); 0 for a push that is not valid. */
+uint64_t vx_kv4_plan_bytes(const vx_kv4_evict_push *pc);
+/* What stays when every sequence of more than `keep` slots is cut to `keep`, for all
+ * layers and each KV head by itself: slots whose position is below sinks or above
+ * newest - recent (newest: the greatest of slot_positions over the filled slots)
+ * first, then by falling weight (NaN last), ties to the lower slot. The plan moves
+ * the i-th slot that stays at or above keep into the i-th below it that does not
+ * (so at most `keep` rows move, and none is both read and written); its other pairs
+ * are VX_KV4_NO_SLOT. sinks + recent may not exceed keep. */
+int vx_kv4_select(vx_ctx *ctx, const vx_buf *weights, const vx_buf *slot_positions, const vx_buf *slots,
+                  vx_buf *plan, const vx_kv4_evict_push *pc);
+/* Carries out a plan of the same push: cache rows, weights and positions (each
+ * nullable, the caches both or neither) move, then slots[s] = min(slots[s], keep).
+ * A pair that is not from [keep, context) to [0, keep) is not carried out. */
+int vx_kv4_compact(vx_ctx *ctx, const vx_buf *plan, vx_buf *k_cache, vx_buf *v_cache, vx_buf *weights,
+                   vx_buf *slot_positions, vx_buf *slots, const vx_kv4_evict_push *pc);
+
+/* ------------------------------------------------------------------------- */
 /* Diagnostics (no reference counterpart): plain streaming kernels that       */
 /* calibrate the HBM roofline and the PMC byte counters.                      */
 /* ------------------------------------------------------------------------- */

@@ -37,6 +37,7 @@ pub const VX_DTYPE_F32: u32 = 0;
 pub const VX_DTYPE_F16: u32 = 1;
 pub const VX_DTYPE_Q8_0: u32 = 8;
 pub const VX_NOALLOC_SCRATCH_BYTES: u32 = 2097152;
+pub const VX_KV4_NO_SLOT: u32 = 4294967295;
 pub const VX_EXEC_GRAPH: u32 = 0;
 pub const VX_EXEC_FUSED: u32 = 1;
 pub const VX_EXEC_REFERENCE: u32 = 2;
@@ -802,6 +803,134 @@ extern "C" {
         hidden: *const VxBuf,
         y: *mut VxBuf,
         a: *const VxFusedSwigluArgs,
+    ) -> c_int;
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct VxKv4Geom {
+    pub layers: u32,
+    pub sequences: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+    pub context: u32,
+}
+
+#[link(name = "voxhip")]
+extern "C" {
+    pub fn vx_kv4_cache_bytes(geom: *const VxKv4Geom) -> u64;
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct VxKv4RowsPush {
+    pub geom: VxKv4Geom,
+    pub layer: u32,
+    pub first_sequence: u32,
+    pub n_sequences: u32,
+    pub tokens: u32,
+    pub k_stride: u32,
+    pub v_stride: u32,
+    pub k_base: u32,
+    pub v_base: u32,
+}
+
+#[link(name = "voxhip")]
+extern "C" {
+    pub fn vx_kv4_store(
+        ctx: *mut VxCtx,
+        k: *const VxBuf,
+        v: *const VxBuf,
+        k_cache: *mut VxBuf,
+        v_cache: *mut VxBuf,
+        slots: *const VxBuf,
+        positions: *const VxBuf,
+        slot_positions: *mut VxBuf,
+        pc: *const VxKv4RowsPush,
+    ) -> c_int;
+    pub fn vx_kv4_load(
+        ctx: *mut VxCtx,
+        k_cache: *const VxBuf,
+        v_cache: *const VxBuf,
+        k: *mut VxBuf,
+        v: *mut VxBuf,
+        slots: *const VxBuf,
+        pc: *const VxKv4RowsPush,
+    ) -> c_int;
+    pub fn vx_kv4_advance(
+        ctx: *mut VxCtx,
+        slots: *mut VxBuf,
+        positions: *mut VxBuf,
+        first_sequence: u32,
+        n_sequences: u32,
+        tokens: u32,
+        context: u32,
+    ) -> c_int;
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct VxKv4AttentionPush {
+    pub geom: VxKv4Geom,
+    pub layer: u32,
+    pub first_sequence: u32,
+    pub n_sequences: u32,
+    pub tokens: u32,
+    pub q_heads: u32,
+    pub q_stride: u32,
+    pub out_stride: u32,
+    pub q_base: u32,
+    pub out_base: u32,
+    pub decay: f32,
+}
+
+#[link(name = "voxhip")]
+extern "C" {
+    pub fn vx_kv4_attention_scratch_bytes(pc: *const VxKv4AttentionPush, with_weights: u32) -> u64;
+    pub fn vx_kv4_attention(
+        ctx: *mut VxCtx,
+        q: *const VxBuf,
+        k_cache: *const VxBuf,
+        v_cache: *const VxBuf,
+        out: *mut VxBuf,
+        weights: *mut VxBuf,
+        slots: *const VxBuf,
+        scratch: *mut VxBuf,
+        pc: *const VxKv4AttentionPush,
+    ) -> c_int;
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct VxKv4EvictPush {
+    pub geom: VxKv4Geom,
+    pub first_sequence: u32,
+    pub n_sequences: u32,
+    pub keep: u32,
+    pub sinks: u32,
+    pub recent: u32,
+}
+
+#[link(name = "voxhip")]
+extern "C" {
+    pub fn vx_kv4_plan_bytes(pc: *const VxKv4EvictPush) -> u64;
+    pub fn vx_kv4_select(
+        ctx: *mut VxCtx,
+        weights: *const VxBuf,
+        slot_positions: *const VxBuf,
+        slots: *const VxBuf,
+        plan: *mut VxBuf,
+        pc: *const VxKv4EvictPush,
+    ) -> c_int;
+    pub fn vx_kv4_compact(
+        ctx: *mut VxCtx,
+        plan: *const VxBuf,
+        k_cache: *mut VxBuf,
+        v_cache: *mut VxBuf,
+        weights: *mut VxBuf,
+        slot_positions: *mut VxBuf,
+        slots: *mut VxBuf,
+        pc: *const VxKv4EvictPush,
     ) -> c_int;
     pub fn vx_diag_stream_read(
         ctx: *mut VxCtx,

@@ -1,0 +1,217 @@
+"""The 4-bit KV cache's host side on the CPU: the format's restatement, geometry and
+argument checks (a stand-in for the HIP runtime counts launches, so that a refused call is
+seen to launch nothing), and the Python class's pushes."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import kv4ref
+from test_refused_memory import child, fake  # noqa: F401  (fixture)
+from voxgen_amd import abi
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_format_round_trip_is_within_half_a_step(hd):
+    """A value is off by at most half a step d, plus the roundings of o and of the value to f16
+    (half a unit each: 2^-11 of the largest magnitude), plus 15 times d's own (2^-11 of d, or half
+    of f16's least step 2^-24) at the far end."""
+    rng = np.random.default_rng(hd)
+    x = (rng.standard_normal((40, hd)) * np.exp(rng.uniform(-6, 6, (40, 1)))).astype(np.float32)
+    c, d, o = kv4ref.encode(x)
+    step = np.repeat(d.astype(np.float64), 32, -1)
+    off = np.abs(kv4ref.values(c, d, o) - x)
+    assert np.all(off <= step / 2 + 2 * 2.0 ** -11 * np.abs(x).max(-1, keepdims=True) + 15 * (step * 2.0 ** -11 + 2.0 ** -25))
+    assert c.max() == 15 and c.min() == 0
+
+
+@pytest.mark.parametrize("hd,context", [(64, 33), (128, 64), (256, 1)])
+def test_blocks_hold_what_was_put(hd, context):
+    rng = np.random.default_rng(1)
+    for is_v in (False, True):
+        cache = kv4ref.blank(2, 1, 2, hd, context, rng)
+        other = cache[0].copy()
+        x = rng.standard_normal((context, hd)).astype(np.float32)
+        for s in rng.permutation(context):
+            kv4ref.put(cache, (1, 0, 1), int(s), *(a[s] for a in kv4ref.encode(x)), is_v)
+        assert np.array_equal(kv4ref.rows(cache, (1, 0, 1), context, is_v), kv4ref.stored(x))
+        assert np.array_equal(cache[0], other)
+
+
+def test_cache_bytes():
+    lib = abi.load()
+    size = lambda *g: lib.vx_kv4_cache_bytes(C.byref(abi.Kv4Geom(*g)))  # noqa: E731
+    assert size(28, 1, 2, 128, 8192) == 28 * 2 * 8192 * 80
+    assert size(1, 3, 5, 64, 33) == 3 * 5 * 2 * 20 * 64          # whole blocks of 32 slots
+    assert size(1, 1, 1, 256, 1) == 20 * 256
+    for bad in ((0, 1, 1, 64, 1), (1, 0, 1, 64, 1), (1, 1, 0, 64, 1), (1, 1, 1, 64, 0), (1, 1, 1, 96, 1),
+                (1, 1, 1, 0, 1), (1, 1, 1, 128, (1 << 28) + 1), (1, 65536, 1, 64, 1), (1, 256, 256, 64, 1),
+                (65535, 65535, 1, 256, 1 << 28)):
+        assert size(*bad) == 0, bad
+    assert lib.vx_kv4_cache_bytes(None) == 0
+
+
+REFUSALS = """
+from voxgen_amd.kv4 import Kv4Cache
+import ctypes as C
+lib = abi.load()
+def kernels():
+    return launches("k_kv4")
+def row_push(**kw):
+    f = dict(layer=0, first_sequence=0, n_sequences=2, tokens=3, k_stride=256, v_stride=256, k_base=0, v_base=0)
+    g = dict(layers=2, sequences=2, kv_heads=2, head_dim=128, context=40)
+    for n, v in kw.items():
+        (g if n in g else f)[n] = v
+    return abi.Kv4RowsPush(abi.Kv4Geom(*g.values()), *f.values())
+def attn_push(**kw):
+    f = dict(layer=0, first_sequence=0, n_sequences=2, tokens=3, q_heads=8, q_stride=1024, out_stride=1024, q_base=0,
+             out_base=0, decay=1.0)
+    g = dict(layers=2, sequences=2, kv_heads=2, head_dim=128, context=40)
+    for n, v in kw.items():
+        (g if n in g else f)[n] = v
+    return abi.Kv4AttentionPush(abi.Kv4Geom(*g.values()), *f.values())
+def evict_push(**kw):
+    f = dict(first_sequence=0, n_sequences=2, keep=20, sinks=2, recent=4)
+    g = dict(layers=2, sequences=2, kv_heads=2, head_dim=128, context=40)
+    for n, v in kw.items():
+        (g if n in g else f)[n] = v
+    return abi.Kv4EvictPush(abi.Kv4Geom(*g.values()), *f.values())
+cache_bytes = 2 * 2 * 2 * 2 * 20 * 128
+kc, vc = ctx.alloc(cache_bytes), ctx.alloc(cache_bytes)
+rows = 6 * 256 * 4
+k, v = ctx.alloc(rows), ctx.alloc(rows)
+slots, pos = ctx.alloc(8), ctx.alloc(8)
+table = 2 * 2 * 2 * 40 * 4
+w, sp = ctx.alloc(table), ctx.alloc(table)
+q, out = ctx.alloc(6 * 1024 * 4), ctx.alloc(6 * 1024 * 4)
+small = ctx.alloc(4)
+H = lambda b: b.handle if b is not None else None
+def store(pc, k=k, v=v, kc=kc, vc=vc, slots=slots, pos=pos, sp=sp):
+    return refused(abi.call, "vx_kv4_store", ctx.handle, H(k), H(v), H(kc), H(vc), H(slots), H(pos), H(sp), pc)
+def load(pc, k=k, v=v, kc=kc, vc=vc, slots=slots):
+    return refused(abi.call, "vx_kv4_load", ctx.handle, H(kc), H(vc), H(k), H(v), H(slots), pc)
+def attn(pc, q=q, out=out, kc=kc, vc=vc, w=w, slots=slots, scratch=None):
+    need = lib.vx_kv4_attention_scratch_bytes(pc, 1 if w is not None else 0)
+    s = ctx.alloc(max(need, 4)) if scratch is None else scratch
+    return refused(abi.call, "vx_kv4_attention", ctx.handle, H(q), H(kc), H(vc), H(out), H(w), H(slots), H(s), pc)
+def select(pc, w=w, sp=sp, slots=slots, plan=None):
+    p = plan or ctx.alloc(max(4, lib.vx_kv4_plan_bytes(pc)))
+    return refused(abi.call, "vx_kv4_select", ctx.handle, H(w), H(sp), H(slots), H(p), pc)
+def compact(pc, kc=kc, vc=vc, w=w, sp=sp, slots=slots, plan=None):
+    p = plan or ctx.alloc(max(4, lib.vx_kv4_plan_bytes(pc)))
+    return refused(abi.call, "vx_kv4_compact", ctx.handle, H(p), H(kc), H(vc), H(w), H(sp), H(slots), pc)
+"""
+
+
+def test_row_calls_are_refused_before_a_launch(fake):  # noqa: F811
+    child(fake, REFUSALS + """
+for call in (store, load):
+    for want, kw in (("VX_ERR_INVALID_ARG", dict(tokens=0)), ("VX_ERR_INVALID_ARG", dict(n_sequences=0)),
+                     ("VX_ERR_INVALID_ARG", dict(layers=0)), ("VX_ERR_SHAPE", dict(layer=2)),
+                     ("VX_ERR_SHAPE", dict(first_sequence=2)), ("VX_ERR_SHAPE", dict(first_sequence=1)),
+                     ("VX_ERR_SHAPE", dict(n_sequences=4294967295, first_sequence=1)),
+                     ("VX_ERR_SHAPE", dict(tokens=41)), ("VX_ERR_SHAPE", dict(k_stride=255)),
+                     ("VX_ERR_SHAPE", dict(v_stride=0)), ("VX_ERR_UNSUPPORTED", dict(head_dim=96)),
+                     ("VX_ERR_BOUNDS", dict(k_stride=257)), ("VX_ERR_BOUNDS", dict(k_base=1)),
+                     ("VX_ERR_BOUNDS", dict(v_base=4294967295, v_stride=4294967295)),
+                     ("VX_ERR_BOUNDS", dict(tokens=4)), ("VX_ERR_BOUNDS", dict(layers=3)),
+                     ("VX_ERR_BOUNDS", dict(context=65)), ("VX_ERR_BOUNDS", dict(sequences=3)),
+                     ("VX_ERR_UNSUPPORTED", dict(context=1 << 29))):
+        assert call(row_push(**kw)) == want, (call, kw)
+    for want, kw in (("VX_ERR_INVALID_ARG", dict(kc=None)), ("VX_ERR_INVALID_ARG", dict(slots=None)),
+                     ("VX_ERR_INVALID_ARG", dict(vc=kc)), ("VX_ERR_BOUNDS", dict(slots=small)),
+                     ("VX_ERR_BOUNDS", dict(vc=small)), ("VX_ERR_BOUNDS", dict(v=small))):
+        assert call(row_push(), **kw) == want, (call, kw)
+assert store(row_push(), k=None) == "VX_ERR_INVALID_ARG"
+assert store(row_push(), pos=small) == "VX_ERR_BOUNDS"
+assert store(row_push(), sp=small) == "VX_ERR_BOUNDS"
+assert load(row_push(), k=None, v=None) == "VX_ERR_INVALID_ARG"
+adv = lambda *a: refused(abi.call, "vx_kv4_advance", ctx.handle, *a)
+for a, want in (((H(slots), None, 0, 0, 1, 40), "VX_ERR_INVALID_ARG"), ((H(slots), None, 0, 2, 0, 40), "VX_ERR_INVALID_ARG"),
+                ((H(slots), None, 0, 2, 1, 0), "VX_ERR_INVALID_ARG"), ((H(slots), None, 0, 2, 41, 40), "VX_ERR_SHAPE"),
+                ((H(slots), None, 1, 2, 1, 40), "VX_ERR_BOUNDS"), ((None, None, 0, 2, 1, 40), "VX_ERR_INVALID_ARG"),
+                ((H(slots), H(small), 0, 2, 1, 40), "VX_ERR_BOUNDS"),
+                ((H(slots), None, 4294967295, 4294967295, 1, 40), "VX_ERR_BOUNDS")):
+    assert adv(*a) == want, a
+assert refused(abi.call, "vx_kv4_store", None, H(k), H(v), H(kc), H(vc), H(slots), None, None, row_push()) == "VX_ERR_INVALID_ARG"
+assert refused(abi.call, "vx_kv4_store", ctx.handle, H(k), H(v), H(kc), H(vc), H(slots), None, None, None) == "VX_ERR_INVALID_ARG"
+assert kernels() == 0
+assert store(row_push()) == "VX_OK" and store(row_push(), pos=None, sp=None) == "VX_OK"
+assert load(row_push()) == "VX_OK" and load(row_push(), k=None) == "VX_OK" and load(row_push(), v=None) == "VX_OK"
+assert adv(H(slots), H(pos), 0, 2, 1, 40) == "VX_OK"
+assert kernels() == 6
+""")
+
+
+def test_attention_is_refused_before_a_launch(fake):  # noqa: F811
+    child(fake, REFUSALS + """
+for want, kw in (("VX_ERR_INVALID_ARG", dict(tokens=0)), ("VX_ERR_SHAPE", dict(q_heads=7)), ("VX_ERR_SHAPE", dict(q_heads=0)),
+                 ("VX_ERR_SHAPE", dict(layer=2)), ("VX_ERR_SHAPE", dict(first_sequence=1)), ("VX_ERR_SHAPE", dict(tokens=41)),
+                 ("VX_ERR_SHAPE", dict(q_stride=1023)), ("VX_ERR_SHAPE", dict(out_stride=1)),
+                 ("VX_ERR_BOUNDS", dict(q_base=1)), ("VX_ERR_BOUNDS", dict(out_base=1)), ("VX_ERR_BOUNDS", dict(tokens=4)),
+                 ("VX_ERR_UNSUPPORTED", dict(head_dim=32)), ("VX_ERR_UNSUPPORTED", dict(q_heads=2050)),
+                 ("VX_ERR_INVALID_ARG", dict(decay=-0.1)), ("VX_ERR_INVALID_ARG", dict(decay=1.5)),
+                 ("VX_ERR_INVALID_ARG", dict(decay=float("nan"))), ("VX_ERR_BOUNDS", dict(context=65))):
+    pc = attn_push(**kw)
+    assert attn(pc) == want, kw
+for want, kw in (("VX_ERR_INVALID_ARG", dict(q=None)), ("VX_ERR_INVALID_ARG", dict(out=None)),
+                 ("VX_ERR_INVALID_ARG", dict(out=q)), ("VX_ERR_INVALID_ARG", dict(slots=None)),
+                 ("VX_ERR_INVALID_ARG", dict(vc=kc)), ("VX_ERR_BOUNDS", dict(w=small)), ("VX_ERR_BOUNDS", dict(slots=small)),
+                 ("VX_ERR_BOUNDS", dict(scratch=small))):
+    assert attn(attn_push(), **kw) == want, kw
+assert kernels() == 0
+both = ctx.alloc(12 * 1024 * 4)                      # q and out in one buffer, apart
+assert attn(attn_push(out_base=6 * 1024), q=both, out=both) == "VX_OK"
+assert attn(attn_push(out_base=6 * 1024 - 1), q=both, out=both) == "VX_ERR_INVALID_ARG"
+assert attn(attn_push()) == "VX_OK" and attn(attn_push(), w=None) == "VX_OK"
+for kw in (dict(tokens=0), dict(q_heads=3), dict(layer=2)):
+    assert lib.vx_kv4_attention_scratch_bytes(attn_push(**kw), 1) == 0
+assert lib.vx_kv4_attention_scratch_bytes(None, 0) == 0
+""")
+
+
+def test_eviction_is_refused_before_a_launch(fake):  # noqa: F811
+    child(fake, REFUSALS + """
+for call in (select, compact):
+    for want, kw in (("VX_ERR_SHAPE", dict(keep=0)), ("VX_ERR_SHAPE", dict(keep=40)), ("VX_ERR_SHAPE", dict(sinks=17)),
+                     ("VX_ERR_SHAPE", dict(recent=4294967295)), ("VX_ERR_INVALID_ARG", dict(n_sequences=0)),
+                     ("VX_ERR_SHAPE", dict(first_sequence=1)), ("VX_ERR_UNSUPPORTED", dict(head_dim=100)),
+                     ("VX_ERR_INVALID_ARG", dict(kv_heads=0)), ("VX_ERR_BOUNDS", dict(context=41)),
+                     ("VX_ERR_BOUNDS", dict(layers=3))):
+        assert call(evict_push(**kw)) == want, (call, kw)
+    for want, kw in (("VX_ERR_BOUNDS", dict(plan=small)), ("VX_ERR_BOUNDS", dict(w=small)), ("VX_ERR_BOUNDS", dict(sp=small)),
+                     ("VX_ERR_BOUNDS", dict(slots=small)), ("VX_ERR_INVALID_ARG", dict(slots=None))):
+        assert call(evict_push(), **kw) == want, (call, kw)
+assert select(evict_push(), w=None) == "VX_ERR_INVALID_ARG" and select(evict_push(), sp=None) == "VX_ERR_INVALID_ARG"
+assert compact(evict_push(), kc=None) == "VX_ERR_INVALID_ARG" and compact(evict_push(), vc=None) == "VX_ERR_INVALID_ARG"
+assert compact(evict_push(), vc=kc) == "VX_ERR_INVALID_ARG"
+assert kernels() == 0
+assert select(evict_push()) == "VX_OK" and compact(evict_push()) == "VX_OK"
+assert compact(evict_push(), kc=None, vc=None, w=None, sp=None) == "VX_OK"
+assert kernels() == 3
+assert lib.vx_kv4_plan_bytes(evict_push()) == 2 * 2 * 2 * 20 * 8
+assert lib.vx_kv4_plan_bytes(evict_push(keep=33)) == 2 * 2 * 2 * 7 * 8
+assert lib.vx_kv4_plan_bytes(None) == 0
+""")
+
+
+def test_python_class_checks_and_keeps_its_pushes(fake):  # noqa: F811
+    child(fake, REFUSALS + """
+assert refused(Kv4Cache, ctx, 1, 1, 1, 96, 8) == "VX_ERR_SHAPE"
+c = Kv4Cache(ctx, 2, 2, 2, 128, 40, track=True)
+assert c.nbytes == 2 * cache_bytes
+c.store(1, k, v, tokens=3)
+c.load(1, k, None, tokens=3)
+c.attention(1, q, out, 8, tokens=3)
+c.advance(3)
+plan = c.plan(20)
+assert plan.nbytes == 2 * 2 * 2 * 20 * 8 and c.plan_moves(33) == 7
+c.evict(plan, 20, sinks=1, recent=2)
+assert refused(c.store, 2, k, v) == "VX_ERR_SHAPE"
+assert refused(c.attention, 0, q, out, 8, 4) == "VX_ERR_BOUNDS"
+bare = Kv4Cache(ctx, 1, 1, 1, 64, 8)
+assert refused(bare.select, plan, 4) == "VX_ERR_STATE"
+before = len(c._pushes)
+c.store(1, k, v, tokens=3)
+assert len(c._pushes) == before
+""")

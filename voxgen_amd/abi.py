@@ -179,6 +179,15 @@ AudioDecodeStats = _struct("AudioDecodeStats", [
     ("latent_frames", u32), ("latent_patches", u32), ("output_samples", u32), ("output_sample_rate", u32),
     ("duration_seconds", f64), ("checksum", f64), ("l2", f64), ("peak", f32), ("decode_ms", f64),
     ("scratch_bytes", u64)])
+Kv4Geom = _struct("Kv4Geom", [(n, u32) for n in ("layers", "sequences", "kv_heads", "head_dim", "context")])
+Kv4RowsPush = _struct("Kv4RowsPush", [("geom", Kv4Geom)] + [(n, u32) for n in (
+    "layer", "first_sequence", "n_sequences", "tokens", "k_stride", "v_stride", "k_base", "v_base")])
+Kv4AttentionPush = _struct("Kv4AttentionPush", [("geom", Kv4Geom)] + [(n, u32) for n in (
+    "layer", "first_sequence", "n_sequences", "tokens", "q_heads", "q_stride", "out_stride", "q_base", "out_base")] +
+    [("decay", f32)])
+Kv4EvictPush = _struct("Kv4EvictPush", [("geom", Kv4Geom)] + [(n, u32) for n in (
+    "first_sequence", "n_sequences", "keep", "sinks", "recent")])
+KV4_NO_SLOT = 0xFFFFFFFF  # VX_KV4_NO_SLOT
 RESIDUAL_BUF = dict(OUTPUT=0, CURRENT_LM=1, FSQ_LATENT=2, FSQ_OUTPUT=3, FUSION_SNAPSHOT=4, HIDDEN=5,
                     KV_K=6, KV_V=7, STOP_LOGITS=8)
 
@@ -273,6 +282,15 @@ PROTOTYPES = {
     "vx_fused_attention_noalloc": (i32, [CTX, BUFP, BUFP, BUFP, BUFP, BUFP, P(FusedAttnArgs)]),
     "vx_fused_matvec_residual": (i32, [CTX, MODEL, BUFP, BUFP, BUFP, P(FusedResidualArgs)]),
     "vx_fused_rms_swiglu": (i32, [CTX, MODEL, BUFP, BUFP, P(FusedSwigluArgs)]),
+    "vx_kv4_cache_bytes": (u64, [P(Kv4Geom)]),
+    "vx_kv4_store": (i32, [CTX, BUFP, BUFP, BUFP, BUFP, BUFP, BUFP, BUFP, P(Kv4RowsPush)]),
+    "vx_kv4_load": (i32, [CTX, BUFP, BUFP, BUFP, BUFP, BUFP, P(Kv4RowsPush)]),
+    "vx_kv4_advance": (i32, [CTX, BUFP, BUFP, u32, u32, u32, u32]),
+    "vx_kv4_attention_scratch_bytes": (u64, [P(Kv4AttentionPush), u32]),
+    "vx_kv4_attention": (i32, [CTX, BUFP, BUFP, BUFP, BUFP, BUFP, BUFP, BUFP, P(Kv4AttentionPush)]),
+    "vx_kv4_plan_bytes": (u64, [P(Kv4EvictPush)]),
+    "vx_kv4_select": (i32, [CTX, BUFP, BUFP, BUFP, BUFP, P(Kv4EvictPush)]),
+    "vx_kv4_compact": (i32, [CTX, BUFP, BUFP, BUFP, BUFP, BUFP, BUFP, P(Kv4EvictPush)]),
     "vx_diag_stream_read": (i32, [CTX, BUFP, u64, u64, BUFP, u32, u32]),
     "vx_diag_stream_copy": (i32, [CTX, BUFP, BUFP, u64, u32]),
     "vx_diag_timeline_arm": (i32, [CTX, u64]),
@@ -366,6 +384,8 @@ STRUCT_SIZES = {  # C name -> ctypes struct
     "vx_residual_gpu_step": ResidualGpuStep, "vx_residual_benchmark_result": ResidualBenchmark,
     "vx_stop_prediction": StopPrediction, "vx_vae_conv_push": VaeConvPush, "vx_vae_convt_push": VaeConvTPush,
     "vx_vae_snake_push": VaeSnakePush, "vx_vae_scale_push": VaeScalePush, "vx_vae_grid_push": VaeGridPush,
+    "vx_kv4_geom": Kv4Geom, "vx_kv4_rows_push": Kv4RowsPush, "vx_kv4_attention_push": Kv4AttentionPush,
+    "vx_kv4_evict_push": Kv4EvictPush,
     "vx_audiovae_config": AudioVaeConfig, "vx_audio_decode_stats": AudioDecodeStats,
 }
 
