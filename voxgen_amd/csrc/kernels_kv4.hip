@@ -10,6 +10,8 @@
 // slots of K's rows are taken in the order that leaves, in S^T, each lane with eight
 // consecutive slots of its query row: the P^T operand of the second product, already in
 // the lane's registers.
+#include <type_traits>
+
 #include "kv4.h"
 
 namespace vx {
@@ -17,6 +19,7 @@ namespace {
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLimit = 61440.0f;   // inputs are clamped to this: o + 15 d then stays inside f16
@@ -46,33 +49,43 @@ __device__ __forceinline__ float dpp(float v) {
 __device__ __forceinline__ constexpr int code_bit(int e) { return 4 * (e / 2) + 16 * (e % 2); }
 
 // Eight codes as f16 pairs: 1024 + c and 64 + c are made by or-ing a nibble under the
-// exponent for which its lowest bit counts one, and the difference is exact.
-__device__ __forceinline__ void codes8(uint32_t w, h2 *c) {
+// exponent for which its lowest bit counts one, and the difference is exact. The masks are
+// kept in registers, so that a pair takes one v_and_or_b32 (which takes no literals).
+struct Masks {
+    uint32_t low = 0x000f000fu, high = 0x00f000f0u, k1024 = 0x64006400u, k64 = 0x54005400u;
+    __device__ __forceinline__ Masks() {
+        asm("" : "+s"(low), "+s"(high));
+        asm("" : "+v"(k1024), "+v"(k64));
+    }
+};
+__device__ __forceinline__ void codes8(const Masks &k, uint32_t w, h2 *c) {
     const h2 k1024 = {1024.f16, 1024.f16}, k64 = {64.f16, 64.f16};
     const uint32_t u = w >> 8;
-    c[0] = __builtin_bit_cast(h2, (w & 0x000f000fu) | 0x64006400u) - k1024;
-    c[1] = __builtin_bit_cast(h2, (w & 0x00f000f0u) | 0x54005400u) - k64;
-    c[2] = __builtin_bit_cast(h2, (u & 0x000f000fu) | 0x64006400u) - k1024;
-    c[3] = __builtin_bit_cast(h2, (u & 0x00f000f0u) | 0x54005400u) - k64;
+    c[0] = __builtin_bit_cast(h2, (w & k.low) | k.k1024) - k1024;
+    c[1] = __builtin_bit_cast(h2, (w & k.high) | k.k64) - k64;
+    c[2] = __builtin_bit_cast(h2, (u & k.low) | k.k1024) - k1024;
+    c[3] = __builtin_bit_cast(h2, (u & k.high) | k.k64) - k64;
 }
-// The values of eight codes: f16(o + d * c), one rounding; of one (d, o) or of eight.
-__device__ __forceinline__ h8 values8(uint32_t w, h2 d, h2 o) {
-    h2 c[4];
-    codes8(w, c);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = __builtin_elementwise_fma(c[i], d, o);
+__device__ __forceinline__ h8 join8(const h2 *c) {
     return __builtin_shufflevector(__builtin_shufflevector(c[0], c[1], 0, 1, 2, 3),
                                    __builtin_shufflevector(c[2], c[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
 }
-__device__ __forceinline__ h8 values8(uint32_t w, h8 d, h8 o) {
+// The values of eight codes: f16(o + d * c), one rounding; of one (d, o) or of eight.
+__device__ __forceinline__ h8 values8(const Masks &k, uint32_t w, h2 d, h2 o) {
     h2 c[4];
-    codes8(w, c);
+    codes8(k, w, c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = __builtin_elementwise_fma(c[i], d, o);
+    return join8(c);
+}
+__device__ __forceinline__ h8 values8(const Masks &k, uint32_t w, h8 d, h8 o) {
+    h2 c[4];
+    codes8(k, w, c);
     c[0] = __builtin_elementwise_fma(c[0], __builtin_shufflevector(d, d, 0, 1), __builtin_shufflevector(o, o, 0, 1));
     c[1] = __builtin_elementwise_fma(c[1], __builtin_shufflevector(d, d, 2, 3), __builtin_shufflevector(o, o, 2, 3));
     c[2] = __builtin_elementwise_fma(c[2], __builtin_shufflevector(d, d, 4, 5), __builtin_shufflevector(o, o, 4, 5));
     c[3] = __builtin_elementwise_fma(c[3], __builtin_shufflevector(d, d, 6, 7), __builtin_shufflevector(o, o, 6, 7));
-    return __builtin_shufflevector(__builtin_shufflevector(c[0], c[1], 0, 1, 2, 3),
-                                   __builtin_shufflevector(c[2], c[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+    return join8(c);
 }
 
 // ------------------------------------------------------------------- rows
@@ -190,7 +203,7 @@ __global__ __launch_bounds__(HD) void k_kv4_load(Kv4Rows a) {
         const uint8_t *const kb = a.kc + block;
         const uint32_t w = reinterpret_cast<const uint32_t *>(kb)[(slot % 32u) * W + c];
         const h2 p = __builtin_bit_cast(h2, reinterpret_cast<const uint32_t *>(kb + L::CODES)[(slot % 32u) * L::G + c / 4u]);
-        const h8 x = values8(w, h2{p[0], p[0]}, h2{p[1], p[1]});
+        const h8 x = values8(Masks(), w, h2{p[0], p[0]}, h2{p[1], p[1]});
         float *const to = a.k + (first_row + slot - base) * a.k_stride + head * HD + c * 8u;
         if (a.vec) {
             reinterpret_cast<f4 *>(to)[0] = f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
@@ -204,7 +217,7 @@ __global__ __launch_bounds__(HD) void k_kv4_load(Kv4Rows a) {
         const uint8_t *const vb = a.vc + block;
         const uint32_t w = reinterpret_cast<const uint32_t *>(vb)[((oct % 4u) * 32u + tid % 32u) * L::G + tid / 32u];
         const h8 *const sc = reinterpret_cast<const h8 *>(vb + L::CODES) + ((oct % 4u) * L::G + tid / 32u) * 2u;
-        const h8 x = values8(w, sc[0], sc[1]);
+        const h8 x = values8(Masks(), w, sc[0], sc[1]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const uint32_t sl = oct * 8u + e;
@@ -224,48 +237,60 @@ __global__ __launch_bounds__(256) void k_kv4_advance(uint32_t *slots, uint32_t *
 }
 
 // ------------------------------------------------------------------- attention
-constexpr uint32_t kRows = 16;       // query rows of a tile
-constexpr uint32_t kWaves = 4;
 constexpr float kLazy = 8.0f;        // a row's reference moves when a score exceeds it by this
 constexpr float kRaise = 7.0f;       // weights are taken 2^7 up, so that their low f16 terms stay normal
 
 struct AttnArgs {
     Kv4Attn a;
-    uint32_t group, tiles, splits;   // query heads a KV head, tiles of 16 rows, key splits of the grid
-    float *ml, *acc, *lse;           // [unit][split][16][2], [unit][split][16][HD], [unit][16]
+    uint32_t group, rows, tiles;     // query heads a KV head, rows (tokens x group), tiles of them
+    uint32_t splits, per;            // key splits of the grid, blocks of one
+    float *ml, *acc, *lse;           // [unit][split][tile rows][2], [..][tile rows][HD], [sequence x KV head][rows]
+    // for the weights of prompts: the query rows as operands [sequence x KV head][16 rows][HD / 32][hi, lo][64],
+    // the factors of their scores [sequence x KV head][rows], sums by row split [split][sequence x KV head][slots]
+    h8 *qp;
+    float *factors, *sums;
+    uint32_t qtiles, row_splits, slots32;
 };
 
-// Keys of a tile's rows: `base` filled slots ahead of the call, rows r0.. of rows.
+// Keys of a tile: all that its last row attends to. A split is `per` blocks whatever the
+// sequence's length: sequences of unequal length then make splits of equal work.
 struct Span {
-    uint32_t base, keys, blocks, per, active;   // blocks of the tile, blocks a split, splits in use
+    uint32_t base, keys, blocks, active;   // slots filled ahead of the call; blocks and splits of the tile
 };
-__device__ __forceinline__ Span span_of(const AttnArgs &p, uint32_t seq, uint32_t tile) {
+__device__ __forceinline__ Span span_of(const AttnArgs &p, uint32_t seq, uint32_t last_row) {
     Span s;
     s.base = p.a.slots[seq];
-    const uint32_t last = min((tile + 1u) * kRows, p.a.tokens * p.group) - 1u;   // last row of the tile
-    s.keys = s.base >= p.a.g.context ? 0u : min(s.base + last / p.group + 1u, p.a.g.context);
+    s.keys = s.base >= p.a.g.context ? 0u : min(s.base + last_row / p.group + 1u, p.a.g.context);
     s.blocks = (s.keys + 31u) / 32u;
-    s.per = max(kWaves, (s.blocks + p.splits - 1u) / p.splits);
-    s.active = (s.blocks + s.per - 1u) / s.per;
+    s.active = (s.blocks + p.per - 1u) / p.per;
     return s;
 }
 
 __device__ __forceinline__ f4 mfma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// Over the four lanes l, l + 16, l + 32, l + 48 that share a query row.
+// Over the four lanes l, l + 16, l + 32, l + 48 that share a query row: v_permlane16_swap
+// and v_permlane32_swap put both partners' values into every lane.
 __device__ __forceinline__ float row_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+    u = __builtin_bit_cast(uint32_t, v);
+    const auto t = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)t[0]), __builtin_bit_cast(float, (uint32_t)t[1]));
 }
 __device__ __forceinline__ float row_sum(float v) {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
+    uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    v = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+    u = __builtin_bit_cast(uint32_t, v);
+    const auto t = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_bit_cast(float, (uint32_t)t[0]) + __builtin_bit_cast(float, (uint32_t)t[1]);
 }
 
-// A tile's query rows as the B operand: lane (i, q) holds row i, dimensions
-// q HD / 4 + 8 u + 0..7 in step u, as two f16 terms of the row scaled to below 2^10 (the
-// low term of a value down to 2^-13 of the row's largest is then still normal). Returns
-// the factor of the scores: the row's scale, log2(e) and 1 / sqrt(HD).
+// Sixteen query rows as the B operand: lane (i, q) holds row i, dimensions q HD / 4 + 8 u
+// + 0..7 in step u, as two f16 terms of the row scaled to below 2^10 (the low term of a
+// value down to 2^-13 of the row's largest is then still normal). Returns the factor of
+// the scores: the row's scale, log2(e) and 1 / sqrt(HD).
 template <int HD>
 __device__ __forceinline__ float load_q(const AttnArgs &p, uint32_t s, uint32_t head, uint32_t row, bool valid, uint32_t q,
                                         h8 *qh, h8 *ql) {
@@ -300,238 +325,533 @@ __device__ __forceinline__ float load_q(const AttnArgs &p, uint32_t s, uint32_t 
     return ldexpf(kLog2e / sqrtf((float)HD), e - 10);
 }
 
-// S^T of a block's 32 slots with the tile's rows: lane (i, q) gets the scores of row i and
-// slots 8 q + 0..7.
+// A lane's share of a block of K: for both of the product's row tiles tt, the codes of
+// slot 8 (i / 4) + 4 tt + i % 4 in dimensions q HD / 4.. and their (d, o). Lane (i, q) of
+// the product S^T then holds the scores of query row i and slots 8 q + 4 tt + r: eight
+// consecutive ones.
 template <int HD>
-__device__ __forceinline__ void scores(const uint8_t *kb, uint32_t i, uint32_t q, const h8 *qh, const h8 *ql, float *s) {
-    using L = Lay<HD>;
-    constexpr int U = HD / 32;
+struct KFrag {
+    static constexpr int U = HD / 32, SC = HD == 256 ? 2 : 1;
+    uint32_t code[2][U], scale[2][SC];
+    __device__ __forceinline__ void load(const uint8_t *kb, uint32_t i, uint32_t q) {
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt) {
-        const uint32_t slot = 8u * (i / 4u) + 4u * tt + i % 4u;
-        const uint32_t *const codes = reinterpret_cast<const uint32_t *>(kb + slot * (HD / 2) + q * (HD / 8));
-        const uint32_t *const sc = reinterpret_cast<const uint32_t *>(kb + L::CODES) + slot * L::G;
-        f4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            // dimensions q HD / 4 + 8 u..: group q HD / 128 + u / 4
-            const h2 p = __builtin_bit_cast(h2, sc[HD == 64 ? q / 2u : q * (HD / 128) + u / 4]);
-            const h8 k = values8(codes[u], h2{p[0], p[0]}, h2{p[1], p[1]});
-            x = mfma16(k, qh[u], x);
-            x = mfma16(k, ql[u], x);
+        for (int tt = 0; tt < 2; ++tt) {
+            const uint32_t slot = 8u * (i / 4u) + 4u * tt + i % 4u;
+            __builtin_memcpy(code[tt], __builtin_assume_aligned(kb + slot * (HD / 2) + q * (HD / 8), HD == 64 ? 8 : 16), 4 * U);
+            const uint32_t g = HD == 64 ? q / 2u : q * (HD / 128);
+            __builtin_memcpy(scale[tt], __builtin_assume_aligned(kb + Lay<HD>::CODES + (slot * Lay<HD>::G + g) * 4u, 4 * SC), 4 * SC);
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[4 * tt + r] = x[r];
     }
-}
-
-// One workgroup: a tile of 16 query rows (tokens x the KV head's query heads) of a
-// sequence over one split of its blocks, which four waves take in turn, each with its own
-// running maximum and sum; they join in LDS. A tile with one split in use is finished
-// here, the others' partial sums go to scratch.
+    __device__ __forceinline__ h8 value(const Masks &k, int tt, int u) const {
+        const h2 p = __builtin_bit_cast(h2, scale[tt][u / 4]);
+        return values8(k, code[tt][u], h2{p[0], p[0]}, h2{p[1], p[1]});
+    }
+};
+// A lane's share of a block of V^T: octet q, dimensions 32 g + 16 h + i, and the (d, o) of
+// the octet's slots in group g.
 template <int HD>
-__global__ __launch_bounds__(256) void k_kv4_attn(AttnArgs p) {
+struct VFrag {
+    static constexpr int G = HD / 32;
+    uint32_t code[2][G];
+    __device__ __forceinline__ void load(const uint8_t *vb, uint32_t i, uint32_t q) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            __builtin_memcpy(code[h], __builtin_assume_aligned(vb + (q * 32u + 16u * h + i) * (4u * G), HD == 64 ? 8 : 16), 4 * G);
+    }
+};
+struct VScale {
+    h8 d, o;
+    template <int HD>
+    __device__ __forceinline__ void load(const uint8_t *vb, int g, uint32_t q) {
+        const h8 *const sc = reinterpret_cast<const h8 *>(vb + Lay<HD>::CODES) + (q * Lay<HD>::G + g) * 2u;
+        d = sc[0];
+        o = sc[1];
+    }
+    // Slots from `some` on may hold anything: their values count as zero.
+    __device__ __forceinline__ void keep(uint32_t some) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            d[e] = (uint32_t)e < some ? d[e] : 0.f16;
+            o[e] = (uint32_t)e < some ? o[e] : 0.f16;
+        }
+    }
+};
+
+// One workgroup: a tile of 16 NT query rows (tokens x the KV head's query heads) of a
+// sequence over one split of its blocks, which the waves take in turn, each with its own
+// running maximum and sum; they join in LDS. A tile with one split in use is finished
+// here, the others' partial sums go to scratch. A block's values are made once and meet
+// all NT column tiles, whose query rows lie in LDS in the order of the operand (NT 1: in
+// registers).
+template <int HD, int NT, int W>
+__global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
     using L = Lay<HD>;
-    constexpr int U = HD / 32, DT = HD / 16, OROW = HD + 4;
-    __shared__ __attribute__((aligned(16))) float os[kWaves][kRows][OROW];
-    __shared__ float ms[kWaves][kRows], ls[kWaves][kRows];
+    constexpr int U = HD / 32, DT = HD / 16, OROW = HD + 4, R = 16 * NT, B = W > 4 ? 4 : W;
+    constexpr int QLDS = NT > 1 ? R * HD : 0;   // floats: two f16 planes
+    constexpr int LDS = B * R * OROW > QLDS ? B * R * OROW : QLDS;
+    __shared__ __attribute__((aligned(16))) float lds[LDS];
+    __shared__ float ms[W][R], ls[W][R], fs[R];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
     const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // the tiles with the most keys first
     const uint32_t split = blockIdx.x / p.tiles, tile = p.tiles - 1u - blockIdx.x % p.tiles;
     const uint32_t head = blockIdx.y, s = blockIdx.z, seq = p.a.first + s;
-    const Span sp = span_of(p, seq, tile);
-    const uint32_t rows = p.a.tokens * p.group, r0 = tile * kRows;
-    if (split >= sp.active && !(split == 0 && sp.active == 0)) return;
-    const uint32_t b0 = split * sp.per, b1 = min(b0 + sp.per, sp.blocks);
-    const uint32_t row = min(r0 + i, rows - 1u);
-    const bool valid = r0 + i < rows;
-    const uint32_t limit = sp.base + row / p.group;   // last slot the row attends to (sp.blocks == 0 where idle)
-    const uint32_t sees_all = sp.base + r0 / p.group; // last slot that every row attends to
-
-    h8 qh[U], ql[U];
-    const float factor = load_q<HD>(p, s, head, row, valid, q, qh, ql);
+    const uint32_t rows = p.rows, r0 = tile * R;
+    const Span sp = span_of(p, seq, min(r0 + R, rows) - 1u);
+    if (split != 0 && split >= sp.active) return;
+    const uint32_t b0 = split * p.per, b1 = min(b0 + p.per, sp.blocks);
     const size_t plane = plane_of(p.a.g, p.a.layer, seq, head) * plane_bytes<HD>(p.a.g);
-    float m = -INFINITY, l = 0.f;
-    f4 o[DT];
+    const uint8_t *const kp = p.a.kc + plane, *const vp = p.a.vc + plane;
+    KFrag<HD> kf;
+    uint32_t b = b0 + w;
+    if (b < b1) kf.load(kp + (size_t)b * L::BLOCK, i, q);
+    h8 qh[U], ql[U];
+    float factor[NT];
+    h8 *const qs = reinterpret_cast<h8 *>(lds);   // [NT][U][hi, lo][64]
+    if constexpr (NT == 1) {
+        factor[0] = load_q<HD>(p, s, head, min(r0 + i, rows - 1u), r0 + i < rows, q, qh, ql);
+    } else {
+        for (uint32_t c = w; c < NT; c += W) {
+            const uint32_t row = r0 + 16u * c + i;
+            const float f = load_q<HD>(p, s, head, min(row, rows - 1u), row < rows, q, qh, ql);
+            if (q == 0) fs[16u * c + i] = f;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] = f4{0.f, 0.f, 0.f, 0.f};
+            for (int u = 0; u < U; ++u) {
+                qs[((c * U + u) * 2u) * 64u + lane] = qh[u];
+                qs[((c * U + u) * 2u + 1u) * 64u + lane] = ql[u];
+            }
+            if (p.qp && split == 0) {   // the weights' kernel reads them again
+                const size_t pair = (size_t)s * p.a.g.kv_heads + head;
+                h8 *const to = p.qp + (pair * p.qtiles + tile * NT + c) * U * 128u;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    to[u * 128 + lane] = qh[u];
+                    to[u * 128 + 64 + lane] = ql[u];
+                }
+                if (q == 0 && row < rows) p.factors[pair * rows + row] = f;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < NT; ++c) factor[c] = fs[16 * c + i];
+    }
+    // last slot that the lane's row of a column tile attends to
+    auto limit = [&](int c) { return sp.base + min(r0 + 16u * c + i, rows - 1u) / p.group; };
+    const uint32_t sees_all = sp.base + r0 / p.group;   // last slot that every row attends to
 
-    for (uint32_t b = b0 + w; b < b1; b += kWaves) {
-        const uint8_t *const kb = p.a.kc + plane + (size_t)b * L::BLOCK, *const vb = p.a.vc + plane + (size_t)b * L::BLOCK;
-        float x[8];
-        scores<HD>(kb, i, q, qh, ql, x);
+    float m[NT], l[NT];
+    f4 o[NT][DT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        m[c] = -INFINITY;
+        l[c] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[c][dt] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const Masks masks;
+    float minus = -1.0f;
+    asm("" : "+v"(minus));   // a product the compiler keeps: v - hi then is one v_fma_mix_f32
+    // A block; at the tile's edge, some row's last slots or the cache's.
+    auto step = [&](auto at_edge) {
+        constexpr bool edge = decltype(at_edge)::value;
+        const uint8_t *const vb = vp + (size_t)b * L::BLOCK;
+        VFrag<HD> vf;
+        vf.load(vb, i, q);
+        f4 x[NT][2];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) x[c][0] = x[c][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const h8 k0 = kf.value(masks, 0, u), k1 = kf.value(masks, 1, u);
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                const h8 hi = NT == 1 ? qh[u] : qs[((c * U + u) * 2u) * 64u + lane];
+                const h8 lo = NT == 1 ? ql[u] : qs[((c * U + u) * 2u + 1u) * 64u + lane];
+                x[c][0] = mfma16(k0, hi, x[c][0]);
+                x[c][1] = mfma16(k1, hi, x[c][1]);
+                x[c][0] = mfma16(k0, lo, x[c][0]);
+                x[c][1] = mfma16(k1, lo, x[c][1]);
+            }
+        }
+        if (b + W < b1) kf.load(kp + (size_t)(b + W) * L::BLOCK, i, q);
+        VScale sc[2];
+        sc[0].template load<HD>(vb, 0, q);
+        __builtin_amdgcn_sched_barrier(0);
         const uint32_t slot0 = b * 32u + 8u * q;
-        const bool edge = b * 32u + 31u > sees_all;   // some row's last slots, or the cache's
-        float top = -INFINITY;
+        if constexpr (edge) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            x[e] *= factor;
-            if (edge && slot0 + e > limit) x[e] = -INFINITY;
-            top = fmaxf(top, x[e]);
-        }
-        if (__any(top > m + kLazy)) {
-            const float t = row_max(top), mn = t > m + kLazy ? t : m;
-            const float alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= alpha;
+            for (int c = 0; c < NT; ++c) {
+                const uint32_t last = limit(c);
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+                for (int e = 0; e < 8; ++e) x[c][e / 4][e % 4] = slot0 + e > last ? -INFINITY : x[c][e / 4][e % 4];
+            }
         }
-        h8 ph, pl;
+        float top[NT];
+        bool moves = false;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float v = __builtin_amdgcn_exp2f(x[e] - (m - kRaise));
-            if (edge && slot0 + e > limit) v = 0.f;
-            l += v;
-            ph[e] = (_Float16)v;
-            pl[e] = (_Float16)(v - (float)ph[e]);
+        for (int c = 0; c < NT; ++c) {
+            top[c] = x[c][0][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) top[c] = fmaxf(top[c], x[c][e / 4][e % 4]);
+            top[c] *= factor[c];
+            moves = moves || top[c] > m[c] + kLazy;
         }
-        // Slots past the tile's keys may hold anything: their values count as zero.
-        const uint32_t some = edge ? min(max(sp.keys, slot0) - slot0, 8u) : 8u;
+        if (__builtin_expect(__any(moves), 0)) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                const float t = row_max(top[c]), mn = t > m[c] + kLazy ? t : m[c];
+                const float alpha = mn == m[c] ? 1.f : __builtin_amdgcn_exp2f(m[c] - mn);
+                m[c] = mn;
+                l[c] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[c][dt] *= alpha;
+            }
+        }
+        h8 ph[NT], pl[NT];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            // A row that attends to nothing of the blocks so far has no reference yet; any serves.
+            const float ref = (m[c] == -INFINITY ? 0.f : m[c]) - kRaise;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[c][e / 4][e % 4], factor[c], -ref));
+                l[c] += v[e];
+            }
+            h2 h[4], r[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                h[e] = __builtin_convertvector((f2{v[2 * e], v[2 * e + 1]}), h2);
+                r[e] = __builtin_convertvector((f2{__builtin_fmaf(minus, (float)h[e][0], v[2 * e]),
+                                                   __builtin_fmaf(minus, (float)h[e][1], v[2 * e + 1])}), h2);
+            }
+            ph[c] = join8(h);
+            pl[c] = join8(r);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const uint32_t some = min(max(sp.keys, slot0) - slot0, 8u);
 #pragma unroll
         for (int g = 0; g < L::G; ++g) {
-            const h8 *const sc = reinterpret_cast<const h8 *>(vb + L::CODES) + (q * L::G + g) * 2u;
-            h8 d = sc[0], off = sc[1];
-            if (edge) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    d[e] = (uint32_t)e < some ? d[e] : 0.f16;
-                    off[e] = (uint32_t)e < some ? off[e] : 0.f16;
-                }
-            }
+            VScale &now = sc[g % 2];
+            if (g + 1 < L::G) sc[(g + 1) % 2].template load<HD>(vb, g + 1, q);
+            if constexpr (edge) now.keep(some);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t code = reinterpret_cast<const uint32_t *>(vb)[(q * 32u + 16u * h + i) * L::G + g];
-                const h8 v = values8(code, d, off);
-                o[2 * g + h] = mfma16(v, ph, o[2 * g + h]);
-                o[2 * g + h] = mfma16(v, pl, o[2 * g + h]);
+                const h8 v = values8(masks, vf.code[h][g], now.d, now.o);
+#pragma unroll
+                for (int c = 0; c < NT; ++c) o[c][2 * g + h] = mfma16(v, ph[c], o[c][2 * g + h]);
+#pragma unroll
+                for (int c = 0; c < NT; ++c) o[c][2 * g + h] = mfma16(v, pl[c], o[c][2 * g + h]);
+            }
+        }
+    };
+    const uint32_t whole = min(b1, (sees_all + 1u) / 32u);   // blocks that every row attends to all of
+    for (; b < whole; b += W) step(std::false_type{});
+    for (; b < b1; b += W) step(std::true_type{});
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        l[c] = row_sum(l[c]);
+        if (q == 0) ms[w][16 * c + i] = m[c], ls[w][16 * c + i] = l[c];
+    }
+    __syncthreads();   // the queries in LDS have been read, every wave's m and l are there
+
+    // A wave's sums are taken to the row's largest reference. One without keys has nothing
+    // to give; one whose every score is NaN has no reference but a NaN sum.
+    auto *const os = reinterpret_cast<float (*)[R][OROW]>(lds);
+    float sum[NT], top[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        top[c] = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < W; ++v) top[c] = fmaxf(top[c], ms[v][16 * c + i]);
+        sum[c] = 0.f;
+#pragma unroll
+        for (int v = 0; v < W; ++v) {
+            const float mv = ms[v][16 * c + i], lv = ls[v][16 * c + i];
+            sum[c] += mv == -INFINITY ? lv : lv * __builtin_amdgcn_exp2f(mv - top[c]);
+        }
+        const float mine = m[c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[c] - top[c]);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[c][dt] *= mine;
+    }
+    if constexpr (W > B) {
+        if (w >= B) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f4 *>(&os[w - B][16 * c + i][16 * dt + 4 * q]) = o[c][dt];
+        }
+        __syncthreads();
+        if (w < B) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[c][dt] += *reinterpret_cast<const f4 *>(&os[w][16 * c + i][16 * dt + 4 * q]);
+        }
+    }
+    if (w < B) {
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f4 *>(&os[w][16 * c + i][16 * dt + 4 * q]) = o[c][dt];
+    }
+    const size_t unit = ((size_t)s * p.a.g.kv_heads + head) * p.tiles + tile, part = unit * p.splits + split;
+    const bool alone = sp.active <= 1u;
+    if (w == 0 && q == 0) {   // ms and ls of wave 0 become the row's: read by all above, written below a barrier
+#pragma unroll
+        for (int c = 0; c < NT; ++c) fs[16 * c + i] = sum[c];
+    }
+    if (w == 0 && q == 0) {
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            const uint32_t row = r0 + 16u * c + i;
+            if (row >= rows) continue;
+            if (alone) {
+                p.lse[((size_t)s * p.a.g.kv_heads + head) * rows + row] = (top[c] - kRaise) + __builtin_amdgcn_logf(sum[c]);
+            } else {
+                p.ml[(part * R + 16u * c + i) * 2u] = top[c];
+                p.ml[(part * R + 16u * c + i) * 2u + 1u] = sum[c];
             }
         }
     }
-    l = row_sum(l);
-    if (q == 0) ms[w][i] = m, ls[w][i] = l;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f4 *>(&os[w][i][16 * dt + 4 * q]) = o[dt];
     __syncthreads();
-
-    const size_t unit = ((size_t)s * p.a.g.kv_heads + head) * p.tiles + tile, part = unit * p.splits + split;
-    constexpr int TPR = 256 / kRows, PER = HD / TPR;   // lanes a row, dimensions a lane
-    const uint32_t orow = tid / TPR, c0 = tid % TPR;
-    if (r0 + orow >= rows) return;
-    float top = -INFINITY;
+    constexpr int V = HD / 4;   // four dimensions a lane
+    for (uint32_t k = tid; k < (uint32_t)R * V; k += 64u * W) {
+        const uint32_t r = k / V, c = 4u * (k % V), row = r0 + r;
+        if (row >= rows) break;
+        f4 v = *reinterpret_cast<const f4 *>(&os[0][r][c]);
 #pragma unroll
-    for (int v = 0; v < (int)kWaves; ++v) top = fmaxf(top, ms[v][orow]);
-    float sc[kWaves], sum = 0.f;
-#pragma unroll
-    for (int v = 0; v < (int)kWaves; ++v) {
-        // a wave without keys has nothing to give; one whose every score is NaN has no maximum but a NaN sum
-        sc[v] = ms[v][orow] == -INFINITY ? (ls[v][orow] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ms[v][orow] - top);
-        sum += ls[v][orow] * sc[v];
-    }
-    const bool alone = sp.active <= 1u;
-    const uint32_t t = (r0 + orow) / p.group, j = (r0 + orow) - t * p.group;
-    const bool attends = sp.base < p.a.g.context && sp.base + t < p.a.g.context;
-    const float inv = !alone ? 1.f : attends ? 1.0f / sum : 0.f;
-    float *const to = alone ? p.a.out + ((size_t)s * p.a.tokens + t) * p.a.out_stride + (size_t)(head * p.group + j) * HD
-                            : p.acc + (part * kRows + orow) * HD;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        const uint32_t c = c0 + k * TPR;
-        float v = 0.f;
-#pragma unroll
-        for (int u = 0; u < (int)kWaves; ++u) v += os[u][orow][c] * sc[u];
-        to[c] = attends || !alone ? v * inv : 0.f;
-    }
-    if (c0 == 0) {
-        if (alone) {
-            p.lse[unit * kRows + orow] = (top - kRaise) + __builtin_amdgcn_logf(sum);
+        for (int u = 1; u < B; ++u) v += *reinterpret_cast<const f4 *>(&os[u][r][c]);
+        const uint32_t t = row / p.group, j = row - t * p.group;
+        if (!alone) {
+            *reinterpret_cast<f4 *>(p.acc + (part * R + r) * HD + c) = v;
+            continue;
+        }
+        const bool attends = sp.base < p.a.g.context && sp.base + t < p.a.g.context;
+        v = attends ? v * (1.0f / fs[r]) : f4{0.f, 0.f, 0.f, 0.f};
+        float *const to = p.a.out + ((size_t)s * p.a.tokens + t) * p.a.out_stride + (size_t)(head * p.group + j) * HD + c;
+        if (p.a.ovec) {
+            *reinterpret_cast<f4 *>(to) = v;
         } else {
-            p.ml[(part * kRows + orow) * 2u] = top;
-            p.ml[(part * kRows + orow) * 2u + 1u] = sum;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[e] = v[e];
         }
     }
 }
 
-// The splits of a tile, joined.
+// The splits of a row, joined: a workgroup a row, its lanes HD / 4 columns by as many
+// splits at once as fit.
+constexpr uint32_t kMaxSplits = 256;
+constexpr uint32_t kWideTiles = 192;   // tiles of 64 rows from which on they are taken
 template <int HD>
-__global__ __launch_bounds__(256) void k_kv4_join(AttnArgs p) {
-    const uint32_t tile = blockIdx.x, head = blockIdx.y, s = blockIdx.z, seq = p.a.first + s;
-    const Span sp = span_of(p, seq, tile);
+__global__ __launch_bounds__(256) void k_kv4_join(AttnArgs p, uint32_t tile_rows) {
+    constexpr int V = HD / 4, Y = 256 / V;
+    __shared__ float sc[kMaxSplits], red[8];
+    __shared__ __attribute__((aligned(16))) float os[Y][HD];
+    const uint32_t tid = threadIdx.x, row = blockIdx.x, head = blockIdx.y, s = blockIdx.z, seq = p.a.first + s;
+    const uint32_t tile = row / tile_rows, r = row - tile * tile_rows;
+    const Span sp = span_of(p, seq, min((tile + 1u) * tile_rows, p.rows) - 1u);
     if (sp.active <= 1u) return;
-    const uint32_t rows = p.a.tokens * p.group, r0 = tile * kRows;
     const size_t unit = ((size_t)s * p.a.g.kv_heads + head) * p.tiles + tile;
-    constexpr int TPR = 256 / kRows, PER = HD / TPR;
-    const uint32_t orow = threadIdx.x / TPR, c0 = threadIdx.x % TPR;
-    if (r0 + orow >= rows) return;
-    const float *const ml = p.ml + (unit * p.splits * kRows + orow) * 2u;
-    const float *const acc = p.acc + (unit * p.splits * kRows + orow) * HD;
-    float top = -INFINITY;
-    for (uint32_t v = 0; v < sp.active; ++v) top = fmaxf(top, ml[(size_t)v * kRows * 2u]);
-    float sum = 0.f, o[PER];
-#pragma unroll
-    for (int k = 0; k < PER; ++k) o[k] = 0.f;
-    for (uint32_t v = 0; v < sp.active; ++v) {
-        const float m = ml[(size_t)v * kRows * 2u], l = ml[(size_t)v * kRows * 2u + 1u];
-        const float sc = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - top);
-        sum += l * sc;
-#pragma unroll
-        for (int k = 0; k < PER; ++k) o[k] += acc[(size_t)v * kRows * HD + c0 + k * TPR] * sc;
+    const size_t first = unit * p.splits * tile_rows + r;   // the row's record in split 0
+    float m = -INFINITY, l = 0.f;
+    if (tid < sp.active) {
+        m = p.ml[(first + (size_t)tid * tile_rows) * 2u];
+        l = p.ml[(first + (size_t)tid * tile_rows) * 2u + 1u];
     }
-    const uint32_t t = (r0 + orow) / p.group, j = (r0 + orow) - t * p.group;
-    const bool attends = sp.base + t < p.a.g.context;
-    float *const to = p.a.out + ((size_t)s * p.a.tokens + t) * p.a.out_stride + (size_t)(head * p.group + j) * HD;
+    float top = m;
 #pragma unroll
-    for (int k = 0; k < PER; ++k) to[c0 + k * TPR] = attends ? o[k] / sum : 0.f;
-    if (c0 == 0) p.lse[unit * kRows + orow] = (top - kRaise) + __builtin_amdgcn_logf(sum);
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    if ((tid & 63u) == 0) red[tid >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float mine = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+    if (tid < sp.active) sc[tid] = mine;
+    float sum = l * mine;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+    if ((tid & 63u) == 0) red[4 + (tid >> 6)] = sum;
+    __syncthreads();
+    sum = (red[4] + red[5]) + (red[6] + red[7]);
+    const uint32_t c = 4u * (tid % V), y = tid / V;
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (uint32_t v = y; v < sp.active; v += Y)
+        o += *reinterpret_cast<const f4 *>(p.acc + (first + (size_t)v * tile_rows) * HD + c) * sc[v];
+    *reinterpret_cast<f4 *>(&os[y][c]) = o;
+    __syncthreads();
+    const uint32_t t = row / p.group, j = row - t * p.group;
+    const bool attends = sp.base + t < p.a.g.context;
+    if (tid < (uint32_t)HD) {
+        float v = os[0][tid];
+#pragma unroll
+        for (int u = 1; u < Y; ++u) v += os[u][tid];
+        p.a.out[((size_t)s * p.a.tokens + t) * p.a.out_stride + (size_t)(head * p.group + j) * HD + tid] = attends ? v / sum : 0.f;
+    }
+    if (tid == 0) p.lse[((size_t)s * p.a.g.kv_heads + head) * p.rows + row] = (top - kRaise) + __builtin_amdgcn_logf(sum);
 }
 
-// Accumulated weights: a wave per block of 32 slots takes the scores of every row that may
-// attend to it again, and sums 2^(score - lse) over the rows.
+// The weight of a slot from its rows' sum: added to what it had, unless the call's own
+// tokens fill it or nothing is kept.
+__device__ __forceinline__ void add_weight(float *to, uint32_t slot, uint32_t base, float decay, float v) {
+    to[slot] = slot >= base || decay == 0.f ? v : decay * to[slot] + v;
+}
+
+// A lane's sum over the 16 lanes of its DPP row: quads, half rows, rows.
+__device__ __forceinline__ float sum16(float v) {
+    v += dpp<0xb1>(v);
+    v += dpp<0x4e>(v);
+    v += dpp<0x141>(v);
+    return v + dpp<0x140>(v);
+}
+
+// Accumulated weights of at most 16 rows: a wave per block of 32 slots takes the scores
+// again, and sums 2^(score - lse) over the rows.
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs p) {
     using L = Lay<HD>;
     constexpr int U = HD / 32;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
-    const uint32_t b = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t b = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t head = blockIdx.y, s = blockIdx.z, seq = p.a.first + s;
-    const uint32_t rows = p.a.tokens * p.group;
     const uint32_t base = p.a.slots[seq];
     if (base >= p.a.g.context) return;
     const uint32_t keys = min(base + p.a.tokens, p.a.g.context);
     if (b * 32u >= keys) return;
     const size_t plane = plane_of(p.a.g, p.a.layer, seq, head);
-    const uint8_t *const kb = p.a.kc + plane * plane_bytes<HD>(p.a.g) + (size_t)b * L::BLOCK;
+    const Masks masks;
+    KFrag<HD> kf;
+    kf.load(p.a.kc + plane * plane_bytes<HD>(p.a.g) + (size_t)b * L::BLOCK, i, q);
     const uint32_t slot0 = b * 32u + 8u * q;
-    // the first token whose row attends to a slot of the block
-    const uint32_t t0 = b * 32u > base ? b * 32u - base : 0u;
-    float sum[8];
+    const uint32_t row = min(i, p.rows - 1u), t = row / p.group;
+    const bool valid = i < p.rows && base + t < p.a.g.context;
+    h8 qh[U], ql[U];
+    const float factor = load_q<HD>(p, s, head, row, true, q, qh, ql);
+    const float lse = p.lse[((size_t)s * p.a.g.kv_heads + head) * p.rows + row];
+    f4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] = 0.f;
-    for (uint32_t tile = t0 * p.group / kRows; tile < p.tiles; ++tile) {
-        const uint32_t row = min(tile * kRows + i, rows - 1u), t = row / p.group;
-        const bool valid = tile * kRows + i < rows && base + t < p.a.g.context;
-        h8 qh[U], ql[U];
-        const float factor = load_q<HD>(p, s, head, row, true, q, qh, ql);
-        const float lse = p.lse[(((size_t)s * p.a.g.kv_heads + head) * p.tiles + tile) * kRows + row % kRows];
-        float x[8];
-        scores<HD>(kb, i, q, qh, ql, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (valid && slot0 + e <= base + t) sum[e] += __builtin_amdgcn_exp2f(x[e] * factor - lse);
+    for (int u = 0; u < U; ++u) {
+        const h8 k0 = kf.value(masks, 0, u), k1 = kf.value(masks, 1, u);
+        x[0] = mfma16(k0, qh[u], x[0]);
+        x[1] = mfma16(k1, qh[u], x[1]);
+        x[0] = mfma16(k0, ql[u], x[0]);
+        x[1] = mfma16(k1, ql[u], x[1]);
     }
     float *const to = p.a.weights + plane * p.a.g.context;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        float v = sum[e];
-        v += dpp<0xb1>(v);    // over the 16 lanes of the rows: quads, half rows, rows
-        v += dpp<0x4e>(v);
-        v += dpp<0x141>(v);
-        v += dpp<0x140>(v);
-        if (i == (uint32_t)e && slot0 + e < keys) {
-            const bool fresh = slot0 + e >= base || p.a.decay == 0.f;
-            to[slot0 + e] = fresh ? v : p.a.decay * to[slot0 + e] + v;
+        const bool sees = valid && slot0 + e <= base + t;
+        const float v = sum16(sees ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[e / 4][e % 4], factor, -lse)) : 0.f);
+        if (i == (uint32_t)e && slot0 + e < keys) add_weight(to, slot0 + e, base, p.a.decay, v);
+    }
+}
+
+// The same of more rows: a workgroup takes 256 slots, 64 a wave, whose values it makes once
+// and keeps in registers, over the row tiles blockIdx.x / chunks, + row_splits, ... The
+// tiles' operands, left by the attention kernel, pass through LDS two at a time, the next
+// two on their way while these are multiplied. A lane sums its slots over the rows it sees;
+// the sums over the row splits are added by k_kv4_add_weights, in order.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
+    using L = Lay<HD>;
+    constexpr int U = HD / 32, TILE = U * 128, PER = 2 * TILE / 256;   // h8 of a tile; of two, a lane
+    __shared__ __attribute__((aligned(16))) h8 qs[2][2 * TILE];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t chunk = blockIdx.x / p.row_splits, part = blockIdx.x % p.row_splits;
+    const uint32_t head = blockIdx.y, s = blockIdx.z, seq = p.a.first + s;
+    const uint32_t base = p.a.slots[seq];
+    if (base >= p.a.g.context) return;
+    const uint32_t keys = min(base + p.a.tokens, p.a.g.context);
+    if (chunk * 256u >= keys) return;
+    const size_t pair = (size_t)s * p.a.g.kv_heads + head;
+    const uint32_t b0 = chunk * 8u + 2u * w, blocks = (keys + 31u) / 32u;
+    const uint8_t *const kp = p.a.kc + plane_of(p.a.g, p.a.layer, seq, head) * plane_bytes<HD>(p.a.g);
+    h8 k[2][2][U];
+    {
+        const Masks masks;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            KFrag<HD> kf;
+            kf.load(kp + (size_t)min(b0 + v, blocks - 1u) * L::BLOCK, i, q);   // a block behind the last: not stored below
+#pragma unroll
+            for (int u = 0; u < U; ++u) k[v][0][u] = kf.value(masks, 0, u), k[v][1][u] = kf.value(masks, 1, u);
         }
     }
+    // pairs of row tiles from the first that attends to a slot of the chunk
+    const uint32_t t0 = chunk * 256u > base ? chunk * 256u - base : 0u;
+    const uint32_t pairs_end = (p.rows + 31u) / 32u, step = p.row_splits;
+    uint32_t j = t0 * p.group / 32u + part;
+    const h8 *const src = p.qp + pair * p.qtiles * TILE;
+    const float *const lses = p.lse + pair * p.rows, *const factors = p.factors + pair * p.rows;
+    h8 next[PER];
+    float sum[2][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[0][e] = sum[1][e] = 0.f;
+    auto fetch = [&](uint32_t to) {
+#pragma unroll
+        for (int n = 0; n < PER; ++n) next[n] = src[(size_t)to * 2u * TILE + n * 256u + tid];
+    };
+    if (j < pairs_end) fetch(j);
+    for (uint32_t turn = 0; j < pairs_end; j += step, turn ^= 1u) {
+        // A buffer is written two turns after it was last read, with a barrier between.
+#pragma unroll
+        for (int n = 0; n < PER; ++n) qs[turn][n * 256u + tid] = next[n];
+        if (j + step < pairs_end) fetch(j + step);
+        float factor[2], lse[2];
+        uint32_t last[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const uint32_t row = j * 32u + 16u * c + i, at = min(row, p.rows - 1u), t = at / p.group;
+            factor[c] = factors[at];
+            last[c] = base + t;
+            lse[c] = row < p.rows && last[c] < p.a.g.context ? lses[at] : INFINITY;   // 2^-inf: counts nothing
+        }
+        const uint32_t first_row_sees = base + j * 32u / p.group;
+        const bool edge = (b0 + 2u) * 32u - 1u > first_row_sees;
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const h8 *const from = qs[turn] + c * TILE + lane;
+            f4 x[2][2] = {{{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}};
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const h8 hi = from[u * 128], lo = from[u * 128 + 64];
+#pragma unroll
+                for (int v = 0; v < 4; ++v) x[v / 2][v % 2] = mfma16(k[v / 2][v % 2][u], hi, x[v / 2][v % 2]);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) x[v / 2][v % 2] = mfma16(k[v / 2][v % 2][u], lo, x[v / 2][v % 2]);
+            }
+#pragma unroll
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[v][e / 4][e % 4], factor[c], -lse[c]));
+                    if (edge) y = (b0 + v) * 32u + 8u * q + e <= last[c] ? y : 0.f;
+                    sum[v][e] += y;
+                }
+        }
+    }
+    float *const sums = p.sums + ((size_t)part * gridDim.y * gridDim.z + pair) * p.slots32;
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float y = sum16(sum[v][e]);
+            const uint32_t slot = (b0 + v) * 32u + 8u * q + e;
+            if (i == (uint32_t)e && slot < keys) sums[slot] = y;
+        }
+}
+
+__global__ __launch_bounds__(256) void k_kv4_add_weights(AttnArgs p) {
+    const uint32_t slot = blockIdx.x * 256u + threadIdx.x, head = blockIdx.y, s = blockIdx.z, seq = p.a.first + s;
+    const uint32_t base = p.a.slots[seq];
+    if (base >= p.a.g.context || slot >= min(base + p.a.tokens, p.a.g.context)) return;
+    const size_t pair = (size_t)s * p.a.g.kv_heads + head, pairs = (size_t)gridDim.y * gridDim.z;
+    float v = 0.f;
+    for (uint32_t k = 0; k < p.row_splits; ++k) v += p.sums[(k * pairs + pair) * p.slots32 + slot];
+    add_weight(p.a.weights + plane_of(p.a.g, p.a.layer, seq, head) * p.a.g.context, slot, base, p.a.decay, v);
 }
 
 // ------------------------------------------------------------------- eviction
@@ -731,59 +1051,122 @@ int launch_kv4_advance(hipStream_t s, uint32_t *slots, uint32_t *positions, uint
 }
 
 namespace {
-// Splits of the key axis: enough workgroups for two on each of 256 CUs, none with less
-// than a block a wave.
+// Tiles of query rows and splits of the key axis. Up to 16 rows: tiles of 16, workgroups
+// of four waves, as many splits as make 2048 workgroups of at least four blocks each (a
+// block a wave). More rows: eight waves a tile of 32 or 64.
 struct Shape {
-    uint32_t group, tiles, splits;
+    uint32_t group, rows, nt, waves, tiles, splits, per;
     uint64_t units;
 };
 Shape shape_of(const Kv4Attn &a) {
     Shape h;
     h.group = a.q_heads / a.g.kv_heads;
-    h.tiles = (a.tokens * h.group + kRows - 1u) / kRows;
-    h.units = (uint64_t)h.tiles * a.g.kv_heads * a.n;
-    const uint32_t blocks = (a.g.context + 31u) / 32u, most = (blocks + kWaves - 1u) / kWaves;
-    const uint64_t want = (512u + h.units - 1u) / h.units;
-    h.splits = (uint32_t)(want < most ? want : most);
+    h.rows = a.tokens * h.group;
+    const uint64_t pairs = (uint64_t)a.g.kv_heads * a.n;
+    const uint32_t blocks = (a.g.context + 31u) / 32u;
+    if (h.rows <= 16u) {
+        h.nt = 1;
+        h.waves = 4;
+    } else {
+        h.nt = a.g.head_dim < 256u && (h.rows + 63u) / 64u * pairs >= kWideTiles ? 4 : 2;
+        h.waves = 8;
+    }
+    h.tiles = (h.rows + 16u * h.nt - 1u) / (16u * h.nt);
+    h.units = h.tiles * pairs;
+    const uint64_t want = ((h.nt == 1 ? 2048u : 256u) + h.units - 1u) / h.units;
+    const uint32_t least = h.nt == 1 ? 4u : 32u;   // blocks of a split
+    uint32_t splits = (blocks + least - 1u) / least;
+    if (splits > want) splits = (uint32_t)want;
+    if (splits > kMaxSplits) splits = kMaxSplits;
+    h.per = (blocks + splits - 1u) / splits;
+    h.splits = (blocks + h.per - 1u) / h.per;
     return h;
 }
 }  // namespace
 
-uint64_t kv4_attn_scratch_bytes(const Kv4Attn &a, bool) {
-    const Shape h = shape_of(a);
-    return h.units * kRows * 4u + (h.splits > 1u ? h.units * h.splits * kRows * (2u + a.g.head_dim) * 4u : 0u);
+namespace {
+// The parts of a call's scratch, in floats from its start; `end` is its size.
+struct Parts {
+    uint64_t acc, ml, qp, lse, factors, sums, end;
+    uint32_t qtiles, row_splits, slots32;
+};
+Parts parts_of(const Kv4Attn &a, const Shape &h, bool with_weights) {
+    Parts t;
+    const uint64_t pairs = (uint64_t)a.g.kv_heads * a.n;
+    const uint64_t records = h.splits > 1u ? h.units * h.splits * 16u * h.nt : 0u;
+    const bool rows = with_weights && h.nt > 1u;   // the weights of prompts
+    t.qtiles = (h.rows + 31u) / 32u * 2u;
+    if (t.qtiles < h.tiles * h.nt) t.qtiles = h.tiles * h.nt;
+    t.slots32 = (a.g.context + 31u) / 32u * 32u;
+    // about 512 workgroups of 256 slots, at least two pairs of row tiles each
+    const uint64_t chunks = (a.g.context + 255u) / 256u * pairs, most = (h.rows + 63u) / 64u;
+    uint64_t splits = (512u + chunks - 1u) / chunks;
+    if (splits > most) splits = most;
+    t.row_splits = (uint32_t)splits;
+    t.acc = 0;
+    t.ml = t.acc + records * a.g.head_dim;
+    t.qp = t.ml + records * 2u;
+    t.lse = t.qp + (rows ? pairs * t.qtiles * 16u * a.g.head_dim : 0u);
+    t.factors = t.lse + (pairs * h.rows + 3u) / 4u * 4u;
+    t.sums = t.factors + (rows ? (pairs * h.rows + 3u) / 4u * 4u : 0u);
+    t.end = t.sums + (rows ? (uint64_t)t.row_splits * pairs * t.slots32 : 0u);
+    return t;
+}
+}  // namespace
+
+uint64_t kv4_attn_scratch_bytes(const Kv4Attn &a, bool with_weights) {
+    return parts_of(a, shape_of(a), with_weights).end * 4u;
 }
 
-int launch_kv4_attention(hipStream_t s, const Kv4Attn &a) {
+template <int HD>
+static int attention(hipStream_t s, const Kv4Attn &a) {
     const Shape h = shape_of(a);
+    const Parts t = parts_of(a, h, a.weights != nullptr);
+    const bool rows = a.weights && h.nt > 1u;
     AttnArgs p;
     p.a = a;
     p.group = h.group;
+    p.rows = h.rows;
     p.tiles = h.tiles;
     p.splits = h.splits;
-    p.acc = a.scratch;
-    p.ml = p.acc + (h.splits > 1u ? h.units * h.splits * kRows * a.g.head_dim : 0u);
-    p.lse = p.ml + (h.splits > 1u ? h.units * h.splits * kRows * 2u : 0u);
+    p.per = h.per;
+    p.acc = a.scratch + t.acc;
+    p.ml = a.scratch + t.ml;
+    p.lse = a.scratch + t.lse;
+    p.qp = rows ? reinterpret_cast<h8 *>(a.scratch + t.qp) : nullptr;
+    p.factors = a.scratch + t.factors;
+    p.sums = a.scratch + t.sums;
+    p.qtiles = t.qtiles;
+    p.row_splits = t.row_splits;
+    p.slots32 = t.slots32;
     const dim3 grid(h.tiles * h.splits, a.g.kv_heads, a.n);
-#define CALL(HD) k_kv4_attn<HD><<<grid, 256, 0, s>>>(p)
-    KV4_HD(a.g.head_dim, CALL)
-#undef CALL
+    if (h.nt == 1) {
+        k_kv4_attn<HD, 1, 4><<<grid, 256, 0, s>>>(p);
+    } else if (h.nt == 2) {
+        k_kv4_attn<HD, 2, 8><<<grid, 512, 0, s>>>(p);
+    } else if constexpr (HD < 256) {
+        k_kv4_attn<HD, 4, 8><<<grid, 512, 0, s>>>(p);
+    }
     VX_LAUNCHED("k_kv4_attn");
     if (h.splits > 1u) {
-        const dim3 jgrid(h.tiles, a.g.kv_heads, a.n);
-#define CALL(HD) k_kv4_join<HD><<<jgrid, 256, 0, s>>>(p)
-        KV4_HD(a.g.head_dim, CALL)
-#undef CALL
+        k_kv4_join<HD><<<dim3(h.rows, a.g.kv_heads, a.n), 256, 0, s>>>(p, 16u * h.nt);
         VX_LAUNCHED("k_kv4_join");
     }
-    if (a.weights) {
-        const dim3 wgrid(((a.g.context + 31u) / 32u + kWaves - 1u) / kWaves, a.g.kv_heads, a.n);
-#define CALL(HD) k_kv4_weights<HD><<<wgrid, 256, 0, s>>>(p)
-        KV4_HD(a.g.head_dim, CALL)
-#undef CALL
+    if (rows) {
+        const uint32_t chunks = (a.g.context + 255u) / 256u;
+        k_kv4_weights_rows<HD><<<dim3(chunks * t.row_splits, a.g.kv_heads, a.n), 256, 0, s>>>(p);
+        VX_LAUNCHED("k_kv4_weights_rows");
+        k_kv4_add_weights<<<dim3(chunks, a.g.kv_heads, a.n), 256, 0, s>>>(p);
+        VX_LAUNCHED("k_kv4_add_weights");
+    } else if (a.weights) {
+        k_kv4_weights<HD><<<dim3(((a.g.context + 31u) / 32u + 3u) / 4u, a.g.kv_heads, a.n), 256, 0, s>>>(p);
         VX_LAUNCHED("k_kv4_weights");
     }
     return VX_OK;
+}
+
+int launch_kv4_attention(hipStream_t s, const Kv4Attn &a) {
+    return a.g.head_dim == 64u ? attention<64>(s, a) : a.g.head_dim == 128u ? attention<128>(s, a) : attention<256>(s, a);
 }
 
 int launch_kv4_select(hipStream_t s, const Kv4Evict &a) {
