@@ -862,7 +862,10 @@ __device__ __forceinline__ uint32_t order_of(float w) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-constexpr uint32_t kSelect = 1024;
+constexpr uint32_t kSelect = 1024;                 // lanes of a plane's workgroup
+constexpr uint32_t kSelectWaves = kSelect / 64;
+constexpr uint32_t kSelectSlots = 16384;           // slots whose orders fit the workgroup's LDS
+constexpr uint32_t kBins = 2048;
 
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 #pragma unroll
@@ -870,12 +873,15 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     return v;
 }
 
-// A workgroup per plane. The keep-th largest weight is found a byte at a time from
-// histograms; a pass over the slots in order then numbers those that leave below `keep`
-// and those that stay above it.
+// A workgroup per plane. The keep-th largest order is found 11, 11 and 10 bits at a time
+// from histograms in LDS; then every wave takes a run of slots, and with the waves' counts
+// numbers, first, the threshold's equals, and then the slots that leave below `keep` and
+// those that stay above it. Orders are worked out once and kept in LDS; a plane of more
+// than kSelectSlots slots works them out in every pass.
+template <bool KEPT>
 __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
-    __shared__ uint32_t hist[256], part[3][kSelect / 64], found[2];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, w = tid >> 6;
+    __shared__ uint32_t orders[KEPT ? kSelectSlots : 1], hist[kBins], part[2][kSelectWaves], found[2];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t head = blockIdx.x, s = blockIdx.y, layer = blockIdx.z, seq = a.first + s;
     const size_t plane = plane_of(a.g, layer, seq, head);
     const float *const weights = a.weights + plane * a.g.context;
@@ -885,134 +891,213 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
     uint32_t moved = 0;
     if (n > keep) {
         uint32_t newest = 0;
-        for (uint32_t j = tid; j < n; j += kSelect) newest = max(newest, positions[j]);
-        newest = wave_max_u32(newest);
-        if (lane == 0) part[0][w] = newest;
-        __syncthreads();
-        newest = wave_max_u32(part[0][lane % (kSelect / 64)]);
+        if constexpr (KEPT) {   // both tables are read once, the orders before it is known which positions are recent
+            constexpr uint32_t PER = kSelectSlots / kSelect;
+            uint32_t at[PER];
+            float wt[PER];
+#pragma unroll
+            for (uint32_t k = 0; k < PER; ++k) {
+                const uint32_t j = k * kSelect + tid;
+                if (k * kSelect < n) {
+                    at[k] = j < n ? positions[j] : 0u;
+                    wt[k] = j < n ? weights[j] : 0.f;
+                    newest = max(newest, at[k]);
+                }
+            }
+            for (uint32_t k = tid; k < kBins; k += kSelect) hist[k] = 0;
+            newest = wave_max_u32(newest);
+            if (lane == 0) part[0][w] = newest;
+            __syncthreads();
+            newest = wave_max_u32(part[0][lane % kSelectWaves]);
+#pragma unroll
+            for (uint32_t k = 0; k < PER; ++k) {
+                const uint32_t j = k * kSelect + tid;
+                if (j < n)
+                    orders[j] = at[k] < a.sinks || (uint64_t)at[k] + a.recent > newest ? 0xFFFFFFFFu : order_of(wt[k]);
+            }
+        } else {
+            for (uint32_t j = tid; j < n; j += kSelect) newest = max(newest, positions[j]);
+            for (uint32_t k = tid; k < kBins; k += kSelect) hist[k] = 0;
+            newest = wave_max_u32(newest);
+            if (lane == 0) part[0][w] = newest;
+            __syncthreads();
+            newest = wave_max_u32(part[0][lane % kSelectWaves]);
+        }
         auto order = [&](uint32_t j) {
+            if constexpr (KEPT) return orders[j];
             const uint32_t at = positions[j];
             return at < a.sinks || (uint64_t)at + a.recent > newest ? 0xFFFFFFFFu : order_of(weights[j]);
         };
-        uint32_t prefix = 0, rest = keep;   // the threshold's bytes so far, slots still to take among its equals
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            __syncthreads();
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
+        __syncthreads();
+        uint32_t prefix = 0, rest = keep;   // the threshold's bits so far, slots still to take among its equals
+        constexpr int kShift[3] = {21, 10, 0};
+#pragma unroll
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = kShift[pass], above_bits = pass == 0 ? 32 : kShift[pass - 1];
+            const uint32_t mask = pass == 2 ? 1023u : 2047u;
             for (uint32_t j = tid; j < n; j += kSelect) {
                 const uint32_t v = order(j);
-                if (shift == 24 || v >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[v >> shift & 255u], 1u);
+                if (pass == 0 || (v ^ prefix) >> (above_bits & 31) == 0) atomicAdd(&hist[v >> shift & mask], 1u);
             }
             __syncthreads();
-            if (tid == 0) {
-                uint32_t bin = 255, above = 0;
-                while (bin > 0 && above + hist[bin] < rest) above += hist[bin--];
-                found[0] = bin;
-                found[1] = above;
+            // The bin that holds the rest-th from the top: each lane two bins, descending.
+            const uint32_t b1 = kBins - 1u - 2u * tid, h1 = hist[b1], h0 = hist[b1 - 1u];
+            uint32_t sum = h1 + h0;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t t = __shfl_up((int)sum, o, 64);
+                if (lane >= (uint32_t)o) sum += t;
+            }
+            if (lane == 63) part[0][w] = sum;
+            hist[b1] = 0, hist[b1 - 1u] = 0;   // for the next pass: only this lane reads them
+            __syncthreads();
+            for (uint32_t k = 0; k < w; ++k) sum += part[0][k];
+            const uint32_t before = sum - h1 - h0;   // slots in the bins above this lane's
+            if (before < rest && sum >= rest) {
+                const bool upper = before + h1 >= rest;
+                found[0] = upper ? b1 : b1 - 1u;
+                found[1] = upper ? before : before + h1;
             }
             __syncthreads();
             prefix |= found[0] << shift;
             rest -= found[1];
         }
-        uint32_t ties = 0, holes = 0, sources = 0;   // so far
-        for (uint32_t j0 = 0; j0 < n; j0 += kSelect) {
-            const uint32_t j = j0 + tid;
-            const uint32_t v = j < n ? order(j) : 0u;
-            const bool tie = j < n && v == prefix;
-            const uint64_t below = (1ull << lane) - 1u;
-            const uint64_t tb = __ballot(tie);
-            __syncthreads();
-            if (lane == 0) part[0][w] = __popcll(tb);
-            __syncthreads();
-            uint32_t rank = ties + __popcll(tb & below), all = 0;
-            for (uint32_t k = 0; k < kSelect / 64; ++k) {
-                if (k < w) rank += part[0][k];
-                all += part[0][k];
+        // Wave w's slots are [run w, run (w + 1)), 64 at a time.
+        const uint32_t run = (n + kSelect - 1u) / kSelect * 64u, j0 = w * run, j1 = min(j0 + run, n);
+        const uint64_t below = (1ull << lane) - 1u;
+        uint32_t ties = 0;
+        for (uint32_t j = j0 + lane; j < j0 + run; j += 64u) ties += __popcll(__ballot(j < j1 && order(j) == prefix));
+        if (lane == 0) part[1][w] = ties;
+        __syncthreads();
+        ties = 0;
+        for (uint32_t k = 0; k < w; ++k) ties += part[1][k];
+        __syncthreads();   // part is written again below
+        uint32_t hr = 0, sr = 0;
+        const uint32_t first_tie = ties;
+        auto pass = [&](bool write) {
+            ties = first_tie;
+            for (uint32_t j = j0 + lane; j < j0 + run; j += 64u) {
+                const uint32_t v = j < j1 ? order(j) : 0u;
+                const bool tie = j < j1 && v == prefix;
+                const uint64_t tb = __ballot(tie);
+                const bool stays = j < j1 && (v > prefix || (tie && ties + __popcll(tb & below) < rest));
+                ties += __popcll(tb);
+                const bool hole = j < keep && j < j1 && !stays, source = j >= keep && stays;
+                const uint64_t hb = __ballot(hole), sb = __ballot(source);
+                if (write) {
+                    const uint32_t h = hr + __popcll(hb & below), r = sr + __popcll(sb & below);
+                    if (hole && h < a.moves) plan[2u * h + 1u] = j;
+                    if (source && r < a.moves) plan[2u * r] = j;
+                }
+                hr += __popcll(hb);
+                sr += __popcll(sb);
             }
-            ties += all;
-            const bool stays = j < n && (v > prefix || (tie && rank < rest));
-            const bool hole = j < keep && !stays, source = j >= keep && stays;
-            const uint64_t hb = __ballot(hole), sb = __ballot(source);
-            if (lane == 0) part[1][w] = __popcll(hb), part[2][w] = __popcll(sb);
-            __syncthreads();
-            uint32_t hr = holes + __popcll(hb & below), sr = sources + __popcll(sb & below);
-            for (uint32_t k = 0; k < kSelect / 64; ++k) {
-                if (k < w) hr += part[1][k], sr += part[2][k];
-                holes += part[1][k];
-                sources += part[2][k];
-            }
-            if (hole && hr < a.moves) plan[2u * hr + 1u] = j;
-            if (source && sr < a.moves) plan[2u * sr] = j;
+        };
+        pass(false);
+        if (lane == 0) part[0][w] = hr, part[1][w] = sr;
+        __syncthreads();
+        hr = sr = 0;
+        for (uint32_t k = 0; k < kSelectWaves; ++k) {
+            if (k < w) hr += part[0][k], sr += part[1][k];
+            moved += part[1][k];
         }
-        moved = min(sources, a.moves);
+        pass(true);
+        moved = min(moved, a.moves);
     }
     for (uint32_t k = 2u * moved + tid; k < 2u * a.moves; k += kSelect) plan[k] = VX_KV4_NO_SLOT;
 }
 
-// Moves of a plan, a workgroup for kMoves of a plane's. V's codes of an octet share dwords,
-// so that the run of moves into one octet (neighbours in the plan, whose targets rise) is
-// made by the workgroup of its first.
+// Moves of a plan, a workgroup of four waves for kMoves of a plane's. V's codes of an octet
+// share dwords, so that the moves into one octet (within eight pairs of the plan, whose
+// targets rise) are made by one wave, of the workgroup of the first: a workgroup looks at
+// seven pairs before its own and seven behind.
 constexpr uint32_t kMoves = 32;
 
 template <int HD>
-__global__ __launch_bounds__(HD) void k_kv4_compact(Kv4Evict a) {
+__global__ __launch_bounds__(256) void k_kv4_compact(Kv4Evict a) {
     using L = Lay<HD>;
-    constexpr int W = HD / 8;
-    const uint32_t tid = threadIdx.x, head = blockIdx.y % a.g.kv_heads, s = blockIdx.y / a.g.kv_heads, layer = blockIdx.z;
-    const uint32_t seq = a.first + s;
+    constexpr uint32_t W = HD / 8, NONE = VX_KV4_NO_SLOT;
+    __shared__ uint32_t froms[kMoves + 14], tos[kMoves + 14];   // of pairs e0 - 7 ..; NONE: no move
+    const uint32_t tid = threadIdx.x, lane = tid & 63u;
+    const uint32_t head = blockIdx.y % a.g.kv_heads, s = blockIdx.y / a.g.kv_heads, layer = blockIdx.z, seq = a.first + s;
     if (blockIdx.x == 0 && layer == 0 && head == 0 && tid == 0) {
         const uint32_t n = a.slots[seq];
-        if (n != VX_KV4_NO_SLOT && n > a.keep) a.slots[seq] = a.keep;
+        if (n != NONE && n > a.keep) a.slots[seq] = a.keep;
     }
     const size_t plane = plane_of(a.g, layer, seq, head);
     const uint32_t *const plan = a.plan_in + (((size_t)layer * a.n + s) * a.g.kv_heads + head) * a.moves * 2u;
-    const uint32_t e0 = blockIdx.x * kMoves, e1 = min(e0 + kMoves, a.moves);
-    auto move = [&](uint32_t e, uint32_t &from, uint32_t &to) {
-        if (e >= a.moves) return false;
-        from = plan[2u * e];
-        to = plan[2u * e + 1u];
-        return from >= a.keep && from < a.g.context && to < a.keep;
-    };
-    uint32_t from, to;
-    if (!move(e0, from, to)) return;   // the moves come first in a plan
-    for (uint32_t e = e0 + tid; e < e1; e += HD) {
-        if (!move(e, from, to)) continue;
-        const size_t base = plane * a.g.context;
-        if (a.weights) a.weights[base + to] = a.weights[base + from];
-        if (a.slot_positions) a.slot_positions[base + to] = a.slot_positions[base + from];
+    const uint32_t e0 = blockIdx.x * kMoves;
+    if (tid < kMoves + 14u) {
+        const uint32_t e = e0 + tid - 7u;   // before pair 0: past every move
+        uint32_t from = NONE, to = NONE;
+        if (e < a.moves) from = plan[2u * e], to = plan[2u * e + 1u];
+        const bool fits = from >= a.keep && from < a.g.context && to < a.keep;
+        froms[tid] = fits ? from : NONE;
+        tos[tid] = fits ? to : NONE;
+    }
+    __syncthreads();
+    if (tid < kMoves && froms[tid + 7u] != NONE) {
+        const size_t base = plane * a.g.context, from = base + froms[tid + 7u], to = base + tos[tid + 7u];
+        if (a.weights) a.weights[to] = a.weights[from];
+        if (a.slot_positions) a.slot_positions[to] = a.slot_positions[from];
     }
     if (!a.kc) return;
     uint8_t *const kp = a.kc + plane * plane_bytes<HD>(a.g), *const vp = a.vc + plane * plane_bytes<HD>(a.g);
-    for (uint32_t e = e0 + tid / W; e < e1; e += HD / W) {
-        if (!move(e, from, to)) continue;
-        uint8_t *const src = kp + (size_t)(from / 32u) * L::BLOCK, *const dst = kp + (size_t)(to / 32u) * L::BLOCK;
-        const uint32_t c = tid % W;
+#pragma unroll
+    for (uint32_t k = tid; k < kMoves * W; k += 256u) {
+        const uint32_t from = froms[k / W + 7u], to = tos[k / W + 7u], c = k % W;
+        if (from == NONE) continue;
+        const uint8_t *const src = kp + (size_t)(from / 32u) * L::BLOCK;
+        uint8_t *const dst = kp + (size_t)(to / 32u) * L::BLOCK;
         reinterpret_cast<uint32_t *>(dst)[(to % 32u) * W + c] = reinterpret_cast<const uint32_t *>(src)[(from % 32u) * W + c];
         if (c < (uint32_t)L::G)
             reinterpret_cast<uint32_t *>(dst + L::CODES)[(to % 32u) * L::G + c] =
                 reinterpret_cast<const uint32_t *>(src + L::CODES)[(from % 32u) * L::G + c];
     }
-    for (uint32_t e = e0; e < e1; ++e) {
-        uint32_t before_from, before_to;
-        if (!move(e, from, to)) continue;
-        const uint32_t oct = to / 8u;
-        if (e > 0 && move(e - 1u, before_from, before_to) && before_to / 8u == oct) continue;   // not the run's first
-        uint8_t *const dst = vp + (size_t)(oct / 4u) * L::BLOCK;
-        uint32_t *const word = reinterpret_cast<uint32_t *>(dst) + (oct % 4u) * HD + tid;
-        uint32_t v = *word;
-        for (uint32_t k = e; move(k, from, to) && to / 8u == oct && k < e + 8u; ++k) {
-            const uint8_t *const src = vp + (size_t)(from / 32u) * L::BLOCK;
-            const uint32_t oct_from = from / 8u % 4u, ef = from % 8u, et = to % 8u;
-            const uint32_t code = reinterpret_cast<const uint32_t *>(src)[oct_from * HD + tid] >> (4u * (ef / 2u) + 16u * (ef % 2u)) & 15u;
-            const uint32_t bit = 4u * (et / 2u) + 16u * (et % 2u);
-            v = (v & ~(15u << bit)) | code << bit;
-            if (tid < 2u * L::G) {   // d and o of every group
-                const uint32_t g = tid / 2u, which = tid % 2u;
-                reinterpret_cast<_Float16 *>(dst + L::CODES)[((oct % 4u) * L::G + g) * 16u + 8u * which + et] =
-                    reinterpret_cast<const _Float16 *>(src + L::CODES)[(oct_from * L::G + g) * 16u + 8u * which + ef];
-            }
+    // The octets' first pairs, wave by wave.
+    bool first = false;
+    if (lane < kMoves) {   // pair e0 + lane
+        const uint32_t to = tos[lane + 7u];
+        first = to != NONE;
+#pragma unroll
+        for (uint32_t k = 0; k < 7; ++k) first = first && tos[lane + k] / 8u != to / 8u;
+    }
+    uint64_t runs = __ballot(first);
+    for (uint32_t turn = 0; runs; ++turn, runs &= runs - 1u) {
+        if (turn % 4u != (uint32_t)__builtin_amdgcn_readfirstlane(tid >> 6)) continue;
+        const uint32_t e = (uint32_t)__builtin_ctzll(runs) + 7u, oct = tos[e] / 8u;
+        bool in[8];
+        uint32_t from[8], to[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            in[k] = tos[e + k] / 8u == oct;   // not so of NONE
+            from[k] = froms[e + k];
+            to[k] = tos[e + k] % 8u;
         }
-        *word = v;
+        uint8_t *const dst = vp + (size_t)(oct / 4u) * L::BLOCK;
+#pragma unroll
+        for (uint32_t d = lane; d < (uint32_t)HD; d += 64u) {
+            uint32_t *const word = reinterpret_cast<uint32_t *>(dst) + (oct % 4u) * HD + d;
+            uint32_t v = *word, got[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (in[k]) got[k] = reinterpret_cast<const uint32_t *>(vp + (size_t)(from[k] / 32u) * L::BLOCK)[from[k] / 8u % 4u * HD + d];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (in[k]) {
+                    const uint32_t code = got[k] >> (4u * (from[k] % 8u / 2u) + 16u * (from[k] % 2u)) & 15u;
+                    const uint32_t bit = 4u * (to[k] / 2u) + 16u * (to[k] % 2u);
+                    v = (v & ~(15u << bit)) | code << bit;
+                }
+            *word = v;
+        }
+        // d and o of every group: lane 2 G k + 2 g + which of pair e + k
+        for (uint32_t k = lane; k < 8u * 2u * L::G; k += 64u) {
+            const uint32_t f = froms[e + k / (2u * L::G)], t = tos[e + k / (2u * L::G)], g = k / 2u % L::G, which = k % 2u;
+            if (t / 8u != oct) continue;
+            reinterpret_cast<_Float16 *>(dst + L::CODES)[((oct % 4u) * L::G + g) * 16u + 8u * which + t % 8u] =
+                reinterpret_cast<const _Float16 *>(vp + (size_t)(f / 32u) * L::BLOCK + L::CODES)[(f / 8u % 4u * L::G + g) * 16u + 8u * which + f % 8u];
+        }
     }
 }
 
@@ -1170,14 +1255,18 @@ int launch_kv4_attention(hipStream_t s, const Kv4Attn &a) {
 }
 
 int launch_kv4_select(hipStream_t s, const Kv4Evict &a) {
-    k_kv4_select<<<dim3(a.g.kv_heads, a.n, a.g.layers), kSelect, 0, s>>>(a);
+    const dim3 grid(a.g.kv_heads, a.n, a.g.layers);
+    if (a.g.context <= kSelectSlots)
+        k_kv4_select<true><<<grid, kSelect, 0, s>>>(a);
+    else
+        k_kv4_select<false><<<grid, kSelect, 0, s>>>(a);
     VX_LAUNCHED("k_kv4_select");
     return VX_OK;
 }
 
 int launch_kv4_compact(hipStream_t s, const Kv4Evict &a) {
     const dim3 grid((a.moves + kMoves - 1u) / kMoves, a.g.kv_heads * a.n, a.g.layers);
-#define CALL(HD) k_kv4_compact<HD><<<grid, HD, 0, s>>>(a)
+#define CALL(HD) k_kv4_compact<HD><<<grid, 256, 0, s>>>(a)
     KV4_HD(a.g.head_dim, CALL)
 #undef CALL
     VX_LAUNCHED("k_kv4_compact");
