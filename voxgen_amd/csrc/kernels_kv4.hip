@@ -244,6 +244,7 @@ struct AttnArgs {
     Kv4Attn a;
     uint32_t group, rows, tiles;     // query heads a KV head, rows (tokens x group), tiles of them
     uint32_t splits, per;            // key splits of the grid, blocks of one
+    bool eager;                      // a wave's first block is fetched before it is known whether slots fill it
     float *ml, *acc, *lse;           // [unit][split][tile rows][2], [..][tile rows][HD], [sequence x KV head][rows]
     // for the weights of prompts: the query rows as operands [sequence x KV head][16 rows][HD / 32][hi, lo][64],
     // the factors of their scores [sequence x KV head][rows], sums by row split [split][sequence x KV head][slots]
@@ -397,14 +398,33 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
     const uint32_t split = blockIdx.x / p.tiles, tile = p.tiles - 1u - blockIdx.x % p.tiles;
     const uint32_t head = blockIdx.y, s = blockIdx.z, seq = p.a.first + s;
     const uint32_t rows = p.rows, r0 = tile * R;
-    const Span sp = span_of(p, seq, min(r0 + R, rows) - 1u);
-    if (split != 0 && split >= sp.active) return;
-    const uint32_t b0 = split * p.per, b1 = min(b0 + p.per, sp.blocks);
+    const uint32_t b0 = split * p.per;
     const size_t plane = plane_of(p.a.g, p.a.layer, seq, head) * plane_bytes<HD>(p.a.g);
     const uint8_t *const kp = p.a.kc + plane, *const vp = p.a.vc + plane;
+    constexpr bool FLAT = NT == 1 && HD <= 128;   // V's (d, o) of a block all at once, and ahead like its codes
     KFrag<HD> kf;
+    VFrag<HD> vf;
+    VScale sc[FLAT ? L::G : 2];
     uint32_t b = b0 + w;
-    if (b < b1) kf.load(kp + (size_t)b * L::BLOCK, i, q);
+    auto load_v = [&]() {
+        const uint8_t *const vb = vp + (size_t)b * L::BLOCK;
+        vf.load(vb, i, q);
+        if constexpr (FLAT) {
+#pragma unroll
+            for (int g = 0; g < L::G; ++g) sc[g].template load<HD>(vb, g, q);
+        }
+    };
+    auto load_first = [&](uint32_t end) {
+        if (b < end) {
+            kf.load(kp + (size_t)b * L::BLOCK, i, q);
+            if constexpr (FLAT) load_v();
+        }
+    };
+    if (p.eager) load_first(min(b0 + p.per, (p.a.g.context + 31u) / 32u));
+    const Span sp = span_of(p, seq, min(r0 + R, rows) - 1u);
+    if (split != 0 && split >= sp.active) return;
+    const uint32_t b1 = min(b0 + p.per, sp.blocks);
+    if (!p.eager) load_first(b1);
     h8 qh[U], ql[U];
     float factor[NT];
     h8 *const qs = reinterpret_cast<h8 *>(lds);   // [NT][U][hi, lo][64]
@@ -456,8 +476,7 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
     auto step = [&](auto at_edge) {
         constexpr bool edge = decltype(at_edge)::value;
         const uint8_t *const vb = vp + (size_t)b * L::BLOCK;
-        VFrag<HD> vf;
-        vf.load(vb, i, q);
+        if constexpr (!FLAT) load_v();
         f4 x[NT][2];
 #pragma unroll
         for (int c = 0; c < NT; ++c) x[c][0] = x[c][1] = f4{0.f, 0.f, 0.f, 0.f};
@@ -475,8 +494,7 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
             }
         }
         if (b + W < b1) kf.load(kp + (size_t)(b + W) * L::BLOCK, i, q);
-        VScale sc[2];
-        sc[0].template load<HD>(vb, 0, q);
+        if constexpr (!FLAT) sc[0].template load<HD>(vb, 0, q);
         __builtin_amdgcn_sched_barrier(0);
         const uint32_t slot0 = b * 32u + 8u * q;
         if constexpr (edge) {
@@ -533,8 +551,8 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
         const uint32_t some = min(max(sp.keys, slot0) - slot0, 8u);
 #pragma unroll
         for (int g = 0; g < L::G; ++g) {
-            VScale &now = sc[g % 2];
-            if (g + 1 < L::G) sc[(g + 1) % 2].template load<HD>(vb, g + 1, q);
+            VScale &now = sc[FLAT ? g : g % 2];
+            if (!FLAT && g + 1 < L::G) sc[(g + 1) % 2].template load<HD>(vb, g + 1, q);
             if constexpr (edge) now.keep(some);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -547,8 +565,13 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
         }
     };
     const uint32_t whole = min(b1, (sees_all + 1u) / 32u);   // blocks that every row attends to all of
-    for (; b < whole; b += W) step(std::false_type{});
-    for (; b < b1; b += W) step(std::true_type{});
+    auto next = [&]() {
+        b += W;
+        if constexpr (FLAT)
+            if (b < b1) load_v();
+    };
+    for (; b < whole; next()) step(std::false_type{});
+    for (; b < b1; next()) step(std::true_type{});
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
         l[c] = row_sum(l[c]);
@@ -643,6 +666,11 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
 // The splits of a row, joined: a workgroup a row, its lanes HD / 4 columns by as many
 // splits at once as fit.
 constexpr uint32_t kMaxSplits = 256;
+#ifndef ALONE
+#define ALONE 16
+#endif
+constexpr uint32_t kAloneBlocks = ALONE;
+constexpr uint32_t kEagerGroups = 256;
 constexpr uint32_t kWideTiles = 192;   // tiles of 64 rows from which on they are taken
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_join(AttnArgs p, uint32_t tile_rows) {
@@ -1142,6 +1170,7 @@ namespace {
 struct Shape {
     uint32_t group, rows, nt, waves, tiles, splits, per;
     uint64_t units;
+    bool eager;
 };
 Shape shape_of(const Kv4Attn &a) {
     Shape h;
@@ -1151,7 +1180,7 @@ Shape shape_of(const Kv4Attn &a) {
     const uint32_t blocks = (a.g.context + 31u) / 32u;
     if (h.rows <= 16u) {
         h.nt = 1;
-        h.waves = 4;
+        h.waves = blocks <= kAloneBlocks ? 8 : 4;
     } else {
         h.nt = a.g.head_dim < 256u && (h.rows + 63u) / 64u * pairs >= kWideTiles ? 4 : 2;
         h.waves = 8;
@@ -1159,12 +1188,13 @@ Shape shape_of(const Kv4Attn &a) {
     h.tiles = (h.rows + 16u * h.nt - 1u) / (16u * h.nt);
     h.units = h.tiles * pairs;
     const uint64_t want = ((h.nt == 1 ? 2048u : 256u) + h.units - 1u) / h.units;
-    const uint32_t least = h.nt == 1 ? 4u : 32u;   // blocks of a split
+    const uint32_t least = h.nt == 1 ? (h.waves == 8 ? kAloneBlocks : 4u) : 32u;   // blocks of a split
     uint32_t splits = (blocks + least - 1u) / least;
     if (splits > want) splits = (uint32_t)want;
     if (splits > kMaxSplits) splits = kMaxSplits;
     h.per = (blocks + splits - 1u) / splits;
     h.splits = (blocks + h.per - 1u) / h.per;
+    h.eager = h.units * h.splits <= kEagerGroups;
     return h;
 }
 }  // namespace
@@ -1215,6 +1245,7 @@ static int attention(hipStream_t s, const Kv4Attn &a) {
     p.tiles = h.tiles;
     p.splits = h.splits;
     p.per = h.per;
+    p.eager = h.eager;
     p.acc = a.scratch + t.acc;
     p.ml = a.scratch + t.ml;
     p.lse = a.scratch + t.lse;
@@ -1225,7 +1256,9 @@ static int attention(hipStream_t s, const Kv4Attn &a) {
     p.row_splits = t.row_splits;
     p.slots32 = t.slots32;
     const dim3 grid(h.tiles * h.splits, a.g.kv_heads, a.n);
-    if (h.nt == 1) {
+    if (h.nt == 1 && h.waves == 8) {
+        k_kv4_attn<HD, 1, 8><<<grid, 512, 0, s>>>(p);
+    } else if (h.nt == 1) {
         k_kv4_attn<HD, 1, 4><<<grid, 256, 0, s>>>(p);
     } else if (h.nt == 2) {
         k_kv4_attn<HD, 2, 8><<<grid, 512, 0, s>>>(p);

@@ -46,7 +46,10 @@ class Kv4Cache:
         self.weights = ctx.zeros(table) if track else None
         self.slot_positions = ctx.zeros(table) if track else None
         self._scratch = None
+        self._outgrown = []
         self._pushes = {}
+        lib = abi.load()
+        self._store, self._load, self._attention = lib.vx_kv4_store, lib.vx_kv4_load, lib.vx_kv4_attention
 
     @property
     def nbytes(self) -> int:
@@ -61,36 +64,45 @@ class Kv4Cache:
     def _range(self, first, n):
         return first, self.sequences - first if n is None else n
 
-    def _push(self, kind, *fields):
-        """The push struct of a call, kept for the next one of the same fields."""
-        got = self._pushes.get((kind, fields))
-        if got is None:
-            if len(self._pushes) > 256:
-                self._pushes.clear()
-            got = self._pushes[(kind, fields)] = kind(self.geom, *fields)
-        return got
+    # A decode loop makes the same few calls over and over: their push structs are made once, by their fields.
+    def _keep(self, key, push):
+        if len(self._pushes) >= 4096:
+            self._pushes.clear()
+        self._pushes[key] = push
+        return push
 
-    def _rows(self, layer, tokens, first, n, k_stride, v_stride, k_base, v_base):
+    def _rows(self, key):
+        layer, tokens, first, n, k_stride, v_stride, k_base, v_base = key
         width = self.kv_heads * self.head_dim
         first, n = self._range(first, n)
-        return self._push(abi.Kv4RowsPush, layer, first, n, tokens, width if k_stride is None else k_stride,
-                          width if v_stride is None else v_stride, k_base, v_base)
+        return self._keep(key, C.byref(abi.Kv4RowsPush(
+            self.geom, layer, first, n, tokens, width if k_stride is None else k_stride,
+            width if v_stride is None else v_stride, k_base, v_base)))
 
     def store(self, layer: int, k: Buffer, v: Buffer, tokens: int = 1, first: int = 0, n: int | None = None,
               k_stride: int | None = None, v_stride: int | None = None, k_base: int = 0, v_base: int = 0) -> None:
         """Rows of `tokens` tokens of each of n sequences from `first` on into their slots."""
-        pc = self._rows(layer, tokens, first, n, k_stride, v_stride, k_base, v_base)
-        abi.call("vx_kv4_store", self.ctx.handle, k.handle, v.handle, self.k.handle, self.v.handle,
-                 self.slots.handle, self.positions.handle if self.track else None,
-                 self.slot_positions.handle if self.track else None, pc)
+        key = (layer, tokens, first, n, k_stride, v_stride, k_base, v_base)
+        pc = self._pushes.get(key) or self._rows(key)
+        if self.track:
+            positions, table = self.positions.handle, self.slot_positions.handle
+        else:
+            positions = table = None
+        status = self._store(self.ctx.handle, k.handle, v.handle, self.k.handle, self.v.handle, self.slots.handle,
+                             positions, table, pc)
+        if status:
+            abi.check(status, "vx_kv4_store")
 
     def load(self, layer: int, k: Buffer | None, v: Buffer | None, tokens: int = 1, first: int = 0,
              n: int | None = None, k_stride: int | None = None, v_stride: int | None = None, k_base: int = 0,
              v_base: int = 0, slots: Buffer | None = None) -> None:
         """The values of the slots that store() with the same arguments fills, or of those from `slots` on."""
-        pc = self._rows(layer, tokens, first, n, k_stride, v_stride, k_base, v_base)
-        abi.call("vx_kv4_load", self.ctx.handle, self.k.handle, self.v.handle, k.handle if k else None,
-                 v.handle if v else None, (slots or self.slots).handle, pc)
+        key = (layer, tokens, first, n, k_stride, v_stride, k_base, v_base)
+        pc = self._pushes.get(key) or self._rows(key)
+        status = self._load(self.ctx.handle, self.k.handle, self.v.handle, k.handle if k else None,
+                            v.handle if v else None, (slots or self.slots).handle, pc)
+        if status:
+            abi.check(status, "vx_kv4_load")
 
     def advance(self, tokens: int = 1, first: int = 0, n: int | None = None) -> None:
         """The sequences' slots and positions after `tokens` tokens went through every layer."""
@@ -103,24 +115,30 @@ class Kv4Cache:
                   out_base: int = 0, decay: float = 1.0, scratch: Buffer | None = None) -> None:
         """Attention of the call's rows over the cache; with `track`, into self.weights too. The scratch is the
         cache's own unless one is given; a call captured into a graph keeps the one that it was captured with."""
-        first, n = self._range(first, n)
-        width = q_heads * self.head_dim
-        pc = self._push(abi.Kv4AttentionPush, layer, first, n, tokens, q_heads, width if q_stride is None else q_stride,
-                        width if out_stride is None else out_stride, q_base, out_base, decay)
+        key = (layer, q_heads, tokens, first, n, q_stride, out_stride, q_base, out_base, decay)
+        pc, nbytes = self._pushes.get(key) or self._rows_of_queries(key)
         if scratch is None:
-            scratch = self.scratch(pc)
-        abi.call("vx_kv4_attention", self.ctx.handle, q.handle, self.k.handle, self.v.handle, out.handle,
-                 self.weights.handle if self.track else None, self.slots.handle, scratch.handle, pc)
+            scratch = self._scratch
+            if scratch is None or scratch.nbytes < nbytes:
+                scratch = self._grow(nbytes)
+        status = self._attention(self.ctx.handle, q.handle, self.k.handle, self.v.handle, out.handle,
+                                 self.weights.handle if self.track else None, self.slots.handle, scratch.handle, pc)
+        if status:
+            abi.check(status, "vx_kv4_attention")
 
-    def scratch(self, pc: abi.Kv4AttentionPush) -> Buffer:
-        """The cache's own scratch, made larger where the call needs it. A smaller one stays allocated: a captured
-        graph may hold it."""
-        nbytes = getattr(pc, "_scratch_bytes", None)
-        if nbytes is None:
-            nbytes = pc._scratch_bytes = max(4, abi.load().vx_kv4_attention_scratch_bytes(pc, 1 if self.track else 0))
-        if self._scratch is None or self._scratch.nbytes < nbytes:
-            self._outgrown = getattr(self, "_outgrown", []) + ([self._scratch] if self._scratch else [])
-            self._scratch = self.ctx.alloc(nbytes)
+    def _rows_of_queries(self, key):
+        layer, q_heads, tokens, first, n, q_stride, out_stride, q_base, out_base, decay = key
+        width = q_heads * self.head_dim
+        first, n = self._range(first, n)
+        pc = abi.Kv4AttentionPush(self.geom, layer, first, n, tokens, q_heads, width if q_stride is None else q_stride,
+                                  width if out_stride is None else out_stride, q_base, out_base, decay)
+        return self._keep(key, (C.byref(pc), abi.load().vx_kv4_attention_scratch_bytes(pc, 1 if self.track else 0)))
+
+    def _grow(self, nbytes: int) -> Buffer:
+        """The cache's own scratch, larger. The smaller one stays allocated: a captured graph may hold it."""
+        if self._scratch is not None:
+            self._outgrown.append(self._scratch)
+        self._scratch = self.ctx.alloc(max(4, nbytes))
         return self._scratch
 
     def plan_moves(self, keep: int) -> int:
@@ -139,14 +157,14 @@ class Kv4Cache:
             raise abi.VxError(abi.STATUS_CODE["VX_ERR_STATE"], "the cache tracks no weights", "vx_kv4_select")
         first, n = self._range(first, n)
         abi.call("vx_kv4_select", self.ctx.handle, self.weights.handle, self.slot_positions.handle, self.slots.handle,
-                 plan.handle, self._push(abi.Kv4EvictPush, first, n, keep, sinks, recent))
+                 plan.handle, abi.Kv4EvictPush(self.geom, first, n, keep, sinks, recent))
 
     def compact(self, plan: Buffer, keep: int, first: int = 0, n: int | None = None) -> None:
         """Carries out the moves of `plan`, and sets the slot counts."""
         first, n = self._range(first, n)
         abi.call("vx_kv4_compact", self.ctx.handle, plan.handle, self.k.handle, self.v.handle,
                  self.weights.handle if self.track else None, self.slot_positions.handle if self.track else None,
-                 self.slots.handle, self._push(abi.Kv4EvictPush, first, n, keep, 0, 0))
+                 self.slots.handle, abi.Kv4EvictPush(self.geom, first, n, keep, 0, 0))
 
     def evict(self, plan: Buffer, keep: int, sinks: int = 0, recent: int = 0, first: int = 0,
               n: int | None = None) -> None:
