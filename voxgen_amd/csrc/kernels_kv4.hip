@@ -21,6 +21,7 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr float kLimit = 61440.0f;   // inputs are clamped to this: o + 15 d then stays inside f16
 constexpr float kLog2e = 1.4426950408889634f;
@@ -240,28 +241,37 @@ __global__ __launch_bounds__(256) void k_kv4_advance(uint32_t *slots, uint32_t *
 constexpr float kLazy = 8.0f;        // a row's reference moves when a score exceeds it by this
 constexpr float kRaise = 7.0f;       // weights are taken 2^7 up, so that their low f16 terms stay normal
 
+constexpr uint32_t kMaxSplits = 256;
+
 struct AttnArgs {
     Kv4Attn a;
     uint32_t group, rows, tiles;     // query heads a KV head, rows (tokens x group), tiles of them
-    uint32_t splits, per;            // key splits of the grid, blocks of one
+    uint32_t by_group;               // 2^32 / group, rounded up; 0 where group is 1
+    uint32_t tile_rows, splits, per; // rows of a tile, key splits of the grid, blocks of one
     bool eager;                      // a wave's first block is fetched before it is known whether slots fill it
     float *ml, *acc, *lse;           // [unit][split][tile rows][2], [..][tile rows][HD], [sequence x KV head][rows]
-    // for the weights of prompts: the query rows as operands [sequence x KV head][16 rows][HD / 32][hi, lo][64],
+    // for the weights of prompts: the query rows as operands [sequence x KV head][32 rows][HD / 16][hi, lo][64],
     // the factors of their scores [sequence x KV head][rows], sums by row split [split][sequence x KV head][slots]
     h8 *qp;
     float *factors, *sums;
     uint32_t qtiles, row_splits, slots32;
 };
 
-// Keys of a tile: all that its last row attends to. A split is `per` blocks whatever the
-// sequence's length: sequences of unequal length then make splits of equal work.
+// The token of a row. The product with 2^32 / group rounded up is exact for rows below 2^22
+// and groups up to 2^10: it is over by less than 2^22 2^10 / 2^32 / group.
+__device__ __forceinline__ uint32_t token_of(const AttnArgs &p, uint32_t row) {
+    return p.by_group ? __umulhi(row, p.by_group) : row;
+}
+
+// Keys of a tile: all that its last row attends to. A split is `per` blocks
+// whatever the sequence's length: sequences of unequal length then make splits of equal work.
 struct Span {
     uint32_t base, keys, blocks, active;   // slots filled ahead of the call; blocks and splits of the tile
 };
 __device__ __forceinline__ Span span_of(const AttnArgs &p, uint32_t seq, uint32_t last_row) {
     Span s;
     s.base = p.a.slots[seq];
-    s.keys = s.base >= p.a.g.context ? 0u : min(s.base + last_row / p.group + 1u, p.a.g.context);
+    s.keys = s.base >= p.a.g.context ? 0u : min(s.base + token_of(p, last_row) + 1u, p.a.g.context);
     s.blocks = (s.keys + 31u) / 32u;
     s.active = (s.blocks + p.per - 1u) / p.per;
     return s;
@@ -288,43 +298,66 @@ __device__ __forceinline__ float row_sum(float v) {
     return __builtin_bit_cast(float, (uint32_t)t[0]) + __builtin_bit_cast(float, (uint32_t)t[1]);
 }
 
+// A row's scale: below 2^10, the low f16 term of a value down to 2^-13 of the row's largest
+// is still normal. The exponent of its largest magnitude; 0 where that is 0 or not finite.
+__device__ __forceinline__ int scale_of(float top) {
+    return top > 0.f && top < INFINITY ? max(__builtin_amdgcn_frexp_expf(top), -100) : 0;
+}
+__device__ __forceinline__ void split8(const float *x, float up, h8 &hi, h8 &lo) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = x[i] * up;
+        hi[i] = (_Float16)v;
+        lo[i] = (_Float16)(v - (float)hi[i]);
+    }
+}
+// Eight weights as two f16 terms; `minus` is -1 that the compiler cannot see, so that v - hi
+// is one v_fma_mix_f32.
+__device__ __forceinline__ void two_terms(const float *v, float minus, h8 &hi, h8 &lo) {
+    h2 h[4], r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        h[e] = __builtin_convertvector((f2{v[2 * e], v[2 * e + 1]}), h2);
+        r[e] = __builtin_convertvector((f2{__builtin_fmaf(minus, (float)h[e][0], v[2 * e]),
+                                           __builtin_fmaf(minus, (float)h[e][1], v[2 * e + 1])}), h2);
+    }
+    hi = join8(h);
+    lo = join8(r);
+}
+
 // Sixteen query rows as the B operand: lane (i, q) holds row i, dimensions q HD / 4 + 8 u
-// + 0..7 in step u, as two f16 terms of the row scaled to below 2^10 (the low term of a
-// value down to 2^-13 of the row's largest is then still normal). Returns the factor of
+// + 0..7 in step u; split() makes two f16 terms of the scaled row and returns the factor of
 // the scores: the row's scale, log2(e) and 1 / sqrt(HD).
 template <int HD>
-__device__ __forceinline__ float load_q(const AttnArgs &p, uint32_t s, uint32_t head, uint32_t row, bool valid, uint32_t q,
-                                        h8 *qh, h8 *ql) {
-    constexpr int U = HD / 32;
+struct QRow {
+    static constexpr int U = HD / 32;
     float x[U][8];
-    float top = 0.f;
-    const uint32_t t = row / p.group, j = row - t * p.group;
-    const float *src = p.a.q + ((size_t)s * p.a.tokens + t) * p.a.q_stride + (size_t)(head * p.group + j) * HD + q * (HD / 4);
+    __device__ __forceinline__ void load(const AttnArgs &p, uint32_t s, uint32_t head, uint32_t row, bool valid, uint32_t q) {
+        const uint32_t t = token_of(p, row), j = row - t * p.group;
+        const float *src = p.a.q + ((size_t)s * p.a.tokens + t) * p.a.q_stride + (size_t)(head * p.group + j) * HD + q * (HD / 4);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (valid) {
-            load8(src + 8 * u, p.a.qvec, x[u]);
-        } else {
+        for (int u = 0; u < U; ++u) {
+            if (valid) {
+                load8(src + 8 * u, p.a.qvec, x[u]);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+                for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+            }
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[u][i]));
     }
-    top = row_max(top);
-    int e = 0;
-    if (top > 0.f && top < INFINITY) e = max(__builtin_amdgcn_frexp_expf(top), -100);
-    const float up = ldexpf(1.0f, 10 - e);
+    __device__ __forceinline__ float split(h8 *qh, h8 *ql) const {
+        float top = 0.f;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float v = x[u][i] * up;
-            qh[u][i] = (_Float16)v;
-            ql[u][i] = (_Float16)(v - (float)qh[u][i]);
-        }
-    return ldexpf(kLog2e / sqrtf((float)HD), e - 10);
-}
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[u][i]));
+        const int e = scale_of(row_max(top));
+        const float up = ldexpf(1.0f, 10 - e);
+#pragma unroll
+        for (int u = 0; u < U; ++u) split8(x[u], up, qh[u], ql[u]);
+        return ldexpf(kLog2e / sqrtf((float)HD), e - 10);
+    }
+};
 
 // A lane's share of a block of K: for both of the product's row tiles tt, the codes of
 // slot 8 (i / 4) + 4 tt + i % 4 in dimensions q HD / 4.. and their (d, o). Lane (i, q) of
@@ -384,44 +417,36 @@ struct VScale {
 // here, the others' partial sums go to scratch. A block's values are made once and meet
 // all NT column tiles, whose query rows lie in LDS in the order of the operand (NT 1: in
 // registers).
-template <int HD, int NT, int W>
-__global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
+// PK, of at most eight rows: columns 0..7 of the products take the high terms of the rows,
+// columns 8..15 the low ones, so that one product does for both; the scores of the two
+// columns of a row are added, and so are its sums at the end.
+template <int HD, int NT, int W, bool PK>
+__global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k_kv4_attn(AttnArgs p) {
     using L = Lay<HD>;
-    constexpr int U = HD / 32, DT = HD / 16, OROW = HD + 4, R = 16 * NT, B = W > 4 ? 4 : W;
+    constexpr int U = HD / 32, DT = HD / 16, OROW = HD + 4, R = 16 * NT, RT = PK ? 8 : R, B = W > 4 || NT > 2 ? W / 2 : W;
     constexpr int QLDS = NT > 1 ? R * HD : 0;   // floats: two f16 planes
     constexpr int LDS = B * R * OROW > QLDS ? B * R * OROW : QLDS;
     __shared__ __attribute__((aligned(16))) float lds[LDS];
+    static_assert(!PK || NT == 1, "one column tile");
     __shared__ float ms[W][R], ls[W][R], fs[R];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
     const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
     // the tiles with the most keys first
     const uint32_t split = blockIdx.x / p.tiles, tile = p.tiles - 1u - blockIdx.x % p.tiles;
     const uint32_t head = blockIdx.y, s = blockIdx.z, seq = p.a.first + s;
-    const uint32_t rows = p.rows, r0 = tile * R;
+    const uint32_t rows = p.rows, r0 = tile * RT, ri = PK ? i & 7u : i;
     const uint32_t b0 = split * p.per;
     const size_t plane = plane_of(p.a.g, p.a.layer, seq, head) * plane_bytes<HD>(p.a.g);
     const uint8_t *const kp = p.a.kc + plane, *const vp = p.a.vc + plane;
-    constexpr bool FLAT = NT == 1 && HD <= 128;   // V's (d, o) of a block all at once, and ahead like its codes
     KFrag<HD> kf;
-    VFrag<HD> vf;
-    VScale sc[FLAT ? L::G : 2];
     uint32_t b = b0 + w;
-    auto load_v = [&]() {
-        const uint8_t *const vb = vp + (size_t)b * L::BLOCK;
-        vf.load(vb, i, q);
-        if constexpr (FLAT) {
-#pragma unroll
-            for (int g = 0; g < L::G; ++g) sc[g].template load<HD>(vb, g, q);
-        }
-    };
     auto load_first = [&](uint32_t end) {
-        if (b < end) {
-            kf.load(kp + (size_t)b * L::BLOCK, i, q);
-            if constexpr (FLAT) load_v();
-        }
+        if (b < end) kf.load(kp + (size_t)b * L::BLOCK, i, q);
     };
     if (p.eager) load_first(min(b0 + p.per, (p.a.g.context + 31u) / 32u));
-    const Span sp = span_of(p, seq, min(r0 + R, rows) - 1u);
+    QRow<HD> qr;
+    if constexpr (NT == 1) qr.load(p, s, head, min(r0 + ri, rows - 1u), r0 + ri < rows, q);
+    const Span sp = span_of(p, seq, min(r0 + RT, rows) - 1u);
     if (split != 0 && split >= sp.active) return;
     const uint32_t b1 = min(b0 + p.per, sp.blocks);
     if (!p.eager) load_first(b1);
@@ -429,24 +454,30 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
     float factor[NT];
     h8 *const qs = reinterpret_cast<h8 *>(lds);   // [NT][U][hi, lo][64]
     if constexpr (NT == 1) {
-        factor[0] = load_q<HD>(p, s, head, min(r0 + i, rows - 1u), r0 + i < rows, q, qh, ql);
+        factor[0] = qr.split(qh, ql);
+        if constexpr (PK) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) qh[u] = i < 8u ? qh[u] : ql[u];
+        }
     } else {
         for (uint32_t c = w; c < NT; c += W) {
             const uint32_t row = r0 + 16u * c + i;
-            const float f = load_q<HD>(p, s, head, min(row, rows - 1u), row < rows, q, qh, ql);
+            qr.load(p, s, head, min(row, rows - 1u), row < rows, q);
+            const float f = qr.split(qh, ql);
             if (q == 0) fs[16u * c + i] = f;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 qs[((c * U + u) * 2u) * 64u + lane] = qh[u];
                 qs[((c * U + u) * 2u + 1u) * 64u + lane] = ql[u];
             }
-            if (p.qp && split == 0) {   // the weights' kernel reads them again
+            if (p.qp && split == 0) {   // the weights' kernel reads them again, in its operand's order
                 const size_t pair = (size_t)s * p.a.g.kv_heads + head;
-                h8 *const to = p.qp + (pair * p.qtiles + tile * NT + c) * U * 128u;
+                h8 *const to = p.qp + (pair * p.qtiles + (tile * NT + c) / 2u) * (HD / 16) * 128u;
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    to[u * 128 + lane] = qh[u];
-                    to[u * 128 + 64 + lane] = ql[u];
+                    const uint32_t d8 = q * U + u, at = (d8 / 2u * 2u) * 64u + d8 % 2u * 32u + c % 2u * 16u + i;
+                    to[at] = qh[u];
+                    to[at + 64u] = ql[u];
                 }
                 if (q == 0 && row < rows) p.factors[pair * rows + row] = f;
             }
@@ -456,8 +487,8 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
         for (int c = 0; c < NT; ++c) factor[c] = fs[16 * c + i];
     }
     // last slot that the lane's row of a column tile attends to
-    auto limit = [&](int c) { return sp.base + min(r0 + 16u * c + i, rows - 1u) / p.group; };
-    const uint32_t sees_all = sp.base + r0 / p.group;   // last slot that every row attends to
+    auto limit = [&](int c) { return sp.base + token_of(p, min(r0 + 16u * c + ri, rows - 1u)); };
+    const uint32_t sees_all = sp.base + token_of(p, r0);   // last slot that every row attends to
 
     float m[NT], l[NT];
     f4 o[NT][DT];
@@ -470,13 +501,14 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
     }
 
     const Masks masks;
-    float minus = -1.0f;
-    asm("" : "+v"(minus));   // a product the compiler keeps: v - hi then is one v_fma_mix_f32
+    float minus = PK && i < 8u ? 0.0f : -1.0f;
+    asm("" : "+v"(minus));
     // A block; at the tile's edge, some row's last slots or the cache's.
     auto step = [&](auto at_edge) {
         constexpr bool edge = decltype(at_edge)::value;
         const uint8_t *const vb = vp + (size_t)b * L::BLOCK;
-        if constexpr (!FLAT) load_v();
+        VFrag<HD> vf;
+        vf.load(vb, i, q);
         f4 x[NT][2];
 #pragma unroll
         for (int c = 0; c < NT; ++c) x[c][0] = x[c][1] = f4{0.f, 0.f, 0.f, 0.f};
@@ -489,14 +521,21 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
                 const h8 lo = NT == 1 ? ql[u] : qs[((c * U + u) * 2u + 1u) * 64u + lane];
                 x[c][0] = mfma16(k0, hi, x[c][0]);
                 x[c][1] = mfma16(k1, hi, x[c][1]);
-                x[c][0] = mfma16(k0, lo, x[c][0]);
-                x[c][1] = mfma16(k1, lo, x[c][1]);
+                if constexpr (!PK) {
+                    x[c][0] = mfma16(k0, lo, x[c][0]);
+                    x[c][1] = mfma16(k1, lo, x[c][1]);
+                }
             }
         }
         if (b + W < b1) kf.load(kp + (size_t)(b + W) * L::BLOCK, i, q);
-        if constexpr (!FLAT) sc[0].template load<HD>(vb, 0, q);
+        VScale sc[2];
+        sc[0].template load<HD>(vb, 0, q);
         __builtin_amdgcn_sched_barrier(0);
         const uint32_t slot0 = b * 32u + 8u * q;
+        if constexpr (PK) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[0][e / 4][e % 4] += dpp<0x128>(x[0][e / 4][e % 4]);   // row_ror:8
+        }
         if constexpr (edge) {
 #pragma unroll
             for (int c = 0; c < NT; ++c) {
@@ -537,41 +576,30 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
                 v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[c][e / 4][e % 4], factor[c], -ref));
                 l[c] += v[e];
             }
-            h2 h[4], r[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                h[e] = __builtin_convertvector((f2{v[2 * e], v[2 * e + 1]}), h2);
-                r[e] = __builtin_convertvector((f2{__builtin_fmaf(minus, (float)h[e][0], v[2 * e]),
-                                                   __builtin_fmaf(minus, (float)h[e][1], v[2 * e + 1])}), h2);
-            }
-            ph[c] = join8(h);
-            pl[c] = join8(r);
+            two_terms(v, minus, ph[c], pl[c]);   // of PK the term of the lane's column, by `minus`
         }
         __builtin_amdgcn_sched_barrier(0);
         const uint32_t some = min(max(sp.keys, slot0) - slot0, 8u);
 #pragma unroll
         for (int g = 0; g < L::G; ++g) {
-            VScale &now = sc[FLAT ? g : g % 2];
-            if (!FLAT && g + 1 < L::G) sc[(g + 1) % 2].template load<HD>(vb, g + 1, q);
-            if constexpr (edge) now.keep(some);
+            VScale &dc = sc[g % 2];
+            if (g + 1 < L::G) sc[(g + 1) % 2].template load<HD>(vb, g + 1, q);
+            if constexpr (edge) dc.keep(some);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const h8 v = values8(masks, vf.code[h][g], now.d, now.o);
+                const h8 v = values8(masks, vf.code[h][g], dc.d, dc.o);
 #pragma unroll
-                for (int c = 0; c < NT; ++c) o[c][2 * g + h] = mfma16(v, ph[c], o[c][2 * g + h]);
+                for (int c = 0; c < NT; ++c) o[c][2 * g + h] = mfma16(v, PK ? pl[c] : ph[c], o[c][2 * g + h]);
+                if constexpr (!PK) {
 #pragma unroll
-                for (int c = 0; c < NT; ++c) o[c][2 * g + h] = mfma16(v, pl[c], o[c][2 * g + h]);
+                    for (int c = 0; c < NT; ++c) o[c][2 * g + h] = mfma16(v, pl[c], o[c][2 * g + h]);
+                }
             }
         }
     };
     const uint32_t whole = min(b1, (sees_all + 1u) / 32u);   // blocks that every row attends to all of
-    auto next = [&]() {
-        b += W;
-        if constexpr (FLAT)
-            if (b < b1) load_v();
-    };
-    for (; b < whole; next()) step(std::false_type{});
-    for (; b < b1; next()) step(std::true_type{});
+    while (b < whole) step(std::false_type{}), b += W;
+    while (b < b1) step(std::true_type{}), b += W;
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
         l[c] = row_sum(l[c]);
@@ -629,26 +657,30 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
             const uint32_t row = r0 + 16u * c + i;
-            if (row >= rows) continue;
+            if (row >= rows || (PK && i >= 8u)) continue;
             if (alone) {
                 p.lse[((size_t)s * p.a.g.kv_heads + head) * rows + row] = (top[c] - kRaise) + __builtin_amdgcn_logf(sum[c]);
             } else {
-                p.ml[(part * R + 16u * c + i) * 2u] = top[c];
-                p.ml[(part * R + 16u * c + i) * 2u + 1u] = sum[c];
+                p.ml[(part * RT + 16u * c + i) * 2u] = top[c];
+                p.ml[(part * RT + 16u * c + i) * 2u + 1u] = sum[c];
             }
         }
     }
     __syncthreads();
     constexpr int V = HD / 4;   // four dimensions a lane
-    for (uint32_t k = tid; k < (uint32_t)R * V; k += 64u * W) {
+    for (uint32_t k = tid; k < (uint32_t)RT * V; k += 64u * W) {
         const uint32_t r = k / V, c = 4u * (k % V), row = r0 + r;
         if (row >= rows) break;
         f4 v = *reinterpret_cast<const f4 *>(&os[0][r][c]);
 #pragma unroll
         for (int u = 1; u < B; ++u) v += *reinterpret_cast<const f4 *>(&os[u][r][c]);
-        const uint32_t t = row / p.group, j = row - t * p.group;
+        if constexpr (PK) {
+#pragma unroll
+            for (int u = 0; u < B; ++u) v += *reinterpret_cast<const f4 *>(&os[u][r + 8u][c]);
+        }
+        const uint32_t t = token_of(p, row), j = row - t * p.group;
         if (!alone) {
-            *reinterpret_cast<f4 *>(p.acc + (part * R + r) * HD + c) = v;
+            *reinterpret_cast<f4 *>(p.acc + (part * RT + r) * HD + c) = v;
             continue;
         }
         const bool attends = sp.base < p.a.g.context && sp.base + t < p.a.g.context;
@@ -661,63 +693,6 @@ __global__ __launch_bounds__(64 * W) void k_kv4_attn(AttnArgs p) {
             for (int e = 0; e < 4; ++e) to[e] = v[e];
         }
     }
-}
-
-// The splits of a row, joined: a workgroup a row, its lanes HD / 4 columns by as many
-// splits at once as fit.
-constexpr uint32_t kMaxSplits = 256;
-#ifndef ALONE
-#define ALONE 16
-#endif
-constexpr uint32_t kAloneBlocks = ALONE;
-constexpr uint32_t kEagerGroups = 256;
-constexpr uint32_t kWideTiles = 192;   // tiles of 64 rows from which on they are taken
-template <int HD>
-__global__ __launch_bounds__(256) void k_kv4_join(AttnArgs p, uint32_t tile_rows) {
-    constexpr int V = HD / 4, Y = 256 / V;
-    __shared__ float sc[kMaxSplits], red[8];
-    __shared__ __attribute__((aligned(16))) float os[Y][HD];
-    const uint32_t tid = threadIdx.x, row = blockIdx.x, head = blockIdx.y, s = blockIdx.z, seq = p.a.first + s;
-    const uint32_t tile = row / tile_rows, r = row - tile * tile_rows;
-    const Span sp = span_of(p, seq, min((tile + 1u) * tile_rows, p.rows) - 1u);
-    if (sp.active <= 1u) return;
-    const size_t unit = ((size_t)s * p.a.g.kv_heads + head) * p.tiles + tile;
-    const size_t first = unit * p.splits * tile_rows + r;   // the row's record in split 0
-    float m = -INFINITY, l = 0.f;
-    if (tid < sp.active) {
-        m = p.ml[(first + (size_t)tid * tile_rows) * 2u];
-        l = p.ml[(first + (size_t)tid * tile_rows) * 2u + 1u];
-    }
-    float top = m;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    if ((tid & 63u) == 0) red[tid >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float mine = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
-    if (tid < sp.active) sc[tid] = mine;
-    float sum = l * mine;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
-    if ((tid & 63u) == 0) red[4 + (tid >> 6)] = sum;
-    __syncthreads();
-    sum = (red[4] + red[5]) + (red[6] + red[7]);
-    const uint32_t c = 4u * (tid % V), y = tid / V;
-    f4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (uint32_t v = y; v < sp.active; v += Y)
-        o += *reinterpret_cast<const f4 *>(p.acc + (first + (size_t)v * tile_rows) * HD + c) * sc[v];
-    *reinterpret_cast<f4 *>(&os[y][c]) = o;
-    __syncthreads();
-    const uint32_t t = row / p.group, j = row - t * p.group;
-    const bool attends = sp.base + t < p.a.g.context;
-    if (tid < (uint32_t)HD) {
-        float v = os[0][tid];
-#pragma unroll
-        for (int u = 1; u < Y; ++u) v += os[u][tid];
-        p.a.out[((size_t)s * p.a.tokens + t) * p.a.out_stride + (size_t)(head * p.group + j) * HD + tid] = attends ? v / sum : 0.f;
-    }
-    if (tid == 0) p.lse[((size_t)s * p.a.g.kv_heads + head) * p.rows + row] = (top - kRaise) + __builtin_amdgcn_logf(sum);
 }
 
 // The weight of a slot from its rows' sum: added to what it had, unless the call's own
@@ -734,29 +709,127 @@ __device__ __forceinline__ float sum16(float v) {
     return v + dpp<0x140>(v);
 }
 
-// Accumulated weights of at most 16 rows: a wave per block of 32 slots takes the scores
-// again, and sums 2^(score - lse) over the rows.
+// A barrier for what lies in LDS: __syncthreads waits for every global load too, which here
+// are on their way for a later turn.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+__device__ __forceinline__ f16v mfma32(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// The splits of a row, joined: a workgroup a row, its lanes HD / 4 columns by as many
+// splits at once as fit.
+constexpr uint32_t kEagerGroups = 256;
+constexpr uint32_t kWideTiles = 192;   // tiles of 64 rows from which on they are taken
 template <int HD>
-__global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs p) {
+__device__ __forceinline__ void join_row(const AttnArgs &p, uint32_t row, uint32_t head, uint32_t s) {
+    constexpr int V = HD / 4, Y = 256 / V;
+    __shared__ float sc[kMaxSplits], red[8];
+    __shared__ __attribute__((aligned(16))) float os[Y][HD];
+    const uint32_t tid = threadIdx.x, seq = p.a.first + s, tile_rows = p.tile_rows;
+    const uint32_t tile = row / tile_rows, r = row - tile * tile_rows;
+    const size_t unit = ((size_t)s * p.a.g.kv_heads + head) * p.tiles + tile;
+    const size_t first = unit * p.splits * tile_rows + r;   // the row's record in split 0
+    const uint32_t c = 4u * (tid % V), y = tid / V;
+    // Few splits are fetched before it is known which are in use.
+    constexpr int E = 8;
+    f4 early[E];
+    float m = -INFINITY, l = 0.f;
+    if (p.eager) {
+        if (tid < p.splits) {
+            m = p.ml[(first + (size_t)tid * tile_rows) * 2u];
+            l = p.ml[(first + (size_t)tid * tile_rows) * 2u + 1u];
+        }
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            const uint32_t v = y + k * Y;
+            if (v < p.splits) early[k] = *reinterpret_cast<const f4 *>(p.acc + (first + (size_t)v * tile_rows) * HD + c);
+        }
+    }
+    const Span sp = span_of(p, seq, min((tile + 1u) * tile_rows, p.rows) - 1u);
+    if (sp.active <= 1u) return;
+    if (!p.eager && tid < sp.active) {
+        m = p.ml[(first + (size_t)tid * tile_rows) * 2u];
+        l = p.ml[(first + (size_t)tid * tile_rows) * 2u + 1u];
+    }
+    if (tid >= sp.active) m = -INFINITY, l = 0.f;
+    float top = m;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    if ((tid & 63u) == 0) red[tid >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const float mine = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+    if (tid < sp.active) sc[tid] = mine;
+    float sum = l * mine;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+    if ((tid & 63u) == 0) red[4 + (tid >> 6)] = sum;
+    __syncthreads();
+    sum = (red[4] + red[5]) + (red[6] + red[7]);
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+    uint32_t v = y;
+    if (p.eager) {
+#pragma unroll
+        for (int k = 0; k < E; ++k, v += Y)
+            if (v < sp.active) o += early[k] * sc[v];
+    }
+#pragma unroll 4
+    for (; v < sp.active; v += Y)
+        o += *reinterpret_cast<const f4 *>(p.acc + (first + (size_t)v * tile_rows) * HD + c) * sc[v];
+    *reinterpret_cast<f4 *>(&os[y][c]) = o;
+    __syncthreads();
+    const uint32_t t = token_of(p, row), j = row - t * p.group;
+    const bool attends = sp.base + t < p.a.g.context;
+    if (tid < (uint32_t)HD) {
+        float x = os[0][tid];
+#pragma unroll
+        for (int u = 1; u < Y; ++u) x += os[u][tid];
+        p.a.out[((size_t)s * p.a.tokens + t) * p.a.out_stride + (size_t)(head * p.group + j) * HD + tid] = attends ? x / sum : 0.f;
+    }
+    if (tid == 0) p.lse[((size_t)s * p.a.g.kv_heads + head) * p.rows + row] = (top - kRaise) + __builtin_amdgcn_logf(sum);
+}
+
+// Accumulated weights of at most 16 rows: a wave per block of 32 slots takes the scores
+// again, and sums 2^(score - lse) over the rows; a row's lse is joined from its splits here
+// too, so that it need not wait for join_row's.
+template <int HD>
+__device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_t head, uint32_t s) {
     using L = Lay<HD>;
     constexpr int U = HD / 32;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
-    const uint32_t b = blockIdx.x * 4u + __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t head = blockIdx.y, s = blockIdx.z, seq = p.a.first + s;
-    const uint32_t base = p.a.slots[seq];
-    if (base >= p.a.g.context) return;
-    const uint32_t keys = min(base + p.a.tokens, p.a.g.context);
-    if (b * 32u >= keys) return;
-    const size_t plane = plane_of(p.a.g, p.a.layer, seq, head);
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4, seq = p.a.first + s;
+    const uint32_t b = group * 4u + __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t row = min(i, p.rows - 1u), t = token_of(p, row);
+    const Span sp = span_of(p, seq, p.rows - 1u);   // one tile
+    if (sp.base >= p.a.g.context || b >= sp.blocks) return;
+    const size_t plane = plane_of(p.a.g, p.a.layer, seq, head), pair = (size_t)s * p.a.g.kv_heads + head;
     const Masks masks;
     KFrag<HD> kf;
     kf.load(p.a.kc + plane * plane_bytes<HD>(p.a.g) + (size_t)b * L::BLOCK, i, q);
-    const uint32_t slot0 = b * 32u + 8u * q;
-    const uint32_t row = min(i, p.rows - 1u), t = row / p.group;
-    const bool valid = i < p.rows && base + t < p.a.g.context;
+    QRow<HD> qr;
+    qr.load(p, s, head, row, true, q);
+    float lse;
+    if (sp.active <= 1u) {
+        lse = p.lse[pair * p.rows + row];
+    } else {
+        float m = -INFINITY, l = 0.f;
+#pragma unroll 4
+        for (uint32_t v = q; v < sp.active; v += 4u) {
+            const f2 ml = *reinterpret_cast<const f2 *>(p.ml + ((pair * p.splits + v) * p.tile_rows + row) * 2u);
+            const float top = fmaxf(m, ml[0]);
+            l = (m == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - top)) +
+                (ml[0] == -INFINITY ? ml[1] : ml[1] * __builtin_amdgcn_exp2f(ml[0] - top));
+            m = top;
+        }
+        const float top = row_max(m);
+        lse = (top - kRaise) + __builtin_amdgcn_logf(row_sum(m == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - top)));
+    }
     h8 qh[U], ql[U];
-    const float factor = load_q<HD>(p, s, head, row, true, q, qh, ql);
-    const float lse = p.lse[((size_t)s * p.a.g.kv_heads + head) * p.rows + row];
+    const float factor = qr.split(qh, ql);
+    const uint32_t slot0 = b * 32u + 8u * q;
+    const bool valid = i < p.rows && sp.base + t < p.a.g.context;
     f4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -769,23 +842,33 @@ __global__ __launch_bounds__(256) void k_kv4_weights(AttnArgs p) {
     float *const to = p.a.weights + plane * p.a.g.context;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const bool sees = valid && slot0 + e <= base + t;
+        const bool sees = valid && slot0 + e <= sp.base + t;
         const float v = sum16(sees ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[e / 4][e % 4], factor, -lse)) : 0.f);
-        if (i == (uint32_t)e && slot0 + e < keys) add_weight(to, slot0 + e, base, p.a.decay, v);
+        if (i == (uint32_t)e && slot0 + e < sp.keys) add_weight(to, slot0 + e, sp.base, p.a.decay, v);
     }
 }
 
+// What follows the attention kernel, in one launch: workgroups 0..joins-1 join a row's
+// splits, the others the weights of 128 slots each.
+template <int HD>
+__global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs p, uint32_t joins) {
+    if (blockIdx.x < joins)
+        join_row<HD>(p, blockIdx.x, blockIdx.y, blockIdx.z);
+    else
+        weigh<HD>(p, blockIdx.x - joins, blockIdx.y, blockIdx.z);
+}
+
 // The same of more rows: a workgroup takes 256 slots, 64 a wave, whose values it makes once
-// and keeps in registers, over the row tiles blockIdx.x / chunks, + row_splits, ... The
-// tiles' operands, left by the attention kernel, pass through LDS two at a time, the next
-// two on their way while these are multiplied. A lane sums its slots over the rows it sees;
-// the sums over the row splits are added by k_kv4_add_weights, in order.
+// and keeps in registers, over every row_splits-th tile of 32 rows. The tiles' operands, left
+// by the attention kernel, pass through LDS, the next on its way while one is multiplied. A
+// lane sums its slots over its row of each tile; the sums over the row splits are added by
+// k_kv4_add_weights, in order.
 template <int HD>
 __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
     using L = Lay<HD>;
-    constexpr int U = HD / 32, TILE = U * 128, PER = 2 * TILE / 256;   // h8 of a tile; of two, a lane
-    __shared__ __attribute__((aligned(16))) h8 qs[2][2 * TILE];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
+    constexpr int S = HD / 16, TILE = S * 128, PER = TILE / 256;   // h8 of a tile; a lane's share
+    __shared__ __attribute__((aligned(16))) h8 qs[2][TILE];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, j = lane & 31u, h = lane >> 5;
     const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t chunk = blockIdx.x / p.row_splits, part = blockIdx.x % p.row_splits;
     const uint32_t head = blockIdx.y, s = blockIdx.z, seq = p.a.first + s;
@@ -796,79 +879,78 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
     const size_t pair = (size_t)s * p.a.g.kv_heads + head;
     const uint32_t b0 = chunk * 8u + 2u * w, blocks = (keys + 31u) / 32u;
     const uint8_t *const kp = p.a.kc + plane_of(p.a.g, p.a.layer, seq, head) * plane_bytes<HD>(p.a.g);
-    h8 k[2][2][U];
+    h8 k[2][S];
     {
         const Masks masks;
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            KFrag<HD> kf;
-            kf.load(kp + (size_t)min(b0 + v, blocks - 1u) * L::BLOCK, i, q);   // a block behind the last: not stored below
+        for (int v = 0; v < 2; ++v) {   // slot j in row j; a block behind the last: not stored below
+            const uint8_t *const kb = kp + (size_t)min(b0 + v, blocks - 1u) * L::BLOCK;
 #pragma unroll
-            for (int u = 0; u < U; ++u) k[v][0][u] = kf.value(masks, 0, u), k[v][1][u] = kf.value(masks, 1, u);
+            for (int u = 0; u < S; ++u) {
+                const uint32_t word = reinterpret_cast<const uint32_t *>(kb)[j * (HD / 8) + 2u * u + h];
+                const h2 sc = __builtin_bit_cast(h2, reinterpret_cast<const uint32_t *>(kb + L::CODES)[j * L::G + u / 2]);
+                k[v][u] = values8(masks, word, h2{sc[0], sc[0]}, h2{sc[1], sc[1]});
+            }
         }
     }
-    // pairs of row tiles from the first that attends to a slot of the chunk
+    // row tiles from the first that attends to a slot of the chunk
     const uint32_t t0 = chunk * 256u > base ? chunk * 256u - base : 0u;
-    const uint32_t pairs_end = (p.rows + 31u) / 32u, step = p.row_splits;
-    uint32_t j = t0 * p.group / 32u + part;
+    const uint32_t tiles = (p.rows + 31u) / 32u;
+    uint32_t tile = t0 * p.group / 32u + part;
     const h8 *const src = p.qp + pair * p.qtiles * TILE;
     const float *const lses = p.lse + pair * p.rows, *const factors = p.factors + pair * p.rows;
     h8 next[PER];
-    float sum[2][8];
+    float sum[2][16];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[0][e] = sum[1][e] = 0.f;
-    auto fetch = [&](uint32_t to) {
+    for (int r = 0; r < 16; ++r) sum[0][r] = sum[1][r] = 0.f;
+    auto fetch = [&](uint32_t from) {
 #pragma unroll
-        for (int n = 0; n < PER; ++n) next[n] = src[(size_t)to * 2u * TILE + n * 256u + tid];
+        for (int n = 0; n < PER; ++n) next[n] = src[(size_t)from * TILE + n * 256u + tid];
     };
-    if (j < pairs_end) fetch(j);
-    for (uint32_t turn = 0; j < pairs_end; j += step, turn ^= 1u) {
+    if (tile < tiles) fetch(tile);
+    for (uint32_t turn = 0; tile < tiles; tile += p.row_splits, turn ^= 1u) {
         // A buffer is written two turns after it was last read, with a barrier between.
 #pragma unroll
         for (int n = 0; n < PER; ++n) qs[turn][n * 256u + tid] = next[n];
-        if (j + step < pairs_end) fetch(j + step);
-        float factor[2], lse[2];
-        uint32_t last[2];
+        if (tile + p.row_splits < tiles) fetch(tile + p.row_splits);
+        const uint32_t row = tile * 32u + j, at = min(row, p.rows - 1u), last = base + token_of(p, at);
+        const float factor = factors[at];
+        const float lse = row < p.rows && last < p.a.g.context ? lses[at] : INFINITY;   // 2^-inf: counts nothing
+        const bool edge = (b0 + 2u) * 32u - 1u > base + token_of(p, tile * 32u);
+        lds_barrier();
+        const h8 *const from = qs[turn] + lane;
+        f16v x[2] = {};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const uint32_t row = j * 32u + 16u * c + i, at = min(row, p.rows - 1u), t = at / p.group;
-            factor[c] = factors[at];
-            last[c] = base + t;
-            lse[c] = row < p.rows && last[c] < p.a.g.context ? lses[at] : INFINITY;   // 2^-inf: counts nothing
+        for (int u = 0; u < S; ++u) {
+            const h8 hi = from[u * 128], lo = from[u * 128 + 64];
+            x[0] = mfma32(k[0][u], hi, x[0]);
+            x[1] = mfma32(k[1][u], hi, x[1]);
+            x[0] = mfma32(k[0][u], lo, x[0]);
+            x[1] = mfma32(k[1][u], lo, x[1]);
         }
-        const uint32_t first_row_sees = base + j * 32u / p.group;
-        const bool edge = (b0 + 2u) * 32u - 1u > first_row_sees;
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const h8 *const from = qs[turn] + c * TILE + lane;
-            f4 x[2][2] = {{{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}};
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const h8 hi = from[u * 128], lo = from[u * 128 + 64];
-#pragma unroll
-                for (int v = 0; v < 4; ++v) x[v / 2][v % 2] = mfma16(k[v / 2][v % 2][u], hi, x[v / 2][v % 2]);
-#pragma unroll
-                for (int v = 0; v < 4; ++v) x[v / 2][v % 2] = mfma16(k[v / 2][v % 2][u], lo, x[v / 2][v % 2]);
-            }
+        if (edge) {
 #pragma unroll
             for (int v = 0; v < 2; ++v)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float y = __builtin_amdgcn_exp2f(__builtin_fmaf(x[v][e / 4][e % 4], factor[c], -lse[c]));
-                    if (edge) y = (b0 + v) * 32u + 8u * q + e <= last[c] ? y : 0.f;
-                    sum[v][e] += y;
-                }
+                for (int r = 0; r < 16; ++r)
+                    x[v][r] = (b0 + v) * 32u + 8u * (r / 4) + 4u * h + r % 4 > last ? -INFINITY : x[v][r];
         }
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum[v][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[v][r], factor, -lse));
     }
     float *const sums = p.sums + ((size_t)part * gridDim.y * gridDim.z + pair) * p.slots32;
 #pragma unroll
     for (int v = 0; v < 2; ++v)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float y = sum16(sum[v][e]);
-            const uint32_t slot = (b0 + v) * 32u + 8u * q + e;
-            if (i == (uint32_t)e && slot < keys) sums[slot] = y;
+        for (int r = 0; r < 16; ++r) {
+            float y = sum16(sum[v][r]);   // and the other 16 rows of the half
+            const uint32_t bits = __builtin_bit_cast(uint32_t, y);
+            const auto t = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
+            y = __builtin_bit_cast(float, (uint32_t)t[0]) + __builtin_bit_cast(float, (uint32_t)t[1]);
+            const uint32_t slot = (b0 + v) * 32u + 8u * (r / 4) + 4u * h + r % 4;
+            if (j == (uint32_t)r && slot < keys) sums[slot] = y;
         }
 }
 
@@ -1168,7 +1250,7 @@ namespace {
 // of four waves, as many splits as make 2048 workgroups of at least four blocks each (a
 // block a wave). More rows: eight waves a tile of 32 or 64.
 struct Shape {
-    uint32_t group, rows, nt, waves, tiles, splits, per;
+    uint32_t group, rows, nt, waves, tile_rows, tiles, splits, per;
     uint64_t units;
     bool eager;
 };
@@ -1180,15 +1262,16 @@ Shape shape_of(const Kv4Attn &a) {
     const uint32_t blocks = (a.g.context + 31u) / 32u;
     if (h.rows <= 16u) {
         h.nt = 1;
-        h.waves = blocks <= kAloneBlocks ? 8 : 4;
+        h.waves = 4;
     } else {
         h.nt = a.g.head_dim < 256u && (h.rows + 63u) / 64u * pairs >= kWideTiles ? 4 : 2;
         h.waves = 8;
     }
-    h.tiles = (h.rows + 16u * h.nt - 1u) / (16u * h.nt);
+    h.tile_rows = h.rows <= 8u ? 8u : 16u * h.nt;
+    h.tiles = (h.rows + h.tile_rows - 1u) / h.tile_rows;
     h.units = h.tiles * pairs;
-    const uint64_t want = ((h.nt == 1 ? 2048u : 256u) + h.units - 1u) / h.units;
-    const uint32_t least = h.nt == 1 ? (h.waves == 8 ? kAloneBlocks : 4u) : 32u;   // blocks of a split
+    const uint64_t wide = h.nt == 1 ? 1536u : 256u, want = wide > h.units ? wide / h.units : 1u;
+    const uint32_t least = h.waves;   // blocks of a split: one a wave
     uint32_t splits = (blocks + least - 1u) / least;
     if (splits > want) splits = (uint32_t)want;
     if (splits > kMaxSplits) splits = kMaxSplits;
@@ -1208,12 +1291,11 @@ struct Parts {
 Parts parts_of(const Kv4Attn &a, const Shape &h, bool with_weights) {
     Parts t;
     const uint64_t pairs = (uint64_t)a.g.kv_heads * a.n;
-    const uint64_t records = h.splits > 1u ? h.units * h.splits * 16u * h.nt : 0u;
+    const uint64_t records = h.splits > 1u ? h.units * h.splits * h.tile_rows : 0u;
     const bool rows = with_weights && h.nt > 1u;   // the weights of prompts
-    t.qtiles = (h.rows + 31u) / 32u * 2u;
-    if (t.qtiles < h.tiles * h.nt) t.qtiles = h.tiles * h.nt;
+    t.qtiles = h.tiles * ((h.nt + 1u) / 2u);
     t.slots32 = (a.g.context + 31u) / 32u * 32u;
-    // about 512 workgroups of 256 slots, at least two pairs of row tiles each
+    // about 512 workgroups of 256 slots, at least two row tiles each
     const uint64_t chunks = (a.g.context + 255u) / 256u * pairs, most = (h.rows + 63u) / 64u;
     uint64_t splits = (512u + chunks - 1u) / chunks;
     if (splits > most) splits = most;
@@ -1221,7 +1303,7 @@ Parts parts_of(const Kv4Attn &a, const Shape &h, bool with_weights) {
     t.acc = 0;
     t.ml = t.acc + records * a.g.head_dim;
     t.qp = t.ml + records * 2u;
-    t.lse = t.qp + (rows ? pairs * t.qtiles * 16u * a.g.head_dim : 0u);
+    t.lse = t.qp + (rows ? pairs * t.qtiles * 32u * a.g.head_dim : 0u);
     t.factors = t.lse + (pairs * h.rows + 3u) / 4u * 4u;
     t.sums = t.factors + (rows ? (pairs * h.rows + 3u) / 4u * 4u : 0u);
     t.end = t.sums + (rows ? (uint64_t)t.row_splits * pairs * t.slots32 : 0u);
@@ -1241,8 +1323,10 @@ static int attention(hipStream_t s, const Kv4Attn &a) {
     AttnArgs p;
     p.a = a;
     p.group = h.group;
+    p.by_group = h.group == 1u ? 0u : (uint32_t)((0x100000000ull + h.group - 1u) / h.group);
     p.rows = h.rows;
     p.tiles = h.tiles;
+    p.tile_rows = h.tile_rows;
     p.splits = h.splits;
     p.per = h.per;
     p.eager = h.eager;
@@ -1256,19 +1340,21 @@ static int attention(hipStream_t s, const Kv4Attn &a) {
     p.row_splits = t.row_splits;
     p.slots32 = t.slots32;
     const dim3 grid(h.tiles * h.splits, a.g.kv_heads, a.n);
-    if (h.nt == 1 && h.waves == 8) {
-        k_kv4_attn<HD, 1, 8><<<grid, 512, 0, s>>>(p);
+    if (h.rows <= 8u) {
+        k_kv4_attn<HD, 1, 4, true><<<grid, 256, 0, s>>>(p);
     } else if (h.nt == 1) {
-        k_kv4_attn<HD, 1, 4><<<grid, 256, 0, s>>>(p);
+        k_kv4_attn<HD, 1, 4, false><<<grid, 256, 0, s>>>(p);
     } else if (h.nt == 2) {
-        k_kv4_attn<HD, 2, 8><<<grid, 512, 0, s>>>(p);
+        k_kv4_attn<HD, 2, 8, false><<<grid, 512, 0, s>>>(p);
     } else if constexpr (HD < 256) {
-        k_kv4_attn<HD, 4, 8><<<grid, 512, 0, s>>>(p);
+        k_kv4_attn<HD, 4, 8, false><<<grid, 512, 0, s>>>(p);
     }
     VX_LAUNCHED("k_kv4_attn");
-    if (h.splits > 1u) {
-        k_kv4_join<HD><<<dim3(h.rows, a.g.kv_heads, a.n), 256, 0, s>>>(p, 16u * h.nt);
-        VX_LAUNCHED("k_kv4_join");
+    const uint32_t joins = h.splits > 1u ? h.rows : 0u;
+    const uint32_t groups = a.weights && !rows ? ((a.g.context + 31u) / 32u + 3u) / 4u : 0u;
+    if (joins + groups) {
+        k_kv4_finish<HD><<<dim3(joins + groups, a.g.kv_heads, a.n), 256, 0, s>>>(p, joins);
+        VX_LAUNCHED("k_kv4_finish");
     }
     if (rows) {
         const uint32_t chunks = (a.g.context + 255u) / 256u;
@@ -1276,9 +1362,6 @@ static int attention(hipStream_t s, const Kv4Attn &a) {
         VX_LAUNCHED("k_kv4_weights_rows");
         k_kv4_add_weights<<<dim3(chunks, a.g.kv_heads, a.n), 256, 0, s>>>(p);
         VX_LAUNCHED("k_kv4_add_weights");
-    } else if (a.weights) {
-        k_kv4_weights<HD><<<dim3(((a.g.context + 31u) / 32u + 3u) / 4u, a.g.kv_heads, a.n), 256, 0, s>>>(p);
-        VX_LAUNCHED("k_kv4_weights");
     }
     return VX_OK;
 }

@@ -8,7 +8,7 @@ namespace vx {
 
 constexpr uint32_t kKv4Block = 32;        // slots of a block
 constexpr uint32_t kKv4MaxContext = 1u << 28;   // these keep every grid below 2^32 threads a dimension
-constexpr uint32_t kKv4MaxRows = 1u << 24;      // tokens of a sequence, times the query heads of a KV head
+constexpr uint32_t kKv4MaxRows = 1u << 22;      // tokens of a sequence, times the query heads of a KV head
 
 inline uint64_t kv4_block_bytes(uint32_t head_dim) { return 20ull * head_dim; }
 inline uint64_t kv4_plane_bytes(const vx_kv4_geom &g) {
