@@ -188,43 +188,53 @@ __global__ __launch_bounds__(HD) void k_kv4_store(Kv4Rows a) {
     *vw = merged;
 }
 
+// A workgroup per octet of slots, KV head and sequence, two lanes a dword of codes: K's rows
+// go out as they are made, four values a lane; V's, made a dimension a lane, pass through LDS
+// to be written the same way.
 template <int HD>
-__global__ __launch_bounds__(HD) void k_kv4_load(Kv4Rows a) {
+__global__ __launch_bounds__(2 * HD) void k_kv4_load(Kv4Rows a) {
     using L = Lay<HD>;
-    constexpr int W = HD / 8;
-    const uint32_t tid = threadIdx.x, r = tid / W, c = tid % W, head = blockIdx.y, s = blockIdx.z, seq = a.first + s;
+    constexpr int W = HD / 8, Q = HD / 4, VROW = HD + 4;   // a row's dwords of codes and quads of values
+    __shared__ __attribute__((aligned(16))) float vrows[8 * VROW];
+    const uint32_t tid = threadIdx.x, head = blockIdx.y, s = blockIdx.z, seq = a.first + s;
     const uint32_t base = a.slots[seq];
     if (base >= a.g.context) return;
     const uint32_t end = min(base + a.tokens, a.g.context);
-    const uint32_t oct = base / 8u + blockIdx.x, slot = oct * 8u + r;
+    const uint32_t oct = base / 8u + blockIdx.x;
     if (oct * 8u >= end) return;
     const size_t plane = plane_of(a.g, a.layer, seq, head), first_row = (size_t)s * a.tokens;
     const size_t block = plane * plane_bytes<HD>(a.g) + (size_t)(oct / 4u) * L::BLOCK;
-    if (a.k && slot >= base && slot < end) {
-        const uint8_t *const kb = a.kc + block;
-        const uint32_t w = reinterpret_cast<const uint32_t *>(kb)[(slot % 32u) * W + c];
-        const h2 p = __builtin_bit_cast(h2, reinterpret_cast<const uint32_t *>(kb + L::CODES)[(slot % 32u) * L::G + c / 4u]);
-        const h8 x = values8(Masks(), w, h2{p[0], p[0]}, h2{p[1], p[1]});
-        float *const to = a.k + (first_row + slot - base) * a.k_stride + head * HD + c * 8u;
+    const uint32_t r = tid / Q, c = tid % Q, slot = oct * 8u + r;   // row of the octet, quad of the row
+    const bool live = slot >= base && slot < end;
+    auto put = [&](float *to, f4 v) {
         if (a.vec) {
-            reinterpret_cast<f4 *>(to)[0] = f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
-            reinterpret_cast<f4 *>(to)[1] = f4{(float)x[4], (float)x[5], (float)x[6], (float)x[7]};
+            *reinterpret_cast<f4 *>(to) = v;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) to[i] = (float)x[i];
+            for (int i = 0; i < 4; ++i) to[i] = v[i];
         }
-    }
-    if (a.v) {   // dimension tid of the octet's slots
+    };
+    if (a.v && tid < (uint32_t)HD) {   // dimension tid of the octet's slots
         const uint8_t *const vb = a.vc + block;
         const uint32_t w = reinterpret_cast<const uint32_t *>(vb)[((oct % 4u) * 32u + tid % 32u) * L::G + tid / 32u];
         const h8 *const sc = reinterpret_cast<const h8 *>(vb + L::CODES) + ((oct % 4u) * L::G + tid / 32u) * 2u;
         const h8 x = values8(Masks(), w, sc[0], sc[1]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t sl = oct * 8u + e;
-            if (sl >= base && sl < end) a.v[(first_row + sl - base) * a.v_stride + head * HD + tid] = (float)x[e];
-        }
+        for (int e = 0; e < 8; ++e) vrows[e * VROW + tid] = (float)x[e];
     }
+    if (a.k && live) {
+        const uint8_t *const kb = a.kc + block;
+        const uint32_t w = reinterpret_cast<const uint32_t *>(kb)[(slot % 32u) * W + c / 2u];
+        const h2 p = __builtin_bit_cast(h2, reinterpret_cast<const uint32_t *>(kb + L::CODES)[(slot % 32u) * L::G + c / 8u]);
+        const h8 x = values8(Masks(), w, h2{p[0], p[0]}, h2{p[1], p[1]});
+        const bool upper = c % 2u;
+        put(a.k + (first_row + slot - base) * a.k_stride + head * HD + c * 4u,
+            f4{(float)(upper ? x[4] : x[0]), (float)(upper ? x[5] : x[1]), (float)(upper ? x[6] : x[2]), (float)(upper ? x[7] : x[3])});
+    }
+    if (!a.v) return;
+    __syncthreads();
+    if (live)
+        put(a.v + (first_row + slot - base) * a.v_stride + head * HD + c * 4u, *reinterpret_cast<const f4 *>(&vrows[r * VROW + c * 4u]));
 }
 
 __global__ __launch_bounds__(256) void k_kv4_advance(uint32_t *slots, uint32_t *positions, uint32_t n, uint32_t tokens,
@@ -974,23 +984,44 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 
 constexpr uint32_t kSelect = 1024;                 // lanes of a plane's workgroup
 constexpr uint32_t kSelectWaves = kSelect / 64;
-constexpr uint32_t kSelectSlots = 16384;           // slots whose orders fit the workgroup's LDS
-constexpr uint32_t kBins = 2048;
+constexpr uint32_t kSelectTurns = 16;              // 64 slots of a wave's run that a lane keeps in registers
+constexpr uint32_t kBins = 2048, kCopies = 4;
 
+// Over a wave, without LDS: lane l's sum over lanes 0..l (shifts within rows of 16, then the
+// last lanes of rows and row pairs broadcast upwards), and the largest, which lane 63 ends up
+// with.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += dpp_u32<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8
+    v += dpp_u32<0x112, 0xf>(v);
+    v += dpp_u32<0x114, 0xf>(v);
+    v += dpp_u32<0x118, 0xf>(v);
+    v += dpp_u32<0x142, 0xa>(v);   // row_bcast 15, 31
+    return v + dpp_u32<0x143, 0xc>(v);
+}
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
-    return v;
+    v = max(v, dpp_u32<0x111, 0xf>(v));
+    v = max(v, dpp_u32<0x112, 0xf>(v));
+    v = max(v, dpp_u32<0x114, 0xf>(v));
+    v = max(v, dpp_u32<0x118, 0xf>(v));
+    v = max(v, dpp_u32<0x142, 0xa>(v));
+    v = max(v, dpp_u32<0x143, 0xc>(v));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
-// A workgroup per plane. The keep-th largest order is found 11, 11 and 10 bits at a time
-// from histograms in LDS; then every wave takes a run of slots, and with the waves' counts
-// numbers, first, the threshold's equals, and then the slots that leave below `keep` and
-// those that stay above it. Orders are worked out once and kept in LDS; a plane of more
-// than kSelectSlots slots works them out in every pass.
+// A workgroup per plane, a wave per run of slots. The keep-th largest order is found 11, 11
+// and 10 bits at a time from histograms in LDS. With the waves' counts of orders above the
+// threshold and of its equals, S(j), the slots below j that stay, follows; slot j < keep that
+// leaves is then the (j - S(j))-th, slot j >= keep that stays the (S(j) - S(keep))-th. A lane keeps its slots' orders in registers; of more than 16384 slots it works
+// them out in every pass. Four copies of the histogram, by lane: many weights are alike (zero,
+// say), and additions to one word take turns.
 template <bool KEPT>
 __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
-    __shared__ uint32_t orders[KEPT ? kSelectSlots : 1], hist[kBins], part[2][kSelectWaves], found[2];
+    __shared__ uint32_t part[2][kSelectWaves], found[3];
+    __shared__ __attribute__((aligned(16))) uint32_t hist[kBins * kCopies];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t head = blockIdx.x, s = blockIdx.y, layer = blockIdx.z, seq = a.first + s;
     const size_t plane = plane_of(a.g, layer, seq, head);
@@ -1000,68 +1031,73 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
     const uint32_t had = a.slots[seq], n = had == VX_KV4_NO_SLOT ? 0u : min(had, a.g.context), keep = a.keep;
     uint32_t moved = 0;
     if (n > keep) {
-        uint32_t newest = 0;
-        if constexpr (KEPT) {   // both tables are read once, the orders before it is known which positions are recent
-            constexpr uint32_t PER = kSelectSlots / kSelect;
-            uint32_t at[PER];
-            float wt[PER];
+        // Wave w's slots are [run w, run (w + 1)), 64 a turn.
+        const uint32_t turns = (n + kSelect - 1u) / kSelect, j0 = w * turns * 64u + lane;
+        constexpr uint32_t KEEP = KEPT ? kSelectTurns : 1;
+        uint32_t kept[KEEP], newest = 0;
+        for (uint32_t k = tid; k < kBins * kCopies; k += kSelect) hist[k] = 0;
+        if constexpr (KEPT) {
+            float wt[KEEP];
 #pragma unroll
-            for (uint32_t k = 0; k < PER; ++k) {
-                const uint32_t j = k * kSelect + tid;
-                if (k * kSelect < n) {
-                    at[k] = j < n ? positions[j] : 0u;
-                    wt[k] = j < n ? weights[j] : 0.f;
-                    newest = max(newest, at[k]);
+            for (uint32_t k = 0; k < KEEP; ++k)
+                if (k < turns) {
+                    const uint32_t j = min(j0 + 64u * k, n - 1u);
+                    kept[k] = positions[j];
+                    wt[k] = weights[j];
                 }
-            }
-            for (uint32_t k = tid; k < kBins; k += kSelect) hist[k] = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < KEEP; ++k)
+                if (k < turns) newest = max(newest, kept[k]);
             newest = wave_max_u32(newest);
             if (lane == 0) part[0][w] = newest;
             __syncthreads();
             newest = wave_max_u32(part[0][lane % kSelectWaves]);
 #pragma unroll
-            for (uint32_t k = 0; k < PER; ++k) {
-                const uint32_t j = k * kSelect + tid;
-                if (j < n)
-                    orders[j] = at[k] < a.sinks || (uint64_t)at[k] + a.recent > newest ? 0xFFFFFFFFu : order_of(wt[k]);
-            }
+            for (uint32_t k = 0; k < KEEP; ++k)
+                if (k < turns)
+                    kept[k] = kept[k] < a.sinks || (uint64_t)kept[k] + a.recent > newest ? 0xFFFFFFFFu : order_of(wt[k]);
         } else {
             for (uint32_t j = tid; j < n; j += kSelect) newest = max(newest, positions[j]);
-            for (uint32_t k = tid; k < kBins; k += kSelect) hist[k] = 0;
             newest = wave_max_u32(newest);
             if (lane == 0) part[0][w] = newest;
             __syncthreads();
             newest = wave_max_u32(part[0][lane % kSelectWaves]);
         }
-        auto order = [&](uint32_t j) {
-            if constexpr (KEPT) return orders[j];
-            const uint32_t at = positions[j];
-            return at < a.sinks || (uint64_t)at + a.recent > newest ? 0xFFFFFFFFu : order_of(weights[j]);
+        // f(slot, its order, whether there is such a slot) for the lane's slots, in order
+        auto each = [&](auto f) {
+            if constexpr (KEPT) {
+#pragma unroll
+                for (uint32_t k = 0; k < KEEP; ++k)
+                    if (k < turns) f(j0 + 64u * k, kept[k], j0 + 64u * k < n);
+            } else {
+                for (uint32_t k = 0; k < turns; ++k) {
+                    const uint32_t j = j0 + 64u * k, at = j < n ? positions[j] : 0u;
+                    const bool held = at < a.sinks || (uint64_t)at + a.recent > newest;
+                    f(j, j >= n ? 0u : held ? 0xFFFFFFFFu : order_of(weights[j]), j < n);
+                }
+            }
         };
-        __syncthreads();
         uint32_t prefix = 0, rest = keep;   // the threshold's bits so far, slots still to take among its equals
         constexpr int kShift[3] = {21, 10, 0};
 #pragma unroll
         for (int pass = 0; pass < 3; ++pass) {
-            const int shift = kShift[pass], above_bits = pass == 0 ? 32 : kShift[pass - 1];
+            const int shift = kShift[pass], known = pass == 0 ? 0 : kShift[pass - 1];
             const uint32_t mask = pass == 2 ? 1023u : 2047u;
-            for (uint32_t j = tid; j < n; j += kSelect) {
-                const uint32_t v = order(j);
-                if (pass == 0 || (v ^ prefix) >> (above_bits & 31) == 0) atomicAdd(&hist[v >> shift & mask], 1u);
-            }
+            each([&](uint32_t, uint32_t v, bool is) {
+                if (is && (pass == 0 || (v ^ prefix) >> known == 0))
+                    atomicAdd(&hist[(v >> shift & mask) * kCopies + (tid & (kCopies - 1u))], 1u);
+            });
             __syncthreads();
             // The bin that holds the rest-th from the top: each lane two bins, descending.
-            const uint32_t b1 = kBins - 1u - 2u * tid, h1 = hist[b1], h0 = hist[b1 - 1u];
-            uint32_t sum = h1 + h0;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t t = __shfl_up((int)sum, o, 64);
-                if (lane >= (uint32_t)o) sum += t;
-            }
+            const uint32_t b1 = kBins - 1u - 2u * tid;
+            uint4 *const pair = reinterpret_cast<uint4 *>(hist + (b1 - 1u) * kCopies);
+            const uint4 n0 = pair[0], n1 = pair[1];
+            const uint32_t h0 = n0.x + n0.y + n0.z + n0.w, h1 = n1.x + n1.y + n1.z + n1.w;
+            uint32_t sum = wave_scan(h1 + h0);
             if (lane == 63) part[0][w] = sum;
-            hist[b1] = 0, hist[b1 - 1u] = 0;   // for the next pass: only this lane reads them
+            pair[0] = pair[1] = make_uint4(0, 0, 0, 0);   // for the next pass: only this lane reads them
             __syncthreads();
-            for (uint32_t k = 0; k < w; ++k) sum += part[0][k];
+            for (uint32_t k = 0; k < kSelectWaves; ++k) sum += k < w ? part[0][k] : 0u;
             const uint32_t before = sum - h1 - h0;   // slots in the bins above this lane's
             if (before < rest && sum >= rest) {
                 const bool upper = before + h1 >= rest;
@@ -1072,46 +1108,44 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
             prefix |= found[0] << shift;
             rest -= found[1];
         }
-        // Wave w's slots are [run w, run (w + 1)), 64 at a time.
-        const uint32_t run = (n + kSelect - 1u) / kSelect * 64u, j0 = w * run, j1 = min(j0 + run, n);
         const uint64_t below = (1ull << lane) - 1u;
-        uint32_t ties = 0;
-        for (uint32_t j = j0 + lane; j < j0 + run; j += 64u) ties += __popcll(__ballot(j < j1 && order(j) == prefix));
-        if (lane == 0) part[1][w] = ties;
+        uint32_t above = 0, ties = 0;
+        each([&](uint32_t, uint32_t v, bool is) {
+            above += __popcll(__ballot(is && v > prefix));
+            ties += __popcll(__ballot(is && v == prefix));
+        });
+        if (lane == 0) part[0][w] = above, part[1][w] = ties;
         __syncthreads();
-        ties = 0;
-        for (uint32_t k = 0; k < w; ++k) ties += part[1][k];
-        __syncthreads();   // part is written again below
-        uint32_t hr = 0, sr = 0;
-        const uint32_t first_tie = ties;
-        auto pass = [&](bool write) {
-            ties = first_tie;
-            for (uint32_t j = j0 + lane; j < j0 + run; j += 64u) {
-                const uint32_t v = j < j1 ? order(j) : 0u;
-                const bool tie = j < j1 && v == prefix;
-                const uint64_t tb = __ballot(tie);
-                const bool stays = j < j1 && (v > prefix || (tie && ties + __popcll(tb & below) < rest));
-                ties += __popcll(tb);
-                const bool hole = j < keep && j < j1 && !stays, source = j >= keep && stays;
-                const uint64_t hb = __ballot(hole), sb = __ballot(source);
-                if (write) {
-                    const uint32_t h = hr + __popcll(hb & below), r = sr + __popcll(sb & below);
-                    if (hole && h < a.moves) plan[2u * h + 1u] = j;
-                    if (source && r < a.moves) plan[2u * r] = j;
-                }
-                hr += __popcll(hb);
-                sr += __popcll(sb);
-            }
-        };
-        pass(false);
-        if (lane == 0) part[0][w] = hr, part[1][w] = sr;
-        __syncthreads();
-        hr = sr = 0;
+        above = ties = 0;
         for (uint32_t k = 0; k < kSelectWaves; ++k) {
-            if (k < w) hr += part[0][k], sr += part[1][k];
-            moved += part[1][k];
+            above += k < w ? part[0][k] : 0u;
+            ties += k < w ? part[1][k] : 0u;
         }
-        pass(true);
+        // f(slot, S(slot), whether it stays, whether there is such a slot)
+        auto ranked = [&](auto f) {
+            uint32_t high = above, same = ties;
+            each([&](uint32_t j, uint32_t v, bool is) {
+                const uint64_t hb = __ballot(is && v > prefix), tb = __ballot(is && v == prefix);
+                const uint32_t rank = same + __popcll(tb & below);
+                f(j, high + __popcll(hb & below) + min(rank, rest), is && (v > prefix || (v == prefix && rank < rest)), is);
+                high += __popcll(hb);
+                same += __popcll(tb);
+            });
+        };
+        if (keep >= j0 - lane && keep < j0 - lane + 64u * turns)   // this wave's run holds slot keep
+            ranked([&](uint32_t j, uint32_t stay, bool, bool) {
+                if (j == keep) found[2] = stay;
+            });
+        __syncthreads();
+        const uint32_t low = found[2];   // slots below keep that stay
+        ranked([&](uint32_t j, uint32_t stay, bool stays, bool is) {
+            if (j < keep) {
+                if (is && !stays && j - stay < a.moves) plan[2u * (j - stay) + 1u] = j;
+            } else if (stays && stay - low < a.moves) {
+                plan[2u * (stay - low)] = j;
+            }
+        });
+        moved = keep - low;
         moved = min(moved, a.moves);
     }
     for (uint32_t k = 2u * moved + tid; k < 2u * a.moves; k += kSelect) plan[k] = VX_KV4_NO_SLOT;
@@ -1231,7 +1265,7 @@ int launch_kv4_store(hipStream_t s, const Kv4Rows &a) {
 
 int launch_kv4_load(hipStream_t s, const Kv4Rows &a) {
     const dim3 grid((a.tokens + 14u) / 8u, a.g.kv_heads, a.n);
-#define CALL(HD) k_kv4_load<HD><<<grid, HD, 0, s>>>(a)
+#define CALL(HD) k_kv4_load<HD><<<grid, 2 * HD, 0, s>>>(a)
     KV4_HD(a.g.head_dim, CALL)
 #undef CALL
     VX_LAUNCHED("k_kv4_load");
@@ -1372,7 +1406,7 @@ int launch_kv4_attention(hipStream_t s, const Kv4Attn &a) {
 
 int launch_kv4_select(hipStream_t s, const Kv4Evict &a) {
     const dim3 grid(a.g.kv_heads, a.n, a.g.layers);
-    if (a.g.context <= kSelectSlots)
+    if (a.g.context <= kSelect * kSelectTurns)
         k_kv4_select<true><<<grid, kSelect, 0, s>>>(a);
     else
         k_kv4_select<false><<<grid, kSelect, 0, s>>>(a);
