@@ -1151,11 +1151,12 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
     for (uint32_t k = 2u * moved + tid; k < 2u * a.moves; k += kSelect) plan[k] = VX_KV4_NO_SLOT;
 }
 
-// Moves of a plan, a workgroup of four waves for kMoves of a plane's. V's codes of an octet
+// Moves of a plan, a workgroup of four waves for kMoves of a plane's: the first moves K and
+// the tables, the others V; each issues all its reads before its writes. V's codes of an octet
 // share dwords, so that the moves into one octet (within eight pairs of the plan, whose
 // targets rise) are made by one wave, of the workgroup of the first: a workgroup looks at
 // seven pairs before its own and seven behind.
-constexpr uint32_t kMoves = 32;
+constexpr uint32_t kMoves = 16;
 
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_compact(Kv4Evict a) {
@@ -1180,25 +1181,42 @@ __global__ __launch_bounds__(256) void k_kv4_compact(Kv4Evict a) {
         tos[tid] = fits ? to : NONE;
     }
     __syncthreads();
-    if (tid < kMoves && froms[tid + 7u] != NONE) {
-        const size_t base = plane * a.g.context, from = base + froms[tid + 7u], to = base + tos[tid + 7u];
-        if (a.weights) a.weights[to] = a.weights[from];
-        if (a.slot_positions) a.slot_positions[to] = a.slot_positions[from];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (wave == 0) {
+        // K: 16 bytes a lane of the codes, a dword of the (d, o)
+        constexpr uint32_t C = HD / 32, NC = (kMoves * C + 63u) / 64u;   // lanes a row; turns
+        uint8_t *const kp = a.kc + (a.kc ? plane * plane_bytes<HD>(a.g) : 0);
+        uint4 codes[NC];
+        uint32_t scales[NC];
+        const uint32_t mine = lane < kMoves ? froms[lane + 7u] : NONE;
+        float weight = 0.f;
+        uint32_t position = 0;
+        const size_t table = plane * a.g.context;
+        if (mine != NONE && a.weights) weight = a.weights[table + mine];
+        if (mine != NONE && a.slot_positions) position = a.slot_positions[table + mine];
+#pragma unroll
+        for (uint32_t n = 0; n < NC; ++n) {
+            const uint32_t k = n * 64u + lane, e = k / C, c = k % C, from = e < kMoves ? froms[e + 7u] : NONE;
+            if (from == NONE || !a.kc) continue;
+            const uint8_t *const src = kp + (size_t)(from / 32u) * L::BLOCK;
+            codes[n] = *reinterpret_cast<const uint4 *>(src + (from % 32u) * (HD / 2) + c * 16u);
+            scales[n] = reinterpret_cast<const uint32_t *>(src + L::CODES)[(from % 32u) * L::G + c];
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < NC; ++n) {
+            const uint32_t k = n * 64u + lane, e = k / C, c = k % C, to = e < kMoves ? tos[e + 7u] : NONE;
+            if (to == NONE || !a.kc) continue;
+            uint8_t *const dst = kp + (size_t)(to / 32u) * L::BLOCK;
+            *reinterpret_cast<uint4 *>(dst + (to % 32u) * (HD / 2) + c * 16u) = codes[n];
+            reinterpret_cast<uint32_t *>(dst + L::CODES)[(to % 32u) * L::G + c] = scales[n];
+        }
+        if (mine != NONE && a.weights) a.weights[table + tos[lane + 7u]] = weight;
+        if (mine != NONE && a.slot_positions) a.slot_positions[table + tos[lane + 7u]] = position;
+        return;
     }
     if (!a.kc) return;
-    uint8_t *const kp = a.kc + plane * plane_bytes<HD>(a.g), *const vp = a.vc + plane * plane_bytes<HD>(a.g);
-#pragma unroll
-    for (uint32_t k = tid; k < kMoves * W; k += 256u) {
-        const uint32_t from = froms[k / W + 7u], to = tos[k / W + 7u], c = k % W;
-        if (from == NONE) continue;
-        const uint8_t *const src = kp + (size_t)(from / 32u) * L::BLOCK;
-        uint8_t *const dst = kp + (size_t)(to / 32u) * L::BLOCK;
-        reinterpret_cast<uint32_t *>(dst)[(to % 32u) * W + c] = reinterpret_cast<const uint32_t *>(src)[(from % 32u) * W + c];
-        if (c < (uint32_t)L::G)
-            reinterpret_cast<uint32_t *>(dst + L::CODES)[(to % 32u) * L::G + c] =
-                reinterpret_cast<const uint32_t *>(src + L::CODES)[(from % 32u) * L::G + c];
-    }
-    // The octets' first pairs, wave by wave.
+    // V: the octets' first pairs, wave by wave.
+    uint8_t *const vp = a.vc + plane * plane_bytes<HD>(a.g);
     bool first = false;
     if (lane < kMoves) {   // pair e0 + lane
         const uint32_t to = tos[lane + 7u];
@@ -1208,8 +1226,9 @@ __global__ __launch_bounds__(256) void k_kv4_compact(Kv4Evict a) {
     }
     uint64_t runs = __ballot(first);
     for (uint32_t turn = 0; runs; ++turn, runs &= runs - 1u) {
-        if (turn % 4u != (uint32_t)__builtin_amdgcn_readfirstlane(tid >> 6)) continue;
+        if (turn % 3u != wave - 1u) continue;
         const uint32_t e = (uint32_t)__builtin_ctzll(runs) + 7u, oct = tos[e] / 8u;
+        uint8_t *const dst = vp + (size_t)(oct / 4u) * L::BLOCK;
         bool in[8];
         uint32_t from[8], to[8];
 #pragma unroll
@@ -1218,30 +1237,42 @@ __global__ __launch_bounds__(256) void k_kv4_compact(Kv4Evict a) {
             from[k] = froms[e + k];
             to[k] = tos[e + k] % 8u;
         }
-        uint8_t *const dst = vp + (size_t)(oct / 4u) * L::BLOCK;
+        constexpr uint32_t ND = (HD + 63) / 64, NS = 8 * 2 * L::G / 64 ? 8 * 2 * L::G / 64 : 1;   // a lane's dwords, its d and o
+        uint32_t *const word = reinterpret_cast<uint32_t *>(dst) + (oct % 4u) * HD + lane;
+        uint32_t v[ND], got[ND][8];
 #pragma unroll
-        for (uint32_t d = lane; d < (uint32_t)HD; d += 64u) {
-            uint32_t *const word = reinterpret_cast<uint32_t *>(dst) + (oct % 4u) * HD + d;
-            uint32_t v = *word, got[8];
+        for (uint32_t n = 0; n < ND; ++n) {
+            v[n] = word[64u * n];
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (in[k]) got[k] = reinterpret_cast<const uint32_t *>(vp + (size_t)(from[k] / 32u) * L::BLOCK)[from[k] / 8u % 4u * HD + d];
+                if (in[k]) got[n][k] = reinterpret_cast<const uint32_t *>(vp + (size_t)(from[k] / 32u) * L::BLOCK)[from[k] / 8u % 4u * HD + 64u * n + lane];
+        }
+        // d and o of every group: lane 2 G k + 2 g + which of pair e + k
+        _Float16 scale[NS], *at[NS];
+#pragma unroll
+        for (uint32_t n = 0; n < NS; ++n) {
+            const uint32_t x = n * 64u + lane, k = x / (2u * L::G), g = x / 2u % L::G, which = x % 2u;
+            at[n] = nullptr;
+            if (k >= 8u) continue;
+            const uint32_t f = froms[e + k], t = tos[e + k];
+            if (t / 8u != oct) continue;
+            scale[n] = reinterpret_cast<const _Float16 *>(vp + (size_t)(f / 32u) * L::BLOCK + L::CODES)[(f / 8u % 4u * L::G + g) * 16u + 8u * which + f % 8u];
+            at[n] = reinterpret_cast<_Float16 *>(dst + L::CODES) + ((oct % 4u) * L::G + g) * 16u + 8u * which + t % 8u;
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < ND; ++n) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (in[k]) {
-                    const uint32_t code = got[k] >> (4u * (from[k] % 8u / 2u) + 16u * (from[k] % 2u)) & 15u;
+                    const uint32_t code = got[n][k] >> (4u * (from[k] % 8u / 2u) + 16u * (from[k] % 2u)) & 15u;
                     const uint32_t bit = 4u * (to[k] / 2u) + 16u * (to[k] % 2u);
-                    v = (v & ~(15u << bit)) | code << bit;
+                    v[n] = (v[n] & ~(15u << bit)) | code << bit;
                 }
-            *word = v;
+            word[64u * n] = v[n];
         }
-        // d and o of every group: lane 2 G k + 2 g + which of pair e + k
-        for (uint32_t k = lane; k < 8u * 2u * L::G; k += 64u) {
-            const uint32_t f = froms[e + k / (2u * L::G)], t = tos[e + k / (2u * L::G)], g = k / 2u % L::G, which = k % 2u;
-            if (t / 8u != oct) continue;
-            reinterpret_cast<_Float16 *>(dst + L::CODES)[((oct % 4u) * L::G + g) * 16u + 8u * which + t % 8u] =
-                reinterpret_cast<const _Float16 *>(vp + (size_t)(f / 32u) * L::BLOCK + L::CODES)[(f / 8u % 4u * L::G + g) * 16u + 8u * which + f % 8u];
-        }
+#pragma unroll
+        for (uint32_t n = 0; n < NS; ++n)
+            if (at[n]) *at[n] = scale[n];
     }
 }
 
