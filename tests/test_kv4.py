@@ -130,7 +130,7 @@ adv = lambda *a: refused(abi.call, "vx_kv4_advance", ctx.handle, *a)
 for a, want in (((H(slots), None, 0, 0, 1, 40), "VX_ERR_INVALID_ARG"), ((H(slots), None, 0, 2, 0, 40), "VX_ERR_INVALID_ARG"),
                 ((H(slots), None, 0, 2, 1, 0), "VX_ERR_INVALID_ARG"), ((H(slots), None, 0, 2, 41, 40), "VX_ERR_SHAPE"),
                 ((H(slots), None, 1, 2, 1, 40), "VX_ERR_BOUNDS"), ((None, None, 0, 2, 1, 40), "VX_ERR_INVALID_ARG"),
-                ((H(slots), H(small), 0, 2, 1, 40), "VX_ERR_BOUNDS"),
+                ((H(slots), H(small), 0, 2, 1, 40), "VX_ERR_BOUNDS"), ((H(slots), H(slots), 0, 2, 1, 40), "VX_ERR_INVALID_ARG"),
                 ((H(slots), None, 4294967295, 4294967295, 1, 40), "VX_ERR_BOUNDS")):
     assert adv(*a) == want, a
 assert refused(abi.call, "vx_kv4_store", None, H(k), H(v), H(kc), H(vc), H(slots), None, None, row_push()) == "VX_ERR_INVALID_ARG"
@@ -184,7 +184,7 @@ for call in (select, compact):
         assert call(evict_push(), **kw) == want, (call, kw)
 assert select(evict_push(), w=None) == "VX_ERR_INVALID_ARG" and select(evict_push(), sp=None) == "VX_ERR_INVALID_ARG"
 assert compact(evict_push(), kc=None) == "VX_ERR_INVALID_ARG" and compact(evict_push(), vc=None) == "VX_ERR_INVALID_ARG"
-assert compact(evict_push(), vc=kc) == "VX_ERR_INVALID_ARG"
+assert compact(evict_push(), vc=kc) == "VX_ERR_INVALID_ARG" and compact(evict_push(), sp=w) == "VX_ERR_INVALID_ARG"
 assert kernels() == 0
 assert select(evict_push()) == "VX_OK" and compact(evict_push()) == "VX_OK"
 assert compact(evict_push(), kc=None, vc=None, w=None, sp=None) == "VX_OK"

@@ -213,6 +213,7 @@ int vx_kv4_advance(vx_ctx *ctx, vx_buf *slots, vx_buf *positions, uint32_t first
     const uint64_t bytes = ((uint64_t)first_sequence + n_sequences) * 4u;
     VX_CHECK(need_buf(slots, bytes, "vx_kv4_advance slots"));
     if (positions) VX_CHECK(need_buf(positions, bytes, "vx_kv4_advance positions"));
+    if (positions == slots) return fail(VX_ERR_INVALID_ARG, "vx_kv4_advance: slots and positions are one buffer");
     OnDevice on(ctx->device);
     ProfSpan span(ctx, "kv4.advance");
     return launch_kv4_advance(ctx->stream, static_cast<uint32_t *>(slots->ptr) + first_sequence,
@@ -296,6 +297,8 @@ int vx_kv4_compact(vx_ctx *ctx, const vx_buf *plan, vx_buf *k_cache, vx_buf *v_c
     if (k_cache || v_cache) VX_CHECK(check_caches(l.g, k_cache, v_cache, "vx_kv4_compact cache"));
     if (weights) VX_CHECK(need_buf(weights, table, "vx_kv4_compact weights"));
     if (slot_positions) VX_CHECK(need_buf(slot_positions, table, "vx_kv4_compact slot_positions"));
+    if (weights && weights == slot_positions)
+        return fail(VX_ERR_INVALID_ARG, "vx_kv4_compact: weights and slot_positions are one buffer");
     VX_CHECK(need_buf(slots, (uint64_t)l.g.sequences * 4u, "vx_kv4_compact slots"));
     l.plan_in = static_cast<const uint32_t *>(plan->ptr);
     l.kc = k_cache ? static_cast<uint8_t *>(k_cache->ptr) : nullptr;
