@@ -325,6 +325,38 @@ def test_a_nan_row_is_nan_and_others_are_not(ctx):
     assert np.isnan(got[0, 1]).all() and np.isfinite(got[0, [0, 2, 3]]).all() and np.isfinite(got[1]).all()
 
 
+@pytest.mark.parametrize("hd,qh,H,tokens,base", [(128, 16, 2, 1, 40), (128, 16, 2, 2, 40), (128, 16, 2, 12, 40),
+                                                (64, 4, 2, 30, 0), (256, 2, 1, 30, 9), (128, 16, 2, 1600, 0)])
+def test_a_stored_nan_reaches_the_rows_that_attend_to_it(ctx, hd, qh, H, tokens, base):
+    """V of one group of a slot in the call's midst, and K of another slot: earlier rows keep their bits, rows that
+    attend to the V have NaN in that group's dimensions alone, rows that attend to the K are NaN."""
+    context, group = base + tokens + 5, qh // H
+    rng = np.random.default_rng(5)
+    cache = Kv4Cache(ctx, 1, 1, H, hd, context)
+    k, v = rows_of(rng, base + tokens, H * hd), rows_of(rng, base + tokens, H * hd)
+    q, out = ctx.array(rng.standard_normal((tokens, qh * hd)).astype(np.float32)), ctx.zeros(tokens * qh * hd * 4)
+    got = []
+    at_v, at_k = base + tokens // 2, base + (3 * tokens) // 4
+    for bad in (False, True):
+        if bad:
+            v[at_v, hd * (H - 1) + 35] = np.nan
+            if tokens > 1:
+                k[at_k, 1] = np.nan      # KV head 0
+        cache.slots.upload(np.array([0], np.uint32))
+        cache.store(0, ctx.array(k), ctx.array(v), tokens=base + tokens)
+        cache.slots.upload(np.array([base], np.uint32))
+        cache.attention(0, q, out, qh, tokens=tokens)
+        got.append(out.download(np.float32).reshape(tokens, H, group, hd))
+    clean, dirty = got
+    assert np.isfinite(clean).all()
+    want = np.zeros(clean.shape, bool)
+    want[at_v - base:, H - 1, :, 32:64] = True
+    if tokens > 1:
+        want[at_k - base:, 0] = True
+    assert np.array_equal(np.isnan(dirty), want)
+    assert np.array_equal(dirty[~want], clean[~want])
+
+
 # ----------------------------------------------------------------- eviction
 def tables(rng, geom, bases, ties=True):
     L, S, H, hd, context = geom

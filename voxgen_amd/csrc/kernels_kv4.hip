@@ -411,13 +411,16 @@ struct VScale {
         d = sc[0];
         o = sc[1];
     }
-    // Slots from `some` on may hold anything: their values count as zero.
-    __device__ __forceinline__ void keep(uint32_t some) {
+    // Slots from `some` on may hold anything: their values count as zero. A NaN offset becomes
+    // the least one, unless that is NaN.
+    __device__ __forceinline__ void keep(uint32_t some, _Float16 least) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             d[e] = (uint32_t)e < some ? d[e] : 0.f16;
             o[e] = (uint32_t)e < some ? o[e] : 0.f16;
         }
+        d = __builtin_elementwise_max(d, (h8)(0.f16));
+        o = __builtin_elementwise_max(o, (h8)(least));
     }
 };
 
@@ -439,8 +442,11 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
     __shared__ __attribute__((aligned(16))) float lds[LDS];
     static_assert(!PK || NT == 1, "one column tile");
     __shared__ float ms[W][R], ls[W][R], fs[R];
+    __shared__ uint32_t nan_at[W][L::G], nan_first[L::G];   // by groups, the first slot at the edge whose V is NaN
     const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
     const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (lane < L::G) nan_at[w][lane] = ~0u;   // a wave's LDS accesses keep their order
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     // the tiles with the most keys first
     const uint32_t split = blockIdx.x / p.tiles, tile = p.tiles - 1u - blockIdx.x % p.tiles;
     const uint32_t head = blockIdx.y, s = blockIdx.z, seq = p.a.first + s;
@@ -513,6 +519,10 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
     const Masks masks;
     float minus = PK && i < 8u ? 0.0f : -1.0f;
     asm("" : "+v"(minus));
+    // 0 x NaN would reach rows that do not attend to the NaN's slot. Tiles of several columns
+    // are taken to have such rows: a constant for them, or registers spill.
+    const bool partly = NT > 1 || sees_all + 1u < sp.keys;
+    const _Float16 least = partly ? (_Float16)-kLimit : (_Float16)__builtin_nanf("");
     // A block; at the tile's edge, some row's last slots or the cache's.
     auto step = [&](auto at_edge) {
         constexpr bool edge = decltype(at_edge)::value;
@@ -594,7 +604,10 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
         for (int g = 0; g < L::G; ++g) {
             VScale &dc = sc[g % 2];
             if (g + 1 < L::G) sc[(g + 1) % 2].template load<HD>(vb, g + 1, q);
-            if constexpr (edge) dc.keep(some);
+            if constexpr (edge) {
+                dc.keep(some, least);
+                __builtin_amdgcn_sched_barrier(0);   // without it the groups' selects mix, and registers spill
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const h8 v = values8(masks, vf.code[h][g], dc.d, dc.o);
@@ -609,7 +622,24 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
     };
     const uint32_t whole = min(b1, (sees_all + 1u) / 32u);   // blocks that every row attends to all of
     while (b < whole) step(std::false_type{}), b += W;
+    const uint32_t b_edge = b;
     while (b < b1) step(std::true_type{}), b += W;
+    // Blocks at the edge took a NaN in V as finite. The first such slot is noted here: the rows
+    // that attend to it have NaN in the group's dimensions.
+    if (partly) {
+        for (b = b_edge; b < b1; b += W) {
+            const uint32_t slot0 = b * 32u + 8u * q;
+#pragma unroll 1
+            for (int g = 0; g < L::G; ++g) {
+                VScale sc;
+                sc.template load<HD>(vp + (size_t)b * L::BLOCK, g, q);
+                uint32_t at = ~0u;
+#pragma unroll
+                for (int e = 7; e >= 0; --e) at = sc.o[e] != sc.o[e] ? slot0 + e : at;
+                if (i == 0 && at < sp.keys) atomicMin(&nan_at[w][g], at);
+            }
+        }
+    }
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
         l[c] = row_sum(l[c]);
@@ -663,6 +693,12 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
 #pragma unroll
         for (int c = 0; c < NT; ++c) fs[16 * c + i] = sum[c];
     }
+    if (tid < L::G) {
+        uint32_t at = nan_at[0][tid];
+#pragma unroll
+        for (int v = 1; v < W; ++v) at = min(at, nan_at[v][tid]);
+        nan_first[tid] = at;
+    }
     if (w == 0 && q == 0) {
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
@@ -689,6 +725,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
             for (int u = 0; u < B; ++u) v += *reinterpret_cast<const f4 *>(&os[u][r + 8u][c]);
         }
         const uint32_t t = token_of(p, row), j = row - t * p.group;
+        if (nan_first[c / 32u] <= sp.base + t) v = v * __builtin_nanf("");
         if (!alone) {
             *reinterpret_cast<f4 *>(p.acc + (part * RT + r) * HD + c) = v;
             continue;
