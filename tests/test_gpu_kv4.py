@@ -249,6 +249,67 @@ def test_ragged_sequences(ctx, tokens, track, hd):
     attend(side, 0, tokens, 8, first=2, n=3, decay=0.0)
 
 
+@pytest.mark.parametrize("track", [False, True])
+@pytest.mark.parametrize("hd,qh,H,tokens,bases,context", [
+    (128, 16, 2, 790, [0], 800), (64, 16, 2, 800, [37], 830), (128, 6, 2, 521, [70, NO_SLOT, 0, 300], 600),
+    (64, 3, 3, 1400, [5, 0, 33], 1440)])
+def test_long_prompts(ctx, hd, qh, H, tokens, bases, context, track):
+    """Tiles of 64 rows, whose last tokens may lie past the context."""
+    filled = [NO_SLOT if b == NO_SLOT else min(b + tokens, context) for b in bases]
+    side = Side(ctx, (1, len(bases), H, hd, context), filled, tokens, track=track)
+    side.bases = bases
+    side.send()
+    attend(side, 0, tokens, qh, pad=4, base=4, decay=0.25)
+
+
+@pytest.mark.parametrize("track", [False, True])
+@pytest.mark.parametrize("hd,qh,H,tokens,bases,context", [
+    (128, 16, 2, 40, [3000], 3100), (256, 8, 1, 40, [1500], 1600), (64, 16, 2, 18, [2100, 64], 2200),
+    (128, 16, 1, 1, [3000], 3001), (64, 6, 2, 4, [2000, 10, NO_SLOT], 2050), (256, 12, 1, 1, [1500], 1600),
+    (128, 8, 1, 1, [12000], 12001)])
+def test_long_caches(ctx, hd, qh, H, tokens, bases, context, track):
+    """Several splits of the slots, joined; weights of many blocks."""
+    filled = [NO_SLOT if b == NO_SLOT else b + tokens for b in bases]
+    side = Side(ctx, (1, len(bases), H, hd, context), filled, tokens, track=track)
+    side.bases = bases
+    side.send()
+    attend(side, 0, tokens, qh, decay=1.0)
+
+
+def test_graphs_that_share_a_scratch(ctx):
+    """Two captured calls of one cache, replayed in turn and in either order, and a larger eager call in between whose
+    scratch outgrows theirs."""
+    hd, H, qh, context = 128, 2, 16, 2048
+    side = Side(ctx, (1, 2, H, hd, context), [1990, 700], 8, track=True)
+    tokens = (1, 5)
+    qs = [ctx.array(side.rng.standard_normal((2 * t, qh * hd)).astype(np.float32)) for t in tokens]
+    outs = [ctx.zeros(2 * t * qh * hd * 4) for t in tokens]
+    side.bases = [1980, 650]
+    side.send()
+    calls = [lambda i=i: side.dev.attention(0, qs[i], outs[i], qh, tokens=tokens[i], decay=0.0) for i in range(2)]
+    want = []
+    for i in (1, 0):
+        calls[i]()
+    want = [o.download(np.float32) for o in outs]
+    graphs = []
+    for call in calls:
+        ctx.graph_begin()
+        call()
+        graphs.append(ctx.graph_end())
+    big = ctx.zeros(2 * 40 * qh * hd * 4)
+    for turn in ((0, 1), (1, 0), (0, 0, 1, 1)):
+        for o in outs:
+            o.upload(np.zeros(o.nbytes // 4, np.float32))
+        for i in turn:
+            ctx.graph_launch(graphs[i])
+        ctx.sync()
+        for o, x in zip(outs, want):
+            assert np.array_equal(o.download(np.float32), x)
+        side.dev.attention(0, ctx.zeros(2 * 40 * qh * hd * 4), big, qh, tokens=40)
+    for g in graphs:
+        ctx.graph_free(g)
+
+
 def test_unused_slots_do_not_matter(ctx):
     """Not a bit of a row depends on what lies behind its last slot, infinities and NaN in d and o among it."""
     outs = []
