@@ -469,11 +469,25 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
     h8 qh[U], ql[U];
     float factor[NT];
     h8 *const qs = reinterpret_cast<h8 *>(lds);   // [NT][U][hi, lo][64]
+    // The weights' kernel reads the operands again, in its own order: a half of one of its tiles.
+    auto leave = [&](uint32_t half, uint32_t row, float f) {
+        const size_t pair = (size_t)s * p.a.g.kv_heads + head;
+        h8 *const to = p.qp + (pair * p.qtiles + half / 2u) * (HD / 16) * 128u;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t d8 = q * U + u, at = (d8 / 2u * 2u) * 64u + d8 % 2u * 32u + half % 2u * 16u + i;
+            to[at] = qh[u];
+            to[at + 64u] = ql[u];
+        }
+        if (q == 0 && row < rows) p.factors[pair * rows + row] = f;
+    };
     if constexpr (NT == 1) {
         factor[0] = qr.split(qh, ql);
         if constexpr (PK) {
 #pragma unroll
             for (int u = 0; u < U; ++u) qh[u] = i < 8u ? qh[u] : ql[u];
+        } else if (p.qp && split == 0 && w == 0) {
+            leave(tile, r0 + i, factor[0]);
         }
     } else {
         for (uint32_t c = w; c < NT; c += W) {
@@ -486,17 +500,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
                 qs[((c * U + u) * 2u) * 64u + lane] = qh[u];
                 qs[((c * U + u) * 2u + 1u) * 64u + lane] = ql[u];
             }
-            if (p.qp && split == 0) {   // the weights' kernel reads them again, in its operand's order
-                const size_t pair = (size_t)s * p.a.g.kv_heads + head;
-                h8 *const to = p.qp + (pair * p.qtiles + (tile * NT + c) / 2u) * (HD / 16) * 128u;
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const uint32_t d8 = q * U + u, at = (d8 / 2u * 2u) * 64u + d8 % 2u * 32u + c % 2u * 16u + i;
-                    to[at] = qh[u];
-                    to[at + 64u] = ql[u];
-                }
-                if (q == 0 && row < rows) p.factors[pair * rows + row] = f;
-            }
+            if (p.qp && split == 0) leave(tile * NT + c, row, f);
         }
         __syncthreads();
 #pragma unroll
@@ -770,6 +774,7 @@ __device__ __forceinline__ f16v mfma32(h8 a, h8 b, f16v c) { return __builtin_am
 // splits at once as fit.
 constexpr uint32_t kEagerGroups = 256;
 constexpr uint32_t kWideTiles = 192;   // tiles of 64 rows from which on they are taken
+constexpr uint64_t kSmallWork = 1ull << 28;
 template <int HD>
 __device__ __forceinline__ void join_row(const AttnArgs &p, uint32_t row, uint32_t head, uint32_t s) {
     constexpr int V = HD / 4, Y = 256 / V;
@@ -952,7 +957,11 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
     for (int r = 0; r < 16; ++r) sum[0][r] = sum[1][r] = 0.f;
     auto fetch = [&](uint32_t from) {
 #pragma unroll
-        for (int n = 0; n < PER; ++n) next[n] = src[(size_t)from * TILE + n * 256u + tid];
+        for (int n = 0; n < PER; ++n) {
+            // of an odd number of 16-row tiles, the last tile's second half was not left
+            const h8 v = src[(size_t)from * TILE + n * 256u + tid];
+            next[n] = from * 32u + (tid & 16u) < p.rows ? v : h8{};
+        }
     };
     if (tile < tiles) fetch(tile);
     for (uint32_t turn = 0; tile < tiles; tile += p.row_splits, turn ^= 1u) {
@@ -1366,13 +1375,18 @@ Shape shape_of(const Kv4Attn &a) {
         h.nt = 1;
         h.waves = 4;
     } else {
-        h.nt = a.g.head_dim < 256u && (h.rows + 63u) / 64u * pairs >= kWideTiles ? 4 : 2;
-        h.waves = 8;
+        const uint64_t work = h.rows * pairs * a.g.context;   // < 2^22 2^16 2^28: no overflow beyond 64 bits below
+        h.nt = 1;
+        h.waves = 4;
+        if (work > kSmallWork / a.g.head_dim) {
+            h.nt = a.g.head_dim < 256u && (h.rows + 63u) / 64u * pairs >= kWideTiles ? 4 : 2;
+            h.waves = 8;
+        }
     }
     h.tile_rows = h.rows <= 8u ? 8u : 16u * h.nt;
     h.tiles = (h.rows + h.tile_rows - 1u) / h.tile_rows;
     h.units = h.tiles * pairs;
-    const uint64_t wide = h.nt == 1 ? 1536u : 256u, want = wide > h.units ? wide / h.units : 1u;
+    const uint64_t wide = h.rows <= 16u ? 1536u : 256u, want = wide > h.units ? wide / h.units : 1u;
     const uint32_t least = h.waves;   // blocks of a split: one a wave
     uint32_t splits = (blocks + least - 1u) / least;
     if (splits > want) splits = (uint32_t)want;
@@ -1394,8 +1408,8 @@ Parts parts_of(const Kv4Attn &a, const Shape &h, bool with_weights) {
     Parts t;
     const uint64_t pairs = (uint64_t)a.g.kv_heads * a.n;
     const uint64_t records = h.splits > 1u ? h.units * h.splits * h.tile_rows : 0u;
-    const bool rows = with_weights && h.nt > 1u;   // the weights of prompts
-    t.qtiles = h.tiles * ((h.nt + 1u) / 2u);
+    const bool rows = with_weights && h.rows > 16u;   // the weights of prompts
+    t.qtiles = (h.tiles * h.tile_rows + 31u) / 32u;
     t.slots32 = (a.g.context + 31u) / 32u * 32u;
     // about 512 workgroups of 256 slots, at least two row tiles each
     const uint64_t chunks = (a.g.context + 255u) / 256u * pairs, most = (h.rows + 63u) / 64u;
@@ -1421,7 +1435,7 @@ template <int HD>
 static int attention(hipStream_t s, const Kv4Attn &a) {
     const Shape h = shape_of(a);
     const Parts t = parts_of(a, h, a.weights != nullptr);
-    const bool rows = a.weights && h.nt > 1u;
+    const bool rows = a.weights && h.rows > 16u;
     AttnArgs p;
     p.a = a;
     p.group = h.group;
