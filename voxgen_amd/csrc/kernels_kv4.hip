@@ -772,6 +772,7 @@ __device__ __forceinline__ f16v mfma32(h8 a, h8 b, f16v c) { return __builtin_am
 
 // The splits of a row, joined: a workgroup a row, its lanes HD / 4 columns by as many
 // splits at once as fit.
+constexpr uint32_t kFewSplits = 8;
 constexpr uint32_t kEagerGroups = 256;
 constexpr uint32_t kWideTiles = 192;   // tiles of 64 rows from which on they are taken
 constexpr uint64_t kSmallWork = 1ull << 28;
@@ -844,6 +845,50 @@ __device__ __forceinline__ void join_row(const AttnArgs &p, uint32_t row, uint32
     if (tid == 0) p.lse[((size_t)s * p.a.g.kv_heads + head) * p.rows + row] = (top - kRaise) + __builtin_amdgcn_logf(sum);
 }
 
+// The same of at most kFewSplits splits: HD / 4 lanes a row, whose splits they fetch at once,
+// before it is known which are in use.
+template <int HD>
+__device__ __forceinline__ void join_rows(const AttnArgs &p, uint32_t group, uint32_t head, uint32_t s) {
+    constexpr uint32_t V = HD / 4, Y = 256 / V;
+    const uint32_t row = group * Y + threadIdx.x / V, c = 4u * (threadIdx.x % V), seq = p.a.first + s;
+    if (row >= p.rows) return;
+    const uint32_t tile = row / p.tile_rows, r = row - tile * p.tile_rows;
+    const size_t pair = (size_t)s * p.a.g.kv_heads + head;
+    const size_t first = (pair * p.tiles + tile) * p.splits * p.tile_rows + r;
+    f4 part[kFewSplits];
+    f2 ml[kFewSplits];
+#pragma unroll
+    for (uint32_t v = 0; v < kFewSplits; ++v)
+        if (v < p.splits) {
+            part[v] = *reinterpret_cast<const f4 *>(p.acc + (first + (size_t)v * p.tile_rows) * HD + c);
+            ml[v] = *reinterpret_cast<const f2 *>(p.ml + (first + (size_t)v * p.tile_rows) * 2u);
+        }
+    const Span sp = span_of(p, seq, min((tile + 1u) * p.tile_rows, p.rows) - 1u);
+    if (sp.active <= 1u) return;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (uint32_t v = 0; v < kFewSplits; ++v)
+        if (v < sp.active) top = fmaxf(top, ml[v][0]);
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (uint32_t v = 0; v < kFewSplits; ++v)
+        if (v < sp.active) {
+            const float scale = ml[v][0] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[v][0] - top);
+            sum += ml[v][1] * scale;
+            o += part[v] * scale;
+        }
+    const uint32_t t = token_of(p, row), j = row - t * p.group;
+    o = sp.base + t < p.a.g.context ? o * (1.0f / sum) : f4{0.f, 0.f, 0.f, 0.f};
+    float *const to = p.a.out + ((size_t)s * p.a.tokens + t) * p.a.out_stride + (size_t)(head * p.group + j) * HD + c;
+    if (p.a.ovec) {
+        *reinterpret_cast<f4 *>(to) = o;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = o[e];
+    }
+    if (c == 0) p.lse[pair * p.rows + row] = (top - kRaise) + __builtin_amdgcn_logf(sum);
+}
+
 // Accumulated weights of at most 16 rows: a wave per block of 32 slots takes the scores
 // again, and sums 2^(score - lse) over the rows; a row's lse is joined from its splits here
 // too, so that it need not wait for join_row's.
@@ -900,14 +945,18 @@ __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_
     }
 }
 
-// What follows the attention kernel, in one launch: workgroups 0..joins-1 join a row's
-// splits, the others the weights of 128 slots each.
+// What follows the attention kernel, in one launch: workgroups 0..joins-1 join rows' splits,
+// the others the weights of 128 slots each.
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs p, uint32_t joins) {
-    if (blockIdx.x < joins)
-        join_row<HD>(p, blockIdx.x, blockIdx.y, blockIdx.z);
-    else
+    if (blockIdx.x < joins) {
+        if (p.splits <= kFewSplits)
+            join_rows<HD>(p, blockIdx.x, blockIdx.y, blockIdx.z);
+        else
+            join_row<HD>(p, blockIdx.x, blockIdx.y, blockIdx.z);
+    } else {
         weigh<HD>(p, blockIdx.x - joins, blockIdx.y, blockIdx.z);
+    }
 }
 
 // The same of more rows: a workgroup takes 256 slots, 64 a wave, whose values it makes once
@@ -1466,7 +1515,8 @@ static int attention(hipStream_t s, const Kv4Attn &a) {
         k_kv4_attn<HD, 4, 8, false><<<grid, 512, 0, s>>>(p);
     }
     VX_LAUNCHED("k_kv4_attn");
-    const uint32_t joins = h.splits > 1u ? h.rows : 0u;
+    const uint32_t per_join = h.splits <= kFewSplits ? 1024u / HD : 1u;   // rows
+    const uint32_t joins = h.splits > 1u ? (h.rows + per_join - 1u) / per_join : 0u;
     const uint32_t groups = a.weights && !rows ? ((a.g.context + 31u) / 32u + 3u) / 4u : 0u;
     if (joins + groups) {
         k_kv4_finish<HD><<<dim3(joins + groups, a.g.kv_heads, a.n), 256, 0, s>>>(p, joins);
