@@ -1414,7 +1414,7 @@ struct Shape {
     uint64_t units;
     bool eager;
 };
-Shape shape_of(const Kv4Attn &a) {
+Shape shape_of(const Kv4Attn &a, bool with_weights) {
     Shape h;
     h.group = a.q_heads / a.g.kv_heads;
     h.rows = a.tokens * h.group;
@@ -1436,8 +1436,8 @@ Shape shape_of(const Kv4Attn &a) {
     h.tiles = (h.rows + h.tile_rows - 1u) / h.tile_rows;
     h.units = h.tiles * pairs;
     const uint64_t wide = h.rows <= 16u ? 1536u : 256u, want = wide > h.units ? wide / h.units : 1u;
-    const uint32_t least = h.waves;   // blocks of a split: one a wave
-    uint32_t splits = (blocks + least - 1u) / least;
+    uint32_t splits = h.nt == 1 ? (blocks + 3u) / 4u : blocks < 32u ? 1u : blocks / 16u;
+    if (h.nt == 1 && blocks * a.g.head_dim <= 2048u && !(with_weights && h.rows <= 16u)) splits = 1;
     if (splits > want) splits = (uint32_t)want;
     if (splits > kMaxSplits) splits = kMaxSplits;
     h.per = (blocks + splits - 1u) / splits;
@@ -1477,12 +1477,12 @@ Parts parts_of(const Kv4Attn &a, const Shape &h, bool with_weights) {
 }  // namespace
 
 uint64_t kv4_attn_scratch_bytes(const Kv4Attn &a, bool with_weights) {
-    return parts_of(a, shape_of(a), with_weights).end * 4u;
+    return parts_of(a, shape_of(a, with_weights), with_weights).end * 4u;
 }
 
 template <int HD>
 static int attention(hipStream_t s, const Kv4Attn &a) {
-    const Shape h = shape_of(a);
+    const Shape h = shape_of(a, a.weights != nullptr);
     const Parts t = parts_of(a, h, a.weights != nullptr);
     const bool rows = a.weights && h.rows > 16u;
     AttnArgs p;
