@@ -262,18 +262,19 @@ def test_long_prompts(ctx, hd, qh, H, tokens, bases, context, track):
     attend(side, 0, tokens, qh, pad=4, base=4, decay=0.25)
 
 
-@pytest.mark.parametrize("track", [False, True])
+@pytest.mark.parametrize("track,pad", [(False, 0), (True, 0), (True, 1)])
 @pytest.mark.parametrize("hd,qh,H,tokens,bases,context", [
+    (128, 8, 1, 1, [700], 800), (64, 16, 2, 7, [1200, 3], 1250), (256, 2, 1, 3, [600], 700), (128, 16, 2, 200, [900], 1104),
     (128, 16, 2, 40, [3000], 3100), (256, 8, 1, 40, [1500], 1600), (64, 16, 2, 18, [2100, 64], 2200),
     (128, 16, 1, 1, [3000], 3001), (64, 6, 2, 4, [2000, 10, NO_SLOT], 2050), (256, 12, 1, 1, [1500], 1600),
     (128, 8, 1, 1, [12000], 12001)])
-def test_long_caches(ctx, hd, qh, H, tokens, bases, context, track):
+def test_long_caches(ctx, hd, qh, H, tokens, bases, context, track, pad):
     """Several splits of the slots, joined; weights of many blocks."""
     filled = [NO_SLOT if b == NO_SLOT else b + tokens for b in bases]
     side = Side(ctx, (1, len(bases), H, hd, context), filled, tokens, track=track)
     side.bases = bases
     side.send()
-    attend(side, 0, tokens, qh, decay=1.0)
+    attend(side, 0, tokens, qh, pad=pad, base=pad, decay=1.0)
 
 
 def test_graphs_that_share_a_scratch(ctx):

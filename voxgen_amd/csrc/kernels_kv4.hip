@@ -1045,7 +1045,9 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) sum[v][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[v][r], factor, -lse));
     }
-    float *const sums = p.sums + ((size_t)part * gridDim.y * gridDim.z + pair) * p.slots32;
+    // The sums of 256 slots through LDS, so that a lane stores its own slot's.
+    __syncthreads();
+    float *const mine = reinterpret_cast<float *>(&qs[0][0]) + w * 64u;
 #pragma unroll
     for (int v = 0; v < 2; ++v)
 #pragma unroll
@@ -1054,9 +1056,16 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
             const uint32_t bits = __builtin_bit_cast(uint32_t, y);
             const auto t = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
             y = __builtin_bit_cast(float, (uint32_t)t[0]) + __builtin_bit_cast(float, (uint32_t)t[1]);
-            const uint32_t slot = (b0 + v) * 32u + 8u * (r / 4) + 4u * h + r % 4;
-            if (j == (uint32_t)r && slot < keys) sums[slot] = y;
+            if (j == (uint32_t)r) mine[v * 32 + 8 * (r / 4) + r % 4 + 4u * h] = y;
         }
+    __syncthreads();
+    const uint32_t slot = chunk * 256u + tid;
+    if (slot >= keys) return;
+    const float y = mine[lane];
+    if (p.row_splits > 1u)
+        p.sums[((size_t)part * gridDim.y * gridDim.z + pair) * p.slots32 + slot] = y;
+    else
+        add_weight(p.a.weights + plane_of(p.a.g, p.a.layer, seq, head) * p.a.g.context, slot, base, p.a.decay, y);
 }
 
 __global__ __launch_bounds__(256) void k_kv4_add_weights(AttnArgs p) {
@@ -1460,8 +1469,10 @@ Parts parts_of(const Kv4Attn &a, const Shape &h, bool with_weights) {
     const bool rows = with_weights && h.rows > 16u;   // the weights of prompts
     t.qtiles = (h.tiles * h.tile_rows + 31u) / 32u;
     t.slots32 = (a.g.context + 31u) / 32u * 32u;
-    // about 512 workgroups of 256 slots, at least two row tiles each
-    const uint64_t chunks = (a.g.context + 255u) / 256u * pairs, most = (h.rows + 63u) / 64u;
+    // about 512 workgroups of 256 slots, at least two row tiles each; up to four row tiles one, which
+    // saves the launch that adds the splits (8 tokens of 16 query heads to 2 over 4000: 22.6 -> 19.2 us
+    // a call), from 5 tiles on that costs more (24 tokens: 24.5 against 26.1)
+    const uint64_t chunks = (a.g.context + 255u) / 256u * pairs, most = h.rows <= 128u ? 1u : (h.rows + 63u) / 64u;
     uint64_t splits = (512u + chunks - 1u) / chunks;
     if (splits > most) splits = most;
     t.row_splits = (uint32_t)splits;
@@ -1471,7 +1482,7 @@ Parts parts_of(const Kv4Attn &a, const Shape &h, bool with_weights) {
     t.lse = t.qp + (rows ? pairs * t.qtiles * 32u * a.g.head_dim : 0u);
     t.factors = t.lse + (pairs * h.rows + 3u) / 4u * 4u;
     t.sums = t.factors + (rows ? (pairs * h.rows + 3u) / 4u * 4u : 0u);
-    t.end = t.sums + (rows ? (uint64_t)t.row_splits * pairs * t.slots32 : 0u);
+    t.end = t.sums + (rows && t.row_splits > 1u ? (uint64_t)t.row_splits * pairs * t.slots32 : 0u);
     return t;
 }
 }  // namespace
@@ -1526,8 +1537,10 @@ static int attention(hipStream_t s, const Kv4Attn &a) {
         const uint32_t chunks = (a.g.context + 255u) / 256u;
         k_kv4_weights_rows<HD><<<dim3(chunks * t.row_splits, a.g.kv_heads, a.n), 256, 0, s>>>(p);
         VX_LAUNCHED("k_kv4_weights_rows");
-        k_kv4_add_weights<<<dim3(chunks, a.g.kv_heads, a.n), 256, 0, s>>>(p);
-        VX_LAUNCHED("k_kv4_add_weights");
+        if (t.row_splits > 1u) {
+            k_kv4_add_weights<<<dim3(chunks, a.g.kv_heads, a.n), 256, 0, s>>>(p);
+            VX_LAUNCHED("k_kv4_add_weights");
+        }
     }
     return VX_OK;
 }
