@@ -265,6 +265,7 @@ def test_long_prompts(ctx, hd, qh, H, tokens, bases, context, track):
 @pytest.mark.parametrize("track,pad", [(False, 0), (True, 0), (True, 1)])
 @pytest.mark.parametrize("hd,qh,H,tokens,bases,context", [
     (128, 8, 1, 1, [700], 800), (64, 16, 2, 7, [1200, 3], 1250), (256, 2, 1, 3, [600], 700), (128, 16, 2, 200, [900], 1104),
+    (128, 16, 2, 520, [1100], 1650),
     (128, 16, 2, 40, [3000], 3100), (256, 8, 1, 40, [1500], 1600), (64, 16, 2, 18, [2100, 64], 2200),
     (128, 16, 1, 1, [3000], 3001), (64, 6, 2, 4, [2000, 10, NO_SLOT], 2050), (256, 12, 1, 1, [1500], 1600),
     (128, 8, 1, 1, [12000], 12001)])

@@ -773,9 +773,6 @@ __device__ __forceinline__ f16v mfma32(h8 a, h8 b, f16v c) { return __builtin_am
 // The splits of a row, joined: a workgroup a row, its lanes HD / 4 columns by as many
 // splits at once as fit.
 constexpr uint32_t kFewSplits = 8;
-constexpr uint32_t kEagerGroups = 256;
-constexpr uint32_t kWideTiles = 192;   // tiles of 64 rows from which on they are taken
-constexpr uint64_t kSmallWork = 1ull << 28;
 template <int HD>
 __device__ __forceinline__ void join_row(const AttnArgs &p, uint32_t row, uint32_t head, uint32_t s) {
     constexpr int V = HD / 4, Y = 256 / V;
@@ -786,28 +783,13 @@ __device__ __forceinline__ void join_row(const AttnArgs &p, uint32_t row, uint32
     const size_t unit = ((size_t)s * p.a.g.kv_heads + head) * p.tiles + tile;
     const size_t first = unit * p.splits * tile_rows + r;   // the row's record in split 0
     const uint32_t c = 4u * (tid % V), y = tid / V;
-    // Few splits are fetched before it is known which are in use.
-    constexpr int E = 8;
-    f4 early[E];
-    float m = -INFINITY, l = 0.f;
-    if (p.eager) {
-        if (tid < p.splits) {
-            m = p.ml[(first + (size_t)tid * tile_rows) * 2u];
-            l = p.ml[(first + (size_t)tid * tile_rows) * 2u + 1u];
-        }
-#pragma unroll
-        for (int k = 0; k < E; ++k) {
-            const uint32_t v = y + k * Y;
-            if (v < p.splits) early[k] = *reinterpret_cast<const f4 *>(p.acc + (first + (size_t)v * tile_rows) * HD + c);
-        }
-    }
     const Span sp = span_of(p, seq, min((tile + 1u) * tile_rows, p.rows) - 1u);
     if (sp.active <= 1u) return;
-    if (!p.eager && tid < sp.active) {
+    float m = -INFINITY, l = 0.f;
+    if (tid < sp.active) {
         m = p.ml[(first + (size_t)tid * tile_rows) * 2u];
         l = p.ml[(first + (size_t)tid * tile_rows) * 2u + 1u];
     }
-    if (tid >= sp.active) m = -INFINITY, l = 0.f;
     float top = m;
 #pragma unroll
     for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
@@ -823,14 +805,8 @@ __device__ __forceinline__ void join_row(const AttnArgs &p, uint32_t row, uint32
     __syncthreads();
     sum = (red[4] + red[5]) + (red[6] + red[7]);
     f4 o = {0.f, 0.f, 0.f, 0.f};
-    uint32_t v = y;
-    if (p.eager) {
-#pragma unroll
-        for (int k = 0; k < E; ++k, v += Y)
-            if (v < sp.active) o += early[k] * sc[v];
-    }
 #pragma unroll 4
-    for (; v < sp.active; v += Y)
+    for (uint32_t v = y; v < sp.active; v += Y)
         o += *reinterpret_cast<const f4 *>(p.acc + (first + (size_t)v * tile_rows) * HD + c) * sc[v];
     *reinterpret_cast<f4 *>(&os[y][c]) = o;
     __syncthreads();
@@ -1415,11 +1391,34 @@ int launch_kv4_advance(hipStream_t s, uint32_t *slots, uint32_t *positions, uint
 }
 
 namespace {
-// Tiles of query rows and splits of the key axis. Up to 16 rows: tiles of 16, workgroups
-// of four waves, as many splits as make 2048 workgroups of at least four blocks each (a
-// block a wave). More rows: eight waves a tile of 32 or 64.
+// Tiles of query rows and splits of the slots, by sizes alone (MI355X, us a call; 16/2 heads of
+// 128 unless stated).
+//
+// Rows. Up to 8 take a tile whose columns hold both terms (PK; 16 sequences over 32768: 33.8
+// against 37.4 as 16 rows). More take tiles of 16 by four waves while rows x planes x context x
+// head_dim is within kSmallWork: a value is then made again for every 16 rows, but a workgroup
+// starts and joins sooner (8 tokens over 508: 10.6, with 32-row tiles 13.2; 64 over 564: 12.0 and
+// 14.3; beyond it 200 over 1200: 16.2 against 18). From there on tiles of 32 rows by eight waves,
+// and of 64 where there are enough of those to fill the card: kWideTiles (1900 tokens: 49 against
+// 59; 500 tokens, 126 such tiles: 18.5 against 12.6). One sequence's 32-row tiles of a long
+// context take a second round over the 256 CUs as soon as there are more than 256 of them, so
+// the wider ones then begin at kWideTilesLong (600 tokens over 4600: 69 against 81; over 600
+// they lose, 19 against 17.5; sequences of unequal length even the rounds out).
+//
+// Splits. As many as make kWideGrid workgroups of up to 16 rows (16 sequences over 32768: 33.8; 768:
+// 35.2; 3000: 38.2), and 256 of more rows (512: 256 tokens over 4256 take 37.4 against 31), a
+// workgroup having at least four blocks, and one of eight waves 16. A split costs the
+// join's launch too: a context of at most 2048 / head_dim blocks is not split (448 slots: 7.7
+// against 9.2) unless a launch for the weights follows anyway.
+constexpr uint64_t kSmallWork = 1ull << 28;
+constexpr uint32_t kWideTiles = 192, kWideTilesLong = 129, kLongContext = 1536;
+constexpr uint32_t kWideGrid = 1536;
+// Workgroups in so small a grid fetch their first block before they know the slot counts (512
+// slots: 7.4 against 7.7 us; of larger grids it is no matter, and idle splits would read for
+// nothing).
+constexpr uint32_t kEagerGroups = 256;
 struct Shape {
-    uint32_t group, rows, nt, waves, tile_rows, tiles, splits, per;
+    uint32_t group, rows, nt, tile_rows, tiles, splits, per;
     uint64_t units;
     bool eager;
 };
@@ -1429,22 +1428,14 @@ Shape shape_of(const Kv4Attn &a, bool with_weights) {
     h.rows = a.tokens * h.group;
     const uint64_t pairs = (uint64_t)a.g.kv_heads * a.n;
     const uint32_t blocks = (a.g.context + 31u) / 32u;
-    if (h.rows <= 16u) {
-        h.nt = 1;
-        h.waves = 4;
-    } else {
-        const uint64_t work = h.rows * pairs * a.g.context;   // < 2^22 2^16 2^28: no overflow beyond 64 bits below
-        h.nt = 1;
-        h.waves = 4;
-        if (work > kSmallWork / a.g.head_dim) {
-            h.nt = a.g.head_dim < 256u && (h.rows + 63u) / 64u * pairs >= kWideTiles ? 4 : 2;
-            h.waves = 8;
-        }
-    }
+    // rows < 2^22 and a cache below 2^47 bytes: no overflow
+    const bool small = h.rows <= 16u || h.rows * pairs * a.g.context <= kSmallWork / a.g.head_dim;
+    const uint32_t wide = a.n == 1u && a.g.context >= kLongContext ? kWideTilesLong : kWideTiles;
+    h.nt = small ? 1 : a.g.head_dim < 256u && (h.rows + 63u) / 64u * pairs >= wide ? 4 : 2;
     h.tile_rows = h.rows <= 8u ? 8u : 16u * h.nt;
     h.tiles = (h.rows + h.tile_rows - 1u) / h.tile_rows;
     h.units = h.tiles * pairs;
-    const uint64_t wide = h.rows <= 16u ? 1536u : 256u, want = wide > h.units ? wide / h.units : 1u;
+    const uint64_t grid = h.rows <= 16u ? kWideGrid : 256u, want = grid > h.units ? grid / h.units : 1u;
     uint32_t splits = h.nt == 1 ? (blocks + 3u) / 4u : blocks < 32u ? 1u : blocks / 16u;
     if (h.nt == 1 && blocks * a.g.head_dim <= 2048u && !(with_weights && h.rows <= 16u)) splits = 1;
     if (splits > want) splits = (uint32_t)want;
