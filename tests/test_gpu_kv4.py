@@ -278,6 +278,31 @@ def test_long_caches(ctx, hd, qh, H, tokens, bases, context, track, pad):
     attend(side, 0, tokens, qh, pad=pad, base=pad, decay=1.0)
 
 
+@pytest.mark.parametrize("track", [False, True])
+@pytest.mark.parametrize("hd,qh,H,tokens,S,context", [
+    (128, 8, 1, 1, 1, 512), (128, 8, 1, 1, 1, 513), (64, 24, 2, 1, 3, 4000), (128, 16, 2, 3, 2, 1500), (256, 5, 1, 17, 1, 700),
+    (128, 16, 2, 9, 1, 900), (128, 16, 2, 130, 2, 2100), (64, 3, 3, 1300, 3, 1400), (128, 16, 2, 530, 1, 1600)])
+def test_scratch_is_kept_to(ctx, hd, qh, H, tokens, S, context, track):
+    """Nothing behind the bytes asked for is written, and what the scratch holds before a call does not matter."""
+    cache = Kv4Cache(ctx, 1, S, H, hd, context, track=track)
+    rng = np.random.default_rng(tokens)
+    k = ctx.array(rows_of(rng, S * context, H * hd))
+    cache.store(0, k, k, tokens=context)
+    cache.slots.upload(np.array([context - tokens, 0, NO_SLOT][:S], np.uint32))
+    pc = abi.Kv4AttentionPush(cache.geom, 0, 0, S, tokens, qh, qh * hd, qh * hd, 0, 0, 0.0)
+    n = abi.load().vx_kv4_attention_scratch_bytes(pc, int(track)) // 4
+    q, got = ctx.array(rng.standard_normal((S * tokens, qh * hd)).astype(np.float32)), []
+    for fill in (0, 0x7FC00000):
+        scratch = ctx.array(np.full(n + 4096, fill, np.uint32))
+        out = ctx.zeros(S * tokens * qh * hd * 4)
+        cache.attention(0, q, out, qh, tokens=tokens, decay=0.0, scratch=scratch)
+        assert (scratch.download(np.uint32)[n:] == fill).all()
+        got.append(out.download(np.float32))
+        if track:
+            got[-1] = np.concatenate([got[-1], cache.weights.download(np.float32)])
+    assert np.isfinite(got[0]).all() and np.array_equal(got[0], got[1])
+
+
 def test_graphs_that_share_a_scratch(ctx):
     """Two captured calls of one cache, replayed in turn and in either order, and a larger eager call in between whose
     scratch outgrows theirs."""

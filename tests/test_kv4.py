@@ -157,8 +157,11 @@ for want, kw in (("VX_ERR_INVALID_ARG", dict(tokens=0)), ("VX_ERR_SHAPE", dict(q
 for want, kw in (("VX_ERR_INVALID_ARG", dict(q=None)), ("VX_ERR_INVALID_ARG", dict(out=None)),
                  ("VX_ERR_INVALID_ARG", dict(out=q)), ("VX_ERR_INVALID_ARG", dict(slots=None)),
                  ("VX_ERR_INVALID_ARG", dict(vc=kc)), ("VX_ERR_BOUNDS", dict(w=small)), ("VX_ERR_BOUNDS", dict(slots=small)),
-                 ("VX_ERR_BOUNDS", dict(scratch=small))):
+                 ("VX_ERR_BOUNDS", dict(scratch=small)), ("VX_ERR_INVALID_ARG", dict(w=out)), ("VX_ERR_INVALID_ARG", dict(w=q))):
     assert attn(attn_push(), **kw) == want, kw
+large = ctx.alloc(lib.vx_kv4_attention_scratch_bytes(attn_push(), 1) + 12 * 1024 * 4)
+for name in ("q", "kc", "vc", "out", "w", "slots"):
+    assert attn(attn_push(), **{name: large, "scratch": large}) == "VX_ERR_INVALID_ARG", name
 assert kernels() == 0
 both = ctx.alloc(12 * 1024 * 4)                      # q and out in one buffer, apart
 assert attn(attn_push(out_base=6 * 1024), q=both, out=both) == "VX_OK"
@@ -183,6 +186,7 @@ for call in (select, compact):
                      ("VX_ERR_BOUNDS", dict(slots=small)), ("VX_ERR_INVALID_ARG", dict(slots=None))):
         assert call(evict_push(), **kw) == want, (call, kw)
 assert select(evict_push(), w=None) == "VX_ERR_INVALID_ARG" and select(evict_push(), sp=None) == "VX_ERR_INVALID_ARG"
+assert select(evict_push(), plan=w, w=w) == "VX_ERR_INVALID_ARG"
 assert compact(evict_push(), kc=None) == "VX_ERR_INVALID_ARG" and compact(evict_push(), vc=None) == "VX_ERR_INVALID_ARG"
 assert compact(evict_push(), vc=kc) == "VX_ERR_INVALID_ARG" and compact(evict_push(), sp=w) == "VX_ERR_INVALID_ARG"
 assert kernels() == 0

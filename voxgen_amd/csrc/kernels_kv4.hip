@@ -134,7 +134,9 @@ __device__ __forceinline__ uint32_t encode8(const float *x, _Float16 &d, _Float1
 // A workgroup per octet of slots, KV head and sequence: eight rows of HD / 8 lanes code
 // eight values each. K's codes go out as they are; V's are transposed through LDS, and a
 // lane then owns one dimension's dword of the octet, which it merges with the codes of
-// the octet's other slots (another call's): no dword has two writers.
+// the octet's other slots (another call's): no dword has two writers. Bound by one launch
+// up to about a thousand tokens, then by the bytes: 2.8 us for a token of 2 KV heads of 128, 4.5
+// for 1900 (9 MB, 2.0 TB/s), 5.8 in a graph for 8192 (19 MB, 3.3 TB/s).
 template <int HD>
 __global__ __launch_bounds__(HD) void k_kv4_store(Kv4Rows a) {
     using L = Lay<HD>;
@@ -190,7 +192,9 @@ __global__ __launch_bounds__(HD) void k_kv4_store(Kv4Rows a) {
 
 // A workgroup per octet of slots, KV head and sequence, two lanes a dword of codes: K's rows
 // go out as they are made, four values a lane; V's, made a dimension a lane, pass through LDS
-// to be written the same way.
+// to be written the same way (2056 tokens of 2 heads of 128 3.4 us; stored a dimension a lane
+// 3.8). Bound by one launch, then by the bytes written: 1.6 us for a token, 5.4 in a graph
+// for 8192 (19 MB, 3.6 TB/s).
 template <int HD>
 __global__ __launch_bounds__(2 * HD) void k_kv4_load(Kv4Rows a) {
     using L = Lay<HD>;
@@ -433,6 +437,12 @@ struct VScale {
 // PK, of at most eight rows: columns 0..7 of the products take the high terms of the rows,
 // columns 8..15 the low ones, so that one product does for both; the scores of the two
 // columns of a row are added, and so are its sums at the end.
+// What bounds it: for few rows over a short context, the instructions of one pass through the
+// kernel at one wave a SIMD (4.2 us for a single block; 7.0 for 512 slots in one split); over a
+// long one the making of the values by the VALU (16 sequences over 32768 slots, 111 MB: 34 us,
+// 3.3 TB/s where a copy reaches 4.7); for prompts the matrix pipes at the clock that the card's power limit leaves
+// them (1024 tokens over 8024 slots, 16/2 heads of 128: 136 us, 930 TFLOP/s of two-term
+// products at 1.8 GHz; a plain f16 product of 8192^3 reaches 1045).
 template <int HD, int NT, int W, bool PK>
 __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k_kv4_attn(AttnArgs p) {
     using L = Lay<HD>;
@@ -922,7 +932,8 @@ __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_
 }
 
 // What follows the attention kernel, in one launch: workgroups 0..joins-1 join rows' splits,
-// the others the weights of 128 slots each.
+// the others the weights of 128 slots each. Bound by launch and latency: 2.6 us (28 rows of 8
+// splits), 4.3 (256 rows of 48), 5.3 with the weights of 8192 slots (as two launches 9.1).
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs p, uint32_t joins) {
     if (blockIdx.x < joins) {
@@ -935,11 +946,13 @@ __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs p, uint32_t joins) 
     }
 }
 
-// The same of more rows: a workgroup takes 256 slots, 64 a wave, whose values it makes once
-// and keeps in registers, over every row_splits-th tile of 32 rows. The tiles' operands, left
-// by the attention kernel, pass through LDS, the next on its way while one is multiplied. A
-// lane sums its slots over its row of each tile; the sums over the row splits are added by
-// k_kv4_add_weights, in order.
+// Weights of more rows, from the scores once more: the sum over rows needs each row's final
+// lse. A workgroup takes 256 slots, 64 a wave, whose values it makes once and keeps in
+// registers, over every row_splits-th tile of 32 rows. The tiles' operands, left by the
+// attention kernel, pass through LDS, the next on its way while one is multiplied. A lane sums
+// its slots over its row of each tile; the sums over the row splits are added by
+// k_kv4_add_weights, in order, so that they do not vary. Bound by the matrix pipes and the
+// exponentials between them: 1024 tokens over 8024 slots 72 us, 870 TFLOP/s of products.
 template <int HD>
 __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
     using L = Lay<HD>;
@@ -1095,9 +1108,11 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 // A workgroup per plane, a wave per run of slots. The keep-th largest order is found 11, 11
 // and 10 bits at a time from histograms in LDS. With the waves' counts of orders above the
 // threshold and of its equals, S(j), the slots below j that stay, follows; slot j < keep that
-// leaves is then the (j - S(j))-th, slot j >= keep that stays the (S(j) - S(keep))-th. A lane keeps its slots' orders in registers; of more than 16384 slots it works
-// them out in every pass. Four copies of the histogram, by lane: many weights are alike (zero,
-// say), and additions to one word take turns.
+// leaves is then the (j - S(j))-th, slot j >= keep that stays the (S(j) - S(keep))-th. A lane
+// keeps its slots' orders in registers; of more than 16384 slots it works them out in every
+// pass. Four copies of the histogram, by lane: many weights are alike (zero, say), and
+// additions to one word take turns. Bound by the latencies of its phases, one workgroup going
+// through them all: 56 planes of 8192 slots 13.2 us, 32 of 2049 9.6.
 template <bool KEPT>
 __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
     __shared__ uint32_t part[2][kSelectWaves], found[3];
@@ -1235,7 +1250,8 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
 // the tables, the others V; each issues all its reads before its writes. V's codes of an octet
 // share dwords, so that the moves into one octet (within eight pairs of the plan, whose
 // targets rise) are made by one wave, of the workgroup of the first: a workgroup looks at
-// seven pairs before its own and seven behind.
+// seven pairs before its own and seven behind. Bound by scattered reads of one or two lines a
+// row: up to 2048 moves in each of 16 planes of 128 take 8.6 us.
 constexpr uint32_t kMoves = 16;
 
 template <int HD>

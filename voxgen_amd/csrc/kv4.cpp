@@ -249,6 +249,10 @@ int vx_kv4_attention(vx_ctx *ctx, const vx_buf *q, const vx_buf *k_cache, const 
     if (overlap(q, pc->q_base, rows_end(rows, pc->q_stride, pc->q_base, width), out, pc->out_base,
                 rows_end(rows, pc->out_stride, pc->out_base, width)))
         return fail(VX_ERR_INVALID_ARG, "vx_kv4_attention: q and out overlap");
+    for (const vx_buf *b : {q, k_cache, v_cache, slots, static_cast<const vx_buf *>(out)})
+        if (b == scratch || b == weights)
+            return fail(VX_ERR_INVALID_ARG, "vx_kv4_attention: one buffer is bound twice");
+    if (weights == scratch) return fail(VX_ERR_INVALID_ARG, "vx_kv4_attention: weights and scratch are one buffer");
     l.q = static_cast<const float *>(q->ptr) + pc->q_base;
     l.kc = static_cast<const uint8_t *>(k_cache->ptr);
     l.vc = static_cast<const uint8_t *>(v_cache->ptr);
@@ -278,6 +282,8 @@ int vx_kv4_select(vx_ctx *ctx, const vx_buf *weights, const vx_buf *slot_positio
     VX_CHECK(need_buf(slot_positions, table, "vx_kv4_select slot_positions"));
     VX_CHECK(need_buf(slots, (uint64_t)l.g.sequences * 4u, "vx_kv4_select slots"));
     VX_CHECK(need_buf(plan, plan_bytes(l), "vx_kv4_select plan"));
+    if (plan == weights || plan == slot_positions || plan == slots)
+        return fail(VX_ERR_INVALID_ARG, "vx_kv4_select: the plan is another buffer of the call");
     l.weights = static_cast<float *>(weights->ptr);
     l.slot_positions = static_cast<uint32_t *>(slot_positions->ptr);
     l.slots = static_cast<uint32_t *>(slots->ptr);
