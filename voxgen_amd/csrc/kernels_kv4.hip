@@ -932,7 +932,7 @@ __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_
 }
 
 // What follows the attention kernel, in one launch: workgroups 0..joins-1 join rows' splits,
-// the others the weights of 128 slots each. Bound by launch and latency: 2.6 us (28 rows of 8
+// the others the weights of 128 slots each. Bound by launch and latency: 3.2 us (224 rows of 8
 // splits), 4.3 (256 rows of 48), 5.3 with the weights of 8192 slots (as two launches 9.1).
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs p, uint32_t joins) {
