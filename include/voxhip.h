@@ -507,9 +507,9 @@ int vx_fused_rms_swiglu(vx_ctx *ctx, const vx_model *model, const vx_buf *hidden
 /* ------------------------------------------------------------------------- */
 #define VX_KV4_NO_SLOT 4294967295u
 typedef struct vx_kv4_geom {
-    uint32_t layers, sequences, kv_heads;
+    uint32_t layers, sequences, kv_heads;   /* layers, and sequences * kv_heads, at most 65535 */
     uint32_t head_dim;              /* 64, 128 or 256 */
-    uint32_t context;               /* slots a sequence, at most 2^28 */
+    uint32_t context;               /* slots a sequence, at most 2^28; a cache below 2^47 bytes */
 } vx_kv4_geom;
 /* Bytes of the K cache, and of the V cache; 0 for a geometry that is not valid. */
 uint64_t vx_kv4_cache_bytes(const vx_kv4_geom *geom);
@@ -517,7 +517,7 @@ uint64_t vx_kv4_cache_bytes(const vx_kv4_geom *geom);
 typedef struct vx_kv4_rows_push {
     vx_kv4_geom geom;
     uint32_t layer, first_sequence, n_sequences;   /* the call's sequences */
-    uint32_t tokens;                /* rows of each; row of (i, t): i * tokens + t */
+    uint32_t tokens;                /* rows of each, at most 2^22; row of (i, t): i * tokens + t */
     uint32_t k_stride, v_stride, k_base, v_base;   /* floats */
 } vx_kv4_rows_push;
 /* Rows k, v (f32, kv_heads * head_dim wide) into their slots. slot_positions
@@ -539,11 +539,14 @@ int vx_kv4_advance(vx_ctx *ctx, vx_buf *slots, vx_buf *positions, uint32_t first
 typedef struct vx_kv4_attention_push {
     vx_kv4_geom geom;
     uint32_t layer, first_sequence, n_sequences, tokens;
-    uint32_t q_heads;               /* a multiple of kv_heads */
+    uint32_t q_heads;               /* a multiple of kv_heads, at most 1024 times it; tokens times
+                                     * q_heads / kv_heads at most 2^22 */
     uint32_t q_stride, out_stride, q_base, out_base;   /* floats */
     float decay;                    /* of the accumulated weights, 0..1 */
 } vx_kv4_attention_push;
-/* Scratch of one call; 0 for a push that is not valid. */
+/* Scratch of one call; 0 for a push that is not valid. What it holds before the
+ * call does not matter. No buffer may be bound twice, but q and out may be parts of
+ * one that do not overlap. */
 uint64_t vx_kv4_attention_scratch_bytes(const vx_kv4_attention_push *pc, uint32_t with_weights);
 /* out = softmax(q . K / sqrt(head_dim)) . V over the slots each row attends to, in
  * f32 (products on the matrix cores, q and the weights as two f16 terms each, sums

@@ -114,7 +114,8 @@ class Kv4Cache:
                   n: int | None = None, q_stride: int | None = None, out_stride: int | None = None, q_base: int = 0,
                   out_base: int = 0, decay: float = 1.0, scratch: Buffer | None = None) -> None:
         """Attention of the call's rows over the cache; with `track`, into self.weights too. The scratch is the
-        cache's own unless one is given; a call captured into a graph keeps the one that it was captured with."""
+        cache's own unless one is given. It grows with the largest call, which a capture cannot do: call once with
+        the same sizes before. A graph keeps the scratch that it was captured with."""
         key = (layer, q_heads, tokens, first, n, q_stride, out_stride, q_base, out_base, decay)
         pc, nbytes = self._pushes.get(key) or self._rows_of_queries(key)
         if scratch is None:
