@@ -1095,6 +1095,18 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
     v += dpp_u32<0x142, 0xa>(v);   // row_bcast 15, 31
     return v + dpp_u32<0x143, 0xc>(v);
 }
+// Of a value per wave, in lanes 0..15 of each 16: the sum of those before wave w.
+__device__ __forceinline__ uint32_t before_wave(uint32_t v, uint32_t w) {
+    v += dpp_u32<0x111, 0xf>(v);
+    v += dpp_u32<0x112, 0xf>(v);
+    v += dpp_u32<0x114, 0xf>(v);
+    v += dpp_u32<0x118, 0xf>(v);
+    return w ? (uint32_t)__builtin_amdgcn_readlane((int)v, (int)w - 1) : 0u;
+}
+// n and the lanes of `mask` below this one.
+__device__ __forceinline__ uint32_t lanes_below(uint64_t mask, uint32_t n) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, n));
+}
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     v = max(v, dpp_u32<0x111, 0xf>(v));
     v = max(v, dpp_u32<0x112, 0xf>(v));
@@ -1115,7 +1127,7 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 // through them all: 56 planes of 8192 slots 13.2 us, 32 of 2049 9.6.
 template <bool KEPT>
 __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
-    __shared__ uint32_t part[2][kSelectWaves], found[3];
+    __shared__ uint32_t part[2][kSelectWaves], found[5];
     __shared__ __attribute__((aligned(16))) uint32_t hist[kBins * kCopies];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t head = blockIdx.x, s = blockIdx.y, layer = blockIdx.z, seq = a.first + s;
@@ -1130,7 +1142,10 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
         const uint32_t turns = (n + kSelect - 1u) / kSelect, j0 = w * turns * 64u + lane;
         constexpr uint32_t KEEP = KEPT ? kSelectTurns : 1;
         uint32_t kept[KEEP], newest = 0;
-        for (uint32_t k = tid; k < kBins * kCopies; k += kSelect) hist[k] = 0;
+        // Positions that stay whatever they weigh: the first ones, and the last ones
+        auto held = [&](uint32_t at) { return at < a.sinks || a.recent > newest || at > newest - a.recent; };
+        for (uint32_t k = 4u * tid; k < kBins * kCopies; k += 4u * kSelect)
+            *reinterpret_cast<uint4 *>(&hist[k]) = make_uint4(0, 0, 0, 0);
         if constexpr (KEPT) {
             float wt[KEEP];
 #pragma unroll
@@ -1150,7 +1165,7 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
 #pragma unroll
             for (uint32_t k = 0; k < KEEP; ++k)
                 if (k < turns)
-                    kept[k] = kept[k] < a.sinks || (uint64_t)kept[k] + a.recent > newest ? 0xFFFFFFFFu : order_of(wt[k]);
+                    kept[k] = held(kept[k]) ? 0xFFFFFFFFu : order_of(wt[k]);
         } else {
             for (uint32_t j = tid; j < n; j += kSelect) newest = max(newest, positions[j]);
             newest = wave_max_u32(newest);
@@ -1167,8 +1182,7 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
             } else {
                 for (uint32_t k = 0; k < turns; ++k) {
                     const uint32_t j = j0 + 64u * k, at = j < n ? positions[j] : 0u;
-                    const bool held = at < a.sinks || (uint64_t)at + a.recent > newest;
-                    f(j, j >= n ? 0u : held ? 0xFFFFFFFFu : order_of(weights[j]), j < n);
+                    f(j, j >= n ? 0u : held(at) ? 0xFFFFFFFFu : order_of(weights[j]), j < n);
                 }
             }
         };
@@ -1192,7 +1206,7 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
             if (lane == 63) part[0][w] = sum;
             pair[0] = pair[1] = make_uint4(0, 0, 0, 0);   // for the next pass: only this lane reads them
             __syncthreads();
-            for (uint32_t k = 0; k < kSelectWaves; ++k) sum += k < w ? part[0][k] : 0u;
+            sum += before_wave(part[0][lane % kSelectWaves], w);
             const uint32_t before = sum - h1 - h0;   // slots in the bins above this lane's
             if (before < rest && sum >= rest) {
                 const bool upper = before + h1 >= rest;
@@ -1203,42 +1217,37 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
             prefix |= found[0] << shift;
             rest -= found[1];
         }
-        const uint64_t below = (1ull << lane) - 1u;
+        // The waves' counts above the threshold and at it, and what the wave whose run holds slot
+        // keep counts below that.
         uint32_t above = 0, ties = 0;
-        each([&](uint32_t, uint32_t v, bool is) {
-            above += __popcll(__ballot(is && v > prefix));
-            ties += __popcll(__ballot(is && v == prefix));
+        each([&](uint32_t j, uint32_t v, bool is) {
+            const uint64_t hb = __ballot(is && v > prefix), tb = __ballot(is && v == prefix);
+            if (keep - (j - lane) < 64u) {
+                const uint64_t below = (1ull << (keep - (j - lane))) - 1u;
+                found[2] = above + __popcll(hb & below);
+                found[3] = ties + __popcll(tb & below);
+                found[4] = w;
+            }
+            above += __popcll(hb);
+            ties += __popcll(tb);
         });
         if (lane == 0) part[0][w] = above, part[1][w] = ties;
         __syncthreads();
-        above = ties = 0;
-        for (uint32_t k = 0; k < kSelectWaves; ++k) {
-            above += k < w ? part[0][k] : 0u;
-            ties += k < w ? part[1][k] : 0u;
-        }
-        // f(slot, S(slot), whether it stays, whether there is such a slot)
-        auto ranked = [&](auto f) {
-            uint32_t high = above, same = ties;
-            each([&](uint32_t j, uint32_t v, bool is) {
-                const uint64_t hb = __ballot(is && v > prefix), tb = __ballot(is && v == prefix);
-                const uint32_t rank = same + __popcll(tb & below);
-                f(j, high + __popcll(hb & below) + min(rank, rest), is && (v > prefix || (v == prefix && rank < rest)), is);
-                high += __popcll(hb);
-                same += __popcll(tb);
-            });
-        };
-        if (keep >= j0 - lane && keep < j0 - lane + 64u * turns)   // this wave's run holds slot keep
-            ranked([&](uint32_t j, uint32_t stay, bool, bool) {
-                if (j == keep) found[2] = stay;
-            });
-        __syncthreads();
-        const uint32_t low = found[2];   // slots below keep that stay
-        ranked([&](uint32_t j, uint32_t stay, bool stays, bool is) {
+        const uint32_t highs = part[0][lane % kSelectWaves], sames = part[1][lane % kSelectWaves];
+        const uint32_t of = __builtin_amdgcn_readfirstlane(found[4]);
+        const uint32_t low = before_wave(highs, of) + found[2] + min(before_wave(sames, of) + found[3], rest);   // S(keep)
+        uint32_t high = before_wave(highs, w), same = before_wave(sames, w);
+        each([&](uint32_t j, uint32_t v, bool is) {
+            const uint64_t hb = __ballot(is && v > prefix), tb = __ballot(is && v == prefix);
+            const uint32_t rank = lanes_below(tb, same), stay = lanes_below(hb, high) + min(rank, rest);
+            const bool stays = v > prefix || (v == prefix && rank < rest);
             if (j < keep) {
                 if (is && !stays && j - stay < a.moves) plan[2u * (j - stay) + 1u] = j;
-            } else if (stays && stay - low < a.moves) {
+            } else if (is && stays && stay - low < a.moves) {
                 plan[2u * (stay - low)] = j;
             }
+            high += __popcll(hb);
+            same += __popcll(tb);
         });
         moved = keep - low;
         moved = min(moved, a.moves);
