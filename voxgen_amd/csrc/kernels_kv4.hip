@@ -1138,8 +1138,10 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
     const uint32_t had = a.slots[seq], n = had == VX_KV4_NO_SLOT ? 0u : min(had, a.g.context), keep = a.keep;
     uint32_t moved = 0;
     if (n > keep) {
-        // Wave w's slots are [run w, run (w + 1)), 64 a turn.
-        const uint32_t turns = (n + kSelect - 1u) / kSelect, j0 = w * turns * 64u + lane;
+        // Wave w's slots are [run w, run (w + 1)), 64 a turn. Lanes behind the last slot count as
+        // slots of the least order: behind every other, they neither stay nor matter to those.
+        const uint32_t run = (n + kSelect - 1u) / kSelect * 64u, jw = w * run, j0 = jw + lane;
+        const uint32_t turns = jw < n ? (min(run, n - jw) + 63u) / 64u : 0u;
         constexpr uint32_t KEEP = KEPT ? kSelectTurns : 1;
         uint32_t kept[KEEP], newest = 0;
         // Positions that stay whatever they weigh: the first ones, and the last ones
@@ -1165,7 +1167,7 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
 #pragma unroll
             for (uint32_t k = 0; k < KEEP; ++k)
                 if (k < turns)
-                    kept[k] = held(kept[k]) ? 0xFFFFFFFFu : order_of(wt[k]);
+                    kept[k] = j0 + 64u * k >= n ? 0u : held(kept[k]) ? 0xFFFFFFFFu : order_of(wt[k]);
         } else {
             for (uint32_t j = tid; j < n; j += kSelect) newest = max(newest, positions[j]);
             newest = wave_max_u32(newest);
@@ -1173,16 +1175,16 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
             __syncthreads();
             newest = wave_max_u32(part[0][lane % kSelectWaves]);
         }
-        // f(slot, its order, whether there is such a slot) for the lane's slots, in order
+        // f(the turn's first slot, the order of the lane's) for the wave's slots, in order
         auto each = [&](auto f) {
             if constexpr (KEPT) {
 #pragma unroll
                 for (uint32_t k = 0; k < KEEP; ++k)
-                    if (k < turns) f(j0 + 64u * k, kept[k], j0 + 64u * k < n);
+                    if (k < turns) f(jw + 64u * k, kept[k]);
             } else {
                 for (uint32_t k = 0; k < turns; ++k) {
                     const uint32_t j = j0 + 64u * k, at = j < n ? positions[j] : 0u;
-                    f(j, j >= n ? 0u : held(at) ? 0xFFFFFFFFu : order_of(weights[j]), j < n);
+                    f(jw + 64u * k, j >= n ? 0u : held(at) ? 0xFFFFFFFFu : order_of(weights[j]));
                 }
             }
         };
@@ -1192,8 +1194,8 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = kShift[pass], known = pass == 0 ? 0 : kShift[pass - 1];
             const uint32_t mask = pass == 2 ? 1023u : 2047u;
-            each([&](uint32_t, uint32_t v, bool is) {
-                if (is && (pass == 0 || (v ^ prefix) >> known == 0))
+            each([&](uint32_t, uint32_t v) {
+                if (pass == 0 || v >> known == prefix >> known)
                     atomicAdd(&hist[(v >> shift & mask) * kCopies + (tid & (kCopies - 1u))], 1u);
             });
             __syncthreads();
@@ -1220,10 +1222,10 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
         // The waves' counts above the threshold and at it, and what the wave whose run holds slot
         // keep counts below that.
         uint32_t above = 0, ties = 0;
-        each([&](uint32_t j, uint32_t v, bool is) {
-            const uint64_t hb = __ballot(is && v > prefix), tb = __ballot(is && v == prefix);
-            if (keep - (j - lane) < 64u) {
-                const uint64_t below = (1ull << (keep - (j - lane))) - 1u;
+        each([&](uint32_t first, uint32_t v) {
+            const uint64_t hb = __ballot(v > prefix), tb = __ballot(v == prefix);
+            if (keep - first < 64u) {
+                const uint64_t below = (1ull << (keep - first)) - 1u;
                 found[2] = above + __popcll(hb & below);
                 found[3] = ties + __popcll(tb & below);
                 found[4] = w;
@@ -1236,18 +1238,23 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
         const uint32_t highs = part[0][lane % kSelectWaves], sames = part[1][lane % kSelectWaves];
         const uint32_t of = __builtin_amdgcn_readfirstlane(found[4]);
         const uint32_t low = before_wave(highs, of) + found[2] + min(before_wave(sames, of) + found[3], rest);   // S(keep)
-        uint32_t high = before_wave(highs, w), same = before_wave(sames, w);
-        each([&](uint32_t j, uint32_t v, bool is) {
-            const uint64_t hb = __ballot(is && v > prefix), tb = __ballot(is && v == prefix);
-            const uint32_t rank = lanes_below(tb, same), stay = lanes_below(hb, high) + min(rank, rest);
-            const bool stays = v > prefix || (v == prefix && rank < rest);
-            if (j < keep) {
-                if (is && !stays && j - stay < a.moves) plan[2u * (j - stay) + 1u] = j;
-            } else if (is && stays && stay - low < a.moves) {
-                plan[2u * (stay - low)] = j;
+        uint32_t same = before_wave(sames, w), stayed = before_wave(highs, w) + min(same, rest);
+        each([&](uint32_t first, uint32_t v) {
+            uint64_t stay = __ballot(v > prefix);
+            const uint64_t tb = __ballot(v == prefix);
+            if (same < rest) {   // of the equals, the first ones
+                const uint32_t equals = __popcll(tb);
+                stay |= same + equals <= rest ? tb : __ballot(v == prefix && lanes_below(tb, same) < rest);
+                same += equals;
             }
-            high += __popcll(hb);
-            same += __popcll(tb);
+            const uint32_t j = first + lane, s_of = lanes_below(stay, stayed);
+            const bool stays = stay >> lane & 1u;
+            if (j < keep) {
+                if (!stays && j - s_of < a.moves) plan[2u * (j - s_of) + 1u] = j;
+            } else if (stays && s_of - low < a.moves) {
+                plan[2u * (s_of - low)] = j;
+            }
+            stayed += __popcll(stay);
         });
         moved = keep - low;
         moved = min(moved, a.moves);
