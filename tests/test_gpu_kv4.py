@@ -459,7 +459,7 @@ def tables(rng, geom, bases, ties=True):
     (1, [40], 1, 64, 20, 0, 0), (2, [64, 33, NO_SLOT, 7, 20], 2, 64, 20, 2, 5), (3, [1500], 2, 1500, 700, 4, 64),
     (1, [2049, 3001], 3, 3001, 2048, 4, 256), (1, [100], 1, 101, 100, 3, 3), (1, [101], 2, 101, 100, 3, 97),
     (1, [9], 1, 9, 1, 1, 0), (1, [5000], 1, 5001, 5000, 0, 0), (2, [1024, 1025], 1, 1100, 1023, 0, 1023),
-    (1, [20000, 16385], 1, 20001, 15000, 4, 64)])
+    (1, [20000, 16385], 1, 20001, 15000, 4, 64), (1, [16384, 16000], 1, 16384, 8192, 4, 64)])
 def test_select_and_compact_are_exact(ctx, L, bases, H, context, keep, sinks, recent):
     hd = 64
     geom = (L, len(bases), H, hd, context)

@@ -1136,6 +1136,8 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
     const uint32_t *const positions = a.slot_positions + plane * a.g.context;
     uint32_t *const plan = a.plan + (((size_t)layer * a.n + s) * a.g.kv_heads + head) * a.moves * 2u;
     const uint32_t had = a.slots[seq], n = had == VX_KV4_NO_SLOT ? 0u : min(had, a.g.context), keep = a.keep;
+    // The moves, while `hist` is free again: at most 8192 pairs of slots below 16384.
+    uint16_t *const pairs = reinterpret_cast<uint16_t *>(hist);
     uint32_t moved = 0;
     if (n > keep) {
         // Wave w's slots are [run w, run (w + 1)), 64 a turn. Lanes behind the last slot count as
@@ -1199,14 +1201,24 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
                     atomicAdd(&hist[(v >> shift & mask) * kCopies + (tid & (kCopies - 1u))], 1u);
             });
             __syncthreads();
-            // The bin that holds the rest-th from the top: each lane two bins, descending.
+            // The bin that holds the rest-th from the top: each lane two bins, descending. Eight lanes
+            // of sixteen read their second bin first: all of them meet different banks.
             const uint32_t b1 = kBins - 1u - 2u * tid;
             uint4 *const pair = reinterpret_cast<uint4 *>(hist + (b1 - 1u) * kCopies);
-            const uint4 n0 = pair[0], n1 = pair[1];
-            const uint32_t h0 = n0.x + n0.y + n0.z + n0.w, h1 = n1.x + n1.y + n1.z + n1.w;
+            const uint32_t turned = lane >> 3 & 1u;
+            uint32_t h0 = 0, h1 = 0;
+            if (pass < 2 || b1 < 1024u) {
+                const uint4 n0 = pair[turned], n1 = pair[turned ^ 1u];
+                h0 = n0.x + n0.y + n0.z + n0.w, h1 = n1.x + n1.y + n1.z + n1.w;
+                if (turned) {
+                    const uint32_t t = h0;
+                    h0 = h1, h1 = t;
+                }
+                // for the next pass: only this lane reads them
+                if (pass == 0 || (pass == 1 && b1 < 1024u)) pair[turned] = pair[turned ^ 1u] = make_uint4(0, 0, 0, 0);
+            }
             uint32_t sum = wave_scan(h1 + h0);
             if (lane == 63) part[0][w] = sum;
-            pair[0] = pair[1] = make_uint4(0, 0, 0, 0);   // for the next pass: only this lane reads them
             __syncthreads();
             sum += before_wave(part[0][lane % kSelectWaves], w);
             const uint32_t before = sum - h1 - h0;   // slots in the bins above this lane's
@@ -1250,16 +1262,33 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
             const uint32_t j = first + lane, s_of = lanes_below(stay, stayed);
             const bool stays = stay >> lane & 1u;
             if (j < keep) {
-                if (!stays && j - s_of < a.moves) plan[2u * (j - s_of) + 1u] = j;
+                if (!stays && j - s_of < a.moves) {
+                    if constexpr (KEPT)
+                        pairs[2u * (j - s_of) + 1u] = (uint16_t)j;
+                    else
+                        plan[2u * (j - s_of) + 1u] = j;
+                }
             } else if (stays && s_of - low < a.moves) {
-                plan[2u * (s_of - low)] = j;
+                if constexpr (KEPT)
+                    pairs[2u * (s_of - low)] = (uint16_t)j;
+                else
+                    plan[2u * (s_of - low)] = j;
             }
             stayed += __popcll(stay);
         });
         moved = keep - low;
         moved = min(moved, a.moves);
     }
-    for (uint32_t k = 2u * moved + tid; k < 2u * a.moves; k += kSelect) plan[k] = VX_KV4_NO_SLOT;
+    if constexpr (KEPT) {
+        __syncthreads();
+        for (uint32_t k = tid; k < a.moves; k += kSelect) {
+            const uint32_t none = VX_KV4_NO_SLOT;
+            reinterpret_cast<uint2 *>(plan)[k] =
+                k < moved ? make_uint2(pairs[2u * k], pairs[2u * k + 1u]) : make_uint2(none, none);
+        }
+    } else {
+        for (uint32_t k = 2u * moved + tid; k < 2u * a.moves; k += kSelect) plan[k] = VX_KV4_NO_SLOT;
+    }
 }
 
 // Moves of a plan, a workgroup of four waves for kMoves of a plane's: the first moves K and
