@@ -1070,9 +1070,8 @@ __global__ __launch_bounds__(256) void k_kv4_add_weights(AttnArgs p) {
 // ------------------------------------------------------------------- eviction
 // An order of weights as integers: rising, NaN below all, both zeros alike.
 __device__ __forceinline__ uint32_t order_of(float w) {
-    if (w != w) return 0u;
-    const uint32_t b = __builtin_bit_cast(uint32_t, w == 0.f ? 0.f : w);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    const uint32_t bits = __builtin_bit_cast(uint32_t, w), b = bits == 0x80000000u ? 0u : bits;
+    return w != w ? 0u : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 
 constexpr uint32_t kSelect = 1024;                 // lanes of a plane's workgroup
@@ -1147,7 +1146,7 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
         constexpr uint32_t KEEP = KEPT ? kSelectTurns : 1;
         uint32_t kept[KEEP], newest = 0;
         // Positions that stay whatever they weigh: the first ones, and the last ones
-        auto held = [&](uint32_t at) { return at < a.sinks || a.recent > newest || at > newest - a.recent; };
+        auto held = [&](uint32_t at) { return (at < a.sinks) | (a.recent > newest) | (at > newest - a.recent); };
         for (uint32_t k = 4u * tid; k < kBins * kCopies; k += 4u * kSelect)
             *reinterpret_cast<uint4 *>(&hist[k]) = make_uint4(0, 0, 0, 0);
         if constexpr (KEPT) {
@@ -1228,8 +1227,8 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
                 found[1] = upper ? before : before + h1;
             }
             __syncthreads();
-            prefix |= found[0] << shift;
-            rest -= found[1];
+            prefix |= __builtin_amdgcn_readfirstlane(found[0]) << shift;
+            rest -= __builtin_amdgcn_readfirstlane(found[1]);
         }
         // The waves' counts above the threshold and at it, and what the wave whose run holds slot
         // keep counts below that.
@@ -1249,7 +1248,8 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
         __syncthreads();
         const uint32_t highs = part[0][lane % kSelectWaves], sames = part[1][lane % kSelectWaves];
         const uint32_t of = __builtin_amdgcn_readfirstlane(found[4]);
-        const uint32_t low = before_wave(highs, of) + found[2] + min(before_wave(sames, of) + found[3], rest);   // S(keep)
+        const uint32_t low = before_wave(highs, of) + __builtin_amdgcn_readfirstlane(found[2]) +
+                             min(before_wave(sames, of) + __builtin_amdgcn_readfirstlane(found[3]), rest);   // S(keep)
         uint32_t same = before_wave(sames, w), stayed = before_wave(highs, w) + min(same, rest);
         each([&](uint32_t first, uint32_t v) {
             uint64_t stay = __ballot(v > prefix);
@@ -1260,19 +1260,13 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
                 same += equals;
             }
             const uint32_t j = first + lane, s_of = lanes_below(stay, stayed);
-            const bool stays = stay >> lane & 1u;
-            if (j < keep) {
-                if (!stays && j - s_of < a.moves) {
-                    if constexpr (KEPT)
-                        pairs[2u * (j - s_of) + 1u] = (uint16_t)j;
-                    else
-                        plan[2u * (j - s_of) + 1u] = j;
-                }
-            } else if (stays && s_of - low < a.moves) {
+            const bool lower = j < keep, stays = __builtin_amdgcn_inverse_ballot_w64(stay);
+            const uint32_t e = lower ? j - s_of : s_of - low, at = 2u * e + (lower ? 1u : 0u);
+            if ((lower != stays) & (e < a.moves)) {
                 if constexpr (KEPT)
-                    pairs[2u * (s_of - low)] = (uint16_t)j;
+                    pairs[at] = (uint16_t)j;
                 else
-                    plan[2u * (s_of - low)] = j;
+                    plan[at] = j;
             }
             stayed += __popcll(stay);
         });
@@ -1281,10 +1275,11 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
     }
     if constexpr (KEPT) {
         __syncthreads();
+#pragma unroll 4
         for (uint32_t k = tid; k < a.moves; k += kSelect) {
             const uint32_t none = VX_KV4_NO_SLOT;
-            reinterpret_cast<uint2 *>(plan)[k] =
-                k < moved ? make_uint2(pairs[2u * k], pairs[2u * k + 1u]) : make_uint2(none, none);
+            const uint32_t pair = reinterpret_cast<const uint32_t *>(pairs)[k];
+            reinterpret_cast<uint2 *>(plan)[k] = k < moved ? make_uint2(pair & 0xffffu, pair >> 16) : make_uint2(none, none);
         }
     } else {
         for (uint32_t k = 2u * moved + tid; k < 2u * a.moves; k += kSelect) plan[k] = VX_KV4_NO_SLOT;
@@ -1295,14 +1290,15 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
 // the tables, the others V; each issues all its reads before its writes. V's codes of an octet
 // share dwords, so that the moves into one octet (within eight pairs of the plan, whose
 // targets rise) are made by one wave, of the workgroup of the first: a workgroup looks at
-// seven pairs before its own and seven behind. Bound by scattered reads of one or two lines a
-// row: up to 2048 moves in each of 16 planes of 128 take 8.6 us.
+// seven pairs before its own and seven behind. Bound by the bytes of V, of
+// which a slot has a nibble in head_dim dwords: up to 2048 moves in each of 16 planes of 128, about
+// 32 MB read and written, take 8.6 us (3.7 TB/s).
 constexpr uint32_t kMoves = 16;
 
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_compact(Kv4Evict a) {
     using L = Lay<HD>;
-    constexpr uint32_t W = HD / 8, NONE = VX_KV4_NO_SLOT;
+    constexpr uint32_t NONE = VX_KV4_NO_SLOT;
     __shared__ uint32_t froms[kMoves + 14], tos[kMoves + 14];   // of pairs e0 - 7 ..; NONE: no move
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const uint32_t head = blockIdx.y % a.g.kv_heads, s = blockIdx.y / a.g.kv_heads, layer = blockIdx.z, seq = a.first + s;
