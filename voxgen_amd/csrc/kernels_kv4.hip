@@ -893,17 +893,34 @@ __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_
     kf.load(p.a.kc + plane * plane_bytes<HD>(p.a.g) + (size_t)b * L::BLOCK, i, q);
     QRow<HD> qr;
     qr.load(p, s, head, row, true, q);
+    // Lane (i, q), i < 8, stores the weight of slot 8 q + i.
+    const uint32_t slot0 = b * 32u + 8u * q, mine = slot0 + (i & 7u);
+    float *const to = p.a.weights + plane * p.a.g.context + mine;
+    const bool stores = i < 8u && mine < sp.keys, adds = mine < sp.base && p.a.decay != 0.f;
+    const float had = stores && adds ? *to : 0.f;
     float lse;
     if (sp.active <= 1u) {
         lse = p.lse[pair * p.rows + row];
     } else {
+        // a lane's splits 16 at a time, so that their loads wait once
         float m = -INFINITY, l = 0.f;
-#pragma unroll 4
-        for (uint32_t v = q; v < sp.active; v += 4u) {
-            const f2 ml = *reinterpret_cast<const f2 *>(p.ml + ((pair * p.splits + v) * p.tile_rows + row) * 2u);
-            const float top = fmaxf(m, ml[0]);
-            l = (m == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - top)) +
-                (ml[0] == -INFINITY ? ml[1] : ml[1] * __builtin_amdgcn_exp2f(ml[0] - top));
+        for (uint32_t v0 = q; v0 < sp.active; v0 += 64u) {
+            f2 ml[16];
+#pragma unroll
+            for (uint32_t k = 0; k < 16; ++k) {
+                const uint32_t v = min(v0 + 4u * k, sp.active - 1u);
+                ml[k] = *reinterpret_cast<const f2 *>(p.ml + ((pair * p.splits + v) * p.tile_rows + row) * 2u);
+            }
+            float top = m;
+#pragma unroll
+            for (uint32_t k = 0; k < 16; ++k) {
+                if (v0 + 4u * k >= sp.active) ml[k] = f2{-INFINITY, 0.f};
+                top = fmaxf(top, ml[k][0]);
+            }
+            if (m != -INFINITY) l *= __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+            for (uint32_t k = 0; k < 16; ++k)
+                l += ml[k][0] == -INFINITY ? ml[k][1] : ml[k][1] * __builtin_amdgcn_exp2f(ml[k][0] - top);
             m = top;
         }
         const float top = row_max(m);
@@ -911,7 +928,6 @@ __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_
     }
     h8 qh[U], ql[U];
     const float factor = qr.split(qh, ql);
-    const uint32_t slot0 = b * 32u + 8u * q;
     const bool valid = i < p.rows && sp.base + t < p.a.g.context;
     f4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -922,13 +938,14 @@ __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_
         x[0] = mfma16(k0, ql[u], x[0]);
         x[1] = mfma16(k1, ql[u], x[1]);
     }
-    float *const to = p.a.weights + plane * p.a.g.context;
+    float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const bool sees = valid && slot0 + e <= sp.base + t;
         const float v = sum16(sees ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[e / 4][e % 4], factor, -lse)) : 0.f);
-        if (i == (uint32_t)e && slot0 + e < sp.keys) add_weight(to, slot0 + e, sp.base, p.a.decay, v);
+        sum = i == (uint32_t)e ? v : sum;
     }
+    if (stores) *to = adds ? p.a.decay * had + sum : sum;
 }
 
 // What follows the attention kernel, in one launch: workgroups 0..joins-1 join rows' splits,
