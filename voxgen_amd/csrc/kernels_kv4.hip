@@ -795,6 +795,13 @@ __device__ __forceinline__ void join_row(const AttnArgs &p, uint32_t row, uint32
     const uint32_t c = 4u * (tid % V), y = tid / V;
     const Span sp = span_of(p, seq, min((tile + 1u) * tile_rows, p.rows) - 1u);
     if (sp.active <= 1u) return;
+    constexpr int E = 8;
+    f4 early[E];   // on their way while the splits' weights are worked out
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const uint32_t v = min(y + k * Y, sp.active - 1u);
+        early[k] = *reinterpret_cast<const f4 *>(p.acc + (first + (size_t)v * tile_rows) * HD + c);
+    }
     float m = -INFINITY, l = 0.f;
     if (tid < sp.active) {
         m = p.ml[(first + (size_t)tid * tile_rows) * 2u];
@@ -815,8 +822,11 @@ __device__ __forceinline__ void join_row(const AttnArgs &p, uint32_t row, uint32
     __syncthreads();
     sum = (red[4] + red[5]) + (red[6] + red[7]);
     f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+        if (y + k * Y < sp.active) o += early[k] * sc[y + k * Y];
 #pragma unroll 4
-    for (uint32_t v = y; v < sp.active; v += Y)
+    for (uint32_t v = y + E * Y; v < sp.active; v += Y)
         o += *reinterpret_cast<const f4 *>(p.acc + (first + (size_t)v * tile_rows) * HD + c) * sc[v];
     *reinterpret_cast<f4 *>(&os[y][c]) = o;
     __syncthreads();
