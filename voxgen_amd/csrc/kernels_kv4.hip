@@ -635,7 +635,18 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
         }
     };
     const uint32_t whole = min(b1, (sees_all + 1u) / 32u);   // blocks that every row attends to all of
-    while (b < whole) step(std::false_type{}), b += W;
+    for (; b < whole; b += W) {
+        // The older of a SIMD's two waves is served first and is done early, the other then runs
+        // alone. Taking precedence in turns they end together: hd 64 and 256 3%, 128 1%.
+        if (NT > 1 && b1 - b0 >= 32u) {
+            if ((b / W ^ w / 4u) & 1u)
+                __builtin_amdgcn_s_setprio(1);
+            else
+                __builtin_amdgcn_s_setprio(0);
+        }
+        step(std::false_type{});
+    }
+    if constexpr (NT > 1) __builtin_amdgcn_s_setprio(0);
     const uint32_t b_edge = b;
     while (b < b1) step(std::true_type{}), b += W;
     // Blocks at the edge took a NaN in V as finite. The first such slot is noted here: the rows
@@ -663,7 +674,8 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
 
     // A wave's sums are taken to the row's largest reference. One without keys has nothing
     // to give; one whose every score is NaN has no reference but a NaN sum.
-    auto *const os = reinterpret_cast<float (*)[R][OROW]>(lds);
+    constexpr int PART = W > B ? R / 2 : R;   // rows of a wave's part
+    auto *const os = reinterpret_cast<float (*)[PART][OROW]>(lds);
     float sum[NT], top[NT];
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
@@ -681,21 +693,35 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
         for (int dt = 0; dt < DT; ++dt) o[c][dt] *= mine;
     }
     if constexpr (W > B) {
-        if (w >= B) {
+        // Waves w and w + 4 exchange halves of their tiles, so that all write and read: each adds
+        // the partner's half to its own, in the partner's part of LDS.
+        constexpr int H = NT / 2;
+        auto give = [&](auto upper) {
 #pragma unroll
-            for (int c = 0; c < NT; ++c)
+            for (int c = 0; c < H; ++c)
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f4 *>(&os[w - B][16 * c + i][16 * dt + 4 * q]) = o[c][dt];
-        }
+                for (int dt = 0; dt < DT; ++dt)
+                    *reinterpret_cast<f4 *>(&os[w][16 * c + i][16 * dt + 4 * q]) = o[decltype(upper)::value ? c : H + c][dt];
+        };
+        auto take = [&](auto upper) {
+#pragma unroll
+            for (int c = 0; c < H; ++c)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    f4 *const at = reinterpret_cast<f4 *>(&os[w ^ B][16 * c + i][16 * dt + 4 * q]);
+                    *at = *at + o[decltype(upper)::value ? H + c : c][dt];
+                }
+        };
+        if (w < B)
+            give(std::false_type{});
+        else
+            give(std::true_type{});
         __syncthreads();
-        if (w < B) {
-#pragma unroll
-            for (int c = 0; c < NT; ++c)
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) o[c][dt] += *reinterpret_cast<const f4 *>(&os[w][16 * c + i][16 * dt + 4 * q]);
-        }
-    }
-    if (w < B) {
+        if (w < B)
+            take(std::false_type{});
+        else
+            take(std::true_type{});
+    } else {
 #pragma unroll
         for (int c = 0; c < NT; ++c)
 #pragma unroll
@@ -731,9 +757,10 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
     for (uint32_t k = tid; k < (uint32_t)RT * V; k += 64u * W) {
         const uint32_t r = k / V, c = 4u * (k % V), row = r0 + r;
         if (row >= rows) break;
-        f4 v = *reinterpret_cast<const f4 *>(&os[0][r][c]);
+        const uint32_t u0 = W > B && r < (uint32_t)PART ? B : 0u, at = r % (uint32_t)PART;   // a half's sums: in the other's parts
+        f4 v = *reinterpret_cast<const f4 *>(&os[u0][at][c]);
 #pragma unroll
-        for (int u = 1; u < B; ++u) v += *reinterpret_cast<const f4 *>(&os[u][r][c]);
+        for (int u = 1; u < B; ++u) v += *reinterpret_cast<const f4 *>(&os[u0 + u][at][c]);
         if constexpr (PK) {
 #pragma unroll
             for (int u = 0; u < B; ++u) v += *reinterpret_cast<const f4 *>(&os[u][r + 8u][c]);
