@@ -987,7 +987,7 @@ __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_
 
 // What follows the attention kernel, in one launch: workgroups 0..joins-1 join rows' splits,
 // the others the weights of 128 slots each. Bound by launch and latency: 3.2 us (224 rows of 8
-// splits), 4.3 (256 rows of 48), 5.3 with the weights of 8192 slots (as two launches 9.1).
+// splits), 4.3 (256 rows of 48), 4.4 with the weights of 8192 slots (as two launches 9.1).
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs p, uint32_t joins) {
     if (blockIdx.x < joins) {
@@ -1177,7 +1177,7 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 // keeps its slots' orders in registers; of more than 16384 slots it works them out in every
 // pass. Four copies of the histogram, by lane: many weights are alike (zero, say), and
 // additions to one word take turns. Bound by the latencies of its phases, one workgroup going
-// through them all: 56 planes of 8192 slots 13.2 us, 32 of 2049 9.6.
+// through them all: 56 planes of 8192 slots 10.2 us, 64 of 2049 7.0.
 template <bool KEPT>
 __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
     __shared__ uint32_t part[2][kSelectWaves], found[5];
