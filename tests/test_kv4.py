@@ -2,12 +2,13 @@
 argument checks (a stand-in for the HIP runtime counts launches, so that a refused call is
 seen to launch nothing), and the Python class's pushes."""
 import ctypes as C
+import subprocess
 
 import numpy as np
 import pytest
 
 import kv4ref
-from test_refused_memory import child, fake  # noqa: F401  (fixture)
+from test_refused_memory import HIP_INCLUDE, child, fake  # noqa: F401  (fixture)
 from voxgen_amd import abi
 
 
@@ -218,4 +219,38 @@ assert refused(bare.select, plan, 4) == "VX_ERR_STATE"
 before = len(c._pushes)
 c.store(1, k, v, tokens=3)
 assert len(c._pushes) == before
+""")
+
+
+TWO_DEVICES = """
+#define __HIP_PLATFORM_AMD__ 1
+#include <hip/hip_runtime_api.h>
+static int now, astray;
+int astray_launches(void) { return astray; }
+hipError_t hipGetDevice(int *d) { *d = now; return hipSuccess; }
+hipError_t hipSetDevice(int d) { now = d; return hipSuccess; }
+hipError_t hipLaunchKernel(const void *fn, dim3 g, dim3 b, void **a, size_t s, hipStream_t st) {
+    astray += now != 0;
+    return hipSuccess;
+}
+"""
+
+
+def test_launches_are_on_the_contexts_device(fake, tmp_path):  # noqa: F811
+    """With another device current, every call launches on its context's, and leaves the caller's current."""
+    source, library = tmp_path / "two.c", tmp_path / "libtwo.so"
+    source.write_text(TWO_DEVICES)
+    subprocess.run(["gcc", "-std=gnu11", "-O1", "-w", "-shared", "-fPIC", "-I", str(HIP_INCLUDE), str(source),
+                    "-Wl,--no-as-needed", str(fake),
+                    f"-Wl,-rpath,{fake.parent}", "-o", str(library)], check=True)
+    child(library, REFUSALS + """
+plan, scratch = ctx.alloc(1 << 20), ctx.alloc(1 << 24)
+now = C.c_int()
+for call in (lambda: store(row_push()), lambda: load(row_push()), lambda: attn(attn_push(), scratch=scratch),
+             lambda: select(evict_push(), plan=plan), lambda: compact(evict_push(), plan=plan),
+             lambda: refused(abi.call, "vx_kv4_advance", ctx.handle, H(slots), H(pos), 0, 2, 1, 40)):
+    fake.hipSetDevice(1)
+    assert call() == "VX_OK"
+    fake.hipGetDevice(C.byref(now))
+    assert now.value == 1 and fake.astray_launches() == 0
 """)
