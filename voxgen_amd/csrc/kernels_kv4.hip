@@ -450,7 +450,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
     constexpr int QLDS = NT > 1 ? R * HD : 0;   // floats: two f16 planes
     constexpr int LDS = B * R * OROW > QLDS ? B * R * OROW : QLDS;
     __shared__ __attribute__((aligned(16))) float lds[LDS];
-    static_assert(!PK || NT == 1, "one column tile");
+    static_assert((!PK || NT == 1) && (W == 4 || W == 8), "one column tile of both terms; a wave or two a SIMD");
     __shared__ float ms[W][R], ls[W][R], fs[R];
     __shared__ uint32_t nan_at[W][L::G], nan_first[L::G];   // by groups, the first slot at the edge whose V is NaN
     const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
@@ -679,15 +679,16 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
     float sum[NT], top[NT];
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
-        top[c] = -INFINITY;
+        // the waves' by the four lanes of a row
+        float mv[W / 4], lv[W / 4];
 #pragma unroll
-        for (int v = 0; v < W; ++v) top[c] = fmaxf(top[c], ms[v][16 * c + i]);
+        for (int v = 0; v < W / 4; ++v) mv[v] = ms[4 * v + q][16 * c + i], lv[v] = ls[4 * v + q][16 * c + i];
+        top[c] = row_max(W > 4 ? fmaxf(mv[0], mv[W / 4 - 1]) : mv[0]);
         sum[c] = 0.f;
 #pragma unroll
-        for (int v = 0; v < W; ++v) {
-            const float mv = ms[v][16 * c + i], lv = ls[v][16 * c + i];
-            sum[c] += mv == -INFINITY ? lv : lv * __builtin_amdgcn_exp2f(mv - top[c]);
-        }
+        for (int v = 0; v < W / 4; ++v)
+            sum[c] += mv[v] == -INFINITY ? lv[v] : lv[v] * __builtin_amdgcn_exp2f(mv[v] - top[c]);
+        sum[c] = row_sum(sum[c]);
         const float mine = m[c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[c] - top[c]);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[c][dt] *= mine;
