@@ -445,6 +445,59 @@ def test_a_stored_nan_reaches_the_rows_that_attend_to_it(ctx, hd, qh, H, tokens,
     assert np.array_equal(dirty[~want], clean[~want])
 
 
+@pytest.mark.parametrize("hd,qh,H", [(128, 16, 2), (64, 4, 2), (256, 4, 1)])
+@pytest.mark.parametrize("tokens", [3, 6, 30, 300])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, 3e38])
+def test_weights_of_rows_that_take_no_part_are_left_out(ctx, hd, qh, H, tokens, bad):
+    """Rows past the context hold anything: not a bit of the others' rows and weights depends on them."""
+    base, got = 50 + tokens // 2, []
+    context = base + (tokens + 1) // 2
+    rng = np.random.default_rng(8)
+    cache = Kv4Cache(ctx, 1, 1, H, hd, context, track=True)
+    k = ctx.array(rows_of(rng, context, H * hd))
+    cache.store(0, k, k, tokens=context)
+    cache.slots.upload(np.array([base], np.uint32))
+    q = rng.standard_normal((tokens, qh * hd)).astype(np.float32)
+    old = rng.random((H, context)).astype(np.float32)
+    for fill in (0.0, bad):
+        q[context - base:] = fill
+        out = ctx.zeros(q.nbytes)
+        cache.weights.upload(old)
+        cache.attention(0, ctx.array(q), out, qh, tokens=tokens, decay=0.5)
+        got.append(np.concatenate([out.download(np.float32), cache.weights.download(np.float32)]))
+    assert np.isfinite(got[0]).all() and np.array_equal(got[1], got[0])
+
+
+@pytest.mark.parametrize("hd,qh,H", [(128, 16, 2), (64, 4, 2), (256, 4, 1)])
+@pytest.mark.parametrize("tokens", [3, 6, 30, 300])
+@pytest.mark.parametrize("where", ["q", "k"])
+def test_weights_of_a_nan_row_end_at_its_last_slot(ctx, hd, qh, H, tokens, where):
+    """A row with a NaN in q, or in a K that it attends to, makes NaN of the weights of the slots that it attends to. The
+    slots of later tokens have what the rows that attend to them give: bit for bit, with the NaN in q."""
+    base, at, got = 70, tokens // 2, []
+    rng = np.random.default_rng(9)
+    cache = Kv4Cache(ctx, 1, 1, H, hd, base + tokens, track=True)
+    k, v = rows_of(rng, base + tokens, H * hd), ctx.array(rows_of(rng, base + tokens, H * hd))
+    q = rng.standard_normal((tokens, qh * hd)).astype(np.float32)
+    for bad in (False, True):
+        if bad and where == "q":
+            q[at, hd * (qh - 1) + 3] = np.nan      # the last KV head's
+        elif bad:
+            k[base + at, H * hd - 1] = np.nan
+        cache.slots.upload(np.array([0], np.uint32))
+        cache.store(0, ctx.array(k), v, tokens=base + tokens)
+        cache.slots.upload(np.array([base], np.uint32))
+        cache.weights.upload(np.ones((H, base + tokens), np.float32))
+        cache.attention(0, ctx.array(q), ctx.zeros(q.nbytes), qh, tokens=tokens, decay=0.5)
+        got.append(cache.weights.download(np.float32).reshape(H, -1))
+    want = np.zeros(got[0].shape, bool)
+    # every row from token `at` on attends to the slot of the K, and so has NaN for all that it attends to
+    want[H - 1, :base + at + 1 if where == "q" else None] = True
+    assert np.isfinite(got[0]).all()
+    assert np.array_equal(np.isnan(got[1]), want)
+    assert np.array_equal(got[1][~want], got[0][~want])
+
+
 # ----------------------------------------------------------------- eviction
 def tables(rng, geom, bases, ties=True):
     L, S, H, hd, context = geom

@@ -1040,7 +1040,8 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
     }
     // row tiles from the first that attends to a slot of the chunk
     const uint32_t t0 = chunk * 256u > base ? chunk * 256u - base : 0u;
-    const uint32_t tiles = (p.rows + 31u) / 32u;
+    const uint32_t live = (keys - base) * p.group;   // rows whose slots the context holds; the others hold anything
+    const uint32_t tiles = (live + 31u) / 32u;
     uint32_t tile = t0 * p.group / 32u + part;
     const h8 *const src = p.qp + pair * p.qtiles * TILE;
     const float *const lses = p.lse + pair * p.rows, *const factors = p.factors + pair * p.rows;
@@ -1062,10 +1063,10 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
 #pragma unroll
         for (int n = 0; n < PER; ++n) qs[turn][n * 256u + tid] = next[n];
         if (tile + p.row_splits < tiles) fetch(tile + p.row_splits);
-        const uint32_t row = tile * 32u + j, at = min(row, p.rows - 1u), last = base + token_of(p, at);
-        const float factor = factors[at];
-        const float lse = row < p.rows && last < p.a.g.context ? lses[at] : INFINITY;   // 2^-inf: counts nothing
-        const bool edge = (b0 + 2u) * 32u - 1u > base + token_of(p, tile * 32u);
+        const uint32_t row = tile * 32u + j, at = min(row, live - 1u);
+        const uint32_t end = row < live ? base + token_of(p, row) + 1u : 0u;   // of the slots that the row attends to
+        const float factor = factors[at], lse = lses[at];
+        const bool edge = (b0 + 2u) * 32u > base + token_of(p, tile * 32u) + 1u || tile * 32u + 32u > live;
         lds_barrier();
         const h8 *const from = qs[turn] + lane;
         f16v x[2] = {};
@@ -1077,17 +1078,22 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
             x[0] = mfma32(k[0][u], lo, x[0]);
             x[1] = mfma32(k[1][u], lo, x[1]);
         }
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[v][r] = __builtin_fmaf(x[v][r], factor, -lse);
+        // What a row does not attend to is 2^-inf whatever the row holds: its lse may be NaN.
         if (edge) {
 #pragma unroll
             for (int v = 0; v < 2; ++v)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    x[v][r] = (b0 + v) * 32u + 8u * (r / 4) + 4u * h + r % 4 > last ? -INFINITY : x[v][r];
+                    x[v][r] = (b0 + v) * 32u + 8u * (r / 4) + 4u * h + r % 4 >= end ? -INFINITY : x[v][r];
         }
 #pragma unroll
         for (int v = 0; v < 2; ++v)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum[v][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[v][r], factor, -lse));
+            for (int r = 0; r < 16; ++r) sum[v][r] += __builtin_amdgcn_exp2f(x[v][r]);
     }
     // The sums of 256 slots through LDS, so that a lane stores its own slot's.
     __syncthreads();
