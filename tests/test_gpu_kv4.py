@@ -401,6 +401,31 @@ def test_large_and_small_weights_of_one_row(ctx):
         assert rel_l2(side.dev.weights.download(np.float32)[:4001], w) < TOL
 
 
+@pytest.mark.parametrize("hd,qh,H,base,tokens", [(128, 16, 2, 2000, 1), (128, 16, 2, 2000, 2), (64, 16, 2, 3000, 1), (256, 4, 1, 700, 3),
+                                                 (128, 16, 2, 1500, 200), (64, 6, 2, 1200, 130), (256, 4, 1, 500, 120),
+                                                 (128, 8, 1, 0, 300), (128, 2, 2, 40, 1)])
+def test_weights_are_not_off_to_one_side(ctx, hd, qh, H, base, tokens):
+    """Rows that weigh all slots about alike (|s| < 0.1, so that scores are exact to 1e-8). The sum of all weights has to
+    be the number of rows: a weight is v / l with the v that l is the sum of, so what errs to one side cancels. A row is
+    off by its reciprocal (2^-24 = 6e-8), by the additions of l, of which a lane makes n <= 380 (0.4 2^-24 sqrt(n / 3) in
+    the mean square, over 16 lanes or more: 7e-8), and by the exponentials that take a wave's and a split's sum to the
+    row's reference (2^-23 = 1.2e-7 each): 3.7e-7, of either sign, so over r rows by r^1/2 less. The additions over rows
+    may all round one way: 2^-24. A single weight is off by the rounding of its exponent, which lies near 7 (2^-22 ln 2 =
+    1.65e-7, as 4..8 has steps of 2^-21), and its exponential (2^-23), both once more in l, by the row's 3.7e-7 and
+    a product (2^-24): 1e-6 at the very most."""
+    context = base + tokens
+    side = Side(ctx, (1, 1, H, hd, context), [context], base + hd, track=True)
+    side.bases = [base]
+    side.send()
+    side.dev.weights.upload(np.full(H * context, 7.0, np.float32))
+    q = (side.rng.standard_normal((tokens, qh * hd)) * 0.005).astype(np.float32)
+    side.dev.attention(0, ctx.array(q), ctx.zeros(q.nbytes), qh, tokens=tokens, decay=0.0)
+    got = side.dev.weights.download(np.float32).reshape(H, context).astype(np.float64)
+    _, want = kv4ref.attention(q.reshape(tokens, H, qh // H, hd), side.k, side.v, 0, 0, base, context)
+    assert rel_l2(got, want) < 1e-6
+    assert abs(got.sum(-1) / (tokens * qh // H) - 1).max() < 3.7e-7 / (tokens * qh // H) ** 0.5 + 2.0 ** -24
+
+
 def test_a_nan_row_is_nan_and_others_are_not(ctx):
     side = Side(ctx, (1, 2, 1, 128, 64), [20, 20], 5)
     side.bases = [19, 19]

@@ -263,7 +263,8 @@ struct AttnArgs {
     uint32_t by_group;               // 2^32 / group, rounded up; 0 where group is 1
     uint32_t tile_rows, splits, per; // rows of a tile, key splits of the grid, blocks of one
     bool eager;                      // a wave's first block is fetched before it is known whether slots fill it
-    float *ml, *acc, *lse;           // [unit][split][tile rows][2], [..][tile rows][HD], [sequence x KV head][rows]
+    float *ml, *acc;                 // [unit][split][tile rows][2], [..][tile rows][HD]
+    f2 *norm;                        // [sequence x KV head][rows]: what a weight is taken from, see norm_of
     // for the weights of prompts: the query rows as operands [sequence x KV head][32 rows][HD / 16][hi, lo][64],
     // the factors of their scores [sequence x KV head][rows], sums by row split [split][sequence x KV head][slots]
     h8 *qp;
@@ -337,6 +338,14 @@ __device__ __forceinline__ void two_terms(const float *v, float minus, h8 &hi, h
     }
     hi = join8(h);
     lo = join8(r);
+}
+
+// What gives a row's softmax weight of a score s: 2^(s - ref) / sum. Kept as the two, not as
+// the logarithm of one number: that rounds to 2^-21 at the usual 8 to 16, v_log_f32 errs to one
+// side by as much, and every weight of the row was 3e-7 to 6e-7 too large by it. A row that is
+// NaN has that in ref, so that a score of -inf still weighs nothing.
+__device__ __forceinline__ f2 norm_of(float top, float sum) {
+    return sum == sum ? f2{top - kRaise, 1.0f / sum} : f2{__builtin_nanf(""), 1.0f};
 }
 
 // Sixteen query rows as the B operand: lane (i, q) holds row i, dimensions q HD / 4 + 8 u
@@ -746,7 +755,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
             const uint32_t row = r0 + 16u * c + i;
             if (row >= rows || (PK && i >= 8u)) continue;
             if (alone) {
-                p.lse[((size_t)s * p.a.g.kv_heads + head) * rows + row] = (top[c] - kRaise) + __builtin_amdgcn_logf(sum[c]);
+                p.norm[((size_t)s * p.a.g.kv_heads + head) * rows + row] = norm_of(top[c], sum[c]);
             } else {
                 p.ml[(part * RT + 16u * c + i) * 2u] = top[c];
                 p.ml[(part * RT + 16u * c + i) * 2u + 1u] = sum[c];
@@ -866,7 +875,7 @@ __device__ __forceinline__ void join_row(const AttnArgs &p, uint32_t row, uint32
         for (int u = 1; u < Y; ++u) x += os[u][tid];
         p.a.out[((size_t)s * p.a.tokens + t) * p.a.out_stride + (size_t)(head * p.group + j) * HD + tid] = attends ? x / sum : 0.f;
     }
-    if (tid == 0) p.lse[((size_t)s * p.a.g.kv_heads + head) * p.rows + row] = (top - kRaise) + __builtin_amdgcn_logf(sum);
+    if (tid == 0) p.norm[((size_t)s * p.a.g.kv_heads + head) * p.rows + row] = norm_of(top, sum);
 }
 
 // The same of at most kFewSplits splits: HD / 4 lanes a row, whose splits they fetch at once,
@@ -910,12 +919,12 @@ __device__ __forceinline__ void join_rows(const AttnArgs &p, uint32_t group, uin
 #pragma unroll
         for (int e = 0; e < 4; ++e) to[e] = o[e];
     }
-    if (c == 0) p.lse[pair * p.rows + row] = (top - kRaise) + __builtin_amdgcn_logf(sum);
+    if (c == 0) p.norm[pair * p.rows + row] = norm_of(top, sum);
 }
 
 // Accumulated weights of at most 16 rows: a wave per block of 32 slots takes the scores
-// again, and sums 2^(score - lse) over the rows; a row's lse is joined from its splits here
-// too, so that it need not wait for join_row's.
+// again, and sums their weights over the rows; a row's splits are joined here too, so that it
+// need not wait for join_row.
 template <int HD>
 __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_t head, uint32_t s) {
     using L = Lay<HD>;
@@ -936,9 +945,9 @@ __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_
     float *const to = p.a.weights + plane * p.a.g.context + mine;
     const bool stores = i < 8u && mine < sp.keys, adds = mine < sp.base && p.a.decay != 0.f;
     const float had = stores && adds ? *to : 0.f;
-    float lse;
+    f2 norm;
     if (sp.active <= 1u) {
-        lse = p.lse[pair * p.rows + row];
+        norm = p.norm[pair * p.rows + row];
     } else {
         // a lane's splits 16 at a time, so that their loads wait once
         float m = -INFINITY, l = 0.f;
@@ -962,7 +971,7 @@ __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_
             m = top;
         }
         const float top = row_max(m);
-        lse = (top - kRaise) + __builtin_amdgcn_logf(row_sum(m == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - top)));
+        norm = norm_of(top, row_sum(m == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - top)));
     }
     h8 qh[U], ql[U];
     const float factor = qr.split(qh, ql);
@@ -980,7 +989,7 @@ __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const bool sees = valid && slot0 + e <= sp.base + t;
-        const float v = sum16(sees ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[e / 4][e % 4], factor, -lse)) : 0.f);
+        const float v = sum16(sees ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[e / 4][e % 4], factor, -norm[0])) * norm[1] : 0.f);
         sum = i == (uint32_t)e ? v : sum;
     }
     if (stores) *to = adds ? p.a.decay * had + sum : sum;
@@ -1002,7 +1011,7 @@ __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs p, uint32_t joins) 
 }
 
 // Weights of more rows, from the scores once more: the sum over rows needs each row's final
-// lse. A workgroup takes 256 slots, 64 a wave, whose values it makes once and keeps in
+// sum. A workgroup takes 256 slots, 64 a wave, whose values it makes once and keeps in
 // registers, over every row_splits-th tile of 32 rows. The tiles' operands, left by the
 // attention kernel, pass through LDS, the next on its way while one is multiplied. A lane sums
 // its slots over its row of each tile; the sums over the row splits are added by
@@ -1044,7 +1053,8 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
     const uint32_t tiles = (live + 31u) / 32u;
     uint32_t tile = t0 * p.group / 32u + part;
     const h8 *const src = p.qp + pair * p.qtiles * TILE;
-    const float *const lses = p.lse + pair * p.rows, *const factors = p.factors + pair * p.rows;
+    const float *const factors = p.factors + pair * p.rows;
+    const f2 *const norms = p.norm + pair * p.rows;
     h8 next[PER];
     float sum[2][16];
 #pragma unroll
@@ -1065,7 +1075,8 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
         if (tile + p.row_splits < tiles) fetch(tile + p.row_splits);
         const uint32_t row = tile * 32u + j, at = min(row, live - 1u);
         const uint32_t end = row < live ? base + token_of(p, row) + 1u : 0u;   // of the slots that the row attends to
-        const float factor = factors[at], lse = lses[at];
+        const float factor = factors[at];
+        const f2 norm = norms[at];
         const bool edge = (b0 + 2u) * 32u > base + token_of(p, tile * 32u) + 1u || tile * 32u + 32u > live;
         lds_barrier();
         const h8 *const from = qs[turn] + lane;
@@ -1081,8 +1092,8 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
 #pragma unroll
         for (int v = 0; v < 2; ++v)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[v][r] = __builtin_fmaf(x[v][r], factor, -lse);
-        // What a row does not attend to is 2^-inf whatever the row holds: its lse may be NaN.
+            for (int r = 0; r < 16; ++r) x[v][r] = __builtin_fmaf(x[v][r], factor, -norm[0]);
+        // What a row does not attend to is 2^-inf whatever the row holds.
         if (edge) {
 #pragma unroll
             for (int v = 0; v < 2; ++v)
@@ -1093,7 +1104,7 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
 #pragma unroll
         for (int v = 0; v < 2; ++v)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum[v][r] += __builtin_amdgcn_exp2f(x[v][r]);
+            for (int r = 0; r < 16; ++r) sum[v][r] = __builtin_fmaf(__builtin_amdgcn_exp2f(x[v][r]), norm[1], sum[v][r]);
     }
     // The sums of 256 slots through LDS, so that a lane stores its own slot's.
     __syncthreads();
@@ -1568,7 +1579,7 @@ Shape shape_of(const Kv4Attn &a, bool with_weights) {
 namespace {
 // The parts of a call's scratch, in floats from its start; `end` is its size.
 struct Parts {
-    uint64_t acc, ml, qp, lse, factors, sums, end;
+    uint64_t acc, ml, qp, norm, factors, sums, end;
     uint32_t qtiles, row_splits, slots32;
 };
 Parts parts_of(const Kv4Attn &a, const Shape &h, bool with_weights) {
@@ -1588,8 +1599,8 @@ Parts parts_of(const Kv4Attn &a, const Shape &h, bool with_weights) {
     t.acc = 0;
     t.ml = t.acc + records * a.g.head_dim;
     t.qp = t.ml + records * 2u;
-    t.lse = t.qp + (rows ? pairs * t.qtiles * 32u * a.g.head_dim : 0u);
-    t.factors = t.lse + (pairs * h.rows + 3u) / 4u * 4u;
+    t.norm = t.qp + (rows ? pairs * t.qtiles * 32u * a.g.head_dim : 0u);
+    t.factors = t.norm + (pairs * h.rows + 1u) / 2u * 4u;
     t.sums = t.factors + (rows ? (pairs * h.rows + 3u) / 4u * 4u : 0u);
     t.end = t.sums + (rows && t.row_splits > 1u ? (uint64_t)t.row_splits * pairs * t.slots32 : 0u);
     return t;
@@ -1617,7 +1628,7 @@ static int attention(hipStream_t s, const Kv4Attn &a) {
     p.eager = h.eager;
     p.acc = a.scratch + t.acc;
     p.ml = a.scratch + t.ml;
-    p.lse = a.scratch + t.lse;
+    p.norm = reinterpret_cast<f2 *>(a.scratch + t.norm);
     p.qp = rows ? reinterpret_cast<h8 *>(a.scratch + t.qp) : nullptr;
     p.factors = a.scratch + t.factors;
     p.sums = a.scratch + t.sums;
