@@ -381,6 +381,36 @@ def test_queries_of_any_size(ctx, scale):
     attend(side, 0, 1, 16, q_scale=1.2 * scale, check=tol)
 
 
+@pytest.mark.parametrize("hd,qh,H,tokens,context", [(128, 16, 2, 1, 512), (64, 16, 2, 2, 700), (256, 4, 1, 1, 90), (128, 16, 2, 60, 1400),
+                                                    (128, 8, 1, 800, 1600)])
+@pytest.mark.parametrize("scale", [1e6, 1e8, 1e10, 1e20, 1e30])
+def test_queries_whose_scores_pass_f32s_integers(ctx, hd, qh, H, tokens, context, scale):
+    """Rows that point at one slot's K with scores of up to 2^117: it takes all the weight, and the row is its V. The
+    scores are off by 2^-24 sqrt(512) of their size, and the two largest differ by a tenth and more. (The weights
+    p <= 1 go in as two f16 terms, f16(p) being exact here; the row is then exact but for the reciprocal, 2^-24 twice.)"""
+    side = Side(ctx, (1, 1, H, hd, context), [context], 3)
+    base, group = context - tokens, qh // H
+    side.bases = [base]
+    side.send()
+    q = np.zeros((tokens, H, group, hd), np.float32)
+    want = np.zeros(q.shape)
+    for h in range(H):
+        k, v = (kv4ref.rows(c, (0, 0, h), context, is_v) for c, is_v in ((side.k, False), (side.v, True)))
+        at = np.argsort(-(k ** 2).sum(-1))      # the longest first, so that nothing lies further along them
+        for t in range(tokens):
+            seen = at[at <= base + t]
+            for g in range(group):
+                x = (k[seen[(g + t) % 4]] - k.mean(0)).astype(np.float32)
+                s = k[:base + t + 1] @ x
+                second, most = np.sort(s)[-2:]
+                assert most - second > 0.1 * most
+                q[t, h, g] = x * np.float32(scale)
+                want[t, h, g] = v[np.argmax(s)]
+    out = ctx.zeros(q.nbytes)
+    side.dev.attention(0, ctx.array(q.reshape(tokens, -1)), out, qh, tokens=tokens)
+    assert rel_l2(out.download(np.float32).reshape(q.shape), want) < 2.0 ** -22
+
+
 def test_large_and_small_weights_of_one_row(ctx):
     """One slot with nearly all the weight, thousands with 2^-14 of it each and values that add up."""
     side = Side(ctx, (1, 1, 1, 64, 4096), [0], 8, track=True)

@@ -252,8 +252,11 @@ __global__ __launch_bounds__(256) void k_kv4_advance(uint32_t *slots, uint32_t *
 }
 
 // ------------------------------------------------------------------- attention
-constexpr float kLazy = 8.0f;        // a row's reference moves when a score exceeds it by this
-constexpr float kRaise = 7.0f;       // weights are taken 2^7 up, so that their low f16 terms stay normal
+// A row's reference m moves when a score s exceeds it by more than kLazy. Weights are taken as
+// 2^(s - ref), ref = m - kRaise rounded: 2^7 up, so that their low f16 terms stay normal. ref is
+// never more than 8 below m, of scores of any size (to multiples of 2, 4, 8 and 16, 7 rounds to 6
+// or 8, 8, 8 and 0), which keeps a weight to 2^15, below f16's 65504.
+constexpr float kLazy = 7.0f, kRaise = 7.0f;
 
 constexpr uint32_t kMaxSplits = 256;
 
@@ -318,10 +321,14 @@ __device__ __forceinline__ float row_sum(float v) {
 __device__ __forceinline__ int scale_of(float top) {
     return top > 0.f && top < INFINITY ? max(__builtin_amdgcn_frexp_expf(top), -100) : 0;
 }
+// Eight values times `up`, rounded to f32, as two f16 terms. The compiler must not see that v is a
+// product: it makes hi of it once in one rounding (v_fma_mixlo_f16) and once in two, and where
+// those differ, one value in 2^13, the low term belongs to another high one.
 __device__ __forceinline__ void split8(const float *x, float up, h8 &hi, h8 &lo) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float v = x[i] * up;
+        float v = x[i] * up;
+        asm("" : "+v"(v));
         hi[i] = (_Float16)v;
         lo[i] = (_Float16)(v - (float)hi[i]);
     }
@@ -349,8 +356,11 @@ __device__ __forceinline__ f2 norm_of(float top, float sum) {
 }
 
 // Sixteen query rows as the B operand: lane (i, q) holds row i, dimensions q HD / 4 + 8 u
-// + 0..7 in step u; split() makes two f16 terms of the scaled row and returns the factor of
-// the scores: the row's scale, log2(e) and 1 / sqrt(HD).
+// + 0..7 in step u; split() makes two f16 terms of the row, with log2(e) / sqrt(HD) in it and
+// scaled, and returns the scale that is left to the scores. It is a power of two: products with it
+// are exact, so that a score less the reference, an fma, is what it would be of rounded scores.
+// (With the constant in the factor, large scores exceeded their own maximum by their rounding:
+// from 2^28 on weights were infinite.)
 template <int HD>
 struct QRow {
     static constexpr int U = HD / 32;
@@ -374,11 +384,12 @@ struct QRow {
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[u][i]));
-        const int e = scale_of(row_max(top));
-        const float up = ldexpf(1.0f, 10 - e);
+        constexpr float c = kLog2e / (HD == 64 ? 8.0f : HD == 128 ? 11.3137085f : 16.0f);
+        const int e = scale_of(row_max(top) * c);
+        const float up = ldexpf(c, 10 - e);
 #pragma unroll
         for (int u = 0; u < U; ++u) split8(x[u], up, qh[u], ql[u]);
-        return ldexpf(kLog2e / sqrtf((float)HD), e - 10);
+        return ldexpf(1.0f, e - 10);
     }
 };
 
@@ -595,12 +606,12 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
 #pragma unroll
             for (int e = 1; e < 8; ++e) top[c] = fmaxf(top[c], x[c][e / 4][e % 4]);
             top[c] *= factor[c];
-            moves = moves || top[c] > m[c] + kLazy;
+            moves = moves || top[c] - m[c] > kLazy;
         }
         if (__builtin_expect(__any(moves), 0)) {
 #pragma unroll
             for (int c = 0; c < NT; ++c) {
-                const float t = row_max(top[c]), mn = t > m[c] + kLazy ? t : m[c];
+                const float t = row_max(top[c]), mn = t - m[c] > kLazy ? t : m[c];
                 const float alpha = mn == m[c] ? 1.f : __builtin_amdgcn_exp2f(m[c] - mn);
                 m[c] = mn;
                 l[c] *= alpha;
