@@ -411,6 +411,25 @@ def test_queries_whose_scores_pass_f32s_integers(ctx, hd, qh, H, tokens, context
     assert rel_l2(out.download(np.float32).reshape(q.shape), want) < 2.0 ** -22
 
 
+@pytest.mark.parametrize("hd,qh,H,base,tokens", [(128, 16, 2, 500, 1), (128, 24, 2, 500, 1), (64, 16, 2, 1200, 3), (256, 4, 1, 90, 1),
+                                                 (128, 16, 2, 1400, 60), (128, 8, 1, 900, 800), (256, 8, 1, 2000, 100)])
+@pytest.mark.parametrize("scale", [30.0, 1e3, 1e5, 1e8, 1e12, 1e30])
+def test_weights_of_large_scores_add_up_to_the_rows(ctx, hd, qh, H, base, tokens, scale):
+    """Scores that are off by 2^-24 of their size, so by more than a weight allows: the weights have to come from the very
+    scores that the rows' sums were made of. Allowed is what test_weights_are_not_off_to_one_side allows, and per row the
+    difference of two references and of a score and one, each rounded to 2^-24 of itself where scores are small beside
+    them: exact otherwise."""
+    context, r = base + tokens, tokens * qh // H
+    side = Side(ctx, (1, 1, H, hd, context), [context], base + hd, track=True)
+    side.bases = [base]
+    side.send()
+    q = (side.rng.standard_normal((tokens, qh * hd)) * scale).astype(np.float32)
+    side.dev.attention(0, ctx.array(q), ctx.zeros(q.nbytes), qh, tokens=tokens, decay=0.0)
+    got = side.dev.weights.download(np.float32).reshape(H, context).astype(np.float64)
+    assert got.min() >= 0 and got.max() <= r * (1 + 1e-6)
+    assert abs(got.sum(-1) / r - 1).max() < 2 * (3.7e-7 / r ** 0.5 + 2.0 ** -24)
+
+
 def test_large_and_small_weights_of_one_row(ctx):
     """One slot with nearly all the weight, thousands with 2^-14 of it each and values that add up."""
     side = Side(ctx, (1, 1, 1, 64, 4096), [0], 8, track=True)

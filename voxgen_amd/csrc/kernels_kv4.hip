@@ -21,7 +21,6 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr float kLimit = 61440.0f;   // inputs are clamped to this: o + 15 d then stays inside f16
 constexpr float kLog2e = 1.4426950408889634f;
@@ -252,11 +251,10 @@ __global__ __launch_bounds__(256) void k_kv4_advance(uint32_t *slots, uint32_t *
 }
 
 // ------------------------------------------------------------------- attention
-// A row's reference m moves when a score s exceeds it by more than kLazy. Weights are taken as
-// 2^(s - ref), ref = m - kRaise rounded: 2^7 up, so that their low f16 terms stay normal. ref is
-// never more than 8 below m, of scores of any size (to multiples of 2, 4, 8 and 16, 7 rounds to 6
-// or 8, 8, 8 and 0), which keeps a weight to 2^15, below f16's 65504.
-constexpr float kLazy = 7.0f, kRaise = 7.0f;
+// Weights are taken as 2^(s - m), of a score s and the row's reference m. m moves to kRaise below
+// a score that exceeds it by more than kMost: a weight is then at most 2^15, within f16, and the
+// largest score's at least about 2^kRaise, so that the low f16 terms of lesser ones stay normal.
+constexpr float kMost = 15.0f, kRaise = 7.0f;
 
 constexpr uint32_t kMaxSplits = 256;
 
@@ -267,8 +265,8 @@ struct AttnArgs {
     uint32_t tile_rows, splits, per; // rows of a tile, key splits of the grid, blocks of one
     bool eager;                      // a wave's first block is fetched before it is known whether slots fill it
     float *ml, *acc;                 // [unit][split][tile rows][2], [..][tile rows][HD]
-    f2 *norm;                        // [sequence x KV head][rows]: what a weight is taken from, see norm_of
-    // for the weights of prompts: the query rows as operands [sequence x KV head][32 rows][HD / 16][hi, lo][64],
+    f2 *norm;                        // [sequence x KV head][rows]: see norm_of
+    // for the weights of prompts: the query rows as operands [sequence x KV head][16 rows][HD / 32][hi, lo][64],
     // the factors of their scores [sequence x KV head][rows], sums by row split [split][sequence x KV head][slots]
     h8 *qp;
     float *factors, *sums;
@@ -347,12 +345,12 @@ __device__ __forceinline__ void two_terms(const float *v, float minus, h8 &hi, h
     lo = join8(r);
 }
 
-// What gives a row's softmax weight of a score s: 2^(s - ref) / sum. Kept as the two, not as
-// the logarithm of one number: that rounds to 2^-21 at the usual 8 to 16, v_log_f32 errs to one
-// side by as much, and every weight of the row was 3e-7 to 6e-7 too large by it. A row that is
-// NaN has that in ref, so that a score of -inf still weighs nothing.
-__device__ __forceinline__ f2 norm_of(float top, float sum) {
-    return sum == sum ? f2{top - kRaise, 1.0f / sum} : f2{__builtin_nanf(""), 1.0f};
+// What gives a row's softmax weight of a score s: 2^(s - m) / sum. Kept as the two, not as the
+// logarithm of one number: that rounds to 2^-21 at the usual 8 to 16, v_log_f32 errs to one side
+// by as much, and every weight of the row was 3e-7 to 6e-7 too large by it. A row that is NaN has
+// that in m, so that a score of -inf still weighs nothing.
+__device__ __forceinline__ f2 norm_of(float m, float sum) {
+    return sum == sum ? f2{m, 1.0f / sum} : f2{__builtin_nanf(""), 1.0f};
 }
 
 // Sixteen query rows as the B operand: lane (i, q) holds row i, dimensions q HD / 4 + 8 u
@@ -499,15 +497,14 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
     h8 qh[U], ql[U];
     float factor[NT];
     h8 *const qs = reinterpret_cast<h8 *>(lds);   // [NT][U][hi, lo][64]
-    // The weights' kernel reads the operands again, in its own order: a half of one of its tiles.
+    // The weights' kernel reads the operands again: a half of one of its tiles.
     auto leave = [&](uint32_t half, uint32_t row, float f) {
         const size_t pair = (size_t)s * p.a.g.kv_heads + head;
-        h8 *const to = p.qp + (pair * p.qtiles + half / 2u) * (HD / 16) * 128u;
+        h8 *const to = p.qp + (pair * p.qtiles * 2u + half) * U * 128u + lane;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const uint32_t d8 = q * U + u, at = (d8 / 2u * 2u) * 64u + d8 % 2u * 32u + half % 2u * 16u + i;
-            to[at] = qh[u];
-            to[at + 64u] = ql[u];
+            to[u * 128u] = qh[u];
+            to[u * 128u + 64u] = ql[u];
         }
         if (q == 0 && row < rows) p.factors[pair * rows + row] = f;
     };
@@ -606,12 +603,12 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
 #pragma unroll
             for (int e = 1; e < 8; ++e) top[c] = fmaxf(top[c], x[c][e / 4][e % 4]);
             top[c] *= factor[c];
-            moves = moves || top[c] - m[c] > kLazy;
+            moves = moves || top[c] - m[c] > kMost;
         }
         if (__builtin_expect(__any(moves), 0)) {
 #pragma unroll
             for (int c = 0; c < NT; ++c) {
-                const float t = row_max(top[c]), mn = t - m[c] > kLazy ? t : m[c];
+                const float t = row_max(top[c]), mn = t - m[c] > kMost ? t - kRaise : m[c];
                 const float alpha = mn == m[c] ? 1.f : __builtin_amdgcn_exp2f(m[c] - mn);
                 m[c] = mn;
                 l[c] *= alpha;
@@ -623,7 +620,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
             // A row that attends to nothing of the blocks so far has no reference yet; any serves.
-            const float ref = (m[c] == -INFINITY ? 0.f : m[c]) - kRaise;
+            const float ref = m[c] == -INFINITY ? 0.f : m[c];
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -826,8 +823,6 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-__device__ __forceinline__ f16v mfma32(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-
 // The splits of a row, joined: a workgroup a row, its lanes HD / 4 columns by as many
 // splits at once as fit.
 constexpr uint32_t kFewSplits = 8;
@@ -987,14 +982,23 @@ __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_
     h8 qh[U], ql[U];
     const float factor = qr.split(qh, ql);
     const bool valid = i < p.rows && sp.base + t < p.a.g.context;
-    f4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    // The scores to the bit: of up to eight rows the terms' products are summed apart (PK).
+    f4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, y[2] = {x[0], x[1]};
+    auto scores = [&](f4 *low) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const h8 k0 = kf.value(masks, 0, u), k1 = kf.value(masks, 1, u);
-        x[0] = mfma16(k0, qh[u], x[0]);
-        x[1] = mfma16(k1, qh[u], x[1]);
-        x[0] = mfma16(k0, ql[u], x[0]);
-        x[1] = mfma16(k1, ql[u], x[1]);
+        for (int u = 0; u < U; ++u) {
+            const h8 k0 = kf.value(masks, 0, u), k1 = kf.value(masks, 1, u);
+            x[0] = mfma16(k0, qh[u], x[0]);
+            x[1] = mfma16(k1, qh[u], x[1]);
+            low[0] = mfma16(k0, ql[u], low[0]);
+            low[1] = mfma16(k1, ql[u], low[1]);
+        }
+    };
+    if (p.rows <= 8u) {
+        scores(y);
+        x[0] += y[0], x[1] += y[1];
+    } else {
+        scores(x);
     }
     float sum = 0.f;
 #pragma unroll
@@ -1022,18 +1026,20 @@ __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs p, uint32_t joins) 
 }
 
 // Weights of more rows, from the scores once more: the sum over rows needs each row's final
-// sum. A workgroup takes 256 slots, 64 a wave, whose values it makes once and keeps in
-// registers, over every row_splits-th tile of 32 rows. The tiles' operands, left by the
-// attention kernel, pass through LDS, the next on its way while one is multiplied. A lane sums
-// its slots over its row of each tile; the sums over the row splits are added by
-// k_kv4_add_weights, in order, so that they do not vary. Bound by the matrix pipes and the
-// exponentials between them: 1024 tokens over 8024 slots 72 us, 870 TFLOP/s of products.
+// sum. The products are those of k_kv4_attn, operands and order alike, so that the scores are the
+// very ones that the sum was made of: large ones round by more than their weights allow. A
+// workgroup takes 256 slots, 64 a wave, whose values it makes once and keeps in registers, over
+// every row_splits-th tile of 32 rows. The tiles' operands, left by the attention kernel, pass
+// through LDS, the next on its way while one is multiplied. A lane sums its slots over its two
+// rows of each tile; the sums over the row splits are added by k_kv4_add_weights, in order, so
+// that they do not vary. Bound by the matrix pipes and the exponentials between them: 1024 tokens
+// over 8024 slots 72 us, 870 TFLOP/s of products.
 template <int HD>
 __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
     using L = Lay<HD>;
-    constexpr int S = HD / 16, TILE = S * 128, PER = TILE / 256;   // h8 of a tile; a lane's share
+    constexpr int U = HD / 32, TILE = U * 256, PER = TILE / 256;   // h8 of a tile; a lane's share
     __shared__ __attribute__((aligned(16))) h8 qs[2][TILE];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, j = lane & 31u, h = lane >> 5;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
     const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t chunk = blockIdx.x / p.row_splits, part = blockIdx.x % p.row_splits;
     const uint32_t head = blockIdx.y, s = blockIdx.z, seq = p.a.first + s;
@@ -1044,18 +1050,17 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
     const size_t pair = (size_t)s * p.a.g.kv_heads + head;
     const uint32_t b0 = chunk * 8u + 2u * w, blocks = (keys + 31u) / 32u;
     const uint8_t *const kp = p.a.kc + plane_of(p.a.g, p.a.layer, seq, head) * plane_bytes<HD>(p.a.g);
-    h8 k[2][S];
+    h8 k[2][2][U];   // of the wave's blocks; one behind the last: not stored below
     {
         const Masks masks;
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {   // slot j in row j; a block behind the last: not stored below
-            const uint8_t *const kb = kp + (size_t)min(b0 + v, blocks - 1u) * L::BLOCK;
+        for (int v = 0; v < 2; ++v) {
+            KFrag<HD> kf;
+            kf.load(kp + (size_t)min(b0 + v, blocks - 1u) * L::BLOCK, i, q);
 #pragma unroll
-            for (int u = 0; u < S; ++u) {
-                const uint32_t word = reinterpret_cast<const uint32_t *>(kb)[j * (HD / 8) + 2u * u + h];
-                const h2 sc = __builtin_bit_cast(h2, reinterpret_cast<const uint32_t *>(kb + L::CODES)[j * L::G + u / 2]);
-                k[v][u] = values8(masks, word, h2{sc[0], sc[0]}, h2{sc[1], sc[1]});
-            }
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int u = 0; u < U; ++u) k[v][tt][u] = kf.value(masks, tt, u);
         }
     }
     // row tiles from the first that attends to a slot of the chunk
@@ -1067,16 +1072,12 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
     const float *const factors = p.factors + pair * p.rows;
     const f2 *const norms = p.norm + pair * p.rows;
     h8 next[PER];
-    float sum[2][16];
+    float sum[2][8];   // of slots 8 q + e of the wave's blocks
 #pragma unroll
-    for (int r = 0; r < 16; ++r) sum[0][r] = sum[1][r] = 0.f;
+    for (int e = 0; e < 8; ++e) sum[0][e] = sum[1][e] = 0.f;
     auto fetch = [&](uint32_t from) {
 #pragma unroll
-        for (int n = 0; n < PER; ++n) {
-            // of an odd number of 16-row tiles, the last tile's second half was not left
-            const h8 v = src[(size_t)from * TILE + n * 256u + tid];
-            next[n] = from * 32u + (tid & 16u) < p.rows ? v : h8{};
-        }
+        for (int n = 0; n < PER; ++n) next[n] = src[(size_t)from * TILE + n * 256u + tid];
     };
     if (tile < tiles) fetch(tile);
     for (uint32_t turn = 0; tile < tiles; tile += p.row_splits, turn ^= 1u) {
@@ -1084,60 +1085,77 @@ __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
 #pragma unroll
         for (int n = 0; n < PER; ++n) qs[turn][n * 256u + tid] = next[n];
         if (tile + p.row_splits < tiles) fetch(tile + p.row_splits);
-        const uint32_t row = tile * 32u + j, at = min(row, live - 1u);
-        const uint32_t end = row < live ? base + token_of(p, row) + 1u : 0u;   // of the slots that the row attends to
-        const float factor = factors[at];
-        const f2 norm = norms[at];
+        uint32_t end[2];   // of the slots that the lane's rows attend to
+        float factor[2];
+        f2 norm[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const uint32_t row = tile * 32u + 16u * c + i, at = min(row, live - 1u);
+            end[c] = row < live ? base + token_of(p, row) + 1u : 0u;
+            factor[c] = factors[at];
+            norm[c] = norms[at];
+        }
         const bool edge = (b0 + 2u) * 32u > base + token_of(p, tile * 32u) + 1u || tile * 32u + 32u > live;
         lds_barrier();
         const h8 *const from = qs[turn] + lane;
-        f16v x[2] = {};
+        f4 x[2][2][2];   // [column tile][block][row tile]
 #pragma unroll
-        for (int u = 0; u < S; ++u) {
-            const h8 hi = from[u * 128], lo = from[u * 128 + 64];
-            x[0] = mfma32(k[0][u], hi, x[0]);
-            x[1] = mfma32(k[1][u], hi, x[1]);
-            x[0] = mfma32(k[0][u], lo, x[0]);
-            x[1] = mfma32(k[1][u], lo, x[1]);
-        }
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int v = 0; v < 2; ++v)
+            for (int v = 0; v < 2; ++v) x[c][v][0] = x[c][v][1] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[v][r] = __builtin_fmaf(x[v][r], factor, -norm[0]);
-        // What a row does not attend to is 2^-inf whatever the row holds.
-        if (edge) {
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int term = 0; term < 2; ++term) {
+                const h8 q0 = from[u * 128 + term * 64], q1 = from[(U + u) * 128 + term * 64];
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int tt = 0; tt < 2; ++tt) {
+                        x[0][v][tt] = mfma16(k[v][tt][u], q0, x[0][v][tt]);
+                        x[1][v][tt] = mfma16(k[v][tt][u], q1, x[1][v][tt]);
+                    }
+            }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int v = 0; v < 2; ++v)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    x[v][r] = (b0 + v) * 32u + 8u * (r / 4) + 4u * h + r % 4 >= end ? -INFINITY : x[v][r];
+                for (int e = 0; e < 8; ++e)
+                    x[c][v][e / 4][e % 4] = __builtin_fmaf(x[c][v][e / 4][e % 4], factor[c], -norm[c][0]);
+        // What a row does not attend to is 2^-inf whatever the row holds.
+        if (edge) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int v = 0; v < 2; ++v)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        x[c][v][e / 4][e % 4] = (b0 + v) * 32u + 8u * q + e >= end[c] ? -INFINITY : x[c][v][e / 4][e % 4];
         }
 #pragma unroll
-        for (int v = 0; v < 2; ++v)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum[v][r] = __builtin_fmaf(__builtin_amdgcn_exp2f(x[v][r]), norm[1], sum[v][r]);
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    sum[v][e] = __builtin_fmaf(__builtin_amdgcn_exp2f(x[c][v][e / 4][e % 4]), norm[c][1], sum[v][e]);
     }
-    // The sums of 256 slots through LDS, so that a lane stores its own slot's.
-    __syncthreads();
-    float *const mine = reinterpret_cast<float *>(&qs[0][0]) + w * 64u;
+    // Lane (i, q) stores the sum of slot 8 q + i % 8 of block i / 8.
+    float mine = 0.f;
 #pragma unroll
     for (int v = 0; v < 2; ++v)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            float y = sum16(sum[v][r]);   // and the other 16 rows of the half
-            const uint32_t bits = __builtin_bit_cast(uint32_t, y);
-            const auto t = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
-            y = __builtin_bit_cast(float, (uint32_t)t[0]) + __builtin_bit_cast(float, (uint32_t)t[1]);
-            if (j == (uint32_t)r) mine[v * 32 + 8 * (r / 4) + r % 4 + 4u * h] = y;
+        for (int e = 0; e < 8; ++e) {
+            const float y = sum16(sum[v][e]);
+            mine = i == (uint32_t)(8 * v + e) ? y : mine;
         }
-    __syncthreads();
-    const uint32_t slot = chunk * 256u + tid;
+    const uint32_t slot = (b0 + i / 8u) * 32u + 8u * q + i % 8u;
     if (slot >= keys) return;
-    const float y = mine[lane];
     if (p.row_splits > 1u)
-        p.sums[((size_t)part * gridDim.y * gridDim.z + pair) * p.slots32 + slot] = y;
+        p.sums[((size_t)part * gridDim.y * gridDim.z + pair) * p.slots32 + slot] = mine;
     else
-        add_weight(p.a.weights + plane_of(p.a.g, p.a.layer, seq, head) * p.a.g.context, slot, base, p.a.decay, y);
+        add_weight(p.a.weights + plane_of(p.a.g, p.a.layer, seq, head) * p.a.g.context, slot, base, p.a.decay, mine);
 }
 
 __global__ __launch_bounds__(256) void k_kv4_add_weights(AttnArgs p) {
