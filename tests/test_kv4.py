@@ -254,3 +254,41 @@ for call in (lambda: store(row_push()), lambda: load(row_push()), lambda: attn(a
     fake.hipGetDevice(C.byref(now))
     assert now.value == 1 and fake.astray_launches() == 0
 """)
+
+
+ROOMY = """
+#define __HIP_PLATFORM_AMD__ 1
+#include <hip/hip_runtime_api.h>
+#include <stdlib.h>
+hipError_t hipMalloc(void **p, size_t n) { *p = malloc(n < 1 << 20 ? n : 4096); return hipSuccess; }   /* nothing touches it */
+"""
+
+
+def test_rows_whose_end_passes_64_bits_are_refused(fake, tmp_path):  # noqa: F811
+    """More than 2^30 rows in caches that a card holds (43 GB each), of a stride for which the bytes of the rows, taken
+    modulo 2^64, would fit a buffer of 4 GB."""
+    source, library = tmp_path / "roomy.c", tmp_path / "libroomy.so"
+    source.write_text(ROOMY)
+    subprocess.run(["gcc", "-std=gnu11", "-O1", "-w", "-shared", "-fPIC", "-I", str(HIP_INCLUDE), str(source),
+                    "-Wl,--no-as-needed", str(fake),
+                    f"-Wl,-rpath,{fake.parent}", "-o", str(library)], check=True)
+    child(library, REFUSALS + """
+g = dict(layers=1, sequences=257, kv_heads=1, head_dim=64, context=1 << 22)
+nbytes = lib.vx_kv4_cache_bytes(C.byref(abi.Kv4Geom(*g.values())))
+kc, vc, slots = ctx.alloc(nbytes), ctx.alloc(nbytes), ctx.alloc(4 * 257)
+rows = 257 << 22
+far = -(-(1 << 62) // (rows - 1))                     # the least stride that wraps
+assert far < 1 << 32 and ((rows - 1) * far + 64) * 4 % (1 << 64) < 1 << 33
+buf, whole = ctx.alloc(1 << 33), ctx.alloc(rows * 64 * 4)
+near = dict(n_sequences=257, tokens=1 << 22, k_stride=64, v_stride=64, **g)
+for call in (store, load):
+    kw = dict(kc=kc, vc=vc, slots=slots)
+    for name, at in (("k_stride", dict(k=buf, v=whole)), ("v_stride", dict(k=whole, v=buf))):
+        for stride in (far, 4294967295):
+            assert call(row_push(**dict(near, **{name: stride})), **kw, **at, **({} if call is load else dict(pos=None, sp=None))) == "VX_ERR_BOUNDS"
+near = dict(n_sequences=257, tokens=1 << 22, q_heads=1, q_stride=64, out_stride=64, **g)
+scratch = ctx.alloc(lib.vx_kv4_attention_scratch_bytes(attn_push(**near), 0))
+for name, at in (("q_stride", dict(q=buf, out=whole)), ("out_stride", dict(q=whole, out=buf))):
+    assert attn(attn_push(**dict(near, **{name: far})), **at, kc=kc, vc=vc, w=None, slots=slots, scratch=scratch) == "VX_ERR_BOUNDS"
+assert kernels() == 0
+""")

@@ -58,14 +58,16 @@ int check_call(const vx_kv4_geom &g, uint32_t layer, uint32_t first, uint32_t n,
     return VX_OK;
 }
 
-// The end, in floats, of `rows` rows of `width` at `base`.
+// The end, in bytes, of `rows` rows of `width` floats at `base`: 2^38 rows of stride 2^32 need
+// more than 64 bits, and count as more than any buffer holds.
 uint64_t rows_end(uint64_t rows, uint32_t stride, uint32_t base, uint32_t width) {
-    return (uint64_t)base + (rows - 1u) * stride + width;
+    const unsigned __int128 end = ((unsigned __int128)(rows - 1u) * stride + base + width) * 4u;
+    return end >> 64 ? UINT64_MAX : (uint64_t)end;
 }
 
 int check_rows(const vx_buf *b, uint64_t rows, uint32_t stride, uint32_t base, uint32_t width, const char *what) {
     if (stride < width) return fail(VX_ERR_SHAPE, "%s: stride %u is less than a row of %u", what, stride, width);
-    return need_buf(b, rows_end(rows, stride, base, width) * 4u, what);
+    return need_buf(b, rows_end(rows, stride, base, width), what);
 }
 
 bool aligned(uint32_t stride, uint32_t base) { return stride % 4u == 0 && base % 4u == 0; }
@@ -78,10 +80,10 @@ int check_caches(const vx_kv4_geom &g, const vx_buf *k_cache, const vx_buf *v_ca
     return VX_OK;
 }
 
-// Whether ranges [a, a_end) and [b, b_end) floats of two buffers share memory.
+// Whether ranges [a, a_end) and [b, b_end) bytes of two buffers share memory.
 bool overlap(const vx_buf *x, uint64_t a, uint64_t a_end, const vx_buf *y, uint64_t b, uint64_t b_end) {
     const char *p = static_cast<const char *>(x->ptr), *q = static_cast<const char *>(y->ptr);
-    return p + 4u * a < q + 4u * b_end && q + 4u * b < p + 4u * a_end;
+    return p + a < q + b_end && q + b < p + a_end;
 }
 
 int rows_call(vx_ctx *ctx, const vx_kv4_rows_push *pc, const vx_buf *slots, const char *what, Kv4Rows *l) {
@@ -246,7 +248,7 @@ int vx_kv4_attention(vx_ctx *ctx, const vx_buf *q, const vx_buf *k_cache, const 
     Kv4Attn l = attn_launch(pc);
     VX_CHECK(need_buf(scratch, kv4_attn_scratch_bytes(l, weights != nullptr), "vx_kv4_attention scratch"));
     // Other workgroups still read q when a row of out is written.
-    if (overlap(q, pc->q_base, rows_end(rows, pc->q_stride, pc->q_base, width), out, pc->out_base,
+    if (overlap(q, 4ull * pc->q_base, rows_end(rows, pc->q_stride, pc->q_base, width), out, 4ull * pc->out_base,
                 rows_end(rows, pc->out_stride, pc->out_base, width)))
         return fail(VX_ERR_INVALID_ARG, "vx_kv4_attention: q and out overlap");
     for (const vx_buf *b : {q, k_cache, v_cache, slots, static_cast<const vx_buf *>(out)})
