@@ -503,7 +503,10 @@ int vx_fused_rms_swiglu(vx_ctx *ctx, const vx_model *model, const vx_buf *hidden
 /* token whose slot is not below context. Nothing outside the cache is read or */
 /* written for any content of a device buffer. Calls on one context are in     */
 /* order; two calls that overlap (other contexts, replayed graphs) need caches */
-/* and scratch of their own.                                                   */
+/* and scratch of their own. A buffer that a call writes may share no memory   */
+/* with another of the call, but rows (q and out of vx_kv4_attention, k and v  */
+/* of vx_kv4_load) may be parts of one buffer: one behind the other, or of one */
+/* stride and side by side. K and V cache are two buffers always.              */
 /* ------------------------------------------------------------------------- */
 #define VX_KV4_NO_SLOT 4294967295u
 typedef struct vx_kv4_geom {
@@ -545,8 +548,7 @@ typedef struct vx_kv4_attention_push {
     float decay;                    /* of the accumulated weights, 0..1 */
 } vx_kv4_attention_push;
 /* Scratch of one call; 0 for a push that is not valid. What it holds before the
- * call does not matter. No buffer may be bound twice, but q and out may be parts of
- * one that do not overlap. */
+ * call does not matter. */
 uint64_t vx_kv4_attention_scratch_bytes(const vx_kv4_attention_push *pc, uint32_t with_weights);
 /* out = softmax(q . K / sqrt(head_dim)) . V over the slots each row attends to, in
  * f32 (products on the matrix cores, q and the weights as two f16 terms each, sums

@@ -146,6 +146,26 @@ def test_store_of_special_values(ctx):
     assert np.isnan(back.download(np.float32).reshape(x.shape)[7]).sum() == 32
 
 
+def test_rows_side_by_side_in_one_buffer(ctx):
+    """k and v, and q and out, as the halves of rows of one buffer: what they give in buffers of their own."""
+    hd, H, qh, tokens, context = 128, 2, 8, 37, 64
+    rng, width, wide = np.random.default_rng(13), H * hd, qh * hd
+    cache = Kv4Cache(ctx, 1, 1, H, hd, context)
+    kv = rows_of(rng, tokens, 2 * width)
+    both = ctx.array(kv)
+    cache.store(0, both, both, tokens=tokens, k_stride=2 * width, v_stride=2 * width, v_base=width)
+    back = ctx.zeros(kv.nbytes)
+    cache.load(0, back, back, tokens=tokens, k_stride=2 * width, v_stride=2 * width, v_base=width)
+    assert np.array_equal(back.download(np.float32).reshape(tokens, 2 * H, hd), kv4ref.stored(kv.reshape(tokens, 2 * H, hd)))
+    q = rng.standard_normal((tokens, wide)).astype(np.float32)
+    out = ctx.zeros(q.nbytes)
+    cache.attention(0, ctx.array(q), out, qh, tokens=tokens)
+    rows = ctx.array(np.concatenate([q, np.zeros_like(q)], 1))
+    cache.attention(0, rows, rows, qh, tokens=tokens, q_stride=2 * wide, out_stride=2 * wide, out_base=wide)
+    got = rows.download(np.float32).reshape(tokens, 2, wide)
+    assert np.array_equal(got[:, 0], q) and np.array_equal(got[:, 1], out.download(np.float32).reshape(tokens, wide))
+
+
 def test_advance(ctx):
     slots, pos = ctx.array(np.array([0, 5, NO_SLOT, 38, 40, 99], np.uint32)), ctx.array(np.arange(6, dtype=np.uint32) * 100)
     abi.call("vx_kv4_advance", ctx.handle, slots.handle, pos.handle, 1, 5, 3, 40)

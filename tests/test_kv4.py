@@ -200,6 +200,43 @@ assert lib.vx_kv4_plan_bytes(None) == 0
 """)
 
 
+def test_a_written_buffer_is_bound_once(fake):  # noqa: F811
+    """Every pair of a buffer that a call writes and another of the call; rows side by side in one buffer are two."""
+    child(fake, REFUSALS + """
+one = ctx.alloc(1 << 20)
+def pairs(call, push, written, read, rows=()):
+    for a in written:
+        for b in [n for n in written if n != a] + list(read):
+            if {a, b} != set(rows):
+                assert call(push(), **{a: one, b: one}) == "VX_ERR_INVALID_ARG", (call, a, b)
+pairs(store, row_push, ("kc", "vc", "sp"), ("k", "v", "slots", "pos"))
+pairs(load, row_push, ("k", "v"), ("kc", "vc", "slots"), rows=("k", "v"))
+scratch = ctx.alloc(1 << 20)
+pairs(lambda pc, **kw: attn(pc, **dict(dict(scratch=scratch), **kw)), attn_push, ("out", "w", "scratch"),
+      ("q", "kc", "vc", "slots"), rows=("q", "out"))
+pairs(select, evict_push, ("plan",), ("w", "sp", "slots"))
+pairs(compact, evict_push, ("kc", "vc", "w", "sp", "slots"), ("plan",))
+assert kernels() == 0
+# k and v, or q and out, in rows of one buffer: of one stride side by side, or one behind the other
+def row_pairs(call, push, width, rows, names):
+    buf, launched = ctx.alloc(3 * rows * width * 4), kernels()
+    s, b = [n + "_stride" for n in names], [n + "_base" for n in names]
+    def run(*v):
+        return call(push(**dict(zip(s + b, v))), **{n: buf for n in names})
+    w = width
+    for ok, v in ((True, (2 * w, 2 * w, 0, w)), (True, (2 * w, 2 * w, w, 0)), (True, (2 * w + 4, 2 * w + 4, 3, w + 5)),
+                  (True, (w, w, 0, rows * w)), (True, (w, 2 * w, 0, rows * w)), (True, (2 * w, 2 * w, 0, 3 * w)),
+                  (False, (2 * w, 2 * w, 0, w - 1)), (False, (2 * w, 2 * w, 0, w + 1)), (False, (2 * w, 2 * w, 1, 0)),
+                  (False, (2 * w, 2 * w, 2 * w, 0)), (False, (w, w, 0, 0)), (False, (w, w, 0, w)),
+                  (False, (w, w, 0, rows * w - 1)), (False, (w, 2 * w, 0, w))):
+        assert run(*v) == ("VX_OK" if ok else "VX_ERR_INVALID_ARG"), (call, v)
+    return kernels() - launched
+assert row_pairs(load, row_push, 256, 6, ("k", "v")) == 6
+row_pairs(lambda pc, **kw: attn(pc, scratch=scratch, w=None, **kw), attn_push, 1024, 6, ("q", "out"))
+assert store(row_push(), k=one, v=one) == "VX_OK" and store(row_push(), pos=slots) == "VX_OK"     # read twice
+""")
+
+
 def test_python_class_checks_and_keeps_its_pushes(fake):  # noqa: F811
     child(fake, REFUSALS + """
 assert refused(Kv4Cache, ctx, 1, 1, 1, 96, 8) == "VX_ERR_SHAPE"

@@ -1,6 +1,9 @@
 // C ABI of the 4-bit KV cache: argument checks and launches (kernels_kv4.hip). Every
 // call checks its push and the bound buffers before it enqueues anything; what device
 // buffers hold (slot counts, positions, a plan) is bounded by the kernels themselves.
+#include <algorithm>
+#include <initializer_list>
+
 #include "kv4.h"
 
 using namespace vx;
@@ -80,10 +83,38 @@ int check_caches(const vx_kv4_geom &g, const vx_buf *k_cache, const vx_buf *v_ca
     return VX_OK;
 }
 
-// Whether ranges [a, a_end) and [b, b_end) bytes of two buffers share memory.
+// Bytes [a, a_end) of one buffer and [b, b_end) of another share memory.
 bool overlap(const vx_buf *x, uint64_t a, uint64_t a_end, const vx_buf *y, uint64_t b, uint64_t b_end) {
     const char *p = static_cast<const char *>(x->ptr), *q = static_cast<const char *>(y->ptr);
     return p + a < q + b_end && q + b < p + a_end;
+}
+
+// A buffer that a call writes, nullable ones among them, may share memory with no other of it:
+// other workgroups read that, or write it.
+int check_apart(const char *what, std::initializer_list<const vx_buf *> written,
+                std::initializer_list<const vx_buf *> read) {
+    for (auto w = written.begin(); w != written.end(); ++w) {
+        if (!*w) continue;
+        auto shares = [&](const vx_buf *b) { return b && overlap(*w, 0, (*w)->bytes, b, 0, b->bytes); };
+        if (std::any_of(w + 1, written.end(), shares) || std::any_of(read.begin(), read.end(), shares))
+            return fail(VX_ERR_INVALID_ARG, "%s: a buffer that is written is bound twice", what);
+    }
+    return VX_OK;
+}
+
+// Rows of two operands, where one is written: apart as a whole, or of one stride and side by side.
+int check_rows_apart(const char *what, const vx_buf *x, uint32_t x_stride, uint32_t x_base, const vx_buf *y,
+                     uint32_t y_stride, uint32_t y_base, uint64_t rows, uint32_t width) {
+    if (!overlap(x, 4ull * x_base, rows_end(rows, x_stride, x_base, width), y, 4ull * y_base,
+                 rows_end(rows, y_stride, y_base, width)))
+        return VX_OK;
+    if (x_stride == y_stride) {
+        const int64_t stride = 4ll * x_stride, wide = 4ll * width;
+        const int64_t off = (static_cast<const char *>(y->ptr) - static_cast<const char *>(x->ptr) + 4ll * y_base - 4ll * x_base) % stride;
+        const int64_t ahead = off < 0 ? off + stride : off;   // of the next row of y from a row of x
+        if (ahead >= wide && stride - ahead >= wide) return VX_OK;
+    }
+    return fail(VX_ERR_INVALID_ARG, "%s overlap", what);
 }
 
 int rows_call(vx_ctx *ctx, const vx_kv4_rows_push *pc, const vx_buf *slots, const char *what, Kv4Rows *l) {
@@ -173,6 +204,7 @@ int vx_kv4_store(vx_ctx *ctx, const vx_buf *k, const vx_buf *v, vx_buf *k_cache,
     if (positions) VX_CHECK(need_buf(positions, (uint64_t)g.sequences * 4u, "vx_kv4_store positions"));
     if (slot_positions)
         VX_CHECK(need_buf(slot_positions, planes(g) * g.context * 4u, "vx_kv4_store slot_positions"));
+    VX_CHECK(check_apart("vx_kv4_store", {k_cache, v_cache, slot_positions}, {k, v, slots, positions}));
     l.k = static_cast<float *>(k->ptr) + pc->k_base;
     l.v = static_cast<float *>(v->ptr) + pc->v_base;
     l.kc = static_cast<uint8_t *>(k_cache->ptr);
@@ -195,6 +227,10 @@ int vx_kv4_load(vx_ctx *ctx, const vx_buf *k_cache, const vx_buf *v_cache, vx_bu
     if (k) VX_CHECK(check_rows(k, rows, pc->k_stride, pc->k_base, width, "vx_kv4_load k"));
     if (v) VX_CHECK(check_rows(v, rows, pc->v_stride, pc->v_base, width, "vx_kv4_load v"));
     VX_CHECK(check_caches(g, k_cache, v_cache, "vx_kv4_load cache"));
+    VX_CHECK(check_apart("vx_kv4_load", {k}, {k_cache, v_cache, slots}));
+    VX_CHECK(check_apart("vx_kv4_load", {v}, {k_cache, v_cache, slots}));
+    if (k && v)
+        VX_CHECK(check_rows_apart("vx_kv4_load: k and v", k, pc->k_stride, pc->k_base, v, pc->v_stride, pc->v_base, rows, width));
     if (k) l.k = static_cast<float *>(k->ptr) + pc->k_base;
     if (v) l.v = static_cast<float *>(v->ptr) + pc->v_base;
     l.kc = static_cast<uint8_t *>(k_cache->ptr);
@@ -215,7 +251,7 @@ int vx_kv4_advance(vx_ctx *ctx, vx_buf *slots, vx_buf *positions, uint32_t first
     const uint64_t bytes = ((uint64_t)first_sequence + n_sequences) * 4u;
     VX_CHECK(need_buf(slots, bytes, "vx_kv4_advance slots"));
     if (positions) VX_CHECK(need_buf(positions, bytes, "vx_kv4_advance positions"));
-    if (positions == slots) return fail(VX_ERR_INVALID_ARG, "vx_kv4_advance: slots and positions are one buffer");
+    VX_CHECK(check_apart("vx_kv4_advance", {slots, positions}, {}));
     OnDevice on(ctx->device);
     ProfSpan span(ctx, "kv4.advance");
     return launch_kv4_advance(ctx->stream, static_cast<uint32_t *>(slots->ptr) + first_sequence,
@@ -247,14 +283,10 @@ int vx_kv4_attention(vx_ctx *ctx, const vx_buf *q, const vx_buf *k_cache, const 
     if (weights) VX_CHECK(need_buf(weights, planes(g) * g.context * 4u, "vx_kv4_attention weights"));
     Kv4Attn l = attn_launch(pc);
     VX_CHECK(need_buf(scratch, kv4_attn_scratch_bytes(l, weights != nullptr), "vx_kv4_attention scratch"));
-    // Other workgroups still read q when a row of out is written.
-    if (overlap(q, 4ull * pc->q_base, rows_end(rows, pc->q_stride, pc->q_base, width), out, 4ull * pc->out_base,
-                rows_end(rows, pc->out_stride, pc->out_base, width)))
-        return fail(VX_ERR_INVALID_ARG, "vx_kv4_attention: q and out overlap");
-    for (const vx_buf *b : {q, k_cache, v_cache, slots, static_cast<const vx_buf *>(out)})
-        if (b == scratch || b == weights)
-            return fail(VX_ERR_INVALID_ARG, "vx_kv4_attention: one buffer is bound twice");
-    if (weights == scratch) return fail(VX_ERR_INVALID_ARG, "vx_kv4_attention: weights and scratch are one buffer");
+    VX_CHECK(check_apart("vx_kv4_attention", {out, weights, scratch}, {k_cache, v_cache, slots}));
+    VX_CHECK(check_apart("vx_kv4_attention", {weights, scratch}, {q}));
+    VX_CHECK(check_rows_apart("vx_kv4_attention: q and out", q, pc->q_stride, pc->q_base, out, pc->out_stride, pc->out_base,
+                              rows, width));
     l.q = static_cast<const float *>(q->ptr) + pc->q_base;
     l.kc = static_cast<const uint8_t *>(k_cache->ptr);
     l.vc = static_cast<const uint8_t *>(v_cache->ptr);
@@ -284,8 +316,7 @@ int vx_kv4_select(vx_ctx *ctx, const vx_buf *weights, const vx_buf *slot_positio
     VX_CHECK(need_buf(slot_positions, table, "vx_kv4_select slot_positions"));
     VX_CHECK(need_buf(slots, (uint64_t)l.g.sequences * 4u, "vx_kv4_select slots"));
     VX_CHECK(need_buf(plan, plan_bytes(l), "vx_kv4_select plan"));
-    if (plan == weights || plan == slot_positions || plan == slots)
-        return fail(VX_ERR_INVALID_ARG, "vx_kv4_select: the plan is another buffer of the call");
+    VX_CHECK(check_apart("vx_kv4_select", {plan}, {weights, slot_positions, slots}));
     l.weights = static_cast<float *>(weights->ptr);
     l.slot_positions = static_cast<uint32_t *>(slot_positions->ptr);
     l.slots = static_cast<uint32_t *>(slots->ptr);
@@ -305,9 +336,8 @@ int vx_kv4_compact(vx_ctx *ctx, const vx_buf *plan, vx_buf *k_cache, vx_buf *v_c
     if (k_cache || v_cache) VX_CHECK(check_caches(l.g, k_cache, v_cache, "vx_kv4_compact cache"));
     if (weights) VX_CHECK(need_buf(weights, table, "vx_kv4_compact weights"));
     if (slot_positions) VX_CHECK(need_buf(slot_positions, table, "vx_kv4_compact slot_positions"));
-    if (weights && weights == slot_positions)
-        return fail(VX_ERR_INVALID_ARG, "vx_kv4_compact: weights and slot_positions are one buffer");
     VX_CHECK(need_buf(slots, (uint64_t)l.g.sequences * 4u, "vx_kv4_compact slots"));
+    VX_CHECK(check_apart("vx_kv4_compact", {k_cache, v_cache, weights, slot_positions, slots}, {plan}));
     l.plan_in = static_cast<const uint32_t *>(plan->ptr);
     l.kc = k_cache ? static_cast<uint8_t *>(k_cache->ptr) : nullptr;
     l.vc = v_cache ? static_cast<uint8_t *>(v_cache->ptr) : nullptr;
