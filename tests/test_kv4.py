@@ -259,6 +259,32 @@ assert len(c._pushes) == before
 """)
 
 
+def test_scratch_that_grows_stays_bounded(fake):  # noqa: F811
+    """Calls of every length: the scratches that are kept for graphs are together no larger than the one in use, and that
+    is at most twice what the largest call needs; exactly that where no more can be had, and nothing is lost to a call
+    that fails for want of memory."""
+    child(fake, REFUSALS + """
+c = Kv4Cache(ctx, 1, 1, 2, 128, 2048, track=True)
+q, out = ctx.alloc(2048 * 2048 * 4), ctx.alloc(2048 * 2048 * 4)
+push = lambda t: attn_push(layers=1, sequences=1, context=2048, n_sequences=1, tokens=t, q_heads=16, q_stride=2048, out_stride=2048)
+need = lambda t: lib.vx_kv4_attention_scratch_bytes(push(t), 1)
+largest = 0
+for t in range(20, 1500):
+    c.attention(0, q, out, 16, tokens=t)
+    largest = max(largest, need(t))
+    assert largest <= c._scratch.nbytes <= 2 * largest
+    assert sum(b.nbytes for b in c._outgrown) <= c._scratch.nbytes
+kept = [b.handle for b in c._outgrown]
+now = c._scratch.nbytes
+t = next(t for t in range(1500, 2049) if need(t) > now)
+refuse(need(t), 1 << 40)
+assert refused(c.attention, 0, q, out, 16, t) == "VX_ERR_OOM"
+assert c._scratch.nbytes == now and [b.handle for b in c._outgrown] == kept
+refuse(2 * now, 1 << 40)
+assert refused(c.attention, 0, q, out, 16, t) == "VX_OK" and c._scratch.nbytes == need(t)
+""")
+
+
 TWO_DEVICES = """
 #define __HIP_PLATFORM_AMD__ 1
 #include <hip/hip_runtime_api.h>

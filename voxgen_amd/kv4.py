@@ -136,10 +136,18 @@ class Kv4Cache:
         return self._keep(key, (C.byref(pc), abi.load().vx_kv4_attention_scratch_bytes(pc, 1 if self.track else 0)))
 
     def _grow(self, nbytes: int) -> Buffer:
-        """The cache's own scratch, larger. The smaller one stays allocated: a captured graph may hold it."""
-        if self._scratch is not None:
-            self._outgrown.append(self._scratch)
-        self._scratch = self.ctx.alloc(max(4, nbytes))
+        """The cache's own scratch, larger. The smaller one stays allocated: a captured graph may hold it. Twice the size,
+        where there is room: all that stay are then no more than the one in use."""
+        old = self._scratch
+        double = 2 * old.nbytes if old is not None else 0
+        try:
+            self._scratch = self.ctx.alloc(max(4, nbytes, double))
+        except abi.VxError as e:
+            if e.name != "VX_ERR_OOM" or double <= nbytes:
+                raise
+            self._scratch = self.ctx.alloc(nbytes)
+        if old is not None:
+            self._outgrown.append(old)
         return self._scratch
 
     def plan_moves(self, keep: int) -> int:
