@@ -298,6 +298,55 @@ def test_long_caches(ctx, hd, qh, H, tokens, bases, context, track, pad):
     attend(side, 0, tokens, qh, pad=pad, base=pad, decay=1.0)
 
 
+@pytest.mark.parametrize("hd,qh,H,tokens,S,context", [
+    # tiles of 32 rows of every head size, over one split of the slots and over several
+    (256, 16, 1, 100, 1, 1104), (256, 16, 1, 300, 1, 320), (256, 12, 2, 131, 2, 840), (64, 16, 2, 200, 1, 1710),
+    (64, 16, 2, 301, 1, 900), (64, 12, 3, 170, 2, 2075), (128, 16, 2, 140, 1, 1000), (128, 16, 2, 150, 1, 1155),
+    # weights that need no second launch, because there are many slots or few rows
+    (64, 1, 1, 1, 1, 1), (128, 32, 1, 1, 1, 1), (128, 1, 1, 17, 1, 700), (256, 1, 1, 17, 1, 400), (64, 3, 3, 120, 2, 6000),
+    (64, 8, 8, 180, 3, 6000), (64, 8, 8, 600, 3, 6000), (128, 8, 8, 120, 2, 1100), (128, 8, 8, 180, 3, 6000),
+    (128, 8, 8, 600, 3, 6000), (256, 8, 8, 120, 1, 1100), (256, 8, 8, 120, 3, 400),
+    # and with it
+    (128, 8, 1, 400, 1, 700), (256, 4, 1, 33, 1, 40)])
+def test_kernels_by_size(ctx, hd, qh, H, tokens, S, context):
+    """Every kernel that the rules on sizes may choose (test_kv4.py looks that none is missing), with weights and without:
+    rows that vx_kv4_store has written, of sequences of unequal length."""
+    rng, group = np.random.default_rng(hd + tokens), qh // H
+    bases = [max(0, context - tokens - 45 * s) for s in range(S)]
+    k, v = rows_of(rng, S, context, H * hd), rows_of(rng, S, context, H * hd)
+    q = (rng.standard_normal((S, tokens, H, group, hd)) * 1.2).astype(np.float32)
+    old = rng.random((S, H, context)).astype(np.float32)
+    outs = []
+    for track in (False, True):
+        cache, out = Kv4Cache(ctx, 1, S, H, hd, context, track=track), ctx.zeros(q.nbytes)
+        cache.store(0, ctx.array(k), ctx.array(v), tokens=context)
+        cache.slots.upload(np.array(bases, np.uint32))
+        if track:
+            cache.weights.upload(old)
+        cache.attention(0, ctx.array(q), out, qh, tokens=tokens, decay=0.5)
+        outs.append(out.download(np.float32).reshape(q.shape))
+    weights = cache.weights.download(np.float32).reshape(old.shape)
+    for s, base in enumerate(bases):
+        n = base + tokens
+        hidden = np.arange(n) > base + np.arange(tokens)[:, None]
+        for h in range(H):
+            kk, vv = (kv4ref.stored(x[s, :n, h * hd:(h + 1) * hd]) for x in (k, v))
+            total = np.where(np.arange(n) < base, 0.5 * old[s, h, :n].astype(np.float64), 0.0)
+            for g in range(group):
+                x = q[s, :, h, g].astype(np.float64) @ kk.T / np.sqrt(hd)
+                x[hidden] = -np.inf
+                p = np.exp(x - x.max(-1, keepdims=True))
+                p /= p.sum(-1, keepdims=True)
+                want = p @ vv
+                for out in outs:
+                    off = np.linalg.norm(out[s, :, h, g] - want, axis=-1) / np.linalg.norm(want, axis=-1)
+                    assert off.max() < 4 * TOL, (s, h, g, off.argmax())
+                    assert rel_l2(out[s, :, h, g], want) < TOL
+                total += p.sum(0)
+            assert rel_l2(weights[s, h, :n], total) < TOL, (s, h)
+            assert np.array_equal(weights[s, h, n:], old[s, h, n:])
+
+
 @pytest.mark.parametrize("track", [False, True])
 @pytest.mark.parametrize("hd,qh,H,tokens,S,context", [
     (128, 8, 1, 1, 1, 512), (128, 8, 1, 1, 1, 513), (64, 24, 2, 1, 3, 4000), (128, 16, 2, 3, 2, 1500), (256, 5, 1, 17, 1, 700),

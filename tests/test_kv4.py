@@ -320,22 +320,34 @@ for call in (lambda: store(row_push()), lambda: load(row_push()), lambda: attn(a
 
 
 ROOMY = """
+#define _GNU_SOURCE
 #define __HIP_PLATFORM_AMD__ 1
 #include <hip/hip_runtime_api.h>
-#include <stdlib.h>
-hipError_t hipMalloc(void **p, size_t n) { *p = malloc(n < 1 << 20 ? n : 4096); return hipSuccess; }   /* nothing touches it */
+#include <sys/mman.h>
+hipError_t hipMalloc(void **p, size_t n) {   /* address space; nothing touches what is large */
+    *p = mmap(0, n, PROT_READ | PROT_WRITE, MAP_PRIVATE | MAP_ANONYMOUS | MAP_NORESERVE, -1, 0);
+    return *p == MAP_FAILED ? hipErrorOutOfMemory : hipSuccess;
+}
+hipError_t hipFree(void *p) { return hipSuccess; }
 """
 
 
-def test_rows_whose_end_passes_64_bits_are_refused(fake, tmp_path):  # noqa: F811
-    """More than 2^30 rows in caches that a card holds (43 GB each), of a stride for which the bytes of the rows, taken
-    modulo 2^64, would fit a buffer of 4 GB."""
-    source, library = tmp_path / "roomy.c", tmp_path / "libroomy.so"
+@pytest.fixture(scope="module")
+def roomy(fake, tmp_path_factory):  # noqa: F811
+    """The stand-in with room for buffers of any size."""
+    where = tmp_path_factory.mktemp("roomy")
+    source, library = where / "roomy.c", where / "libroomy.so"
     source.write_text(ROOMY)
     subprocess.run(["gcc", "-std=gnu11", "-O1", "-w", "-shared", "-fPIC", "-I", str(HIP_INCLUDE), str(source),
                     "-Wl,--no-as-needed", str(fake),
                     f"-Wl,-rpath,{fake.parent}", "-o", str(library)], check=True)
-    child(library, REFUSALS + """
+    return library
+
+
+def test_rows_whose_end_passes_64_bits_are_refused(roomy):
+    """More than 2^30 rows in caches that a card holds (43 GB each), of a stride for which the bytes of the rows, taken
+    modulo 2^64, would fit a buffer of 4 GB."""
+    child(roomy, REFUSALS + """
 g = dict(layers=1, sequences=257, kv_heads=1, head_dim=64, context=1 << 22)
 nbytes = lib.vx_kv4_cache_bytes(C.byref(abi.Kv4Geom(*g.values())))
 kc, vc, slots = ctx.alloc(nbytes), ctx.alloc(nbytes), ctx.alloc(4 * 257)
@@ -354,4 +366,53 @@ scratch = ctx.alloc(lib.vx_kv4_attention_scratch_bytes(attn_push(**near), 0))
 for name, at in (("q_stride", dict(q=buf, out=whole)), ("out_stride", dict(q=whole, out=buf))):
     assert attn(attn_push(**dict(near, **{name: far})), **at, kc=kc, vc=vc, w=None, slots=slots, scratch=scratch) == "VX_ERR_BOUNDS"
 assert kernels() == 0
+""")
+
+
+def test_every_kernel_has_a_case_whose_values_are_compared(roomy):
+    """The kernels of a call go by sizes. All sets of them that a sweep of sizes launches are launched by a case of the
+    GPU tests that compares values with the restatement, so that no change of a rule leaves a kernel untested."""
+    child(roomy, REFUSALS + """
+sys.path[:0] = ["tests", "oracle"]
+import test_gpu_kv4 as gpu
+names = ["k_kv4_attnILi%dELi%dELi%dELb%dE" % (hd, nt, 8 if nt > 1 else 4, pk) for hd in (64, 128, 256)
+         for nt, pk in ((1, 1), (1, 0), (2, 0), (4, 0))]
+names += [n % hd for hd in (64, 128, 256) for n in ("k_kv4_finishILi%dE", "k_kv4_weights_rowsILi%dE")] + ["k_kv4_add_weights"]
+bufs = {n: ctx.alloc(1 << 33) for n in ("q", "out", "kc", "vc", "w", "slots", "scratch")}
+def kernels_of(hd, qh, heads, tokens, S, context, track):
+    before = [launches(n) for n in names]
+    pc = abi.Kv4AttentionPush(abi.Kv4Geom(1, S, heads, hd, context), 0, 0, S, tokens, qh, qh * hd, qh * hd, 0, 0, 1.0)
+    b = dict(bufs, w=bufs["w"] if track else None)
+    assert attn(pc, **b) == "VX_OK"
+    return frozenset(n for n, c in zip(names, before) if launches(n) > c)
+def params(test):
+    marks = [m for m in test.pytestmark if m.name == "parametrize"]
+    sets = [{}]
+    for m in marks:
+        keys = m.args[0].split(",")
+        rows = [dict(zip(keys, v if len(keys) > 1 else (v,))) for v in m.args[1]]
+        sets = [dict(s, **r) for s in sets for r in rows]
+    return sets
+covered = set()
+for p in params(gpu.test_single_token):
+    covered.add(kernels_of(p["hd"], p["qh"], p["H"], 1, 1, p["base"] + 1 + p["base"] % 3, False))
+for p in params(gpu.test_several_tokens_and_prompts):
+    covered.add(kernels_of(p["hd"], p["qh"], p["H"], p["tokens"], 1, p["context"], p["track"]))
+for p in params(gpu.test_long_prompts) + params(gpu.test_long_caches):
+    covered.add(kernels_of(p["hd"], p["qh"], p["H"], p["tokens"], len(p["bases"]), p["context"], p["track"]))
+for p in params(gpu.test_kernels_by_size):
+    for track in (False, True):
+        covered.add(kernels_of(p["hd"], p["qh"], p["H"], p["tokens"], p["S"], p["context"], track))
+reached = {}
+for hd in (64, 128, 256):
+    for qh, heads in ((1, 1), (8, 1), (16, 2), (8, 8), (32, 1), (3, 3)):
+        for S in (1, 3, 16):
+            for tokens in (1, 2, 5, 9, 17, 33, 65, 120, 250, 600, 1500, 4000):
+                for context in (1, 40, 130, 400, 1000, 1100, 1600, 4100, 20000):
+                    if tokens <= context:
+                        for track in (False, True):
+                            reached.setdefault(kernels_of(hd, qh, heads, tokens, S, context, track), (hd, qh, heads, tokens, S, context, track))
+missing = [v for k, v in reached.items() if k not in covered]
+assert not missing, missing
+assert {n for k in reached for n in k} == set(n for n in names if n != "k_kv4_attnILi256ELi4ELi8ELb0E")
 """)
