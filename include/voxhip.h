@@ -557,7 +557,10 @@ uint64_t vx_kv4_attention_scratch_bytes(const vx_kv4_attention_push *pc, uint32_
  * the call may attend to, w = decay * w + the sum of the softmax weights it got
  * from the call's rows and the KV head's query heads (decay 0, or a slot the
  * call's own tokens fill: the sum alone). Other entries are left as they were. A
- * stored NaN reaches the rows that attend to its slot and no other. */
+ * stored NaN reaches the rows that attend to its slot and no other; a NaN row
+ * reaches the weights of the slots that it attends to and no other; rows that take
+ * no part may hold anything. Scores may have any size that f32 holds (a larger one
+ * makes its row NaN). */
 int vx_kv4_attention(vx_ctx *ctx, const vx_buf *q, const vx_buf *k_cache, const vx_buf *v_cache, vx_buf *out,
                      vx_buf *weights, const vx_buf *slots, vx_buf *scratch, const vx_kv4_attention_push *pc);
 

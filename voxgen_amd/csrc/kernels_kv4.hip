@@ -134,8 +134,8 @@ __device__ __forceinline__ uint32_t encode8(const float *x, _Float16 &d, _Float1
 // eight values each. K's codes go out as they are; V's are transposed through LDS, and a
 // lane then owns one dimension's dword of the octet, which it merges with the codes of
 // the octet's other slots (another call's): no dword has two writers. Bound by one launch
-// up to about a thousand tokens, then by the bytes: 2.8 us for a token of 2 KV heads of 128, 4.5
-// for 1900 (9 MB, 2.0 TB/s), 5.8 in a graph for 8192 (19 MB, 3.3 TB/s).
+// up to about a thousand tokens, then more and more by the bytes: 2.8 us for a token of 2 KV heads
+// of 128, 4.6 for 1900 (4.5 MB, 1.0 TB/s), 5.8 in a graph for 8192 (19 MB, 3.3 TB/s).
 template <int HD>
 __global__ __launch_bounds__(HD) void k_kv4_store(Kv4Rows a) {
     using L = Lay<HD>;
@@ -455,12 +455,19 @@ struct VScale {
 // PK, of at most eight rows: columns 0..7 of the products take the high terms of the rows,
 // columns 8..15 the low ones, so that one product does for both; the scores of the two
 // columns of a row are added, and so are its sums at the end.
-// What bounds it: for few rows over a short context, the instructions of one pass through the
-// kernel at one wave a SIMD (4.2 us for a single block; 7.0 for 512 slots in one split); over a
-// long one the making of the values by the VALU (16 sequences over 32768 slots, 111 MB: 34 us,
-// 3.3 TB/s where a copy reaches 4.7); for prompts the matrix pipes at the clock that the card's power limit leaves
-// them (1024 tokens over 8024 slots, 16/2 heads of 128: 136 us, 930 TFLOP/s of two-term
-// products at 1.8 GHz; a plain f16 product of 8192^3 reaches 1045).
+// What bounds it (times of calls back to back, at the clock that the card then keeps; out of idle
+// it is lower for the first hundred calls, which take a tenth longer; 16/2 heads of 128). For few
+// rows over a short context, the instructions of one pass through the kernel at one wave a SIMD
+// (4.2 us for a single block; 7.1 for 512 slots in one split). For few rows over a long one neither
+// memory nor the VALU that makes the values is used up: 16 sequences over 32768 slots, 111 MB, take
+// 34 us, 3.3 TB/s where reads reach 6.0, or 29 out of the last-level cache, with 0.62 of the VALU's
+// issue slots at 3.4 waves a SIMD; a block's V is asked for at the block's start. For prompts, the
+// issue of vector instructions: 1024 tokens over 8024 slots take 120 us, 1060 TFLOP/s of two-term
+// products (a plain f16 product of 8192^3: 1080), in which products take 0.52 and the other vector
+// instructions 0.47 of the SIMDs' cycles; with 1900 tokens (48 us) it is 0.29 and 0.44, the rest
+// going to the start of each of 476 tiles and to its waves' wait and join, while nothing else is on
+// the CU. Heads of 256 with one column tile of rows take 258 registers and more, one wave a SIMD
+// (a token over 8001 slots of one KV head: 9.4 us); two have not been tried.
 template <int HD, int NT, int W, bool PK>
 __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k_kv4_attn(AttnArgs p) {
     using L = Lay<HD>;
@@ -551,7 +558,8 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
     float minus = PK && i < 8u ? 0.0f : -1.0f;
     asm("" : "+v"(minus));
     // 0 x NaN would reach rows that do not attend to the NaN's slot. Tiles of several columns
-    // are taken to have such rows: a constant for them, or registers spill.
+    // are taken to have such rows, a constant for them: NT 4 with heads of 128 has every register
+    // in use and three spilled, more of them without it.
     const bool partly = NT > 1 || sees_all + 1u < sp.keys;
     const _Float16 least = partly ? (_Float16)-kLimit : (_Float16)__builtin_nanf("");
     // A block; at the tile's edge, some row's last slots or the cache's.
@@ -747,7 +755,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
     }
     const size_t unit = ((size_t)s * p.a.g.kv_heads + head) * p.tiles + tile, part = unit * p.splits + split;
     const bool alone = sp.active <= 1u;
-    if (w == 0 && q == 0) {   // ms and ls of wave 0 become the row's: read by all above, written below a barrier
+    if (w == 0 && q == 0) {   // the factors of the scores have been read, a barrier ago and more
 #pragma unroll
         for (int c = 0; c < NT; ++c) fs[16 * c + i] = sum[c];
     }
@@ -1011,8 +1019,8 @@ __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_
 }
 
 // What follows the attention kernel, in one launch: workgroups 0..joins-1 join rows' splits,
-// the others the weights of 128 slots each. Bound by launch and latency: 3.2 us (224 rows of 8
-// splits), 4.3 (256 rows of 48), 4.4 with the weights of 8192 slots (as two launches 9.1).
+// the others the weights of 128 slots each. Bound by launch and latency: 3.3 us (224 rows of 8
+// splits), 4.6 (256 rows of 48), 4.9 with the weights of 8192 slots (as two launches 9.1).
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs p, uint32_t joins) {
     if (blockIdx.x < joins) {
@@ -1032,8 +1040,8 @@ __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs p, uint32_t joins) 
 // every row_splits-th tile of 32 rows. The tiles' operands, left by the attention kernel, pass
 // through LDS, the next on its way while one is multiplied. A lane sums its slots over its two
 // rows of each tile; the sums over the row splits are added by k_kv4_add_weights, in order, so
-// that they do not vary. Bound by the matrix pipes and the exponentials between them: 1024 tokens
-// over 8024 slots 72 us, 870 TFLOP/s of products.
+// that they do not vary. Bound by the issue of vector instructions: 1024 tokens over 8024 slots
+// take 54 us, 1170 TFLOP/s of products, in 0.59 of the SIMDs' cycles, the others taking 0.33.
 template <int HD>
 __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
     using L = Lay<HD>;
@@ -1224,7 +1232,8 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 // keeps its slots' orders in registers; of more than 16384 slots it works them out in every
 // pass. Four copies of the histogram, by lane: many weights are alike (zero, say), and
 // additions to one word take turns. Bound by the latencies of its phases, one workgroup going
-// through them all: 56 planes of 8192 slots 10.2 us, 64 of 2049 7.0.
+// through them all: 56 planes of 8192 slots 9.7 us, 64 of 2049 6.9. Of 32768 slots 61 us (0.3 TB/s
+// of the 15 MB): every pass reads both tables anew.
 template <bool KEPT>
 __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
     __shared__ uint32_t part[2][kSelectWaves], found[5];
@@ -1393,7 +1402,7 @@ __global__ __launch_bounds__(kSelect) void k_kv4_select(Kv4Evict a) {
 // targets rise) are made by one wave, of the workgroup of the first: a workgroup looks at
 // seven pairs before its own and seven behind. Bound by the bytes of V, of
 // which a slot has a nibble in head_dim dwords: up to 2048 moves in each of 16 planes of 128, about
-// 32 MB read and written, take 8.6 us (3.7 TB/s).
+// 32 MB read and written, take 9.1 us (3.5 TB/s).
 constexpr uint32_t kMoves = 16;
 
 template <int HD>
@@ -1560,8 +1569,10 @@ namespace {
 // and of 64 where there are enough of those to fill the card: kWideTiles (1900 tokens: 49 against
 // 59; 500 tokens, 126 such tiles: 18.5 against 12.6). One sequence's 32-row tiles of a long
 // context take a second round over the 256 CUs as soon as there are more than 256 of them, so
-// the wider ones then begin at kWideTilesLong (600 tokens over 4600: 69 against 81; over 600
-// they lose, 19 against 17.5; sequences of unequal length even the rounds out).
+// the wider ones then begin at kWideTilesLong (600 tokens over 4600: 66 against 81; over 600
+// they lose, 19 against 17.5). Several sequences are taken to be of unequal length, which the
+// device alone knows: those even the rounds out (300 tokens each at 4000 and 2000: 49 against 63
+// in wide tiles; both at 4000, it is 81 against 63).
 //
 // Splits. As many as make kWideGrid workgroups of up to 16 rows (16 sequences over 32768: 33.8; 768:
 // 35.2; 3000: 38.2), and 256 of more rows (512: 256 tokens over 4256 take 37.4 against 31), a
@@ -1618,9 +1629,10 @@ Parts parts_of(const Kv4Attn &a, const Shape &h, bool with_weights) {
     const bool rows = with_weights && h.rows > 16u;   // the weights of prompts
     t.qtiles = (h.tiles * h.tile_rows + 31u) / 32u;
     t.slots32 = (a.g.context + 31u) / 32u * 32u;
-    // about 512 workgroups of 256 slots, at least two row tiles each; up to four row tiles one, which
-    // saves the launch that adds the splits (8 tokens of 16 query heads to 2 over 4000: 22.6 -> 19.2 us
-    // a call), from 5 tiles on that costs more (24 tokens: 24.5 against 26.1)
+    // about 512 workgroups of 256 slots, at least two row tiles each; three and four row tiles one,
+    // which saves the launch that adds the splits (16 tokens of 16 query heads to 2 over 4000: 20.3 ->
+    // 19.9 us a call, over 500 18.7 -> 17.6), from 5 tiles on that costs more (24 tokens: 23.5 against
+    // 22.2)
     const uint64_t chunks = (a.g.context + 255u) / 256u * pairs, most = h.rows <= 128u ? 1u : (h.rows + 63u) / 64u;
     uint64_t splits = (512u + chunks - 1u) / chunks;
     if (splits > most) splits = most;
