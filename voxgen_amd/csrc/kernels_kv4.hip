@@ -265,7 +265,7 @@ struct AttnArgs {
     uint32_t tile_rows, splits, per; // rows of a tile, key splits of the grid, blocks of one
     bool eager;                      // a wave's first block is fetched before it is known whether slots fill it
     float *ml, *acc;                 // [unit][split][tile rows][2], [..][tile rows][HD]
-    f2 *norm;                        // [sequence x KV head][rows]: see norm_of
+    f2 *norm;                        // [sequence x KV head][rows]: see norm_of; left where weights are wanted
     // for the weights of prompts: the query rows as operands [sequence x KV head][16 rows][HD / 32][hi, lo][64],
     // the factors of their scores [sequence x KV head][rows], sums by row split [split][sequence x KV head][slots]
     h8 *qp;
@@ -348,9 +348,11 @@ __device__ __forceinline__ void two_terms(const float *v, float minus, h8 &hi, h
 // What gives a row's softmax weight of a score s: 2^(s - m) / sum. Kept as the two, not as the
 // logarithm of one number: that rounds to 2^-21 at the usual 8 to 16, v_log_f32 errs to one side
 // by as much, and every weight of the row was 3e-7 to 6e-7 too large by it. A row that is NaN has
-// that in m, so that a score of -inf still weighs nothing.
+// that in m, so that a score of -inf still weighs nothing. The reciprocal is v_rcp_f32's, one
+// step nearer (Newton): within 2^-24 as a division, which takes ten instructions.
 __device__ __forceinline__ f2 norm_of(float m, float sum) {
-    return sum == sum ? f2{m, 1.0f / sum} : f2{__builtin_nanf(""), 1.0f};
+    const float r = __builtin_amdgcn_rcpf(sum);
+    return sum == sum ? f2{m, __builtin_fmaf(__builtin_fmaf(-sum, r, 1.0f), r, r)} : f2{__builtin_nanf(""), 1.0f};
 }
 
 // Sixteen query rows as the B operand: lane (i, q) holds row i, dimensions q HD / 4 + 8 u
@@ -771,7 +773,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k
             const uint32_t row = r0 + 16u * c + i;
             if (row >= rows || (PK && i >= 8u)) continue;
             if (alone) {
-                p.norm[((size_t)s * p.a.g.kv_heads + head) * rows + row] = norm_of(top[c], sum[c]);
+                if (p.a.weights) p.norm[((size_t)s * p.a.g.kv_heads + head) * rows + row] = norm_of(top[c], sum[c]);
             } else {
                 p.ml[(part * RT + 16u * c + i) * 2u] = top[c];
                 p.ml[(part * RT + 16u * c + i) * 2u + 1u] = sum[c];
@@ -889,7 +891,7 @@ __device__ __forceinline__ void join_row(const AttnArgs &p, uint32_t row, uint32
         for (int u = 1; u < Y; ++u) x += os[u][tid];
         p.a.out[((size_t)s * p.a.tokens + t) * p.a.out_stride + (size_t)(head * p.group + j) * HD + tid] = attends ? x / sum : 0.f;
     }
-    if (tid == 0) p.norm[((size_t)s * p.a.g.kv_heads + head) * p.rows + row] = norm_of(top, sum);
+    if (tid == 0 && p.a.weights) p.norm[((size_t)s * p.a.g.kv_heads + head) * p.rows + row] = norm_of(top, sum);
 }
 
 // The same of at most kFewSplits splits: HD / 4 lanes a row, whose splits they fetch at once,
@@ -933,7 +935,7 @@ __device__ __forceinline__ void join_rows(const AttnArgs &p, uint32_t group, uin
 #pragma unroll
         for (int e = 0; e < 4; ++e) to[e] = o[e];
     }
-    if (c == 0) p.norm[pair * p.rows + row] = norm_of(top, sum);
+    if (c == 0 && p.a.weights) p.norm[pair * p.rows + row] = norm_of(top, sum);
 }
 
 // Accumulated weights of at most 16 rows: a wave per block of 32 slots takes the scores
