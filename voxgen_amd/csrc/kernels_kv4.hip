@@ -464,12 +464,12 @@ struct VScale {
 // memory nor the VALU that makes the values is used up: 16 sequences over 32768 slots, 111 MB, take
 // 34 us, 3.3 TB/s where reads reach 6.0, or 29 out of the last-level cache, with 0.62 of the VALU's
 // issue slots at 3.4 waves a SIMD; a block's V is asked for at the block's start. For prompts, the
-// issue of vector instructions: 1024 tokens over 8024 slots take 120 us, 1060 TFLOP/s of two-term
-// products (a plain f16 product of 8192^3: 1080), in which products take 0.52 and the other vector
+// issue of vector instructions: 1024 tokens over 8024 slots take 126 us, 1010 TFLOP/s of two-term
+// products (a plain f16 product of 8192^3 on that card: 1056), in which products take 0.52 and the other vector
 // instructions 0.47 of the SIMDs' cycles; with 1900 tokens (48 us) it is 0.29 and 0.44, the rest
 // going to the start of each of 476 tiles and to its waves' wait and join, while nothing else is on
 // the CU. Heads of 256 with one column tile of rows take 258 registers and more, one wave a SIMD
-// (a token over 8001 slots of one KV head: 9.4 us); two have not been tried.
+// (a token over 8001 slots of one KV head: 10 us); two have not been tried.
 template <int HD, int NT, int W, bool PK>
 __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : PK ? 4 : 3) void k_kv4_attn(AttnArgs p) {
     using L = Lay<HD>;
@@ -1021,8 +1021,8 @@ __device__ __forceinline__ void weigh(const AttnArgs &p, uint32_t group, uint32_
 }
 
 // What follows the attention kernel, in one launch: workgroups 0..joins-1 join rows' splits,
-// the others the weights of 128 slots each. Bound by launch and latency: 3.3 us (224 rows of 8
-// splits), 4.6 (256 rows of 48), 4.9 with the weights of 8192 slots (as two launches 9.1).
+// the others the weights of 128 slots each. Bound by launch and latency: 2.7 us (224 rows of 8
+// splits), 4.7 (256 rows of 48), 4.8 with the weights of 8192 slots (as two launches 9.1).
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs p, uint32_t joins) {
     if (blockIdx.x < joins) {
@@ -1043,7 +1043,7 @@ __global__ __launch_bounds__(256) void k_kv4_finish(AttnArgs p, uint32_t joins) 
 // through LDS, the next on its way while one is multiplied. A lane sums its slots over its two
 // rows of each tile; the sums over the row splits are added by k_kv4_add_weights, in order, so
 // that they do not vary. Bound by the issue of vector instructions: 1024 tokens over 8024 slots
-// take 54 us, 1170 TFLOP/s of products, in 0.59 of the SIMDs' cycles, the others taking 0.33.
+// take 57 us, 1115 TFLOP/s of products, in 0.59 of the SIMDs' cycles, the others taking 0.33.
 template <int HD>
 __global__ __launch_bounds__(256, 2) void k_kv4_weights_rows(AttnArgs p) {
     using L = Lay<HD>;
