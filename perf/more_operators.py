@@ -4,7 +4,7 @@ the pages that a cheap score selects for each query.
 
 K and V lie in pages of `page_size` slots, f16, per layer [page][kv_head], and within a page
 
-  K: [head_dim / 8][slot][8],   V: [slot / 8][head_dim][8];
+  K: [slot / 16][head_dim / 8][slot % 16][8],   V: [slot / 8][head_dim][8];
 
 a request's position p is slot p % page_size of page table[request][p // page_size]. A step
 has rows of several requests one behind the other, counts[i] of request i, at its positions
@@ -194,16 +194,24 @@ def _caches(g, case, s, spread):
 
 
 def _lay_k(x):
-    return x.unflatten(-1, (-1, 8)).transpose(-3, -2).contiguous()
+    return x.unflatten(-1, (-1, 8)).unflatten(-3, (-1, 16)).transpose(-3, -2).contiguous()
 
 
 def _lay_v(x):
     return x.unflatten(-2, (-1, 8)).transpose(-2, -1).contiguous()
 
 
+def _rows_k(x):
+    return x.transpose(-3, -2).flatten(-2).flatten(-3, -2)
+
+
+def _rows_v(x):
+    return x.transpose(-2, -1).flatten(-3, -2)
+
+
 def _bounds(case, s, k):
     """f16 [pages, kv_heads, 2, head_dim] over the filled slots; zeros where a page has none."""
-    x = k.transpose(-3, -2).flatten(-2)                                             # [pages, kv_heads, slots, head_dim]
+    x = _rows_k(k)                                                                  # [pages, kv_heads, slots, head_dim]
     n = _filled(case, s).view(-1, 1, 1, 1)
     there = torch.arange(case["page_size"], device=GPU).view(1, 1, -1, 1) < n
     lo, hi = torch.where(there, x, math.inf).amin(-2), torch.where(there, x, -math.inf).amax(-2)
@@ -335,7 +343,7 @@ def _store(case, s):
     page, at = slot // ps, slot % ps
     k, v = s["k"].view(-1, kh, hd).half(), s["v"].view(-1, kh, hd).half()
     kc, vc = s["kc"].clone(), s["vc"].clone()
-    kc[page, :, :, at] = k.unflatten(-1, (-1, 8))
+    kc[page, :, at // 16, :, at % 16] = k.unflatten(-1, (-1, 8))
     vc[page, :, at // 8, :, at % 8] = v
     if "bounds" not in s:
         return dict(kc=kc, vc=vc)
@@ -356,8 +364,8 @@ def _attend(case, s):
     q, out, at = s["q"].view(-1, kh, group, hd), [], 0
     for i, a, c in s["taking"]:
         page = s["tables"][i, :-(-(a + c) // ps)].long()
-        k = s["kc"][page].permute(1, 0, 3, 2, 4).reshape(kh, -1, hd).float()        # [kv_heads, slots, head_dim]
-        v = s["vc"][page].permute(1, 0, 2, 4, 3).reshape(kh, -1, hd).float()
+        k = _rows_k(s["kc"][page]).transpose(0, 1).reshape(kh, -1, hd).float()      # [kv_heads, slots, head_dim]
+        v = _rows_v(s["vc"][page]).transpose(0, 1).reshape(kh, -1, hd).float()
         rows = q[at:at + c].permute(1, 2, 0, 3).reshape(kh, group * c, hd)
         x = torch.matmul(rows, k.transpose(-1, -2).contiguous()) / math.sqrt(hd)
         seen = torch.arange(k.shape[1], device=GPU) <= a + torch.arange(c, device=GPU).unsqueeze(-1)
@@ -392,8 +400,8 @@ def _sparse(case, s):
         # attention over the slots of those pages
         physical = table[torch.where(there, order, 0)]                                          # [c, kv_heads, budget]
         head = torch.arange(kh, device=GPU).view(1, -1, 1)
-        k = s["kc"][physical, head].transpose(-3, -2).flatten(-2).flatten(2, 3).float()         # [c, kv_heads, slots, head_dim]
-        v = s["vc"][physical, head].transpose(-2, -1).flatten(-3, -2).flatten(2, 3).float()
+        k = _rows_k(s["kc"][physical, head]).flatten(2, 3).float()                             # [c, kv_heads, slots, head_dim]
+        v = _rows_v(s["vc"][physical, head]).flatten(2, 3).float()
         position = (order.unsqueeze(-1) * ps + torch.arange(ps, device=GPU)).flatten(-2)
         seen = (there.unsqueeze(-1).expand(-1, -1, -1, ps).flatten(-2)
                 & (position <= a + torch.arange(c, device=GPU).view(-1, 1, 1))).unsqueeze(2)
@@ -411,7 +419,7 @@ def _one_row(cache, table, head, n, ps, values):
     page, at = table[p // ps].long(), p % ps
     if values:
         return cache[page, head, at // 8, :, at % 8].double()
-    return cache[page, head, :, at].reshape(n, -1).double()
+    return cache[page, head, at // 16, :, at % 16].reshape(n, -1).double()
 
 
 def exact(case, seed):
@@ -429,7 +437,7 @@ def exact(case, seed):
         kc, vc = s["kc"].cpu().numpy().astype(np.float64), s["vc"].cpu().numpy().astype(np.float64)
         rows = [s[n].cpu().numpy().reshape(-1, kh, hd) for n in ("k", "v")]
         for r, slot in enumerate(s["slots"].tolist()):
-            kc[slot // ps, :, :, slot % ps] = rows[0][r].astype(np.float16).reshape(kh, -1, 8)
+            kc[slot // ps, :, slot % ps // 16, :, slot % 16] = rows[0][r].astype(np.float16).reshape(kh, -1, 8)
             vc[slot // ps, :, slot % ps // 8, :, slot % 8] = rows[1][r].astype(np.float16)
         got = dict(kc=kc, vc=vc)
         if "bounds" in s:
@@ -437,8 +445,8 @@ def exact(case, seed):
             tables = s["tables"].cpu().numpy()
             for i, a, c in s["taking"]:
                 for col in range(a // ps, (a + c - 1) // ps + 1):
-                    x = kc[tables[i, col], :, :, :min(ps, a + c - col * ps)]
-                    b[tables[i, col]] = np.stack([x.min(2), x.max(2)], 1).reshape(kh, 2, hd)
+                    x = kc[tables[i, col]].swapaxes(2, 3).reshape(kh, ps, hd)[:, :min(ps, a + c - col * ps)]
+                    b[tables[i, col]] = np.stack([x.min(1), x.max(1)], 1)
         return got
     if sum(a + c for _, a, c in s["taking"]) * kh > 4_000_000:
         return None if kind == "attend" else dict(pages=None, out=None)
