@@ -590,6 +590,137 @@ int vx_kv4_compact(vx_ctx *ctx, const vx_buf *plan, vx_buf *k_cache, vx_buf *v_c
                    vx_buf *slot_positions, vx_buf *slots, const vx_kv4_evict_push *pc);
 
 /* ------------------------------------------------------------------------- */
+/* Paged KV cache (no reference counterpart: the reference's caches are those  */
+/* of one sequence, with room for its whole context).                          */
+/*                                                                            */
+/* K and V lie in pages of page_size slots, f16, in one vx_buf each of          */
+/* vx_paged_cache_bytes: [layer][page][kv_head], and within a page and head    */
+/*   K: [slot / 16][head_dim / 8][slot % 16][8],                               */
+/*   V: [slot / 8][head_dim][8]   (transposed for the product that reads it).  */
+/* A third buffer may hold the bounds of each page's keys, f16                 */
+/* [layer][page][kv_head][lo, hi][head_dim].                                   */
+/*                                                                            */
+/* Of each of `requests` requests the device holds (u32): how many tokens are  */
+/* cached (lengths), and the pages that they lie in (tables, [requests]        */
+/* [table_width]): position p is slot p % page_size of page                    */
+/* tables[i][p / page_size]. Free pages lie on a stack (pool: their number,    */
+/* then the pages, the next one last).                                         */
+/*                                                                            */
+/* A step has counts[i] rows of request i (0: it takes no part), the requests' */
+/* rows one behind the other in their order: row t of request i is the token   */
+/* at position lengths[i] + t and attends to positions 0..lengths[i] + t.      */
+/*   vx_paged_plan      once a step: pages for the new tokens, the slot map,    */
+/*                      and the division of the attention's work;              */
+/*   vx_paged_store, vx_paged_attention   in every layer;                      */
+/*   vx_paged_advance   after the last: lengths and pool as the plan left them.*/
+/* vx_paged_cut takes tokens back (all of them when a request ends, rejected   */
+/* drafts) and returns their pages. Everything is read from device memory, so  */
+/* a step captures into a graph; sizes of vx_paged_batch are fixed by it.      */
+/*                                                                            */
+/* No content of a device buffer makes a call read or write outside of the     */
+/* buffers: a table entry that is no page holds no slots (nothing is stored     */
+/* there, no row attends to it). Calls on one context are in order; calls that */
+/* overlap (other contexts, replayed graphs) need plans and scratch of their    */
+/* own and may not write what another reads. A buffer that a call writes may    */
+/* share no memory with another of the call, but q and out may be parts of one */
+/* buffer, one behind the other or of one stride and side by side.             */
+/* ------------------------------------------------------------------------- */
+#define VX_PAGED_NONE 4294967295u
+typedef struct vx_paged_geom {
+    uint32_t layers, pages;
+    uint32_t page_size;             /* 16, 32, 64, 128 or 256; pages * page_size below 2^32 - 1 */
+    uint32_t kv_heads;
+    uint32_t head_dim;              /* 64, 128 or 256 */
+} vx_paged_geom;
+/* Bytes of the K cache, and of the V cache; of the bounds. 0 for a geometry that
+ * is not valid (layers and kv_heads at most 65535, a cache below 2^47 bytes). */
+uint64_t vx_paged_cache_bytes(const vx_paged_geom *geom);
+uint64_t vx_paged_bounds_bytes(const vx_paged_geom *geom);
+
+typedef struct vx_paged_batch {
+    vx_paged_geom geom;
+    uint32_t requests;              /* at most 4096 */
+    uint32_t table_width;           /* pages of a request; table_width * page_size at most 2^28 */
+    uint32_t max_rows;              /* rows of a step: what its q, k, v and out buffers hold */
+    uint32_t max_count;             /* rows of one request in it, at most max_rows */
+    uint32_t q_heads;               /* a multiple of kv_heads, at most 1024 times it; max_rows * q_heads at most 2^22 */
+} vx_paged_batch;
+/* Words of a plan. The first eight: rows of the step (up to max_rows), pages taken,
+ * requests and rows that take part, and four of the library's own. Then u32
+ * slots[max_rows], requests[max_rows], positions[max_rows] (VX_PAGED_NONE in rows that
+ * take no part), and granted[requests]: the request's rows that take part, its count
+ * or 0. What follows is the library's own. */
+#define VX_PAGED_PLAN_ROWS 8u
+uint64_t vx_paged_plan_bytes(const vx_paged_batch *batch);
+/* Empties the requests: lengths 0, no pages in tables, every page in the pool
+ * (u32[1 + pages]); the first pages that a plan takes are 0, 1, 2... */
+int vx_paged_reset(vx_ctx *ctx, vx_buf *lengths, vx_buf *tables, vx_buf *pool, const vx_paged_batch *batch);
+/* The plan of a step of counts (u32[requests]). A request takes part, with all its rows,
+ * if its count is 1..max_count, its rows end within max_rows, its tokens fit table_width
+ * pages, and the pool has the pages that it and the requests before it want (a request
+ * that wants no new page takes part in any case); else none of its rows is stored or
+ * attended for, and later ones keep their places. Slot of a row: page * page_size + slot
+ * in the page. The new pages are written into the tables behind those in use; lengths
+ * and pool stay, so that a plan can be made again. */
+int vx_paged_plan(vx_ctx *ctx, const vx_buf *lengths, const vx_buf *counts, vx_buf *tables, const vx_buf *pool,
+                  vx_buf *plan, const vx_paged_batch *batch);
+/* lengths[i] += granted[i], and the pages taken leave the pool. Once a plan. */
+int vx_paged_advance(vx_ctx *ctx, const vx_buf *plan, vx_buf *lengths, vx_buf *pool, const vx_paged_batch *batch);
+/* lengths[i] = min(lengths[i], keep[i]); pages that then hold no token return to the
+ * pool, in the requests' and the tables' order, and their entries are VX_PAGED_NONE. */
+int vx_paged_cut(vx_ctx *ctx, const vx_buf *keep, vx_buf *lengths, vx_buf *tables, vx_buf *pool,
+                 const vx_paged_batch *batch);
+
+typedef struct vx_paged_store_push {
+    vx_paged_batch batch;           /* as the plan's */
+    uint32_t layer, k_stride, v_stride, k_base, v_base;   /* floats */
+} vx_paged_store_push;
+/* Rows k, v (f32, kv_heads * head_dim wide), rounded to f16, into the plan's slots. With
+ * bounds (nullable), those of the pages that rows were stored in: each dimension's least
+ * and greatest key over the page's slots up to the last one stored, NaN if there is one. */
+int vx_paged_store(vx_ctx *ctx, const vx_buf *k, const vx_buf *v, vx_buf *k_cache, vx_buf *v_cache, vx_buf *bounds,
+                   const vx_buf *plan, const vx_paged_store_push *pc);
+
+typedef struct vx_paged_attention_push {
+    vx_paged_batch batch;           /* as the plan's */
+    uint32_t layer, q_stride, out_stride, q_base, out_base;   /* floats */
+    uint32_t budget;                /* entries of a row and head in `selected`, budget * page_size at most 2^28;
+                                     * 0 without it */
+} vx_paged_attention_push;
+/* Scratch of one call; 0 for a push that is not valid. What it holds before the
+ * call does not matter. */
+uint64_t vx_paged_attention_scratch_bytes(const vx_paged_attention_push *pc);
+/* out = softmax(q . K / sqrt(head_dim)) . V over the positions each row attends to, in f32
+ * (products on the matrix cores, q and the weights as two f16 terms each, sums in f32).
+ * Rows that take no part are left as they were. With selected (nullable; u32
+ * [max_rows][kv_heads][budget]) a row attends to those positions only that lie in the
+ * pages of its list: indices into the request's table, each once; of the first
+ * min(budget, position / page_size + 1) entries those that are such pages count, and a
+ * row with none of them has an output of 0. A NaN or an infinity that is stored reaches the rows
+ * that attend to its slot and no other; slots that hold no token may hold anything. */
+int vx_paged_attention(vx_ctx *ctx, const vx_buf *q, const vx_buf *k_cache, const vx_buf *v_cache, vx_buf *out,
+                       const vx_buf *tables, const vx_buf *plan, const vx_buf *selected, vx_buf *scratch,
+                       const vx_paged_attention_push *pc);
+
+typedef struct vx_paged_select_push {
+    vx_paged_batch batch;           /* as the plan's */
+    uint32_t layer, q_stride, q_base;   /* floats */
+    uint32_t budget;                /* pages of each row and KV head, budget * page_size at most 2^28 */
+    uint32_t sinks;                 /* its first pages are among them */
+    uint32_t recent;                /* and its last, its own (the position's) the last: 1 or more */
+} vx_paged_select_push;
+uint64_t vx_paged_select_scratch_bytes(const vx_paged_select_push *pc);
+/* The pages that a row attends to, by the most that a key within the page's bounds could
+ * score: up . hi + down . lo, where up and down are the sums over the KV head's query heads of
+ * max(q, 0) and min(q, 0), in 64 bits. Of each row and KV head the first `sinks` and the last `recent` pages up to its
+ * own, then those of the greatest sums (NaN before all), ties to the lower index, `budget` in all:
+ * u32 indices into the request's table in rising order, VX_PAGED_NONE behind them; rows that
+ * take no part are VX_PAGED_NONE throughout. sinks + recent may not exceed budget. A table entry
+ * that is no page scores NaN. */
+int vx_paged_select(vx_ctx *ctx, const vx_buf *q, const vx_buf *bounds, const vx_buf *tables, const vx_buf *plan,
+                    vx_buf *selected, vx_buf *scratch, const vx_paged_select_push *pc);
+
+/* ------------------------------------------------------------------------- */
 /* Diagnostics (no reference counterpart): plain streaming kernels that       */
 /* calibrate the HBM roofline and the PMC byte counters.                      */
 /* ------------------------------------------------------------------------- */

@@ -38,6 +38,8 @@ pub const VX_DTYPE_F16: u32 = 1;
 pub const VX_DTYPE_Q8_0: u32 = 8;
 pub const VX_NOALLOC_SCRATCH_BYTES: u32 = 2097152;
 pub const VX_KV4_NO_SLOT: u32 = 4294967295;
+pub const VX_PAGED_NONE: u32 = 4294967295;
+pub const VX_PAGED_PLAN_ROWS: u32 = 8;
 pub const VX_EXEC_GRAPH: u32 = 0;
 pub const VX_EXEC_FUSED: u32 = 1;
 pub const VX_EXEC_REFERENCE: u32 = 2;
@@ -931,6 +933,150 @@ extern "C" {
         slot_positions: *mut VxBuf,
         slots: *mut VxBuf,
         pc: *const VxKv4EvictPush,
+    ) -> c_int;
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct VxPagedGeom {
+    pub layers: u32,
+    pub pages: u32,
+    pub page_size: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+}
+
+#[link(name = "voxhip")]
+extern "C" {
+    pub fn vx_paged_cache_bytes(geom: *const VxPagedGeom) -> u64;
+    pub fn vx_paged_bounds_bytes(geom: *const VxPagedGeom) -> u64;
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct VxPagedBatch {
+    pub geom: VxPagedGeom,
+    pub requests: u32,
+    pub table_width: u32,
+    pub max_rows: u32,
+    pub max_count: u32,
+    pub q_heads: u32,
+}
+
+#[link(name = "voxhip")]
+extern "C" {
+    pub fn vx_paged_plan_bytes(batch: *const VxPagedBatch) -> u64;
+    pub fn vx_paged_reset(
+        ctx: *mut VxCtx,
+        lengths: *mut VxBuf,
+        tables: *mut VxBuf,
+        pool: *mut VxBuf,
+        batch: *const VxPagedBatch,
+    ) -> c_int;
+    pub fn vx_paged_plan(
+        ctx: *mut VxCtx,
+        lengths: *const VxBuf,
+        counts: *const VxBuf,
+        tables: *mut VxBuf,
+        pool: *const VxBuf,
+        plan: *mut VxBuf,
+        batch: *const VxPagedBatch,
+    ) -> c_int;
+    pub fn vx_paged_advance(
+        ctx: *mut VxCtx,
+        plan: *const VxBuf,
+        lengths: *mut VxBuf,
+        pool: *mut VxBuf,
+        batch: *const VxPagedBatch,
+    ) -> c_int;
+    pub fn vx_paged_cut(
+        ctx: *mut VxCtx,
+        keep: *const VxBuf,
+        lengths: *mut VxBuf,
+        tables: *mut VxBuf,
+        pool: *mut VxBuf,
+        batch: *const VxPagedBatch,
+    ) -> c_int;
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct VxPagedStorePush {
+    pub batch: VxPagedBatch,
+    pub layer: u32,
+    pub k_stride: u32,
+    pub v_stride: u32,
+    pub k_base: u32,
+    pub v_base: u32,
+}
+
+#[link(name = "voxhip")]
+extern "C" {
+    pub fn vx_paged_store(
+        ctx: *mut VxCtx,
+        k: *const VxBuf,
+        v: *const VxBuf,
+        k_cache: *mut VxBuf,
+        v_cache: *mut VxBuf,
+        bounds: *mut VxBuf,
+        plan: *const VxBuf,
+        pc: *const VxPagedStorePush,
+    ) -> c_int;
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct VxPagedAttentionPush {
+    pub batch: VxPagedBatch,
+    pub layer: u32,
+    pub q_stride: u32,
+    pub out_stride: u32,
+    pub q_base: u32,
+    pub out_base: u32,
+    pub budget: u32,
+}
+
+#[link(name = "voxhip")]
+extern "C" {
+    pub fn vx_paged_attention_scratch_bytes(pc: *const VxPagedAttentionPush) -> u64;
+    pub fn vx_paged_attention(
+        ctx: *mut VxCtx,
+        q: *const VxBuf,
+        k_cache: *const VxBuf,
+        v_cache: *const VxBuf,
+        out: *mut VxBuf,
+        tables: *const VxBuf,
+        plan: *const VxBuf,
+        selected: *const VxBuf,
+        scratch: *mut VxBuf,
+        pc: *const VxPagedAttentionPush,
+    ) -> c_int;
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct VxPagedSelectPush {
+    pub batch: VxPagedBatch,
+    pub layer: u32,
+    pub q_stride: u32,
+    pub q_base: u32,
+    pub budget: u32,
+    pub sinks: u32,
+    pub recent: u32,
+}
+
+#[link(name = "voxhip")]
+extern "C" {
+    pub fn vx_paged_select_scratch_bytes(pc: *const VxPagedSelectPush) -> u64;
+    pub fn vx_paged_select(
+        ctx: *mut VxCtx,
+        q: *const VxBuf,
+        bounds: *const VxBuf,
+        tables: *const VxBuf,
+        plan: *const VxBuf,
+        selected: *mut VxBuf,
+        scratch: *mut VxBuf,
+        pc: *const VxPagedSelectPush,
     ) -> c_int;
     pub fn vx_diag_stream_read(
         ctx: *mut VxCtx,

@@ -188,6 +188,17 @@ Kv4AttentionPush = _struct("Kv4AttentionPush", [("geom", Kv4Geom)] + [(n, u32) f
 Kv4EvictPush = _struct("Kv4EvictPush", [("geom", Kv4Geom)] + [(n, u32) for n in (
     "first_sequence", "n_sequences", "keep", "sinks", "recent")])
 KV4_NO_SLOT = 0xFFFFFFFF  # VX_KV4_NO_SLOT
+PagedGeom = _struct("PagedGeom", [(n, u32) for n in ("layers", "pages", "page_size", "kv_heads", "head_dim")])
+PagedBatch = _struct("PagedBatch", [("geom", PagedGeom)] + [(n, u32) for n in (
+    "requests", "table_width", "max_rows", "max_count", "q_heads")])
+PagedStorePush = _struct("PagedStorePush", [("batch", PagedBatch)] + [(n, u32) for n in (
+    "layer", "k_stride", "v_stride", "k_base", "v_base")])
+PagedAttentionPush = _struct("PagedAttentionPush", [("batch", PagedBatch)] + [(n, u32) for n in (
+    "layer", "q_stride", "out_stride", "q_base", "out_base", "budget")])
+PagedSelectPush = _struct("PagedSelectPush", [("batch", PagedBatch)] + [(n, u32) for n in (
+    "layer", "q_stride", "q_base", "budget", "sinks", "recent")])
+PAGED_NONE = 0xFFFFFFFF  # VX_PAGED_NONE
+PAGED_PLAN_ROWS = 8      # VX_PAGED_PLAN_ROWS
 RESIDUAL_BUF = dict(OUTPUT=0, CURRENT_LM=1, FSQ_LATENT=2, FSQ_OUTPUT=3, FUSION_SNAPSHOT=4, HIDDEN=5,
                     KV_K=6, KV_V=7, STOP_LOGITS=8)
 
@@ -291,6 +302,18 @@ PROTOTYPES = {
     "vx_kv4_plan_bytes": (u64, [P(Kv4EvictPush)]),
     "vx_kv4_select": (i32, [CTX, BUFP, BUFP, BUFP, BUFP, P(Kv4EvictPush)]),
     "vx_kv4_compact": (i32, [CTX, BUFP, BUFP, BUFP, BUFP, BUFP, BUFP, P(Kv4EvictPush)]),
+    "vx_paged_cache_bytes": (u64, [P(PagedGeom)]),
+    "vx_paged_bounds_bytes": (u64, [P(PagedGeom)]),
+    "vx_paged_plan_bytes": (u64, [P(PagedBatch)]),
+    "vx_paged_reset": (i32, [CTX, BUFP, BUFP, BUFP, P(PagedBatch)]),
+    "vx_paged_plan": (i32, [CTX, BUFP, BUFP, BUFP, BUFP, BUFP, P(PagedBatch)]),
+    "vx_paged_advance": (i32, [CTX, BUFP, BUFP, BUFP, P(PagedBatch)]),
+    "vx_paged_cut": (i32, [CTX, BUFP, BUFP, BUFP, BUFP, P(PagedBatch)]),
+    "vx_paged_store": (i32, [CTX, BUFP, BUFP, BUFP, BUFP, BUFP, BUFP, P(PagedStorePush)]),
+    "vx_paged_attention_scratch_bytes": (u64, [P(PagedAttentionPush)]),
+    "vx_paged_attention": (i32, [CTX, BUFP, BUFP, BUFP, BUFP, BUFP, BUFP, BUFP, BUFP, P(PagedAttentionPush)]),
+    "vx_paged_select_scratch_bytes": (u64, [P(PagedSelectPush)]),
+    "vx_paged_select": (i32, [CTX, BUFP, BUFP, BUFP, BUFP, BUFP, BUFP, P(PagedSelectPush)]),
     "vx_diag_stream_read": (i32, [CTX, BUFP, u64, u64, BUFP, u32, u32]),
     "vx_diag_stream_copy": (i32, [CTX, BUFP, BUFP, u64, u32]),
     "vx_diag_timeline_arm": (i32, [CTX, u64]),
@@ -386,6 +409,8 @@ STRUCT_SIZES = {  # C name -> ctypes struct
     "vx_vae_snake_push": VaeSnakePush, "vx_vae_scale_push": VaeScalePush, "vx_vae_grid_push": VaeGridPush,
     "vx_kv4_geom": Kv4Geom, "vx_kv4_rows_push": Kv4RowsPush, "vx_kv4_attention_push": Kv4AttentionPush,
     "vx_kv4_evict_push": Kv4EvictPush,
+    "vx_paged_geom": PagedGeom, "vx_paged_batch": PagedBatch, "vx_paged_store_push": PagedStorePush,
+    "vx_paged_attention_push": PagedAttentionPush, "vx_paged_select_push": PagedSelectPush,
     "vx_audiovae_config": AudioVaeConfig, "vx_audio_decode_stats": AudioDecodeStats,
 }
 

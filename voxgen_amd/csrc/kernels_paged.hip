@@ -1,0 +1,582 @@
+// The paged KV cache but for its attention: the plan of a step, what follows from it for
+// lengths and pool, storing rows, and the choice of the pages that a row attends to
+// (include/voxhip.h, vx_paged_*, has the layouts). Everything that a step depends on is
+// read from device memory, so that a captured step replays.
+#include "attn_dev.h"
+#include "paged.h"
+
+namespace vx {
+namespace {
+
+typedef double d2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ uint32_t add_up_to(uint32_t a, uint32_t b, uint32_t most) { return min(a + b, most); }
+
+// Sums over a workgroup's threads up to and with each, and in `before` without it, each clipped to
+// `most` (clipped addition of numbers below 2^31 is associative). `between` holds a word for each wave.
+template <int N>
+__device__ __forceinline__ void scan(uint32_t (&v)[N], uint32_t (&before)[N], uint32_t most, uint32_t (*between)[N]) {
+    const uint32_t lane = threadIdx.x & 63u, w = threadIdx.x >> 6;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t below = __shfl_up(v[n], d, 64);
+            v[n] = lane >= (uint32_t)d ? add_up_to(v[n], below, most) : v[n];
+        }
+        before[n] = __shfl_up(v[n], 1, 64);
+        if (lane == 0) before[n] = 0;
+        if (lane == 63u) between[w][n] = v[n];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        uint32_t ahead = 0;
+        for (uint32_t u = 0; u < w; ++u) ahead = add_up_to(ahead, between[u][n], most);
+        v[n] = add_up_to(v[n], ahead, most);
+        before[n] = add_up_to(before[n], ahead, most);
+    }
+    __syncthreads();
+}
+
+// The least i with end[i] > x; ends rise, and the last is above x.
+__device__ __forceinline__ uint32_t owner_of(const uint32_t *end, uint32_t n, uint32_t x) {
+    uint32_t lo = 0, hi = n - 1u;
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) / 2u;
+        if (end[mid] > x)
+            hi = mid;
+        else
+            lo = mid + 1u;
+    }
+    return lo;
+}
+
+constexpr uint32_t kPlanThreads = 1024, kPlanEach = kPagedRequests / kPlanThreads;
+
+// Every workgroup scans all requests, and writes its share of what follows from that: so one
+// launch does, and none waits for another. A thread has `each` requests one behind the other.
+__global__ __launch_bounds__(1024) void k_paged_plan(PagedPlan a) {
+    __shared__ uint32_t row_end[kPagedRequests], page_end[kPagedRequests], run_end[kPagedRequests], item_end[kPagedRequests],
+        join_end[kPagedRequests], part_end[kPagedRequests];
+    __shared__ uint32_t between[kPlanThreads / 64][4];
+    __shared__ unsigned long long work[kPlanThreads / 64];
+    const uint32_t tid = threadIdx.x, n = a.b.requests, each = (n + kPlanThreads - 1u) / kPlanThreads;
+    const uint32_t pages = a.b.geom.pages, shift = 31u - __clz(a.b.geom.page_size), ps = a.b.geom.page_size;
+    const uint32_t width = a.b.table_width, cap = width << shift, rows = a.b.max_rows;
+    const uint32_t group = a.b.q_heads / a.b.geom.kv_heads, heads = a.b.geom.kv_heads;
+    const uint32_t free = min(a.pool[0], pages);
+    uint32_t len[kPlanEach], count[kPlanEach], need[kPlanEach];
+    bool takes[kPlanEach];
+    const uint32_t r0 = tid * each;
+
+    uint32_t v[1] = {0};
+#pragma unroll
+    for (uint32_t e = 0; e < kPlanEach; ++e) {
+        const bool there = e < each && r0 + e < n;
+        len[e] = there ? a.lengths[r0 + e] : 0u;
+        count[e] = there ? a.counts[r0 + e] : 0u;
+        v[0] = add_up_to(v[0], min(count[e], rows + 1u), rows + 1u);
+    }
+    uint32_t before[1];
+    scan<1>(v, before, rows + 1u, reinterpret_cast<uint32_t (*)[1]>(between));
+    uint32_t at = before[0];
+    v[0] = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < kPlanEach; ++e) {
+        const uint32_t end = add_up_to(at, min(count[e], rows + 1u), rows + 1u);
+        takes[e] = count[e] != 0u && count[e] <= a.b.max_count && end <= rows && len[e] <= cap && count[e] <= cap - len[e];
+        need[e] = takes[e] ? ((len[e] + count[e] + ps - 1u) >> shift) - ((len[e] + ps - 1u) >> shift) : 0u;
+        v[0] = add_up_to(v[0], need[e], pages + 1u);
+        if (e < each && r0 + e < n) row_end[r0 + e] = end;
+        at = end;
+    }
+    scan<1>(v, before, pages + 1u, reinterpret_cast<uint32_t (*)[1]>(between));
+    at = before[0];
+    // what the attention has to do: chunks of 32 keys by tiles of query rows
+    unsigned long long todo = 0;
+    uint32_t tiles[kPlanEach], chunks[kPlanEach];
+#pragma unroll
+    for (uint32_t e = 0; e < kPlanEach; ++e) {
+        at = add_up_to(at, need[e], pages + 1u);
+        takes[e] = takes[e] && (need[e] == 0u || at <= free);
+        if (e < each && r0 + e < n) page_end[r0 + e] = at;
+        tiles[e] = takes[e] ? (count[e] * group + a.s.tile_rows - 1u) / a.s.tile_rows : 0u;
+        chunks[e] = takes[e] ? (len[e] + count[e] + 31u) / 32u : 0u;
+        todo += (unsigned long long)tiles[e] * chunks[e];
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) todo += __shfl_xor(todo, d, 64);
+    if ((tid & 63u) == 0) work[tid >> 6] = todo;
+    __syncthreads();
+    todo = 0;
+    for (uint32_t u = 0; u < kPlanThreads / 64; ++u) todo += work[u];
+    const unsigned long long share = (todo * heads + (1u << a.s.workgroups) - 1u) >> a.s.workgroups;
+    const uint32_t per = max((uint32_t)min(share, 1ull << 30), a.s.least);
+    // runs, then items, joins and parts of each request; a request's tiles are all divided alike
+    uint32_t splits[kPlanEach], by[kPlanEach];
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t e = 0; e < kPlanEach; ++e) {
+        splits[e] = min((chunks[e] + per - 1u) / per, kPagedMaxSplits);
+        by[e] = splits[e] ? (chunks[e] + splits[e] - 1u) / splits[e] : 1u;
+        splits[e] = (chunks[e] + by[e] - 1u) / by[e];
+        w[0] += takes[e] ? ((len[e] + count[e] - 1u) >> shift) - (len[e] >> shift) + 1u : 0u;
+        w[1] += tiles[e] * splits[e];
+        w[2] += splits[e] > 1u ? tiles[e] : 0u;
+        w[3] += splits[e] > 1u ? tiles[e] * splits[e] : 0u;
+    }
+    uint32_t done[4];
+    scan<4>(w, done, 0x7fffffffu, between);
+    uint32_t run = done[0], item = done[1], join = done[2], part = done[3];
+#pragma unroll
+    for (uint32_t e = 0; e < kPlanEach; ++e) {
+        run += takes[e] ? ((len[e] + count[e] - 1u) >> shift) - (len[e] >> shift) + 1u : 0u;
+        item += tiles[e] * splits[e];
+        join += splits[e] > 1u ? tiles[e] : 0u;
+        part += splits[e] > 1u ? tiles[e] * splits[e] : 0u;
+        if (e < each && r0 + e < n) {
+            run_end[r0 + e] = run;
+            item_end[r0 + e] = item;
+            join_end[r0 + e] = join;
+            part_end[r0 + e] = part;
+        }
+    }
+    __syncthreads();
+
+    const uint32_t all_rows = min(row_end[n - 1u], rows), all_runs = min(run_end[n - 1u], a.s.runs);
+    const uint32_t all_items = min(item_end[n - 1u], a.s.items), all_joins = min(join_end[n - 1u], a.s.joins);
+    const uint32_t g0 = blockIdx.x * kPlanThreads + tid, step = gridDim.x * kPlanThreads;
+    auto begin = [&](const uint32_t *end, uint32_t i) { return i ? end[i - 1u] : 0u; };
+    auto taking = [&](uint32_t i) { return run_end[i] != begin(run_end, i); };
+    // the page of position p of request i that takes part: one in use, or one from the top of the pool
+    auto page_of = [&](uint32_t i, uint32_t length, uint32_t p) {
+        const uint32_t have = (length + ps - 1u) >> shift, k = p >> shift;
+        if (k < have) return a.tables[(size_t)i * width + k];
+        const uint32_t nth = begin(page_end, i) + k - have;
+        return nth < free ? a.pool[free - nth] : VX_PAGED_NONE;
+    };
+    for (uint32_t r = g0; r < rows; r += step) {
+        uint32_t slot = VX_PAGED_NONE, request = VX_PAGED_NONE, position = VX_PAGED_NONE;
+        if (r < all_rows) {
+            const uint32_t i = owner_of(row_end, n, r);
+            if (taking(i)) {
+                const uint32_t length = a.lengths[i];
+                request = i;
+                position = length + r - begin(row_end, i);
+                const uint32_t page = page_of(i, length, position);
+                if (page < pages) slot = (page << shift) + (position & (ps - 1u));
+            }
+        }
+        a.plan[a.s.slots + r] = slot;
+        a.plan[a.s.requests + r] = request;
+        a.plan[a.s.positions + r] = position;
+    }
+    for (uint32_t g = g0; g < all_runs; g += step) {
+        const uint32_t i = owner_of(run_end, n, g), length = a.lengths[i], cnt = a.counts[i], k = g - begin(run_end, i);
+        const uint32_t first = k ? ((length >> shift) + k) << shift : length;       // position of the run's first row
+        const uint32_t last = min(((first >> shift) + 1u) << shift, length + cnt);
+        const uint32_t page = page_of(i, length, first);
+        PagedRun run_of = {begin(row_end, i) + first - length, last - first,
+                           page < pages ? (page << shift) + (first & (ps - 1u)) : VX_PAGED_NONE, 0u};
+        reinterpret_cast<PagedRun *>(a.plan + a.s.run_at)[g] = run_of;
+    }
+    // the division, as it was made above
+    auto divided = [&](uint32_t i, uint32_t length, uint32_t cnt, uint32_t &tiles_of, uint32_t &by_of) {
+        const uint32_t many = (length + cnt + 31u) / 32u;
+        tiles_of = (cnt * group + a.s.tile_rows - 1u) / a.s.tile_rows;
+        uint32_t s = min((many + per - 1u) / per, kPagedMaxSplits);
+        by_of = (many + s - 1u) / s;
+        return (many + by_of - 1u) / by_of;
+    };
+    for (uint32_t g = g0; g < all_items; g += step) {
+        const uint32_t i = owner_of(item_end, n, g), length = a.lengths[i], cnt = a.counts[i], k = g - begin(item_end, i);
+        uint32_t tiles_of, by_of;
+        const uint32_t s = divided(i, length, cnt, tiles_of, by_of);
+        // the tiles with the most keys first
+        const uint32_t tile = tiles_of - 1u - k / s, split = k % s;
+        const uint32_t last_row = min((tile + 1u) * a.s.tile_rows, cnt * group) - 1u;
+        const uint32_t many = (length + last_row / group) / 32u + 1u;
+        const uint32_t first = split * by_of;
+        PagedItem it = {i, begin(row_end, i), length, cnt, tile * a.s.tile_rows, first,
+                        first < many ? min(by_of, many - first) : 0u,
+                        many > by_of ? begin(part_end, i) + tile * s + split : VX_PAGED_NONE};
+        reinterpret_cast<PagedItem *>(a.plan + a.s.item_at)[g] = it;
+    }
+    for (uint32_t g = g0; g < all_joins; g += step) {
+        const uint32_t i = owner_of(join_end, n, g), length = a.lengths[i], cnt = a.counts[i], tile = g - begin(join_end, i);
+        uint32_t tiles_of, by_of;
+        const uint32_t s = divided(i, length, cnt, tiles_of, by_of);
+        PagedJoin j = {begin(row_end, i), length, cnt, tile * a.s.tile_rows, begin(part_end, i) + tile * s, by_of, {0, 0}};
+        reinterpret_cast<PagedJoin *>(a.plan + a.s.join_at)[g] = j;
+    }
+    // new pages into the tables, granted rows, the header
+    for (uint32_t i = g0; i < n; i += step) {
+        const bool t = taking(i);
+        const uint32_t cnt = a.counts[i];
+        a.plan[a.s.granted + i] = t ? cnt : 0u;
+    }
+    uint32_t taken = 0;
+    {   // pages that requests that take part want: they are the first of all wanted
+        uint32_t lo = 0;
+#pragma unroll
+        for (uint32_t e = 0; e < kPlanEach; ++e)
+            if (e < each && r0 + e < n && takes[e] && need[e]) lo = page_end[r0 + e];
+#pragma unroll
+        for (int d = 32; d; d >>= 1) lo = max(lo, (uint32_t)__shfl_xor(lo, d, 64));
+        if ((tid & 63u) == 0) between[tid >> 6][0] = lo;
+        __syncthreads();
+        for (uint32_t u = 0; u < kPlanThreads / 64; ++u) taken = max(taken, between[u][0]);
+        __syncthreads();
+    }
+    for (uint32_t g = g0; g < taken; g += step) {
+        const uint32_t i = owner_of(page_end, n, g), have = (a.lengths[i] + ps - 1u) >> shift;
+        a.tables[(size_t)i * width + have + g - begin(page_end, i)] = a.pool[free - g];
+    }
+    if (blockIdx.x == 0) {
+        uint32_t some = 0, sum = 0;
+#pragma unroll
+        for (uint32_t e = 0; e < kPlanEach; ++e)
+            if (takes[e]) some += 1u, sum += count[e];
+#pragma unroll
+        for (int d = 32; d; d >>= 1) some += __shfl_xor(some, d, 64), sum += __shfl_xor(sum, d, 64);
+        if ((tid & 63u) == 0) between[tid >> 6][0] = some, between[tid >> 6][1] = sum;
+        __syncthreads();
+        if (tid == 0) {
+            some = sum = 0;
+            for (uint32_t u = 0; u < kPlanThreads / 64; ++u) some += between[u][0], sum += between[u][1];
+            const uint32_t head[8] = {all_rows, taken, some, sum, all_runs, all_items, all_joins, 0u};
+            for (uint32_t u = 0; u < 8; ++u) a.plan[u] = head[u];
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void k_paged_reset(vx_paged_batch b, uint32_t *lengths, uint32_t *tables, uint32_t *pool) {
+    const size_t at = (size_t)blockIdx.x * 256u + threadIdx.x, step = (size_t)gridDim.x * 256u;
+    if (at == 0) pool[0] = b.geom.pages;
+    for (size_t i = at; i < b.requests; i += step) lengths[i] = 0u;
+    for (size_t i = at; i < (size_t)b.requests * b.table_width; i += step) tables[i] = VX_PAGED_NONE;
+    for (size_t i = at; i < b.geom.pages; i += step) pool[1u + i] = b.geom.pages - 1u - (uint32_t)i;
+}
+
+__global__ __launch_bounds__(256) void k_paged_advance(vx_paged_batch b, const uint32_t *plan, uint64_t granted, uint32_t *lengths,
+                                                       uint32_t *pool) {
+    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
+    if (i == 0) {
+        const uint32_t free = min(pool[0], b.geom.pages);
+        pool[0] = free - min(plan[1], free);
+    }
+    if (i >= b.requests) return;
+    const uint32_t length = lengths[i], cap = b.table_width * b.geom.page_size, more = plan[granted + i];
+    if (more && length <= cap) lengths[i] = length + min(more, cap - length);
+}
+
+// One workgroup: the pages that requests give back, in order, go on top of the pool.
+__global__ __launch_bounds__(1024) void k_paged_cut(vx_paged_batch b, const uint32_t *keep, uint32_t *lengths, uint32_t *tables,
+                                                    uint32_t *pool) {
+    __shared__ uint32_t end[kPagedRequests], from[kPagedRequests];
+    __shared__ uint32_t between[kPlanThreads / 64][1];
+    const uint32_t tid = threadIdx.x, n = b.requests, each = (n + kPlanThreads - 1u) / kPlanThreads, r0 = tid * each;
+    const uint32_t shift = 31u - __clz(b.geom.page_size), ps = b.geom.page_size, pages = b.geom.pages;
+    const uint32_t cap = b.table_width << shift, free = min(pool[0], pages);
+    uint32_t back[kPlanEach], v[1] = {0}, before[1];
+#pragma unroll
+    for (uint32_t e = 0; e < kPlanEach; ++e) {
+        back[e] = 0;
+        if (e >= each || r0 + e >= n) continue;
+        const uint32_t i = r0 + e, length = min(lengths[i], cap), stay = min(length, keep[i]);
+        from[i] = (stay + ps - 1u) >> shift;
+        back[e] = ((length + ps - 1u) >> shift) - from[i];
+        if (stay != length) lengths[i] = stay;
+        v[0] += back[e];
+    }
+    scan<1>(v, before, 0x7fffffffu, between);
+    uint32_t at = before[0];
+#pragma unroll
+    for (uint32_t e = 0; e < kPlanEach; ++e) {
+        at += back[e];
+        if (e < each && r0 + e < n) end[r0 + e] = at;
+    }
+    __syncthreads();
+    const uint32_t all = end[n - 1u];
+    for (uint32_t g = tid; g < all; g += kPlanThreads) {
+        const uint32_t i = owner_of(end, n, g), k = g - (i ? end[i - 1u] : 0u);
+        uint32_t *const entry = tables + (size_t)i * b.table_width + from[i] + k;
+        if (g < pages - free) pool[1u + free + g] = *entry;
+        *entry = VX_PAGED_NONE;
+    }
+    if (tid == 0) pool[0] = free + min(all, pages - free);
+}
+
+// ------------------------------------------------------------------- rows
+// A workgroup per run (rows of one request in one page) and KV head: lanes of eight dimensions,
+// 256 / (HD / 8) slots at once. K's eighths go out as they are; V's are transposed through LDS, and
+// a lane then owns an octet of slots of one dimension.
+template <int HD, bool BOUNDS>
+__global__ __launch_bounds__(256) void k_paged_store(PagedStore a) {
+    constexpr int W = HD / 8, R = 256 / W;
+    __shared__ __attribute__((aligned(16))) _Float16 rows[R][HD + 8];
+    const uint32_t tid = threadIdx.x, r = tid / W, c = tid % W, heads = a.b.geom.kv_heads;
+    const uint32_t run = blockIdx.x / heads, head = blockIdx.x % heads, ps = a.b.geom.page_size, shift = 31u - __clz(ps);
+    if (run >= min(a.plan[4], a.s.runs)) return;
+    const PagedRun at = reinterpret_cast<const PagedRun *>(a.plan + a.s.run_at)[run];
+    const uint32_t page = at.slot >> shift, first = at.slot & (ps - 1u);
+    if (at.slot == VX_PAGED_NONE || page >= a.b.geom.pages || at.n > ps - first || at.row >= a.b.max_rows ||
+        at.n > a.b.max_rows - at.row)
+        return;
+    const uint32_t end = first + at.n;
+    const size_t in_cache = (((size_t)a.layer * a.b.geom.pages + page) * heads + head) * ps * HD;   // values
+    _Float16 *const kc = reinterpret_cast<_Float16 *>(a.kc) + in_cache, *const vc = reinterpret_cast<_Float16 *>(a.vc) + in_cache;
+    h8 lo = (h8)((_Float16)INFINITY), hi = -lo;
+    uint32_t bad = 0;
+    auto bound = [&](h8 x) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bad |= x[i] != x[i] ? 1u << i : 0u;
+        lo = __builtin_elementwise_min(lo, x);
+        hi = __builtin_elementwise_max(hi, x);
+    };
+    for (uint32_t s0 = BOUNDS ? 0u : first / 8u * 8u; s0 < end; s0 += R) {
+        const uint32_t s = s0 + r;
+        const bool live = s >= first && s < end;
+        _Float16 *const to = kc + ((s / 16u * W + c) * 16u + s % 16u) * 8u;
+        if (BOUNDS && s < first) bound(*reinterpret_cast<const h8 *>(to));
+        float x[8], y[8];
+        if (live) {
+            const size_t row = at.row + s - first;
+            load8(a.k + row * a.k_stride + head * HD + c * 8u, a.vec, x);
+            load8(a.v + row * a.v_stride + head * HD + c * 8u, a.vec, y);
+            h8 kx, vx;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) kx[i] = (_Float16)x[i], vx[i] = (_Float16)y[i];
+            *reinterpret_cast<h8 *>(to) = kx;
+            if (BOUNDS) bound(kx);
+            *reinterpret_cast<h8 *>(&rows[r][c * 8u]) = vx;
+        }
+        __syncthreads();
+        const uint32_t o = tid / HD * 8u, dim = tid % HD, so = s0 + o;   // R / 8 octets of HD dimensions
+        _Float16 *const vt = vc + ((size_t)(so / 8u) * HD + dim) * 8u;
+        if (so >= first && so + 8u <= end) {
+            h8 x;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = rows[o + e][dim];
+            *reinterpret_cast<h8 *>(vt) = x;
+        } else if (so + 8u > first && so < end) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (so + e >= first && so + e < end) vt[e] = rows[o + e][dim];
+        }
+        __syncthreads();
+    }
+    if constexpr (BOUNDS) {
+        __shared__ __attribute__((aligned(16))) _Float16 most[2][R][HD + 8];
+        const _Float16 nan = (_Float16)__builtin_nanf("");
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (bad >> i & 1u) lo[i] = hi[i] = nan;
+        *reinterpret_cast<h8 *>(&most[0][r][c * 8u]) = lo;
+        *reinterpret_cast<h8 *>(&most[1][r][c * 8u]) = hi;
+        __syncthreads();
+        for (uint32_t t = tid; t < 2u * HD; t += 256u) {
+            const uint32_t which = t / HD, dim = t % HD;
+            float x = (float)most[which][0][dim];
+#pragma unroll
+            for (int u = 1; u < R; ++u) {
+                const float y = (float)most[which][u][dim];
+                x = x != x ? x : y != y ? y : which ? fmaxf(x, y) : fminf(x, y);
+            }
+            reinterpret_cast<_Float16 *>(a.bounds)[(((size_t)a.layer * a.b.geom.pages + page) * heads + head) * 2u * HD + t] = (_Float16)x;
+        }
+    }
+}
+
+// ------------------------------------------------------------------- selection
+// The most that a key within a page's bounds can score: sum over the group's heads j and the
+// dimensions of max(q_j lo, q_j hi) = up . hi + down . lo, with up and down the sums over j of
+// max(q_j, 0) and min(q_j, 0). In 64 bits: the choice falls at a border between sums that 32 bits,
+// added up in one order or another, would swap.
+//
+// A page's order: sums as unsigned numbers that rise with them; NaN above all of them, pages that
+// stay in any case above that.
+constexpr uint64_t kHeld = ~0ull, kNaN = ~0ull - 1u;
+__device__ __forceinline__ uint64_t order_of(double x) {
+    if (x != x) return kNaN;
+    const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);   // -0 as 0
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+constexpr uint32_t kScorePages = 64;   // pages of a workgroup
+
+template <int HD>
+__global__ __launch_bounds__(256) void k_paged_score(PagedSelect a, uint32_t blocks) {
+    constexpr int L = HD / 4;              // lanes of a page: eight values each of lo, then hi
+    constexpr int AT = 64 / L;             // pages of a wave at once
+    constexpr int P = kScorePages / 4;     // pages of a wave
+    __shared__ double ends[2][HD];         // down, up
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, w = tid >> 6, heads = a.b.geom.kv_heads;
+    const uint32_t pair = blockIdx.x / blocks, block = blockIdx.x % blocks;
+    const uint32_t row = pair / heads, head = pair % heads, shift = 31u - __clz(a.b.geom.page_size);
+    const uint32_t request = a.plan[a.s.requests + row], position = a.plan[a.s.positions + row];
+    if (request >= a.b.requests) return;
+    const uint32_t last = min(position >> shift, a.b.table_width - 1u);
+    if (block * kScorePages > last) return;
+    const uint32_t group = a.b.q_heads / heads;
+    const float *const q = a.q + (size_t)row * a.q_stride + (size_t)head * group * HD;
+    for (uint32_t d = tid; d < (uint32_t)HD; d += 256u) {
+        double up = 0, down = 0;
+        for (uint32_t j = 0; j < group; ++j) {
+            const float x = q[(size_t)j * HD + d];
+            up += x > 0.f || x != x ? (double)x : 0.0;
+            down += x < 0.f || x != x ? (double)x : 0.0;
+        }
+        ends[0][d] = down;
+        ends[1][d] = up;
+    }
+    __syncthreads();
+    double coef[8];
+    const uint32_t l = lane % L;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) coef[i] = ends[l / (L / 2)][l % (L / 2) * 8 + i];
+    uint64_t *const to = a.scratch + ((size_t)row * heads + head) * a.b.table_width;
+    for (uint32_t k = block * kScorePages + w * P, end = k + P; k <= last; k += AT) {
+        if (k == end) {            // the workgroup's next pages
+            k += blocks * kScorePages - P;
+            end = k + P;
+            if (k > last) break;
+        }
+        const uint32_t p = k + lane / L;
+        const bool there = p <= last;
+        const uint32_t page = there ? a.tables[(size_t)request * a.b.table_width + p] : VX_PAGED_NONE;
+        double s = 0;
+        if (page < a.b.geom.pages) {
+            const h8 x = reinterpret_cast<const h8 *>(a.bounds)[(((size_t)a.layer * a.b.geom.pages + page) * heads + head) * L + l];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += coef[i] * (double)(float)x[i];
+        } else {
+            s = __builtin_nan("");
+        }
+#pragma unroll
+        for (int d = L / 2; d; d >>= 1) s += __shfl_xor(s, d, 64);
+        if (there && l == 0) to[p] = p < a.sinks || last - p < a.recent ? kHeld : order_of(s);
+    }
+}
+
+// A workgroup a row and KV head: the order of the budget-th page by eight digits of eight bits,
+// then the pages above it, and of those equal to it the first.
+constexpr uint32_t kChoose = 512;
+__global__ __launch_bounds__(512) void k_paged_choose(PagedSelect a) {
+    __shared__ uint32_t bins[256], between[kChoose / 64][2], chosen[2];
+    const uint32_t tid = threadIdx.x, heads = a.b.geom.kv_heads, row = blockIdx.x / heads, head = blockIdx.x % heads;
+    const uint32_t shift = 31u - __clz(a.b.geom.page_size);
+    const uint32_t request = a.plan[a.s.requests + row], position = a.plan[a.s.positions + row];
+    uint32_t *const out = a.selected + ((size_t)row * heads + head) * a.budget;
+    const uint32_t n = request < a.b.requests ? min(position >> shift, a.b.table_width - 1u) + 1u : 0u;
+    if (n <= a.budget) {
+        for (uint32_t k = tid; k < a.budget; k += kChoose) out[k] = k < n ? k : VX_PAGED_NONE;
+        return;
+    }
+    const uint64_t *const keys = a.scratch + ((size_t)row * heads + head) * a.b.table_width;
+    uint64_t prefix = 0;
+    uint32_t left = a.budget;      // pages to take of those that agree with the prefix
+    for (int digit = 56; digit >= 0; digit -= 8) {
+        if (tid < 256u) bins[tid] = 0;
+        __syncthreads();
+        for (uint32_t k = tid; k < n; k += kChoose) {
+            const uint64_t x = keys[k];
+            if (digit == 56 || x >> (digit + 8) == prefix) atomicAdd(&bins[x >> digit & 255u], 1u);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            uint32_t above = 0;
+            int b = 255;
+            for (; b > 0 && above + bins[b] < left; --b) above += bins[b];
+            chosen[0] = (uint32_t)b;
+            chosen[1] = left - above;
+        }
+        __syncthreads();
+        prefix = prefix << 8 | chosen[0];
+        left = chosen[1];
+        __syncthreads();
+    }
+    // in rising order: a thread has pages one behind the other
+    const uint32_t each = (n + kChoose - 1u) / kChoose, k0 = min(tid * each, n), k1 = min(k0 + each, n);
+    uint32_t v[2] = {0, 0};        // above, equal
+    for (uint32_t k = k0; k < k1; ++k) v[0] += keys[k] > prefix, v[1] += keys[k] == prefix;
+    uint32_t before[2];
+    scan<2>(v, before, 0x7fffffffu, between);
+    uint32_t above = before[0], equal = before[1];
+    for (uint32_t k = k0; k < k1; ++k) {
+        const uint64_t x = keys[k];
+        const bool take = x > prefix || (x == prefix && equal < left);
+        if (take) out[above + min(equal, left)] = k;
+        above += x > prefix;
+        equal += x == prefix;
+    }
+}
+
+}  // namespace
+
+int launch_paged_reset(hipStream_t s, const vx_paged_batch &b, uint32_t *lengths, uint32_t *tables, uint32_t *pool) {
+    const uint64_t n = std::max<uint64_t>(std::max<uint64_t>(b.requests, (uint64_t)b.requests * b.table_width), b.geom.pages);
+    k_paged_reset<<<(uint32_t)std::min<uint64_t>((n + 255u) / 256u, 4096u), 256, 0, s>>>(b, lengths, tables, pool);
+    VX_LAUNCHED("k_paged_reset");
+    return VX_OK;
+}
+
+int launch_paged_plan(hipStream_t s, const PagedPlan &a) {
+    const uint32_t most = std::max(std::max(a.b.max_rows, a.b.requests), a.s.items);
+    k_paged_plan<<<std::min((most + kPlanThreads - 1u) / kPlanThreads, 64u), kPlanThreads, 0, s>>>(a);
+    VX_LAUNCHED("k_paged_plan");
+    return VX_OK;
+}
+
+int launch_paged_advance(hipStream_t s, const vx_paged_batch &b, const uint32_t *plan, uint32_t *lengths, uint32_t *pool) {
+    k_paged_advance<<<(b.requests + 255u) / 256u, 256, 0, s>>>(b, plan, paged_shape(b).granted, lengths, pool);
+    VX_LAUNCHED("k_paged_advance");
+    return VX_OK;
+}
+
+int launch_paged_cut(hipStream_t s, const vx_paged_batch &b, const uint32_t *keep, uint32_t *lengths, uint32_t *tables,
+                     uint32_t *pool) {
+    k_paged_cut<<<1, kPlanThreads, 0, s>>>(b, keep, lengths, tables, pool);
+    VX_LAUNCHED("k_paged_cut");
+    return VX_OK;
+}
+
+#define PAGED_HD(hd, call)                \
+    switch (hd) {                         \
+        case 64: call(64); break;         \
+        case 128: call(128); break;       \
+        default: call(256); break;        \
+    }
+
+int launch_paged_store(hipStream_t s, const PagedStore &a) {
+    const dim3 grid(a.s.runs * a.b.geom.kv_heads);
+#define CALL(HD)                                        \
+    if (a.bounds)                                       \
+        k_paged_store<HD, true><<<grid, 256, 0, s>>>(a); \
+    else                                                \
+        k_paged_store<HD, false><<<grid, 256, 0, s>>>(a)
+    PAGED_HD(a.b.geom.head_dim, CALL)
+#undef CALL
+    VX_LAUNCHED("k_paged_store");
+    return VX_OK;
+}
+
+uint64_t paged_select_scratch_bytes(const vx_paged_batch &b) {
+    return (uint64_t)b.max_rows * b.geom.kv_heads * b.table_width * 8u;
+}
+
+int launch_paged_select(hipStream_t s, const PagedSelect &a) {
+    const uint32_t pairs = a.b.max_rows * a.b.geom.kv_heads;
+    // at most 2^14 workgroups, or one a pair: the pages beyond are taken in turns
+    const uint32_t blocks = std::min((a.b.table_width + kScorePages - 1u) / kScorePages, std::max(16384u / pairs, 1u));
+#define CALL(HD) k_paged_score<HD><<<blocks * pairs, 256, 0, s>>>(a, blocks)
+    PAGED_HD(a.b.geom.head_dim, CALL)
+#undef CALL
+    VX_LAUNCHED("k_paged_score");
+    k_paged_choose<<<pairs, kChoose, 0, s>>>(a);
+    VX_LAUNCHED("k_paged_choose");
+    return VX_OK;
+}
+
+}  // namespace vx

@@ -1,0 +1,690 @@
+// Attention over the paged KV cache (include/voxhip.h, vx_paged_attention): all pages that a row
+// attends to, or those of a selection.
+//
+// With S^T = K . Q^T and O^T = V^T . P^T, a lane of v_mfma_f32_16x16x32_f16 holds as its A operand
+// eight values along the summed axis of one row: of K eight dimensions of a slot, of V^T eight
+// slots of a dimension, 16 bytes each as the pages have them. Which row of the first product is
+// which slot is free, so K's slots are taken in the order that leaves each lane with eight
+// consecutive slots of its query row in S^T: the P^T operand of the second product, already in the
+// lane's registers. Keys go by chunks of 32 slots, of two units of 16; a unit lies in one page, and
+// K's and V's 16 slots at the same 32 * head_dim bytes of their caches.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_dev.h"
+#include "paged.h"
+
+namespace vx {
+namespace {
+
+constexpr uint32_t kFar = 1u << 30;   // the position of a unit that holds no slots: above every row's
+
+struct AttnArgs {
+    PagedAttn a;
+    uint32_t group, by_group;        // query heads a KV head; 2^32 / group, rounded up (0 where group is 1)
+    uint32_t shift, units;           // log2 of the page size, units of a page
+    size_t layer_at;                 // bytes of the layers before
+    uint32_t tiles, splits, per;     // of a selection: tiles of a row, splits of its list, chunks of one
+    float *ml, *acc;                 // [KV head][part][tile rows][2], [..][tile rows][HD]
+    uint32_t parts;                  // of one KV head
+};
+
+// The token of a row. The product with 2^32 / group rounded up is exact for rows below 2^22
+// and groups up to 2^10: it is over by less than 2^22 2^10 / 2^32 / group.
+__device__ __forceinline__ uint32_t token_of(const AttnArgs &p, uint32_t row) {
+    return p.by_group ? __umulhi(row, p.by_group) : row;
+}
+
+// A tile of query rows: those of one request from `tile` on, the request's row 0 being row `row`
+// of the step at position `base`. In bounds whatever the plan's buffer holds.
+struct Tile {
+    uint32_t request, row, base, count, tile, first, n, part;
+    bool ok;
+};
+__device__ __forceinline__ Tile tile_of(const AttnArgs &p, uint32_t index) {
+    const PagedAttn &a = p.a;
+    Tile t;
+    if (a.selected) {
+        const uint32_t split = index % p.splits, rest = index / p.splits;
+        t.row = rest / p.tiles;
+        t.tile = rest % p.tiles * a.s.tile_rows;
+        t.request = a.plan[a.s.requests + t.row];
+        t.base = a.plan[a.s.positions + t.row];
+        t.count = 1;
+        t.ok = t.request < a.b.requests && t.base < a.b.table_width << p.shift;
+        const uint32_t pages = min(a.budget, (t.base >> p.shift) + 1u), chunks = ((pages << p.shift) + 31u) / 32u;
+        t.first = split * p.per;
+        t.n = t.first < chunks ? min(p.per, chunks - t.first) : 0u;
+        t.part = chunks > p.per ? index : VX_PAGED_NONE;
+        return t;
+    }
+    const PagedItem it = reinterpret_cast<const PagedItem *>(a.plan + a.s.item_at)[index];
+    t = {it.request, it.row, it.base, it.count, it.tile, it.first, it.n, it.part, false};
+    const uint32_t cap = a.b.table_width << p.shift;
+    t.ok = index < a.plan[5] && it.request < a.b.requests && it.row < a.b.max_rows && it.count <= a.b.max_rows - it.row &&
+           it.base <= cap && it.count <= cap - it.base && it.tile < it.count * p.group &&
+           (it.part < p.parts || it.part == VX_PAGED_NONE) && it.first <= cap && it.n <= cap;
+    return t;
+}
+
+// Into scalar registers: the compiler does not see that loads by the workgroup's index are uniform.
+__device__ __forceinline__ Tile uniform(Tile t) {
+    uint32_t *const f[8] = {&t.request, &t.row, &t.base, &t.count, &t.tile, &t.first, &t.n, &t.part};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) *f[k] = __builtin_amdgcn_readfirstlane(*f[k]);
+    t.ok = __builtin_amdgcn_readfirstlane(t.ok) != 0;
+    return t;
+}
+
+// Sixteen query rows as the B operand: lane (i, q) holds row i, dimensions 32 u + 8 q + 0..7 in
+// step u; split() makes two f16 terms of the row, with log2(e) / sqrt(HD) in it and scaled, and
+// returns the scale that is left to the scores. It is a power of two: products with it are exact,
+// so that a score less the reference, an fma, is what it would be of rounded scores.
+template <int HD>
+struct QRow {
+    static constexpr int U = HD / 32;
+    float x[U][8];
+    __device__ __forceinline__ void load(const AttnArgs &p, const Tile &t, uint32_t head, uint32_t row, bool valid, uint32_t q) {
+        const uint32_t k = token_of(p, row), j = row - k * p.group;
+        const float *src = p.a.q + (size_t)(t.row + k) * p.a.q_stride + (size_t)(head * p.group + j) * HD + q * 8u;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (valid) {
+                load8(src + 32 * u, p.a.qvec, x[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ float split(h8 *qh, h8 *ql) const {
+        float top = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[u][i]));
+        constexpr float c = kLog2e / (HD == 64 ? 8.0f : HD == 128 ? 11.3137085f : 16.0f);
+        const int e = scale_of(row_max(top) * c);
+        const float up = ldexpf(c, 10 - e);
+#pragma unroll
+        for (int u = 0; u < U; ++u) split8(x[u], up, qh[u], ql[u]);
+        return ldexpf(1.0f, e - 10);
+    }
+};
+
+// A lane's share of a chunk of K: for both of the product's row tiles tt, slot 8 (i / 4) + 4 tt +
+// i % 4. Lane (i, q) of the product S^T then holds the scores of query row i and slots 8 q + 4 tt + r:
+// eight consecutive ones.
+template <int HD>
+struct KFrag {
+    static constexpr int U = HD / 32;
+    h8 x[2][U];
+    __device__ __forceinline__ void load(const uint8_t *unit, uint32_t i, uint32_t q) {
+        const uint8_t *const at = unit + (8u * (i / 4u % 2u) + i % 4u) * 16u + q * 256u;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[tt][u] = *reinterpret_cast<const h8 *>(at + tt * 64 + u * 1024);
+    }
+};
+// Of V^T: octet q of the chunk's slots, dimensions 16 dt + i.
+template <int HD>
+struct VFrag {
+    static constexpr int DT = HD / 16;
+    h8 x[DT];
+    __device__ __forceinline__ void load(const uint8_t *unit, uint32_t i, uint32_t q) {
+        const uint8_t *const at = unit + (q % 2u) * (HD * 16u) + i * 16u;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) x[dt] = *reinterpret_cast<const h8 *>(at + dt * 256);
+    }
+};
+
+typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+// All ones in the first n of eight halves.
+__device__ __forceinline__ U4 halves_below(uint32_t n) {
+    U4 m;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) m[k] = n > 2u * k + 1u ? ~0u : n > 2u * k ? 0xffffu : 0u;
+    return m;
+}
+__device__ __forceinline__ bool finite(_Float16 x) {
+    return (__builtin_bit_cast(uint16_t, x) & 0x7c00u) != 0x7c00u;
+}
+
+// One workgroup: a tile of 16 NT query rows (tokens x the KV head's query heads) of a request over
+// a part of its chunks, which the waves take in turn, each with its own running maximum and sum;
+// they join in LDS. A tile with one part is finished here, the others' partial sums go to scratch.
+// PK, of at most eight rows: columns 0..7 of the products take the high terms of the rows,
+// columns 8..15 the low ones, so that one product does for both; the scores of the two
+// columns of a row are added, and so are its sums at the end.
+template <int HD, int NT, int W, bool PK>
+__global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_attn(AttnArgs p) {
+    constexpr int U = HD / 32, DT = HD / 16, OROW = HD + 4, R = 16 * NT, RT = PK ? 8 : R, B = W > 4 ? W / 2 : W;
+    constexpr int QLDS = NT > 1 ? R * HD : 0;   // floats: two f16 planes
+    constexpr int LDS = B * R * OROW > QLDS ? B * R * OROW : QLDS;
+    constexpr size_t UNIT = 32 * HD;            // bytes
+    __shared__ __attribute__((aligned(16))) float lds[LDS];
+    static_assert((!PK || NT == 1) && (W == 4 || (W == 8 && NT > 1)), "one column tile of both terms; a wave or two a SIMD");
+    __shared__ float ms[W][R], ls[W][R], fs[R];
+    // by dimension the first position of a +inf or NaN in V, and of a -inf or NaN
+    __shared__ uint32_t odd[2][HD], odd_in[W];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t heads = p.a.b.geom.kv_heads, head = blockIdx.x % heads;
+    const Tile t = uniform(tile_of(p, blockIdx.x / heads));
+    if (!t.ok || t.n == 0) return;
+    const uint32_t rows = t.count * p.group, r0 = t.tile, ri = PK ? i & 7u : i;
+    const uint32_t sees_all = t.base + token_of(p, r0);                               // last position that every row attends to
+    const uint32_t last_pos = t.base + token_of(p, min(r0 + RT, rows) - 1u);          // and that some row does
+    const uint8_t *const kc = p.a.kc + p.layer_at, *const vc = p.a.vc + p.layer_at;
+
+    // The wave's chunks t.first + w + W j: lane 2 j + h holds unit h of the j-th, 32 chunks at once.
+    uint32_t unit = 0, where = kFar;
+    auto look_up = [&](uint32_t j0) {
+        const uint32_t c = w + W * (j0 + lane / 2u), at = (t.first + c) * 32u + kPagedUnit * (lane & 1u);
+        unit = 0;
+        where = kFar;
+        if (c >= t.n) return;
+        uint32_t index = at >> p.shift;
+        if (p.a.selected) {
+            index = index < min(p.a.budget, (t.base >> p.shift) + 1u)
+                        ? p.a.selected[((size_t)t.row * heads + head) * p.a.budget + index] : VX_PAGED_NONE;
+            if (index > t.base >> p.shift) return;
+        }
+        if (index >= p.a.b.table_width) return;
+        const uint32_t off = at & (p.a.b.geom.page_size - 1u), pos = (index << p.shift) + off;
+        if (pos > last_pos) return;
+        const uint32_t page = p.a.tables[(size_t)t.request * p.a.b.table_width + index];
+        if (page >= p.a.b.geom.pages) return;
+        unit = (page * heads + head) * p.units + off / kPagedUnit;
+        where = pos;
+    };
+    auto unit_of = [&](uint32_t j, bool second) {   // bytes
+        const uint32_t u0 = __builtin_amdgcn_readlane(unit, (j & 31u) * 2u), u1 = __builtin_amdgcn_readlane(unit, (j & 31u) * 2u + 1u);
+        return (size_t)(second ? u1 : u0) * UNIT;
+    };
+    look_up(0);
+    const uint32_t mine = t.n > w ? (t.n - w + W - 1u) / W : 0u;   // the wave's chunks
+    KFrag<HD> kf;
+    // K of a chunk is fetched before the one ahead is done with, where registers allow.
+    constexpr bool AHEAD = NT == 1;
+    if (AHEAD && mine) kf.load(kc + unit_of(0, i >= 8u), i, q);
+
+    for (uint32_t d = tid; d < 2u * HD; d += 64u * W) odd[d / HD][d % HD] = ~0u;
+    uint32_t found = 0;
+    h8 qh[U], ql[U];
+    float factor[NT];
+    h8 *const qs = reinterpret_cast<h8 *>(lds);   // [NT][U][hi, lo][64]
+    if constexpr (NT == 1) {
+        QRow<HD> qr;
+        qr.load(p, t, head, min(r0 + ri, rows - 1u), r0 + ri < rows, q);
+        factor[0] = qr.split(qh, ql);
+        if constexpr (PK) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) qh[u] = i < 8u ? qh[u] : ql[u];
+        }
+    } else {
+        for (uint32_t c = w; c < NT; c += W) {
+            const uint32_t row = r0 + 16u * c + i;
+            QRow<HD> qr;
+            qr.load(p, t, head, min(row, rows - 1u), row < rows, q);
+            const float f = qr.split(qh, ql);
+            if (q == 0) fs[16u * c + i] = f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                qs[((c * U + u) * 2u) * 64u + lane] = qh[u];
+                qs[((c * U + u) * 2u + 1u) * 64u + lane] = ql[u];
+            }
+        }
+    }
+    if constexpr (NT > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < NT; ++c) factor[c] = fs[16 * c + i];
+    }
+    // last position that the lane's row of a column tile attends to
+    auto limit = [&](int c) { return t.base + token_of(p, min(r0 + 16u * c + ri, rows - 1u)); };
+
+    float m[NT], l[NT];
+    bool saw[NT];   // the lane's row attends to some slot
+    f4 o[NT][DT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        saw[c] = false;
+        m[c] = -INFINITY;
+        l[c] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[c][dt] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    float minus = PK && i < 8u ? 0.0f : -1.0f;
+    asm("" : "+v"(minus));
+    const bool partly = last_pos != sees_all;   // some row does not attend to all that another does
+
+    // A chunk; at an edge, some row attends to a part of it only.
+    auto step = [&](uint32_t j, uint32_t w0, uint32_t w1, auto at_edge) {
+        constexpr bool edge = decltype(at_edge)::value;
+        VFrag<HD> vf;
+        const uint8_t *const vu = vc + unit_of(j, q >= 2u);
+        if constexpr (AHEAD)
+            vf.load(vu, i, q);
+        else
+            kf.load(kc + unit_of(j, i >= 8u), i, q);
+        // Behind the last chunk unit 0 is fetched once more, which is cheaper than a branch: in one between
+        // the products and what reads them, this compiler lost count of the wait that that needs.
+        if (((j + 1u) & 31u) == 0) look_up(j + 1u);
+        const uint8_t *const ku = kc + unit_of(j + 1u, i >= 8u);
+        f4 x[NT][2];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) x[c][0] = x[c][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                const h8 hi = NT == 1 ? qh[u] : qs[((c * U + u) * 2u) * 64u + lane];
+                const h8 lo = NT == 1 ? ql[u] : qs[((c * U + u) * 2u + 1u) * 64u + lane];
+                x[c][0] = mfma16(kf.x[0][u], hi, x[c][0]);
+                x[c][1] = mfma16(kf.x[1][u], hi, x[c][1]);
+                if constexpr (!PK) {
+                    x[c][0] = mfma16(kf.x[0][u], lo, x[c][0]);
+                    x[c][1] = mfma16(kf.x[1][u], lo, x[c][1]);
+                }
+            }
+        }
+        if constexpr (AHEAD)
+            kf.load(ku, i, q);
+        else
+            vf.load(vu, i, q);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (PK) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[0][e / 4][e % 4] += dpp<0x128>(x[0][e / 4][e % 4]);   // row_ror:8
+        }
+        const uint32_t slot0 = (q < 2u ? w0 : w1) + 8u * (q % 2u);   // the lane's first position
+        if constexpr (edge) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                const uint32_t last = limit(c);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[c][e / 4][e % 4] = slot0 + e > last ? -INFINITY : x[c][e / 4][e % 4];
+                saw[c] = saw[c] || slot0 <= last;
+            }
+        }
+        if constexpr (!edge) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) saw[c] = true;
+        }
+        float top[NT];
+        bool moves = false;
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            top[c] = x[c][0][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) top[c] = fmaxf(top[c], x[c][e / 4][e % 4]);
+            top[c] *= factor[c];
+            moves = moves || top[c] - m[c] > kMost;
+        }
+        if (__builtin_expect(__any(moves), 0)) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                const float s = row_max(top[c]), mn = s - m[c] > kMost ? s - kRaise : m[c];
+                const float alpha = mn == m[c] ? 1.f : __builtin_amdgcn_exp2f(m[c] - mn);
+                m[c] = mn;
+                l[c] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[c][dt] *= alpha;
+            }
+        }
+        h8 ph[NT], pl[NT];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            // A row that attends to nothing of the chunks so far has no reference yet; any serves.
+            const float ref = m[c] == -INFINITY ? 0.f : m[c];
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[c][e / 4][e % 4], factor[c], -ref));
+                l[c] += v[e];
+            }
+            two_terms(v, minus, ph[c], pl[c]);   // of PK the term of the lane's column, by `minus`
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (edge) {
+            // Slots behind the last position may hold anything: their values count as zero, as do
+            // infinities and NaN among those that some row does not attend to, which `odd` notes.
+            const U4 keep = halves_below(last_pos + 1u > slot0 ? last_pos + 1u - slot0 : 0u);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) vf.x[dt] = __builtin_bit_cast(h8, __builtin_bit_cast(U4, vf.x[dt]) & keep);
+            if (partly) {
+                const U4 own = ~halves_below(sees_all + 1u > slot0 ? sees_all + 1u - slot0 : 0u);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    const U4 x = __builtin_bit_cast(U4, vf.x[dt]);
+                    const U4 top = ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u;   // of each half whose exponent is all ones
+                    const U4 bad = (top | (top - (top >> 15))) & own;
+                    found |= (bad[0] | bad[1]) | (bad[2] | bad[3]);
+                    vf.x[dt] = __builtin_bit_cast(h8, x & ~bad);
+                }
+            }
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) o[c][dt] = mfma16(vf.x[dt], PK ? pl[c] : ph[c], o[c][dt]);
+            if constexpr (!PK) {
+#pragma unroll
+                for (int c = 0; c < NT; ++c) o[c][dt] = mfma16(vf.x[dt], pl[c], o[c][dt]);
+            }
+        }
+    };
+    for (uint32_t j = 0; j < mine; ++j) {
+        const uint32_t w0 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u), w1 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u + 1u);
+        if (max(w0, w1) + kPagedUnit - 1u <= sees_all)
+            step(j, w0, w1, std::false_type{});
+        else
+            step(j, w0, w1, std::true_type{});
+    }
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        l[c] = row_sum(l[c]);
+        if (row_max(saw[c] ? 1.f : 0.f) == 0.f) l[c] = -1.f;   // nothing to add
+        if (q == 0) ms[w][16 * c + i] = m[c], ls[w][16 * c + i] = l[c];
+    }
+    // Infinities in V have no two terms to be multiplied by, and some were taken as zero: where a sum
+    // is not finite or such a value was found, the chunks are gone through again (rare).
+    float zero = found ? __builtin_nanf("") : 0.f;
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) zero = __builtin_fmaf(o[c][dt][e], 0.f, zero);
+    const bool finite_here = __all(zero == 0.f);
+    if (lane == 0) odd_in[w] = !finite_here;
+    __syncthreads();   // the queries in LDS have been read, every wave's m and l are there
+    bool any_odd = false;
+#pragma unroll
+    for (int v = 0; v < W; ++v) any_odd = any_odd || odd_in[v] != 0;
+    if (__builtin_expect(any_odd, 0)) {
+        for (uint32_t j = 0; j < mine; ++j) {
+            if ((j & 31u) == 0) look_up(j);
+            const uint32_t w0 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u), w1 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u + 1u);
+            const uint32_t slot0 = (q < 2u ? w0 : w1) + 8u * (q % 2u);
+            const uint8_t *const at = vc + unit_of(j, q >= 2u) + (q % 2u) * (HD * 16u) + i * 16u;
+#pragma unroll 1
+            for (int dt = 0; dt < DT; ++dt) {
+                const h8 x = *reinterpret_cast<const h8 *>(at + dt * 256);
+                uint32_t up = ~0u, down = ~0u;
+#pragma unroll
+                for (int e = 7; e >= 0; --e) {
+                    const bool counts = !finite(x[e]) && slot0 + e <= last_pos;
+                    up = counts && !(x[e] < 0.f16) ? slot0 + e : up;
+                    down = counts && !(x[e] > 0.f16) ? slot0 + e : down;
+                }
+                if (up != ~0u) atomicMin(&odd[0][16 * dt + i], up);
+                if (down != ~0u) atomicMin(&odd[1][16 * dt + i], down);
+            }
+        }
+    }
+
+    // A wave's sums are taken to the row's largest reference. One without keys has nothing
+    // to give; one whose every score is NaN has no reference but a NaN sum.
+    constexpr int PART = W > B ? R / 2 : R;   // rows of a wave's part
+    auto *const os = reinterpret_cast<float (*)[PART][OROW]>(lds);
+    float sum[NT], top[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        // the waves' by the four lanes of a row
+        float mv[W / 4], lv[W / 4];
+#pragma unroll
+        for (int v = 0; v < W / 4; ++v) mv[v] = ms[4 * v + q][16 * c + i], lv[v] = ls[4 * v + q][16 * c + i];
+        top[c] = row_max(W > 4 ? fmaxf(mv[0], mv[W / 4 - 1]) : mv[0]);
+        sum[c] = 0.f;
+#pragma unroll
+        for (int v = 0; v < W / 4; ++v)
+            sum[c] += lv[v] < 0.f ? 0.f : mv[v] == -INFINITY ? lv[v] : lv[v] * __builtin_amdgcn_exp2f(mv[v] - top[c]);
+        sum[c] = row_sum(sum[c]);
+        if (row_max(lv[0] < 0.f && lv[W / 4 - 1] < 0.f ? 0.f : 1.f) == 0.f) sum[c] = -1.f;
+        const float share = m[c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[c] - top[c]);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[c][dt] *= share;
+    }
+    if constexpr (W > B) {
+        // Waves w and w + 4 exchange halves of their tiles, so that all write and read: each adds
+        // the partner's half to its own, in the partner's part of LDS.
+        constexpr int H = NT / 2;
+        auto give = [&](auto upper) {
+#pragma unroll
+            for (int c = 0; c < H; ++c)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+                    *reinterpret_cast<f4 *>(&os[w][16 * c + i][16 * dt + 4 * q]) = o[decltype(upper)::value ? c : H + c][dt];
+        };
+        auto take = [&](auto upper) {
+#pragma unroll
+            for (int c = 0; c < H; ++c)
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    f4 *const at = reinterpret_cast<f4 *>(&os[w ^ B][16 * c + i][16 * dt + 4 * q]);
+                    *at = *at + o[decltype(upper)::value ? H + c : c][dt];
+                }
+        };
+        if (w < B)
+            give(std::false_type{});
+        else
+            give(std::true_type{});
+        __syncthreads();
+        if (w < B)
+            take(std::false_type{});
+        else
+            take(std::true_type{});
+    } else {
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f4 *>(&os[w][16 * c + i][16 * dt + 4 * q]) = o[c][dt];
+    }
+    const bool alone = t.part == VX_PAGED_NONE;
+    const size_t part = (size_t)head * p.parts + (alone ? 0u : t.part);
+    if (w == 0 && q == 0) {   // the factors of the scores have been read, a barrier ago and more
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            fs[16 * c + i] = sum[c];
+            if (alone || (PK && i >= 8u)) continue;
+            p.ml[(part * RT + 16u * c + i) * 2u] = top[c];
+            p.ml[(part * RT + 16u * c + i) * 2u + 1u] = sum[c];
+        }
+    }
+    __syncthreads();
+    constexpr int V = HD / 4;   // four dimensions a lane
+    for (uint32_t k = tid; k < (uint32_t)RT * V; k += 64u * W) {
+        const uint32_t r = k / V, c = 4u * (k % V), row = r0 + r;
+        if (row >= rows) break;
+        const uint32_t u0 = W > B && r < (uint32_t)PART ? B : 0u, at = r % (uint32_t)PART;   // a half's sums: in the other's parts
+        f4 v = *reinterpret_cast<const f4 *>(&os[u0][at][c]);
+#pragma unroll
+        for (int u = 1; u < B; ++u) v += *reinterpret_cast<const f4 *>(&os[u0 + u][at][c]);
+        if constexpr (PK) {
+#pragma unroll
+            for (int u = 0; u < B; ++u) v += *reinterpret_cast<const f4 *>(&os[u][r + 8u][c]);
+        }
+        const uint32_t k0 = token_of(p, row), j = row - k0 * p.group;
+        if (any_odd) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool up = odd[0][c + e] <= t.base + k0, down = odd[1][c + e] <= t.base + k0;
+                v[e] = up ? down ? __builtin_nanf("") : INFINITY : down ? -INFINITY : v[e];
+            }
+        }
+        if (!alone) {
+            *reinterpret_cast<f4 *>(p.acc + (part * RT + r) * HD + c) = v;
+            continue;
+        }
+        v = fs[r] < 0.f ? f4{0.f, 0.f, 0.f, 0.f} : v * (1.0f / fs[r]);   // attends to nothing: 0
+        float *const to = p.a.out + (size_t)(t.row + k0) * p.a.out_stride + (size_t)(head * p.group + j) * HD + c;
+        if (p.a.ovec) {
+            *reinterpret_cast<f4 *>(to) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[e] = v[e];
+        }
+    }
+}
+
+// The parts of a tile's row, joined: a workgroup a row, its lanes HD / 4 columns by as many parts at
+// once as fit.
+template <int HD>
+__global__ __launch_bounds__(256) void k_paged_join(AttnArgs p) {
+    constexpr int V = HD / 4, Y = 256 / V;
+    __shared__ float sc[kPagedMaxSplits], red[3][4];
+    __shared__ __attribute__((aligned(16))) float os[Y][HD];
+    const PagedAttn &a = p.a;
+    const uint32_t tid = threadIdx.x, heads = a.b.geom.kv_heads, head = blockIdx.x % heads, tile_rows = a.s.tile_rows;
+    const uint32_t r = blockIdx.x / heads % tile_rows, index = blockIdx.x / heads / tile_rows;
+    uint32_t step_row, base, first, n, row;   // the tile's request's first row, position of that; the parts; the query row
+    if (a.selected) {
+        step_row = index / p.tiles;
+        row = index % p.tiles * tile_rows + r;
+        base = a.plan[a.s.positions + step_row];
+        first = index * p.splits;
+        if (a.plan[a.s.requests + step_row] >= a.b.requests || row >= p.group || base >= a.b.table_width << p.shift) return;
+        const uint32_t pages = min(a.budget, (base >> p.shift) + 1u), chunks = ((pages << p.shift) + 31u) / 32u;
+        n = (chunks + p.per - 1u) / p.per;
+    } else {
+        if (index >= a.plan[6]) return;
+        const PagedJoin j = reinterpret_cast<const PagedJoin *>(a.plan + a.s.join_at)[index];
+        const uint32_t cap = a.b.table_width << p.shift;
+        if (j.row >= a.b.max_rows || j.count > a.b.max_rows - j.row || j.base > cap || j.count > cap - j.base ||
+            j.tile >= j.count * p.group || j.per == 0u || j.part >= p.parts)
+            return;
+        step_row = j.row;
+        base = j.base;
+        row = j.tile + r;
+        first = j.part;
+        if (row >= j.count * p.group) return;
+        const uint32_t last = base + token_of(p, min(j.tile + tile_rows, j.count * p.group) - 1u);
+        n = min((last / 32u + j.per) / j.per, p.parts - first);   // of the tile's chunks
+    }
+    if (n <= 1u || n > kPagedMaxSplits) return;
+    const size_t at = ((size_t)head * p.parts + first) * tile_rows + r;   // the row's record in the first part
+    const uint32_t c = 4u * (tid % V), y = tid / V;
+    float m = -INFINITY, l = -1.f;
+    if (tid < n) {
+        m = p.ml[(at + (size_t)tid * tile_rows) * 2u];
+        l = p.ml[(at + (size_t)tid * tile_rows) * 2u + 1u];
+    }
+    float top = m, some = l < 0.f ? 0.f : 1.f;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64)), some = fmaxf(some, __shfl_xor(some, d, 64));
+    if ((tid & 63u) == 0) red[0][tid >> 6] = top, red[1][tid >> 6] = some;
+    __syncthreads();
+    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    some = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+    const float mine = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+    if (tid < n) sc[tid] = mine;
+    float sum = l < 0.f ? 0.f : l * mine;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+    if ((tid & 63u) == 0) red[2][tid >> 6] = sum;
+    __syncthreads();
+    sum = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (uint32_t v = y; v < n; v += Y)
+        o += *reinterpret_cast<const f4 *>(p.acc + (at + (size_t)v * tile_rows) * HD + c) * sc[v];
+    *reinterpret_cast<f4 *>(&os[y][c]) = o;
+    __syncthreads();
+    if (tid < (uint32_t)HD) {
+        float x = os[0][tid];
+#pragma unroll
+        for (int u = 1; u < Y; ++u) x += os[u][tid];
+        const uint32_t k = token_of(p, row), j = row - k * p.group;
+        a.out[(size_t)(step_row + k) * a.out_stride + (size_t)(head * p.group + j) * HD + tid] = some == 0.f ? 0.f : x / sum;
+    }
+}
+
+// Of a selection: tiles of a row, and how its list is divided: so that about as many workgroups
+// come out as of a step without one, of least chunks or more.
+void divide(const vx_paged_batch &b, const PagedShape &s, uint32_t budget, uint32_t *tiles, uint32_t *splits, uint32_t *per) {
+    const uint32_t group = b.q_heads / b.geom.kv_heads;
+    *tiles = (group + s.tile_rows - 1u) / s.tile_rows;
+    const uint64_t chunks = ((uint64_t)std::min(budget, b.table_width) * b.geom.page_size + 31u) / 32u;
+    const uint64_t units = (uint64_t)b.max_rows * b.geom.kv_heads * *tiles;
+    uint64_t n = std::min<uint64_t>(std::max<uint64_t>((1u << s.workgroups) / units, 1u), kPagedMaxSplits);
+    *per = (uint32_t)std::max<uint64_t>((chunks + n - 1u) / n, s.least);
+    *splits = (uint32_t)((chunks + *per - 1u) / *per);
+}
+
+// A selection is each row's own: its tiles are a row's query heads.
+vx_paged_batch of_rows(vx_paged_batch b, uint32_t budget) {
+    if (budget) b.max_count = 1;
+    return b;
+}
+
+uint64_t parts_of(const vx_paged_batch &b, const PagedShape &s, uint32_t budget) {
+    if (!budget) return s.parts;
+    uint32_t tiles, splits, per;
+    divide(b, s, budget, &tiles, &splits, &per);
+    return splits > 1u ? (uint64_t)b.max_rows * tiles * splits : 0u;
+}
+
+template <int HD>
+void run(hipStream_t s, const AttnArgs &p, uint64_t grid) {
+    const dim3 g((uint32_t)grid);
+    if (p.a.s.packed)
+        k_paged_attn<HD, 1, 4, true><<<g, 256, 0, s>>>(p);
+    else if (p.a.s.tile_rows == 16u)
+        k_paged_attn<HD, 1, 4, false><<<g, 256, 0, s>>>(p);
+    else if constexpr (HD < 256)
+        k_paged_attn<HD, 2, 8, false><<<g, 512, 0, s>>>(p);
+}
+
+}  // namespace
+
+uint64_t paged_attn_scratch_bytes(const vx_paged_batch &batch, uint32_t budget) {
+    const vx_paged_batch b = of_rows(batch, budget);
+    const PagedShape s = paged_shape(b);
+    return parts_of(b, s, budget) * b.geom.kv_heads * s.tile_rows * (b.geom.head_dim + 2u) * 4u;
+}
+
+int launch_paged_attention(hipStream_t s, const PagedAttn &a) {
+    AttnArgs p{};
+    p.a = a;
+    const vx_paged_batch rows = of_rows(a.b, a.budget);
+    const vx_paged_geom &g = a.b.geom;
+    if (a.selected) {   // the plan stays where it is
+        const PagedShape own = paged_shape(rows);
+        p.a.s.tile_rows = own.tile_rows;
+        p.a.s.packed = own.packed;
+        divide(rows, own, a.budget, &p.tiles, &p.splits, &p.per);
+    }
+    p.group = a.b.q_heads / g.kv_heads;
+    p.by_group = p.group > 1u ? (uint32_t)(((1ull << 32) + p.group - 1u) / p.group) : 0u;
+    p.shift = paged_shift(g.page_size);
+    p.units = g.page_size / kPagedUnit;
+    p.layer_at = (size_t)a.layer * g.pages * g.kv_heads * g.page_size * g.head_dim * 2u;
+    p.parts = (uint32_t)parts_of(rows, a.selected ? paged_shape(rows) : a.s, a.budget);
+    const uint64_t records = (uint64_t)p.parts * g.kv_heads * p.a.s.tile_rows;
+    p.acc = a.scratch;
+    p.ml = a.scratch + records * g.head_dim;
+    const uint64_t items = a.selected ? (uint64_t)a.b.max_rows * p.tiles * p.splits : a.s.items;
+#define CALL(HD) run<HD>(s, p, items * g.kv_heads)
+    switch (g.head_dim) {
+        case 64: CALL(64); break;
+        case 128: CALL(128); break;
+        default: CALL(256); break;
+    }
+#undef CALL
+    VX_LAUNCHED("k_paged_attn");
+    if (a.selected && p.splits == 1u) return VX_OK;
+    const uint64_t joins = (a.selected ? (uint64_t)a.b.max_rows * p.tiles : a.s.joins) * p.a.s.tile_rows * g.kv_heads;
+    const dim3 grid((uint32_t)joins);
+    switch (g.head_dim) {
+        case 64: k_paged_join<64><<<grid, 256, 0, s>>>(p); break;
+        case 128: k_paged_join<128><<<grid, 256, 0, s>>>(p); break;
+        default: k_paged_join<256><<<grid, 256, 0, s>>>(p); break;
+    }
+    VX_LAUNCHED("k_paged_join");
+    return VX_OK;
+}
+
+}  // namespace vx

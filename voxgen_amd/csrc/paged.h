@@ -1,0 +1,94 @@
+// The paged KV cache (include/voxhip.h, vx_paged_*): the plan's layout and the launch
+// descriptions shared by the C ABI checks (paged.cpp) and the kernels (kernels_paged*.hip).
+#pragma once
+
+#include "vx_internal.h"
+
+namespace vx {
+
+constexpr uint32_t kPagedRequests = 4096;        // what one workgroup's scan of the requests holds in LDS
+constexpr uint32_t kPagedMaxTokens = 1u << 28;   // positions of a request
+constexpr uint32_t kPagedMaxRowHeads = 1u << 22; // rows of a step times query heads: bounds every grid
+constexpr uint32_t kPagedUnit = 16;              // slots of a unit: 32 * head_dim bytes of K, and of V
+constexpr uint32_t kPagedMaxSplits = 256;        // of a tile of query rows
+
+inline uint32_t paged_shift(uint32_t page_size) { return 31u - (uint32_t)__builtin_clz(page_size); }
+
+// How the attention divides a step, from the sizes that a batch fixes. A tile is tile_rows query
+// rows (tokens times query heads of a KV head) of one request; its keys, in chunks of 32, are
+// divided so that about `workgroups` workgroups come out, of least chunks or more.
+struct PagedShape {
+    uint32_t tile_rows, waves;
+    bool packed;                     // both f16 terms of eight rows in one column tile
+    uint32_t workgroups, least;      // 2^workgroups
+    uint32_t runs, items, joins, parts;              // most of each; items, joins and parts of one KV head
+    // words of the plan
+    uint64_t slots, requests, positions, granted, run_at, item_at, join_at, words;
+};
+PagedShape paged_shape(const vx_paged_batch &b);
+
+// Records of a plan. Rows of a request that lie in one page.
+struct PagedRun {
+    uint32_t row, n, slot, unused;   // first row, rows, slot of the first (VX_PAGED_NONE: no page)
+};
+// One workgroup's share: a tile of query rows over chunks [first, first + n) of its keys.
+struct PagedItem {
+    uint32_t request, row, base, count;   // the request, its first row, tokens cached before it, its rows
+    uint32_t tile, first, n, part;        // the tile's first query row; where its partial sums go (VX_PAGED_NONE: none)
+};
+// A tile whose keys are divided: partial sums first_part.. + parts.
+struct PagedJoin {
+    uint32_t row, base, count, tile, part, per, unused[2];   // per: chunks of a part
+};
+
+struct PagedPlan {
+    vx_paged_batch b;
+    PagedShape s;
+    const uint32_t *lengths = nullptr, *counts = nullptr, *pool = nullptr;
+    uint32_t *tables = nullptr, *plan = nullptr;
+};
+int launch_paged_reset(hipStream_t s, const vx_paged_batch &b, uint32_t *lengths, uint32_t *tables, uint32_t *pool);
+int launch_paged_plan(hipStream_t s, const PagedPlan &a);
+int launch_paged_advance(hipStream_t s, const vx_paged_batch &b, const uint32_t *plan, uint32_t *lengths, uint32_t *pool);
+int launch_paged_cut(hipStream_t s, const vx_paged_batch &b, const uint32_t *keep, uint32_t *lengths, uint32_t *tables,
+                     uint32_t *pool);
+
+struct PagedStore {
+    vx_paged_batch b;
+    PagedShape s;
+    uint32_t layer = 0, k_stride = 0, v_stride = 0;
+    const float *k = nullptr, *v = nullptr;     // at the push's base
+    uint8_t *kc = nullptr, *vc = nullptr, *bounds = nullptr;
+    const uint32_t *plan = nullptr;
+    bool vec = false;                           // every row's address is 16-byte aligned
+};
+int launch_paged_store(hipStream_t s, const PagedStore &a);
+
+struct PagedAttn {
+    vx_paged_batch b;
+    PagedShape s;
+    uint32_t layer = 0, q_stride = 0, out_stride = 0, budget = 0;
+    const float *q = nullptr;
+    const uint8_t *kc = nullptr, *vc = nullptr;
+    float *out = nullptr, *scratch = nullptr;
+    const uint32_t *tables = nullptr, *plan = nullptr, *selected = nullptr;
+    bool qvec = false, ovec = false;            // rows 16-byte aligned
+};
+uint64_t paged_attn_scratch_bytes(const vx_paged_batch &b, uint32_t budget);
+int launch_paged_attention(hipStream_t s, const PagedAttn &a);
+
+struct PagedSelect {
+    vx_paged_batch b;
+    PagedShape s;
+    uint32_t layer = 0, q_stride = 0, budget = 0, sinks = 0, recent = 0;
+    const float *q = nullptr;
+    const uint8_t *bounds = nullptr;
+    const uint32_t *tables = nullptr, *plan = nullptr;
+    uint32_t *selected = nullptr;
+    uint64_t *scratch = nullptr;
+    bool qvec = false;
+};
+uint64_t paged_select_scratch_bytes(const vx_paged_batch &b);
+int launch_paged_select(hipStream_t s, const PagedSelect &a);
+
+}  // namespace vx
