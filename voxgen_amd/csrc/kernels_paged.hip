@@ -395,22 +395,48 @@ __global__ __launch_bounds__(256) void k_paged_store(PagedStore a) {
 // max(q_j, 0) and min(q_j, 0). In 64 bits: the choice falls at a border between sums that 32 bits,
 // added up in one order or another, would swap.
 //
-// A page's order: sums as unsigned numbers that rise with them; NaN above all of them, pages that
-// stay in any case above that.
-constexpr uint64_t kHeld = ~0ull, kNaN = ~0ull - 1u;
+// A page's order: sums as unsigned numbers that rise with them, NaN above all of them.
 __device__ __forceinline__ uint64_t order_of(double x) {
-    if (x != x) return kNaN;
+    if (x != x) return ~0ull;
     const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);   // -0 as 0
     return u >> 63 ? ~u : u | 1ull << 63;
 }
 
 constexpr uint32_t kScorePages = 64;   // pages of a workgroup
 
+// Sums of 2^k values a lane over the L lanes of its group (L 16, 32 or 64, N a divisor of L): each
+// step halves what a lane holds, so that in the end lane l has the whole sum of value l % N.
+template <int N, int L>
+__device__ __forceinline__ double fold(double (&s)[N]) {
+    const uint32_t lane = threadIdx.x & 63u;
+    int n = N;
+#pragma unroll
+    for (int d = 1; d < N; d <<= 1) {
+        n /= 2;
+        const bool odd = lane & (uint32_t)d;
+#pragma unroll
+        for (int k = 0; k < N / 2; ++k)
+            if (k < n) {
+                // values 2 k and 2 k + 1 of those left are the ones that differ in this step's bit
+                const double keep = odd ? s[2 * k + 1] : s[2 * k], give = odd ? s[2 * k] : s[2 * k + 1];
+                s[k] = keep + __shfl_xor(give, d, 64);
+            }
+    }
+    double x = s[0];
+#pragma unroll
+    for (int d = N; d < L; d <<= 1) x += __shfl_xor(x, d, 64);
+    return x;
+}
+
+// A workgroup takes 64 pages of a row and KV head, a wave 16, L lanes a page. What is fetched does
+// not wait for what it is multiplied by. Bound by four loads that need each other (the row's
+// request, the table, the bounds; the queries beside them), then by the bytes of the bounds.
 template <int HD>
 __global__ __launch_bounds__(256) void k_paged_score(PagedSelect a, uint32_t blocks) {
     constexpr int L = HD / 4;              // lanes of a page: eight values each of lo, then hi
     constexpr int AT = 64 / L;             // pages of a wave at once
     constexpr int P = kScorePages / 4;     // pages of a wave
+    constexpr int N = P / AT;              // of a group of L lanes: page n AT + lane / L
     __shared__ double ends[2][HD];         // down, up
     const uint32_t tid = threadIdx.x, lane = tid & 63u, w = tid >> 6, heads = a.b.geom.kv_heads;
     const uint32_t pair = blockIdx.x / blocks, block = blockIdx.x % blocks;
@@ -419,54 +445,65 @@ __global__ __launch_bounds__(256) void k_paged_score(PagedSelect a, uint32_t blo
     if (request >= a.b.requests) return;
     const uint32_t last = min(position >> shift, a.b.table_width - 1u);
     if (block * kScorePages > last) return;
-    const uint32_t group = a.b.q_heads / heads;
+    const uint32_t group = a.b.q_heads / heads, l = lane % L;
+    const uint32_t *const table = a.tables + (size_t)request * a.b.table_width;
+    const h8 *const bounds = reinterpret_cast<const h8 *>(a.bounds) + ((size_t)a.layer * a.b.geom.pages * heads + head) * L + l;
+    uint64_t *const to = a.scratch + ((size_t)row * heads + head) * a.b.table_width;
+    h8 x[N];
+    uint32_t page[N];
+    auto fetch = [&](uint32_t k) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) page[n] = table[min(k + n * AT + lane / L, last)];
+#pragma unroll
+        for (int n = 0; n < N; ++n) x[n] = bounds[(size_t)min(page[n], a.b.geom.pages - 1u) * heads * L];
+    };
+    uint32_t k = block * kScorePages + w * P;
+    if (k <= last) fetch(k);
     const float *const q = a.q + (size_t)row * a.q_stride + (size_t)head * group * HD;
     for (uint32_t d = tid; d < (uint32_t)HD; d += 256u) {
         double up = 0, down = 0;
+#pragma unroll 8
         for (uint32_t j = 0; j < group; ++j) {
-            const float x = q[(size_t)j * HD + d];
-            up += x > 0.f || x != x ? (double)x : 0.0;
-            down += x < 0.f || x != x ? (double)x : 0.0;
+            const float v = q[(size_t)j * HD + d];
+            up += v > 0.f || v != v ? (double)v : 0.0;
+            down += v < 0.f || v != v ? (double)v : 0.0;
         }
         ends[0][d] = down;
         ends[1][d] = up;
     }
     __syncthreads();
     double coef[8];
-    const uint32_t l = lane % L;
 #pragma unroll
     for (int i = 0; i < 8; ++i) coef[i] = ends[l / (L / 2)][l % (L / 2) * 8 + i];
-    uint64_t *const to = a.scratch + ((size_t)row * heads + head) * a.b.table_width;
-    for (uint32_t k = block * kScorePages + w * P, end = k + P; k <= last; k += AT) {
-        if (k == end) {            // the workgroup's next pages
-            k += blocks * kScorePages - P;
-            end = k + P;
-            if (k > last) break;
-        }
-        const uint32_t p = k + lane / L;
-        const bool there = p <= last;
-        const uint32_t page = there ? a.tables[(size_t)request * a.b.table_width + p] : VX_PAGED_NONE;
-        double s = 0;
-        if (page < a.b.geom.pages) {
-            const h8 x = reinterpret_cast<const h8 *>(a.bounds)[(((size_t)a.layer * a.b.geom.pages + page) * heads + head) * L + l];
+    for (; k <= last; k += blocks * kScorePages) {
+        if (k != block * kScorePages + w * P) fetch(k);
+        double s[N];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += coef[i] * (double)(float)x[i];
-        } else {
-            s = __builtin_nan("");
-        }
+        for (int n = 0; n < N; ++n) {
+            s[n] = 0;
 #pragma unroll
-        for (int d = L / 2; d; d >>= 1) s += __shfl_xor(s, d, 64);
-        if (there && l == 0) to[p] = p < a.sinks || last - p < a.recent ? kHeld : order_of(s);
+            for (int i = 0; i < 8; ++i) s[n] += coef[i] * (double)(float)x[n][i];
+            if (page[n] >= a.b.geom.pages) s[n] = __builtin_nan("");
+        }
+        const double sum = fold<N, L>(s);
+        const uint32_t p = k + l % N * AT + lane / L;
+        if (l < (uint32_t)N && p <= last) to[p] = order_of(sum);
     }
 }
 
-// A workgroup a row and KV head: the order of the budget-th page by eight digits of eight bits,
-// then the pages above it, and of those equal to it the first.
-constexpr uint32_t kChoose = 512;
+// A workgroup a row and KV head, E orders a thread one behind the other (E 0: as many as it takes,
+// read again each time). The pages that stay in any case are known by index. Of the others the least
+// order that stays is found by histograms of 2048 bins over the range that is left: orders from lo to hi are
+// binned by their distance from lo, and the bin that the border falls in is the next range, until it
+// is taken whole or holds equal orders only, of which the first pages stay. Two passes as a rule.
+constexpr uint32_t kChoose = 512, kBins = 2048;
+template <int E>
 __global__ __launch_bounds__(512) void k_paged_choose(PagedSelect a) {
-    __shared__ uint32_t bins[256], between[kChoose / 64][2], chosen[2];
+    __shared__ uint32_t bins[kBins], between[kChoose / 64][2], chosen[3];
+    __shared__ uint64_t ends[2][kChoose / 64];
     const uint32_t tid = threadIdx.x, heads = a.b.geom.kv_heads, row = blockIdx.x / heads, head = blockIdx.x % heads;
-    const uint32_t shift = 31u - __clz(a.b.geom.page_size);
+    const uint32_t lane = tid & 63u, w = tid >> 6, shift = 31u - __clz(a.b.geom.page_size);
+    const uint64_t *const keys = a.scratch + ((size_t)row * heads + head) * a.b.table_width;
     const uint32_t request = a.plan[a.s.requests + row], position = a.plan[a.s.positions + row];
     uint32_t *const out = a.selected + ((size_t)row * heads + head) * a.budget;
     const uint32_t n = request < a.b.requests ? min(position >> shift, a.b.table_width - 1u) + 1u : 0u;
@@ -474,42 +511,107 @@ __global__ __launch_bounds__(512) void k_paged_choose(PagedSelect a) {
         for (uint32_t k = tid; k < a.budget; k += kChoose) out[k] = k < n ? k : VX_PAGED_NONE;
         return;
     }
-    const uint64_t *const keys = a.scratch + ((size_t)row * heads + head) * a.b.table_width;
-    uint64_t prefix = 0;
-    uint32_t left = a.budget;      // pages to take of those that agree with the prefix
-    for (int digit = 56; digit >= 0; digit -= 8) {
-        if (tid < 256u) bins[tid] = 0;
-        __syncthreads();
-        for (uint32_t k = tid; k < n; k += kChoose) {
-            const uint64_t x = keys[k];
-            if (digit == 56 || x >> (digit + 8) == prefix) atomicAdd(&bins[x >> digit & 255u], 1u);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            uint32_t above = 0;
-            int b = 255;
-            for (; b > 0 && above + bins[b] < left; --b) above += bins[b];
-            chosen[0] = (uint32_t)b;
-            chosen[1] = left - above;
-        }
-        __syncthreads();
-        prefix = prefix << 8 | chosen[0];
-        left = chosen[1];
-        __syncthreads();
+    const uint32_t each = E ? E : (n + kChoose - 1u) / kChoose, k0 = min(tid * each, n), k1 = min(k0 + each, n);
+    const uint32_t held0 = a.sinks, held1 = n - a.recent;           // pages below and from there on stay
+    uint64_t mine[E ? E : 1];
+    if constexpr (E != 0) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) mine[e] = k0 + e < n ? keys[k0 + e] : 0;
     }
-    // in rising order: a thread has pages one behind the other
-    const uint32_t each = (n + kChoose - 1u) / kChoose, k0 = min(tid * each, n), k1 = min(k0 + each, n);
-    uint32_t v[2] = {0, 0};        // above, equal
-    for (uint32_t k = k0; k < k1; ++k) v[0] += keys[k] > prefix, v[1] += keys[k] == prefix;
-    uint32_t before[2];
+    // every page that has to be chosen, with its order
+    auto each_free = [&](auto &&f) {
+        if constexpr (E != 0) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (k0 + e >= held0 && k0 + e < held1) f(k0 + e, mine[e]);
+        } else {
+            for (uint32_t k = max(k0, held0); k < min(k1, held1); ++k) f(k, keys[k]);
+        }
+    };
+    uint64_t lo = ~0ull, hi = 0;
+    each_free([&](uint32_t, uint64_t x) { lo = min(lo, x), hi = max(hi, x); });
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        lo = min(lo, (uint64_t)__shfl_xor((unsigned long long)lo, d, 64));
+        hi = max(hi, (uint64_t)__shfl_xor((unsigned long long)hi, d, 64));
+    }
+    if (lane == 0) ends[0][w] = lo, ends[1][w] = hi;
+    for (uint32_t k = tid; k < kBins; k += kChoose) bins[k] = 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t u = 0; u < kChoose / 64; ++u) lo = min(lo, ends[0][u]), hi = max(hi, ends[1][u]);
+    uint32_t left = a.budget - a.sinks - a.recent;   // pages to take of those from lo to hi
+    bool some = false;                               // not all that equal lo are taken
+    while (left) {
+        const uint64_t range = hi - lo;
+        const int by = range >> 11 ? 53 - __clzll(range) : 0;        // (hi - lo) >> by is below 2048
+        each_free([&](uint32_t, uint64_t x) {
+            if (x >= lo && x <= hi) atomicAdd(&bins[(x - lo) >> by], 1u);
+        });
+        __syncthreads();
+        // four bins a thread, the highest first
+        constexpr uint32_t BE = kBins / kChoose;
+        uint32_t count[BE], v[1] = {0}, before[1];
+#pragma unroll
+        for (uint32_t e = 0; e < BE; ++e) count[e] = bins[kBins - 1u - (tid * BE + e)], v[0] += count[e];
+        scan<1>(v, before, 0x7fffffffu, reinterpret_cast<uint32_t (*)[1]>(between));
+        if (before[0] < left && v[0] >= left) {
+            uint32_t above = before[0];
+            bool done = false;
+#pragma unroll
+            for (uint32_t e = 0; e < BE; ++e) {
+                if (!done && above + count[e] >= left) {
+                    done = true;
+                    chosen[0] = kBins - 1u - (tid * BE + e);
+                    chosen[1] = left - above;
+                    chosen[2] = count[e];
+                }
+                if (!done) above += count[e];
+            }
+        }
+        for (uint32_t k = tid; k < kBins; k += kChoose) bins[k] = 0;
+        __syncthreads();
+        lo += (uint64_t)chosen[0] << by;
+        const uint64_t span = (1ull << by) - 1ull;
+        hi = hi - lo < span ? hi : lo + span;
+        left = chosen[1];
+        const bool whole = chosen[2] == left;
+        __syncthreads();
+        if (whole) break;
+        if (by == 0) {
+            some = true;
+            break;
+        }
+    }
+    if (a.budget == a.sinks + a.recent) lo = ~0ull, some = true, left = 0;   // none but those that stay
+    // in rising order; of those equal to lo the first `left` where not all are taken
+    uint32_t v[2] = {0, 0}, before[2];
+    auto count = [&](uint32_t k, uint64_t x) {
+        const bool held = k < held0 || k >= held1;
+        v[0] += held || x > lo || (x == lo && !some);
+        v[1] += !held && some && x == lo;
+    };
+    if constexpr (E != 0) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (k0 + e < n) count(k0 + e, mine[e]);
+    } else {
+        for (uint32_t k = k0; k < k1; ++k) count(k, keys[k]);
+    }
     scan<2>(v, before, 0x7fffffffu, between);
-    uint32_t above = before[0], equal = before[1];
-    for (uint32_t k = k0; k < k1; ++k) {
-        const uint64_t x = keys[k];
-        const bool take = x > prefix || (x == prefix && equal < left);
-        if (take) out[above + min(equal, left)] = k;
-        above += x > prefix;
-        equal += x == prefix;
+    uint32_t sure = before[0], equal = before[1];
+    auto put = [&](uint32_t k, uint64_t x) {
+        const bool held = k < held0 || k >= held1, take = held || x > lo || (x == lo && !some), tie = !held && some && x == lo;
+        if (take || (tie && equal < left)) out[sure + min(equal, left)] = k;
+        sure += take;
+        equal += tie;
+    };
+    if constexpr (E != 0) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (k0 + e < n) put(k0 + e, mine[e]);
+    } else {
+        for (uint32_t k = k0; k < k1; ++k) put(k, keys[k]);
     }
 }
 
@@ -574,7 +676,18 @@ int launch_paged_select(hipStream_t s, const PagedSelect &a) {
     PAGED_HD(a.b.geom.head_dim, CALL)
 #undef CALL
     VX_LAUNCHED("k_paged_score");
-    k_paged_choose<<<pairs, kChoose, 0, s>>>(a);
+    // orders in registers up to 16 a thread
+    const uint32_t each = (a.b.table_width + kChoose - 1u) / kChoose;
+    if (each <= 1u)
+        k_paged_choose<1><<<pairs, kChoose, 0, s>>>(a);
+    else if (each <= 2u)
+        k_paged_choose<2><<<pairs, kChoose, 0, s>>>(a);
+    else if (each <= 4u)
+        k_paged_choose<4><<<pairs, kChoose, 0, s>>>(a);
+    else if (each <= 16u)
+        k_paged_choose<16><<<pairs, kChoose, 0, s>>>(a);
+    else
+        k_paged_choose<0><<<pairs, kChoose, 0, s>>>(a);
     VX_LAUNCHED("k_paged_choose");
     return VX_OK;
 }
