@@ -203,12 +203,19 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
         const uint32_t u0 = __builtin_amdgcn_readlane(unit, (j & 31u) * 2u), u1 = __builtin_amdgcn_readlane(unit, (j & 31u) * 2u + 1u);
         return (size_t)(second ? u1 : u0) * UNIT;
     };
+    // Loads come back in order: the queries first, which are worked on while the first chunk is on its way.
+    QRow<HD> qr;
+    if constexpr (NT == 1) qr.load(p, t, head, min(r0 + ri, rows - 1u), r0 + ri < rows, q);
     look_up(0);
     const uint32_t mine = t.n > w ? (t.n - w + W - 1u) / W : 0u;   // the wave's chunks
     KFrag<HD> kf;
-    // K of a chunk is fetched before the one ahead is done with, where registers allow.
+    VFrag<HD> vf;
+    // K and V of a chunk are fetched when the one ahead is done with them, where registers allow.
     constexpr bool AHEAD = NT == 1;
-    if (AHEAD && mine) kf.load(kc + unit_of(0, i >= 8u), i, q);
+    if (AHEAD && mine) {
+        kf.load(kc + unit_of(0, i >= 8u), i, q);
+        vf.load(vc + unit_of(0, q >= 2u), i, q);
+    }
 
     for (uint32_t d = tid; d < 2u * HD; d += 64u * W) odd[d / HD][d % HD] = ~0u;
     uint32_t found = 0;
@@ -216,8 +223,6 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     float factor[NT];
     h8 *const qs = reinterpret_cast<h8 *>(lds);   // [NT][U][hi, lo][64]
     if constexpr (NT == 1) {
-        QRow<HD> qr;
-        qr.load(p, t, head, min(r0 + ri, rows - 1u), r0 + ri < rows, q);
         factor[0] = qr.split(qh, ql);
         if constexpr (PK) {
 #pragma unroll
@@ -226,7 +231,6 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     } else {
         for (uint32_t c = w; c < NT; c += W) {
             const uint32_t row = r0 + 16u * c + i;
-            QRow<HD> qr;
             qr.load(p, t, head, min(row, rows - 1u), row < rows, q);
             const float f = qr.split(qh, ql);
             if (q == 0) fs[16u * c + i] = f;
@@ -263,16 +267,13 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     // A chunk; at an edge, some row attends to a part of it only.
     auto step = [&](uint32_t j, uint32_t w0, uint32_t w1, auto at_edge) {
         constexpr bool edge = decltype(at_edge)::value;
-        VFrag<HD> vf;
         const uint8_t *const vu = vc + unit_of(j, q >= 2u);
-        if constexpr (AHEAD)
-            vf.load(vu, i, q);
-        else
-            kf.load(kc + unit_of(j, i >= 8u), i, q);
-        // Behind the last chunk unit 0 is fetched once more, which is cheaper than a branch: in one between
-        // the products and what reads them, this compiler lost count of the wait that that needs.
-        if (((j + 1u) & 31u) == 0) look_up(j + 1u);
-        const uint8_t *const ku = kc + unit_of(j + 1u, i >= 8u);
+        if constexpr (!AHEAD) kf.load(kc + unit_of(j, i >= 8u), i, q);
+        // Behind the last chunk it is fetched once more, without a branch: with one between the products
+        // and what reads them, this compiler lost count of the wait that that needs.
+        const uint32_t next = min(j + 1u, mine - 1u);
+        if ((next & 31u) == 0 && next != j) look_up(next);
+        const uint8_t *const ku = kc + unit_of(next, i >= 8u), *const vnext = vc + unit_of(next, q >= 2u);
         f4 x[NT][2];
 #pragma unroll
         for (int c = 0; c < NT; ++c) x[c][0] = x[c][1] = f4{0.f, 0.f, 0.f, 0.f};
@@ -375,6 +376,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
                 for (int c = 0; c < NT; ++c) o[c][dt] = mfma16(vf.x[dt], pl[c], o[c][dt]);
             }
         }
+        if constexpr (AHEAD) vf.load(vnext, i, q);
     };
     for (uint32_t j = 0; j < mine; ++j) {
         const uint32_t w0 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u), w1 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u + 1u);
@@ -675,7 +677,7 @@ int launch_paged_attention(hipStream_t s, const PagedAttn &a) {
     }
 #undef CALL
     VX_LAUNCHED("k_paged_attn");
-    if (a.selected && p.splits == 1u) return VX_OK;
+    if (a.selected ? p.splits == 1u : a.s.joins == 0u) return VX_OK;   // nothing is divided
     const uint64_t joins = (a.selected ? (uint64_t)a.b.max_rows * p.tiles : a.s.joins) * p.a.s.tile_rows * g.kv_heads;
     const dim3 grid((uint32_t)joins);
     switch (g.head_dim) {

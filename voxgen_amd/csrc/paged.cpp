@@ -17,11 +17,15 @@ PagedShape paged_shape(const vx_paged_batch &b) {
     s.waves = s.tile_rows > 16u ? 8u : 4u;
     s.workgroups = s.tile_rows > 16u ? 9u : 10u;
     s.least = s.waves;
-    const uint64_t tiles = (uint64_t)b.max_rows * group / s.tile_rows + std::min(b.requests, b.max_rows);
-    const uint32_t share = ((1u << s.workgroups) + b.geom.kv_heads - 1u) / b.geom.kv_heads;   // workgroups of a KV head
-    s.items = (uint32_t)tiles + share;
-    s.joins = share;
-    s.parts = 2u * share;
+    // Tiles: at most one for each request of so few rows, else a request's last may be part of one. Parts
+    // of a tile: what its keys divide into, of which in all a KV head's share of the workgroups comes on top.
+    const uint32_t requests = std::min(b.requests, b.max_rows);
+    const uint64_t tiles = rows <= s.tile_rows ? requests : (uint64_t)b.max_rows * group / s.tile_rows + requests;
+    const uint32_t share = ((1u << s.workgroups) + b.geom.kv_heads - 1u) / b.geom.kv_heads;
+    const uint64_t chunks = ((uint64_t)b.table_width * b.geom.page_size + 31u) / 32u, most = (chunks + s.least - 1u) / s.least;
+    s.items = (uint32_t)std::min(tiles + share, tiles * most);
+    s.joins = most > 1u ? (uint32_t)std::min<uint64_t>(share, tiles) : 0u;
+    s.parts = most > 1u ? (uint32_t)std::min<uint64_t>(2u * share, tiles * most) : 0u;
     s.runs = (uint32_t)std::min<uint64_t>(b.max_rows, (uint64_t)b.max_rows / b.geom.page_size + 2ull * b.requests);
     s.slots = VX_PAGED_PLAN_ROWS;
     s.requests = s.slots + b.max_rows;
