@@ -112,14 +112,15 @@ __global__ __launch_bounds__(1024) void k_paged_plan(PagedPlan a) {
     todo = 0;
     for (uint32_t u = 0; u < kPlanThreads / 64; ++u) todo += work[u];
     const unsigned long long share = (todo * heads + (1u << a.s.workgroups) - 1u) >> a.s.workgroups;
-    const uint32_t per = max((uint32_t)min(share, 1ull << 30), a.s.least);
+    // a wave's chunks are alike in number
+    const uint32_t per = max(((uint32_t)min(share, 1ull << 30) + a.s.waves - 1u) / a.s.waves * a.s.waves, a.s.least);
     // runs, then items, joins and parts of each request; a request's tiles are all divided alike
     uint32_t splits[kPlanEach], by[kPlanEach];
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (uint32_t e = 0; e < kPlanEach; ++e) {
         splits[e] = min((chunks[e] + per - 1u) / per, kPagedMaxSplits);
-        by[e] = splits[e] ? (chunks[e] + splits[e] - 1u) / splits[e] : 1u;
+        by[e] = splits[e] ? ((chunks[e] + splits[e] - 1u) / splits[e] + a.s.waves - 1u) / a.s.waves * a.s.waves : 1u;
         splits[e] = (chunks[e] + by[e] - 1u) / by[e];
         w[0] += takes[e] ? ((len[e] + count[e] - 1u) >> shift) - (len[e] >> shift) + 1u : 0u;
         w[1] += tiles[e] * splits[e];
@@ -186,7 +187,7 @@ __global__ __launch_bounds__(1024) void k_paged_plan(PagedPlan a) {
         const uint32_t many = (length + cnt + 31u) / 32u;
         tiles_of = (cnt * group + a.s.tile_rows - 1u) / a.s.tile_rows;
         uint32_t s = min((many + per - 1u) / per, kPagedMaxSplits);
-        by_of = (many + s - 1u) / s;
+        by_of = ((many + s - 1u) / s + a.s.waves - 1u) / a.s.waves * a.s.waves;
         return (many + by_of - 1u) / by_of;
     };
     for (uint32_t g = g0; g < all_items; g += step) {

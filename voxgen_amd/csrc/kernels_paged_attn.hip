@@ -569,6 +569,11 @@ __global__ __launch_bounds__(256) void k_paged_join(AttnArgs p) {
     if (n <= 1u || n > kPagedMaxSplits) return;
     const size_t at = ((size_t)head * p.parts + first) * tile_rows + r;   // the row's record in the first part
     const uint32_t c = 4u * (tid % V), y = tid / V;
+    constexpr int E = 8;
+    f4 early[E];   // on their way while the parts' weights are worked out
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+        early[k] = *reinterpret_cast<const f4 *>(p.acc + (at + (size_t)min(y + k * Y, n - 1u) * tile_rows) * HD + c);
     float m = -INFINITY, l = -1.f;
     if (tid < n) {
         m = p.ml[(at + (size_t)tid * tile_rows) * 2u];
@@ -590,8 +595,11 @@ __global__ __launch_bounds__(256) void k_paged_join(AttnArgs p) {
     __syncthreads();
     sum = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
     f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+        if (y + k * Y < n) o += early[k] * sc[y + k * Y];
 #pragma unroll 8
-    for (uint32_t v = y; v < n; v += Y)
+    for (uint32_t v = y + E * Y; v < n; v += Y)
         o += *reinterpret_cast<const f4 *>(p.acc + (at + (size_t)v * tile_rows) * HD + c) * sc[v];
     *reinterpret_cast<f4 *>(&os[y][c]) = o;
     __syncthreads();
