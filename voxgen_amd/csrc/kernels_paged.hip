@@ -12,27 +12,40 @@ typedef double d2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ uint32_t add_up_to(uint32_t a, uint32_t b, uint32_t most) { return min(a + b, most); }
 
-// Sums over a workgroup's threads up to and with each, and in `before` without it, each clipped to
-// `most` (clipped addition of numbers below 2^31 is associative). `between` holds a word for each wave.
-template <int N>
-__device__ __forceinline__ void scan(uint32_t (&v)[N], uint32_t (&before)[N], uint32_t most, uint32_t (*between)[N]) {
+// v of another lane of the wave by a DPP control, 0 where there is none or ROWS does not have the lane's row.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lane_of(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+
+// Sums over a workgroup's T threads up to and with each, and in `before` without it, each clipped to
+// `most` (clipped addition of numbers below 2^31 is associative); all of them in `all`. `between`
+// holds a word for each wave.
+template <int N, uint32_t T>
+__device__ __forceinline__ void scan(uint32_t (&v)[N], uint32_t (&before)[N], uint32_t (&all)[N], uint32_t most,
+                                     uint32_t (*between)[N]) {
     const uint32_t lane = threadIdx.x & 63u, w = threadIdx.x >> 6;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t below = __shfl_up(v[n], d, 64);
-            v[n] = lane >= (uint32_t)d ? add_up_to(v[n], below, most) : v[n];
-        }
-        before[n] = __shfl_up(v[n], 1, 64);
-        if (lane == 0) before[n] = 0;
+        v[n] = add_up_to(v[n], lane_of<0x111, 0xf>(v[n]), most);   // row_shr 1, 2, 4, 8
+        v[n] = add_up_to(v[n], lane_of<0x112, 0xf>(v[n]), most);
+        v[n] = add_up_to(v[n], lane_of<0x114, 0xf>(v[n]), most);
+        v[n] = add_up_to(v[n], lane_of<0x118, 0xf>(v[n]), most);
+        v[n] = add_up_to(v[n], lane_of<0x142, 0xa>(v[n]), most);   // row_bcast 15, 31
+        v[n] = add_up_to(v[n], lane_of<0x143, 0xc>(v[n]), most);
+        before[n] = lane_of<0x138, 0xf>(v[n]);                     // wave_shr 1
         if (lane == 63u) between[w][n] = v[n];
     }
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         uint32_t ahead = 0;
-        for (uint32_t u = 0; u < w; ++u) ahead = add_up_to(ahead, between[u][n], most);
+        all[n] = 0;
+#pragma unroll
+        for (uint32_t u = 0; u < T / 64u; ++u) {
+            ahead = u == w ? all[n] : ahead;
+            all[n] = add_up_to(all[n], between[u][n], most);
+        }
         v[n] = add_up_to(v[n], ahead, most);
         before[n] = add_up_to(before[n], ahead, most);
     }
@@ -52,120 +65,128 @@ __device__ __forceinline__ uint32_t owner_of(const uint32_t *end, uint32_t n, ui
     return lo;
 }
 
-constexpr uint32_t kPlanThreads = 1024, kPlanEach = kPagedRequests / kPlanThreads;
-
 // Every workgroup scans all requests, and writes its share of what follows from that: so one
-// launch does, and none waits for another. A thread has `each` requests one behind the other.
-__global__ __launch_bounds__(1024) void k_paged_plan(PagedPlan a) {
-    __shared__ uint32_t row_end[kPagedRequests], page_end[kPagedRequests], run_end[kPagedRequests], item_end[kPagedRequests],
-        join_end[kPagedRequests], part_end[kPagedRequests];
-    __shared__ uint32_t between[kPlanThreads / 64][4];
-    __shared__ unsigned long long work[kPlanThreads / 64];
-    const uint32_t tid = threadIdx.x, n = a.b.requests, each = (n + kPlanThreads - 1u) / kPlanThreads;
+// launch does, and none waits for another. A thread has E requests one behind the other. Bound by
+// what needs each other: lengths and counts, three sums over the requests, for each row the
+// request that it is of, and its page.
+template <uint32_t T, uint32_t E>
+__global__ __launch_bounds__(T) void k_paged_plan(PagedPlan a) {
+    constexpr uint32_t N = T * E;
+    __shared__ uint32_t length_of[N], count_of[N], row_end[N], page_end[N], run_end[N], item_end[N], join_end[N], part_end[N];
+    __shared__ uint32_t between[T / 64][6];
+    __shared__ float work[T / 64];
+    const uint32_t tid = threadIdx.x, n = a.b.requests, r0 = tid * E;
     const uint32_t pages = a.b.geom.pages, shift = 31u - __clz(a.b.geom.page_size), ps = a.b.geom.page_size;
     const uint32_t width = a.b.table_width, cap = width << shift, rows = a.b.max_rows;
     const uint32_t group = a.b.q_heads / a.b.geom.kv_heads, heads = a.b.geom.kv_heads;
+    const uint32_t tile_shift = 31u - __clz(a.s.tile_rows), wave_shift = 31u - __clz(a.s.waves);
     const uint32_t free = min(a.pool[0], pages);
-    uint32_t len[kPlanEach], count[kPlanEach], need[kPlanEach];
-    bool takes[kPlanEach];
-    const uint32_t r0 = tid * each;
-
-    uint32_t v[1] = {0};
+    uint32_t len[E], count[E], need[E], v[1] = {0}, before[1], all[1];
+    bool takes[E];
 #pragma unroll
-    for (uint32_t e = 0; e < kPlanEach; ++e) {
-        const bool there = e < each && r0 + e < n;
-        len[e] = there ? a.lengths[r0 + e] : 0u;
-        count[e] = there ? a.counts[r0 + e] : 0u;
+    for (uint32_t e = 0; e < E; ++e) {
+        len[e] = r0 + e < n ? a.lengths[r0 + e] : 0u;
+        count[e] = r0 + e < n ? a.counts[r0 + e] : 0u;
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) {
+        length_of[r0 + e] = len[e];
+        count_of[r0 + e] = count[e];
         v[0] = add_up_to(v[0], min(count[e], rows + 1u), rows + 1u);
     }
-    uint32_t before[1];
-    scan<1>(v, before, rows + 1u, reinterpret_cast<uint32_t (*)[1]>(between));
-    uint32_t at = before[0];
+    scan<1, T>(v, before, all, rows + 1u, reinterpret_cast<uint32_t (*)[1]>(between));
+    const uint32_t all_rows = min(all[0], rows);
+    // What the attention has to do, chunks of 32 keys by tiles of query rows, of requests that may take
+    // part; rounded up enough for the sums' order not to matter.
+    uint32_t at = before[0], tiles[E], chunks[E];
+    float todo = 0.f;
     v[0] = 0;
 #pragma unroll
-    for (uint32_t e = 0; e < kPlanEach; ++e) {
-        const uint32_t end = add_up_to(at, min(count[e], rows + 1u), rows + 1u);
-        takes[e] = count[e] != 0u && count[e] <= a.b.max_count && end <= rows && len[e] <= cap && count[e] <= cap - len[e];
+    for (uint32_t e = 0; e < E; ++e) {
+        at = add_up_to(at, min(count[e], rows + 1u), rows + 1u);
+        row_end[r0 + e] = at;
+        takes[e] = count[e] != 0u && count[e] <= a.b.max_count && at <= rows && len[e] <= cap && count[e] <= cap - len[e];
         need[e] = takes[e] ? ((len[e] + count[e] + ps - 1u) >> shift) - ((len[e] + ps - 1u) >> shift) : 0u;
         v[0] = add_up_to(v[0], need[e], pages + 1u);
-        if (e < each && r0 + e < n) row_end[r0 + e] = end;
-        at = end;
-    }
-    scan<1>(v, before, pages + 1u, reinterpret_cast<uint32_t (*)[1]>(between));
-    at = before[0];
-    // what the attention has to do: chunks of 32 keys by tiles of query rows
-    unsigned long long todo = 0;
-    uint32_t tiles[kPlanEach], chunks[kPlanEach];
-#pragma unroll
-    for (uint32_t e = 0; e < kPlanEach; ++e) {
-        at = add_up_to(at, need[e], pages + 1u);
-        takes[e] = takes[e] && (need[e] == 0u || at <= free);
-        if (e < each && r0 + e < n) page_end[r0 + e] = at;
-        tiles[e] = takes[e] ? (count[e] * group + a.s.tile_rows - 1u) / a.s.tile_rows : 0u;
+        tiles[e] = takes[e] ? (count[e] * group + a.s.tile_rows - 1u) >> tile_shift : 0u;
         chunks[e] = takes[e] ? (len[e] + count[e] + 31u) / 32u : 0u;
-        todo += (unsigned long long)tiles[e] * chunks[e];
+        todo += (float)tiles[e] * (float)chunks[e];
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) todo += __shfl_xor(todo, d, 64);
     if ((tid & 63u) == 0) work[tid >> 6] = todo;
-    __syncthreads();
-    todo = 0;
-    for (uint32_t u = 0; u < kPlanThreads / 64; ++u) todo += work[u];
-    const unsigned long long share = (todo * heads + (1u << a.s.workgroups) - 1u) >> a.s.workgroups;
-    // a wave's chunks are alike in number
-    const uint32_t per = max(((uint32_t)min(share, 1ull << 30) + a.s.waves - 1u) / a.s.waves * a.s.waves, a.s.least);
-    // runs, then items, joins and parts of each request; a request's tiles are all divided alike
-    uint32_t splits[kPlanEach], by[kPlanEach];
-    uint32_t w[4] = {0, 0, 0, 0};
+    scan<1, T>(v, before, all, pages + 1u, reinterpret_cast<uint32_t (*)[1]>(between));
+    todo = 0.f;
 #pragma unroll
-    for (uint32_t e = 0; e < kPlanEach; ++e) {
-        splits[e] = min((chunks[e] + per - 1u) / per, kPagedMaxSplits);
-        by[e] = splits[e] ? ((chunks[e] + splits[e] - 1u) / splits[e] + a.s.waves - 1u) / a.s.waves * a.s.waves : 1u;
-        splits[e] = (chunks[e] + by[e] - 1u) / by[e];
-        w[0] += takes[e] ? ((len[e] + count[e] - 1u) >> shift) - (len[e] >> shift) + 1u : 0u;
+    for (uint32_t u = 0; u < T / 64u; ++u) todo += work[u];
+    todo = todo * 1.0001f * (float)heads / (float)(1u << a.s.workgroups);
+    // a wave's chunks are alike in number
+    const uint32_t per = max(((uint32_t)fminf(ceilf(todo), 1e9f) + a.s.waves - 1u) >> wave_shift << wave_shift, a.s.least);
+    // Chunks of a part, of which there are `splits`; a request's tiles are all divided alike.
+    auto divided = [&](uint32_t many, uint32_t &splits) {
+        splits = min((many + per - 1u) / per, kPagedMaxSplits);
+        const uint32_t by = splits > 1u ? ((many + splits - 1u) / splits + a.s.waves - 1u) >> wave_shift << wave_shift : max(many, 1u);
+        splits = splits > 1u ? (many + by - 1u) / by : splits;
+        return by;
+    };
+    // runs, items, joins and parts of each request, and pages, rows and requests that take part
+    uint32_t splits[E], w[6] = {0, 0, 0, 0, 0, 0}, done[6], sum[6], taking = 0;
+    at = before[0];
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) {
+        at = add_up_to(at, need[e], pages + 1u);
+        page_end[r0 + e] = at;
+        takes[e] = takes[e] && (need[e] == 0u || at <= free);
+        divided(chunks[e], splits[e]);
+        if (!takes[e]) continue;
+        w[0] += ((len[e] + count[e] - 1u) >> shift) - (len[e] >> shift) + 1u;
         w[1] += tiles[e] * splits[e];
         w[2] += splits[e] > 1u ? tiles[e] : 0u;
         w[3] += splits[e] > 1u ? tiles[e] * splits[e] : 0u;
+        w[4] += need[e];
+        w[5] += count[e];
+        taking += 1u;
     }
-    uint32_t done[4];
-    scan<4>(w, done, 0x7fffffffu, between);
-    uint32_t run = done[0], item = done[1], join = done[2], part = done[3];
+    scan<6, T>(w, done, sum, 0x7fffffffu, between);
+    {
+        uint32_t run = done[0], item = done[1], join = done[2], part = done[3];
 #pragma unroll
-    for (uint32_t e = 0; e < kPlanEach; ++e) {
-        run += takes[e] ? ((len[e] + count[e] - 1u) >> shift) - (len[e] >> shift) + 1u : 0u;
-        item += tiles[e] * splits[e];
-        join += splits[e] > 1u ? tiles[e] : 0u;
-        part += splits[e] > 1u ? tiles[e] * splits[e] : 0u;
-        if (e < each && r0 + e < n) {
+        for (uint32_t e = 0; e < E; ++e) {
+            if (takes[e]) {
+                run += ((len[e] + count[e] - 1u) >> shift) - (len[e] >> shift) + 1u;
+                item += tiles[e] * splits[e];
+                join += splits[e] > 1u ? tiles[e] : 0u;
+                part += splits[e] > 1u ? tiles[e] * splits[e] : 0u;
+            }
             run_end[r0 + e] = run;
             item_end[r0 + e] = item;
             join_end[r0 + e] = join;
             part_end[r0 + e] = part;
         }
     }
-    __syncthreads();
+    const uint32_t most_taking = __syncthreads_count(taking != 0u);   // of E 1 the requests that take part
 
-    const uint32_t all_rows = min(row_end[n - 1u], rows), all_runs = min(run_end[n - 1u], a.s.runs);
-    const uint32_t all_items = min(item_end[n - 1u], a.s.items), all_joins = min(join_end[n - 1u], a.s.joins);
-    const uint32_t g0 = blockIdx.x * kPlanThreads + tid, step = gridDim.x * kPlanThreads;
+    const uint32_t all_runs = min(sum[0], a.s.runs), all_items = min(sum[1], a.s.items), all_joins = min(sum[2], a.s.joins);
+    const uint32_t taken = min(sum[4], free);
+    const uint32_t g0 = blockIdx.x * T + tid, step = gridDim.x * T;
     auto begin = [&](const uint32_t *end, uint32_t i) { return i ? end[i - 1u] : 0u; };
-    auto taking = [&](uint32_t i) { return run_end[i] != begin(run_end, i); };
+    auto part_of = [&](uint32_t i) { return run_end[i] != begin(run_end, i); };
     // the page of position p of request i that takes part: one in use, or one from the top of the pool
     auto page_of = [&](uint32_t i, uint32_t length, uint32_t p) {
         const uint32_t have = (length + ps - 1u) >> shift, k = p >> shift;
-        if (k < have) return a.tables[(size_t)i * width + k];
         const uint32_t nth = begin(page_end, i) + k - have;
-        return nth < free ? a.pool[free - nth] : VX_PAGED_NONE;
+        const uint32_t *const from = k < have ? a.tables + (size_t)i * width + k : a.pool + (nth < free ? free - nth : 0u);
+        const uint32_t page = *from;
+        return k < have || nth < free ? page : VX_PAGED_NONE;
     };
     for (uint32_t r = g0; r < rows; r += step) {
         uint32_t slot = VX_PAGED_NONE, request = VX_PAGED_NONE, position = VX_PAGED_NONE;
         if (r < all_rows) {
             const uint32_t i = owner_of(row_end, n, r);
-            if (taking(i)) {
-                const uint32_t length = a.lengths[i];
+            if (part_of(i)) {
                 request = i;
-                position = length + r - begin(row_end, i);
-                const uint32_t page = page_of(i, length, position);
+                position = length_of[i] + r - begin(row_end, i);
+                const uint32_t page = page_of(i, length_of[i], position);
                 if (page < pages) slot = (page << shift) + (position & (ps - 1u));
             }
         }
@@ -174,79 +195,53 @@ __global__ __launch_bounds__(1024) void k_paged_plan(PagedPlan a) {
         a.plan[a.s.positions + r] = position;
     }
     for (uint32_t g = g0; g < all_runs; g += step) {
-        const uint32_t i = owner_of(run_end, n, g), length = a.lengths[i], cnt = a.counts[i], k = g - begin(run_end, i);
+        const uint32_t i = owner_of(run_end, n, g), length = length_of[i], k = g - begin(run_end, i);
         const uint32_t first = k ? ((length >> shift) + k) << shift : length;       // position of the run's first row
-        const uint32_t last = min(((first >> shift) + 1u) << shift, length + cnt);
+        const uint32_t last = min(((first >> shift) + 1u) << shift, length + count_of[i]);
         const uint32_t page = page_of(i, length, first);
-        PagedRun run_of = {begin(row_end, i) + first - length, last - first,
-                           page < pages ? (page << shift) + (first & (ps - 1u)) : VX_PAGED_NONE, 0u};
-        reinterpret_cast<PagedRun *>(a.plan + a.s.run_at)[g] = run_of;
+        const PagedRun run = {begin(row_end, i) + first - length, last - first,
+                              page < pages ? (page << shift) + (first & (ps - 1u)) : VX_PAGED_NONE, 0u};
+        reinterpret_cast<PagedRun *>(a.plan + a.s.run_at)[g] = run;
     }
-    // the division, as it was made above
-    auto divided = [&](uint32_t i, uint32_t length, uint32_t cnt, uint32_t &tiles_of, uint32_t &by_of) {
-        const uint32_t many = (length + cnt + 31u) / 32u;
-        tiles_of = (cnt * group + a.s.tile_rows - 1u) / a.s.tile_rows;
-        uint32_t s = min((many + per - 1u) / per, kPagedMaxSplits);
-        by_of = ((many + s - 1u) / s + a.s.waves - 1u) / a.s.waves * a.s.waves;
-        return (many + by_of - 1u) / by_of;
-    };
     for (uint32_t g = g0; g < all_items; g += step) {
-        const uint32_t i = owner_of(item_end, n, g), length = a.lengths[i], cnt = a.counts[i], k = g - begin(item_end, i);
-        uint32_t tiles_of, by_of;
-        const uint32_t s = divided(i, length, cnt, tiles_of, by_of);
+        const uint32_t i = owner_of(item_end, n, g), length = length_of[i], cnt = count_of[i], k = g - begin(item_end, i);
+        uint32_t s;
+        const uint32_t by = divided((length + cnt + 31u) / 32u, s);
         // the tiles with the most keys first
-        const uint32_t tile = tiles_of - 1u - k / s, split = k % s;
-        const uint32_t last_row = min((tile + 1u) * a.s.tile_rows, cnt * group) - 1u;
-        const uint32_t many = (length + last_row / group) / 32u + 1u;
-        const uint32_t first = split * by_of;
-        PagedItem it = {i, begin(row_end, i), length, cnt, tile * a.s.tile_rows, first,
-                        first < many ? min(by_of, many - first) : 0u,
-                        many > by_of ? begin(part_end, i) + tile * s + split : VX_PAGED_NONE};
+        const uint32_t tile = ((cnt * group + a.s.tile_rows - 1u) >> tile_shift) - 1u - k / s, split = k % s;
+        const uint32_t last_row = min((tile + 1u) << tile_shift, cnt * group) - 1u;
+        const uint32_t many = (length + last_row / group) / 32u + 1u, first = split * by;
+        const PagedItem it = {i, begin(row_end, i), length, cnt, tile << tile_shift, first,
+                              first < many ? min(by, many - first) : 0u,
+                              many > by ? begin(part_end, i) + tile * s + split : VX_PAGED_NONE};
         reinterpret_cast<PagedItem *>(a.plan + a.s.item_at)[g] = it;
     }
     for (uint32_t g = g0; g < all_joins; g += step) {
-        const uint32_t i = owner_of(join_end, n, g), length = a.lengths[i], cnt = a.counts[i], tile = g - begin(join_end, i);
-        uint32_t tiles_of, by_of;
-        const uint32_t s = divided(i, length, cnt, tiles_of, by_of);
-        PagedJoin j = {begin(row_end, i), length, cnt, tile * a.s.tile_rows, begin(part_end, i) + tile * s, by_of, {0, 0}};
+        const uint32_t i = owner_of(join_end, n, g), length = length_of[i], cnt = count_of[i], tile = g - begin(join_end, i);
+        uint32_t s;
+        const uint32_t by = divided((length + cnt + 31u) / 32u, s);
+        const PagedJoin j = {begin(row_end, i), length, cnt, tile << tile_shift, begin(part_end, i) + tile * s, by, {0, 0}};
         reinterpret_cast<PagedJoin *>(a.plan + a.s.join_at)[g] = j;
     }
-    // new pages into the tables, granted rows, the header
-    for (uint32_t i = g0; i < n; i += step) {
-        const bool t = taking(i);
-        const uint32_t cnt = a.counts[i];
-        a.plan[a.s.granted + i] = t ? cnt : 0u;
-    }
-    uint32_t taken = 0;
-    {   // pages that requests that take part want: they are the first of all wanted
-        uint32_t lo = 0;
-#pragma unroll
-        for (uint32_t e = 0; e < kPlanEach; ++e)
-            if (e < each && r0 + e < n && takes[e] && need[e]) lo = page_end[r0 + e];
-#pragma unroll
-        for (int d = 32; d; d >>= 1) lo = max(lo, (uint32_t)__shfl_xor(lo, d, 64));
-        if ((tid & 63u) == 0) between[tid >> 6][0] = lo;
-        __syncthreads();
-        for (uint32_t u = 0; u < kPlanThreads / 64; ++u) taken = max(taken, between[u][0]);
-        __syncthreads();
-    }
-    for (uint32_t g = g0; g < taken; g += step) {
-        const uint32_t i = owner_of(page_end, n, g), have = (a.lengths[i] + ps - 1u) >> shift;
+    for (uint32_t i = g0; i < n; i += step) a.plan[a.s.granted + i] = part_of(i) ? count_of[i] : 0u;
+    for (uint32_t g = g0; g < taken; g += step) {   // pages that requests that take part want: they are the first of all wanted
+        const uint32_t i = owner_of(page_end, n, g), have = (length_of[i] + ps - 1u) >> shift;
         a.tables[(size_t)i * width + have + g - begin(page_end, i)] = a.pool[free - g];
     }
     if (blockIdx.x == 0) {
-        uint32_t some = 0, sum = 0;
+        uint32_t some = most_taking;
+        if constexpr (E > 1) {
+            some = taking;
 #pragma unroll
-        for (uint32_t e = 0; e < kPlanEach; ++e)
-            if (takes[e]) some += 1u, sum += count[e];
-#pragma unroll
-        for (int d = 32; d; d >>= 1) some += __shfl_xor(some, d, 64), sum += __shfl_xor(sum, d, 64);
-        if ((tid & 63u) == 0) between[tid >> 6][0] = some, between[tid >> 6][1] = sum;
-        __syncthreads();
+            for (int d = 32; d; d >>= 1) some += __shfl_xor(some, d, 64);
+            if ((tid & 63u) == 0) between[tid >> 6][0] = some;
+            __syncthreads();
+            some = 0;
+            for (uint32_t u = 0; u < T / 64u; ++u) some += between[u][0];
+        }
+        const uint32_t head[8] = {all_rows, taken, some, sum[5], all_runs, all_items, all_joins, 0u};
         if (tid == 0) {
-            some = sum = 0;
-            for (uint32_t u = 0; u < kPlanThreads / 64; ++u) some += between[u][0], sum += between[u][1];
-            const uint32_t head[8] = {all_rows, taken, some, sum, all_runs, all_items, all_joins, 0u};
+#pragma unroll
             for (uint32_t u = 0; u < 8; ++u) a.plan[u] = head[u];
         }
     }
@@ -272,17 +267,18 @@ __global__ __launch_bounds__(256) void k_paged_advance(vx_paged_batch b, const u
     if (more && length <= cap) lengths[i] = length + min(more, cap - length);
 }
 
+constexpr uint32_t kCutThreads = 1024, kCutEach = kPagedRequests / kCutThreads;
 // One workgroup: the pages that requests give back, in order, go on top of the pool.
 __global__ __launch_bounds__(1024) void k_paged_cut(vx_paged_batch b, const uint32_t *keep, uint32_t *lengths, uint32_t *tables,
                                                     uint32_t *pool) {
     __shared__ uint32_t end[kPagedRequests], from[kPagedRequests];
-    __shared__ uint32_t between[kPlanThreads / 64][1];
-    const uint32_t tid = threadIdx.x, n = b.requests, each = (n + kPlanThreads - 1u) / kPlanThreads, r0 = tid * each;
+    __shared__ uint32_t between[kCutThreads / 64][1];
+    const uint32_t tid = threadIdx.x, n = b.requests, each = (n + kCutThreads - 1u) / kCutThreads, r0 = tid * each;
     const uint32_t shift = 31u - __clz(b.geom.page_size), ps = b.geom.page_size, pages = b.geom.pages;
     const uint32_t cap = b.table_width << shift, free = min(pool[0], pages);
-    uint32_t back[kPlanEach], v[1] = {0}, before[1];
+    uint32_t back[kCutEach], v[1] = {0}, before[1], all[1];
 #pragma unroll
-    for (uint32_t e = 0; e < kPlanEach; ++e) {
+    for (uint32_t e = 0; e < kCutEach; ++e) {
         back[e] = 0;
         if (e >= each || r0 + e >= n) continue;
         const uint32_t i = r0 + e, length = min(lengths[i], cap), stay = min(length, keep[i]);
@@ -291,22 +287,21 @@ __global__ __launch_bounds__(1024) void k_paged_cut(vx_paged_batch b, const uint
         if (stay != length) lengths[i] = stay;
         v[0] += back[e];
     }
-    scan<1>(v, before, 0x7fffffffu, between);
+    scan<1, kCutThreads>(v, before, all, 0x7fffffffu, between);
     uint32_t at = before[0];
 #pragma unroll
-    for (uint32_t e = 0; e < kPlanEach; ++e) {
+    for (uint32_t e = 0; e < kCutEach; ++e) {
         at += back[e];
         if (e < each && r0 + e < n) end[r0 + e] = at;
     }
     __syncthreads();
-    const uint32_t all = end[n - 1u];
-    for (uint32_t g = tid; g < all; g += kPlanThreads) {
+    for (uint32_t g = tid; g < all[0]; g += kCutThreads) {
         const uint32_t i = owner_of(end, n, g), k = g - (i ? end[i - 1u] : 0u);
         uint32_t *const entry = tables + (size_t)i * b.table_width + from[i] + k;
         if (g < pages - free) pool[1u + free + g] = *entry;
         *entry = VX_PAGED_NONE;
     }
-    if (tid == 0) pool[0] = free + min(all, pages - free);
+    if (tid == 0) pool[0] = free + min(all[0], pages - free);
 }
 
 // ------------------------------------------------------------------- rows
@@ -552,10 +547,10 @@ __global__ __launch_bounds__(512) void k_paged_choose(PagedSelect a) {
         __syncthreads();
         // four bins a thread, the highest first
         constexpr uint32_t BE = kBins / kChoose;
-        uint32_t count[BE], v[1] = {0}, before[1];
+        uint32_t count[BE], v[1] = {0}, before[1], all[1];
 #pragma unroll
         for (uint32_t e = 0; e < BE; ++e) count[e] = bins[kBins - 1u - (tid * BE + e)], v[0] += count[e];
-        scan<1>(v, before, 0x7fffffffu, reinterpret_cast<uint32_t (*)[1]>(between));
+        scan<1, kChoose>(v, before, all, 0x7fffffffu, reinterpret_cast<uint32_t (*)[1]>(between));
         if (before[0] < left && v[0] >= left) {
             uint32_t above = before[0];
             bool done = false;
@@ -586,7 +581,7 @@ __global__ __launch_bounds__(512) void k_paged_choose(PagedSelect a) {
     }
     if (a.budget == a.sinks + a.recent) lo = ~0ull, some = true, left = 0;   // none but those that stay
     // in rising order; of those equal to lo the first `left` where not all are taken
-    uint32_t v[2] = {0, 0}, before[2];
+    uint32_t v[2] = {0, 0}, before[2], all[2];
     auto count = [&](uint32_t k, uint64_t x) {
         const bool held = k < held0 || k >= held1;
         v[0] += held || x > lo || (x == lo && !some);
@@ -599,7 +594,7 @@ __global__ __launch_bounds__(512) void k_paged_choose(PagedSelect a) {
     } else {
         for (uint32_t k = k0; k < k1; ++k) count(k, keys[k]);
     }
-    scan<2>(v, before, 0x7fffffffu, between);
+    scan<2, kChoose>(v, before, all, 0x7fffffffu, between);
     uint32_t sure = before[0], equal = before[1];
     auto put = [&](uint32_t k, uint64_t x) {
         const bool held = k < held0 || k >= held1, take = held || x > lo || (x == lo && !some), tie = !held && some && x == lo;
@@ -626,8 +621,15 @@ int launch_paged_reset(hipStream_t s, const vx_paged_batch &b, uint32_t *lengths
 }
 
 int launch_paged_plan(hipStream_t s, const PagedPlan &a) {
+    // one workgroup for so many rows, items or requests as it has threads; 64 for more
     const uint32_t most = std::max(std::max(a.b.max_rows, a.b.requests), a.s.items);
-    k_paged_plan<<<std::min((most + kPlanThreads - 1u) / kPlanThreads, 64u), kPlanThreads, 0, s>>>(a);
+    auto blocks = [&](uint32_t threads) { return std::min((most + threads - 1u) / threads, 64u); };
+    if (a.b.requests <= 256u)
+        k_paged_plan<256, 1><<<blocks(256), 256, 0, s>>>(a);
+    else if (a.b.requests <= 1024u)
+        k_paged_plan<512, 2><<<blocks(512), 512, 0, s>>>(a);
+    else
+        k_paged_plan<1024, 4><<<blocks(1024), 1024, 0, s>>>(a);
     VX_LAUNCHED("k_paged_plan");
     return VX_OK;
 }
@@ -640,7 +642,7 @@ int launch_paged_advance(hipStream_t s, const vx_paged_batch &b, const uint32_t 
 
 int launch_paged_cut(hipStream_t s, const vx_paged_batch &b, const uint32_t *keep, uint32_t *lengths, uint32_t *tables,
                      uint32_t *pool) {
-    k_paged_cut<<<1, kPlanThreads, 0, s>>>(b, keep, lengths, tables, pool);
+    k_paged_cut<<<1, kCutThreads, 0, s>>>(b, keep, lengths, tables, pool);
     VX_LAUNCHED("k_paged_cut");
     return VX_OK;
 }
