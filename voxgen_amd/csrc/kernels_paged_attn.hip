@@ -264,9 +264,10 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     asm("" : "+v"(minus));
     const bool partly = last_pos != sees_all;   // some row does not attend to all that another does
 
-    // A chunk; at an edge, some row attends to a part of it only.
-    auto step = [&](uint32_t j, uint32_t w0, uint32_t w1, auto at_edge) {
-        constexpr bool edge = decltype(at_edge)::value;
+    // A chunk; at an edge, some row attends to a part of it only. (One body for both: with two, the
+    // compiler moves the sums from registers to registers between them.)
+    bool whole = false;   // some chunk was none at an edge
+    auto step = [&](uint32_t j, uint32_t w0, uint32_t w1, bool edge) {
         const uint8_t *const vu = vc + unit_of(j, q >= 2u);
         if constexpr (!AHEAD) kf.load(kc + unit_of(j, i >= 8u), i, q);
         // Behind the last chunk it is fetched once more, without a branch: with one between the products
@@ -301,7 +302,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
             for (int e = 0; e < 8; ++e) x[0][e / 4][e % 4] += dpp<0x128>(x[0][e / 4][e % 4]);   // row_ror:8
         }
         const uint32_t slot0 = (q < 2u ? w0 : w1) + 8u * (q % 2u);   // the lane's first position
-        if constexpr (edge) {
+        if (edge) {
 #pragma unroll
             for (int c = 0; c < NT; ++c) {
                 const uint32_t last = limit(c);
@@ -310,10 +311,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
                 saw[c] = saw[c] || slot0 <= last;
             }
         }
-        if constexpr (!edge) {
-#pragma unroll
-            for (int c = 0; c < NT; ++c) saw[c] = true;
-        }
+        whole = whole || !edge;
         float top[NT];
         bool moves = false;
 #pragma unroll
@@ -349,7 +347,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
             two_terms(v, minus, ph[c], pl[c]);   // of PK the term of the lane's column, by `minus`
         }
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (edge) {
+        if (edge) {
             // Slots behind the last position may hold anything: their values count as zero, as do
             // infinities and NaN among those that some row does not attend to, which `odd` notes.
             const U4 keep = halves_below(last_pos + 1u > slot0 ? last_pos + 1u - slot0 : 0u);
@@ -380,15 +378,12 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     };
     for (uint32_t j = 0; j < mine; ++j) {
         const uint32_t w0 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u), w1 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u + 1u);
-        if (max(w0, w1) + kPagedUnit - 1u <= sees_all)
-            step(j, w0, w1, std::false_type{});
-        else
-            step(j, w0, w1, std::true_type{});
+        step(j, w0, w1, max(w0, w1) + kPagedUnit - 1u > sees_all);
     }
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
         l[c] = row_sum(l[c]);
-        if (row_max(saw[c] ? 1.f : 0.f) == 0.f) l[c] = -1.f;   // nothing to add
+        if (!whole && row_max(saw[c] ? 1.f : 0.f) == 0.f) l[c] = -1.f;   // nothing to add
         if (q == 0) ms[w][16 * c + i] = m[c], ls[w][16 * c + i] = l[c];
     }
     // Infinities in V have no two terms to be multiplied by, and some were taken as zero: where a sum
@@ -532,6 +527,318 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     }
 }
 
+// Prompts: a tile of 32 RG query rows, RG x KG waves (8). Wave (rg, kg) has 32 rows and every KG-th
+// chunk; the KG chunks of a stage lie in LDS, where RG waves read them, and the next stage's are on
+// their way to registers meanwhile. (A wave with chunks of its own from memory, as above, is bound by
+// the 64 bytes a clock that reach a CU: 16 KB for 64 products of 32 rows.)
+template <int HD, int KG>
+__global__ __launch_bounds__(512, 1) void k_paged_prompt(AttnArgs p) {
+    constexpr int U = HD / 32, DT = HD / 16, NT = 2, RG = 8 / KG, R = 32 * RG, OROW = HD + 4;
+    constexpr uint32_t UNIT = 32 * HD, US = 2 * UNIT + 64, STAGE = 2 * KG * US;   // bytes; 64: a chunk's two units in other banks
+    constexpr int PIECES = KG / 2 * UNIT * 2 / 2048;   // 16 bytes a lane: of a wave's unit, K or V (KG 2) or both
+    constexpr uint32_t JOIN = 8 * 16 * OROW * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE > JOIN ? 2 * STAGE : JOIN];
+    __shared__ uint32_t where_of[2][2 * KG], odd[2][HD], odd_in[8];
+    __shared__ float ms[8][32], ls[8][32];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6), rg = w / KG, kg = w % KG;
+    const uint32_t heads = p.a.b.geom.kv_heads, head = blockIdx.x % heads;
+    const Tile t = uniform(tile_of(p, blockIdx.x / heads));
+    if (!t.ok || t.n == 0) return;
+    const uint32_t rows = t.count * p.group, r0 = t.tile + 32u * rg;
+    const uint32_t sees_all = t.base + token_of(p, min(r0, rows - 1u));                    // last position that every row of the wave attends to
+    const uint32_t last_pos = t.base + token_of(p, min(t.tile + R, rows) - 1u);            // and that some row of the tile does
+    const uint8_t *const kc = p.a.kc + p.layer_at, *const vc = p.a.vc + p.layer_at;
+
+    // The wave fetches unit mine_u of every stage: lane s has stage s0 + s's.
+    const uint32_t mine_u = KG == 2 ? w >> 1 : w;
+    uint32_t unit = 0, where = kFar;
+    auto look_up = [&](uint32_t s0) {
+        const uint32_t c = (s0 + lane) * KG + mine_u / 2u, at = (t.first + c) * 32u + kPagedUnit * (mine_u & 1u);
+        unit = 0;
+        where = kFar;
+        const uint32_t index = at >> p.shift;
+        if (c >= t.n || at > last_pos || index >= p.a.b.table_width) return;
+        const uint32_t page = p.a.tables[(size_t)t.request * p.a.b.table_width + index];
+        if (page >= p.a.b.geom.pages) return;
+        unit = (page * heads + head) * p.units + (at & (p.a.b.geom.page_size - 1u)) / kPagedUnit;
+        where = at;
+    };
+    h8 piece[PIECES];
+    auto fetch = [&](uint32_t s) {
+        const size_t from = (size_t)(uint32_t)__builtin_amdgcn_readlane(unit, s & 63u) * UNIT + lane * 16u;
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+            const bool v = KG == 2 ? w & 1u : k >= PIECES / 2;
+            piece[k] = *reinterpret_cast<const h8 *>((v ? vc : kc) + from + (KG == 2 ? k : k % (PIECES / 2)) * 1024);
+        }
+    };
+    auto lay = [&](uint32_t s) {
+        uint8_t *const to = lds + (s & 1u) * STAGE + mine_u * US + (KG == 2 && (w & 1u) ? UNIT : 0u) + lane * 16u;
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) *reinterpret_cast<h8 *>(to + k * 1024) = piece[k];   // KG 4: V lies behind K
+        if (lane == 0 && (KG == 4 || !(w & 1u))) where_of[s & 1u][mine_u] = __builtin_amdgcn_readlane(where, s & 63u);
+    };
+    const uint32_t stages = (t.n + KG - 1u) / KG;
+    look_up(0);
+    fetch(0);
+
+    for (uint32_t d = tid; d < 2u * HD; d += 512u) odd[d / HD][d % HD] = ~0u;
+    h8 qh[NT][U], ql[NT][U];
+    float factor[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        const uint32_t row = r0 + 16u * c + i;
+        QRow<HD> qr;
+        qr.load(p, t, head, min(row, rows - 1u), row < rows, q);
+        factor[c] = qr.split(qh[c], ql[c]);
+    }
+    uint32_t last[NT];   // last position that the lane's row of a column tile attends to
+    float m[NT], l[NT];
+    bool saw[NT];
+    f4 o[NT][DT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        last[c] = t.base + token_of(p, min(r0 + 16u * c + i, rows - 1u));
+        m[c] = -INFINITY;
+        l[c] = 0.f;
+        saw[c] = false;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[c][dt] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    float minus = -1.0f;
+    asm("" : "+v"(minus));
+    uint32_t found = 0;
+
+    bool whole = false;
+    auto step = [&](const uint8_t *chunk, uint32_t w0, uint32_t w1, uint32_t next, bool edge) {
+        const uint8_t *const kat = chunk + (i >= 8u ? US : 0u) + (8u * (i / 4u % 2u) + i % 4u) * 16u + q * 256u;
+        const uint8_t *const vat = chunk + (q >= 2u ? US : 0u) + UNIT + (q % 2u) * (HD * 16u) + i * 16u;
+        f4 x[NT][2];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) x[c][0] = x[c][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+                const h8 k = *reinterpret_cast<const h8 *>(kat + tt * 64 + u * 1024);
+#pragma unroll
+                for (int c = 0; c < NT; ++c) x[c][tt] = mfma16(k, qh[c][u], x[c][tt]);
+#pragma unroll
+                for (int c = 0; c < NT; ++c) x[c][tt] = mfma16(k, ql[c][u], x[c][tt]);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(next);
+        const uint32_t slot0 = (q < 2u ? w0 : w1) + 8u * (q % 2u);
+        if (edge) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[c][e / 4][e % 4] = slot0 + e > last[c] ? -INFINITY : x[c][e / 4][e % 4];
+                saw[c] = saw[c] || slot0 <= last[c];
+            }
+        }
+        whole = whole || !edge;
+        float top[NT];
+        bool moves = false;
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            top[c] = x[c][0][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) top[c] = fmaxf(top[c], x[c][e / 4][e % 4]);
+            top[c] *= factor[c];
+            moves = moves || top[c] - m[c] > kMost;
+        }
+        if (__builtin_expect(__any(moves), 0)) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                const float s = row_max(top[c]), mn = s - m[c] > kMost ? s - kRaise : m[c];
+                const float alpha = mn == m[c] ? 1.f : __builtin_amdgcn_exp2f(m[c] - mn);
+                m[c] = mn;
+                l[c] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[c][dt] *= alpha;
+            }
+        }
+        h8 ph[NT], pl[NT];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+            const float ref = m[c] == -INFINITY ? 0.f : m[c];   // as in k_paged_attn
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[c][e / 4][e % 4], factor[c], -ref));
+                l[c] += v[e];
+            }
+            two_terms(v, minus, ph[c], pl[c]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        h8 v[DT];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) v[dt] = *reinterpret_cast<const h8 *>(vat + dt * 256);
+        if (edge) {   // as in k_paged_attn
+            const U4 keep = halves_below(last_pos + 1u > slot0 ? last_pos + 1u - slot0 : 0u);
+            const U4 own = ~halves_below(sees_all + 1u > slot0 ? sees_all + 1u - slot0 : 0u);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const U4 y = __builtin_bit_cast(U4, v[dt]) & keep, up = ((y & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+                const U4 bad = (up | (up - (up >> 15))) & own;
+                found |= (bad[0] | bad[1]) | (bad[2] | bad[3]);
+                v[dt] = __builtin_bit_cast(h8, y & ~bad);
+            }
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c) o[c][dt] = mfma16(v[dt], ph[c], o[c][dt]);
+#pragma unroll
+            for (int c = 0; c < NT; ++c) o[c][dt] = mfma16(v[dt], pl[c], o[c][dt]);
+        }
+    };
+    lay(0);
+    for (uint32_t s = 0; s < stages; ++s) {
+        __syncthreads();   // stage s lies in LDS, the other buffer has been read
+        const uint32_t next = min(s + 1u, stages - 1u);
+        if ((next & 63u) == 0 && next != s) look_up(next);
+        const uint8_t *const chunk = lds + (s & 1u) * STAGE + 2u * kg * US;
+        const uint32_t w0 = __builtin_amdgcn_readfirstlane(where_of[s & 1u][2u * kg]), w1 = __builtin_amdgcn_readfirstlane(where_of[s & 1u][2u * kg + 1u]);
+        step(chunk, w0, w1, next, max(w0, w1) + kPagedUnit - 1u > sees_all);   // of a chunk behind the last nothing counts
+        if (s + 1u < stages) lay(s + 1u);
+    }
+    float zero = found ? __builtin_nanf("") : 0.f;
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        l[c] = row_sum(l[c]);
+        if (!whole && row_max(saw[c] ? 1.f : 0.f) == 0.f) l[c] = -1.f;   // nothing to add
+        if (q == 0) ms[w][16 * c + i] = m[c], ls[w][16 * c + i] = l[c];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) zero = __builtin_fmaf(o[c][dt][e], 0.f, zero);
+    }
+    const bool finite_here = __all(zero == 0.f);
+    if (lane == 0) odd_in[w] = !finite_here;
+    __syncthreads();   // the chunks in LDS have been read, every wave's m and l are there
+    bool any_odd = false;
+#pragma unroll
+    for (int v = 0; v < 8; ++v) any_odd = any_odd || odd_in[v] != 0;
+    if (__builtin_expect(any_odd, 0)) {   // rare: V again, a unit a wave, for where its infinities and NaN are
+        for (uint32_t n = w; n < 2u * t.n; n += 8u) {
+            const uint32_t at = t.first * 32u + n * kPagedUnit, index = at >> p.shift;
+            if (at > last_pos || index >= p.a.b.table_width) break;
+            const uint32_t page = p.a.tables[(size_t)t.request * p.a.b.table_width + index];
+            if (page >= p.a.b.geom.pages) continue;
+            const size_t from = (size_t)((page * heads + head) * p.units + (at & (p.a.b.geom.page_size - 1u)) / kPagedUnit) * UNIT;
+            for (uint32_t x = lane; x < 2u * HD; x += 64u) {   // octet x / HD, dimension x % HD
+                const h8 v = *reinterpret_cast<const h8 *>(vc + from + x * 16u);
+                uint32_t up = ~0u, down = ~0u;
+#pragma unroll
+                for (int e = 7; e >= 0; --e) {
+                    const uint32_t slot = at + x / HD * 8u + e;
+                    const bool counts = !finite(v[e]) && slot <= last_pos;
+                    up = counts && !(v[e] < 0.f16) ? slot : up;
+                    down = counts && !(v[e] > 0.f16) ? slot : down;
+                }
+                if (up != ~0u) atomicMin(&odd[0][x % HD], up);
+                if (down != ~0u) atomicMin(&odd[1][x % HD], down);
+            }
+        }
+    }
+    // The KG waves of a row group are joined: their sums to the rows' largest references, then added.
+    float sum[NT], top[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        float mv[KG], lv[KG];
+        top[c] = -INFINITY;
+        sum[c] = -1.f;
+#pragma unroll
+        for (int v = 0; v < KG; ++v) {
+            mv[v] = ms[rg * KG + v][16 * c + i], lv[v] = ls[rg * KG + v][16 * c + i];
+            top[c] = fmaxf(top[c], mv[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < KG; ++v)
+            if (!(lv[v] < 0.f))
+                sum[c] = (sum[c] < 0.f ? 0.f : sum[c]) + (mv[v] == -INFINITY ? lv[v] : lv[v] * __builtin_amdgcn_exp2f(mv[v] - top[c]));
+        const float share = m[c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[c] - top[c]);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[c][dt] *= share;
+    }
+    auto *const os = reinterpret_cast<float (*)[16][OROW]>(lds);
+    // a wave keeps column tile kg % 2 and gives the other to its partner
+    auto give = [&](auto keeps) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+            *reinterpret_cast<f4 *>(&os[w][i][16 * dt + 4 * q]) = o[decltype(keeps)::value ? 0 : 1][dt];
+    };
+    auto take = [&](auto keeps, uint32_t from) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+            o[decltype(keeps)::value ? 1 : 0][dt] += *reinterpret_cast<const f4 *>(&os[from][i][16 * dt + 4 * q]);
+    };
+    if (kg & 1u)
+        give(std::true_type{});
+    else
+        give(std::false_type{});
+    __syncthreads();
+    if (kg & 1u)
+        take(std::true_type{}, w ^ 1u);
+    else
+        take(std::false_type{}, w ^ 1u);
+    if constexpr (KG == 4) {
+        __syncthreads();
+        if (kg >= 2u) {
+            if (kg & 1u)
+                give(std::false_type{});
+            else
+                give(std::true_type{});
+        }
+        __syncthreads();
+        if (kg >= 2u) return;
+        if (kg & 1u)
+            take(std::true_type{}, w + 2u);
+        else
+            take(std::false_type{}, w + 2u);
+    }
+    const bool alone = t.part == VX_PAGED_NONE;
+    const size_t part = (size_t)head * p.parts + (alone ? 0u : t.part);
+    auto finish = [&](auto keeps) {
+        constexpr int c = decltype(keeps)::value ? 1 : 0;
+        const uint32_t row = r0 + 16u * c + i, in_tile = 32u * rg + 16u * c + i;
+        if (row >= rows) return;
+        if (!alone && q == 0) {
+            p.ml[(part * R + in_tile) * 2u] = top[c];
+            p.ml[(part * R + in_tile) * 2u + 1u] = sum[c];
+        }
+        const uint32_t k0 = token_of(p, row), j = row - k0 * p.group;
+        float *const to = alone ? p.a.out + (size_t)(t.row + k0) * p.a.out_stride + (size_t)(head * p.group + j) * HD + 4u * q
+                                : p.acc + (part * R + in_tile) * HD + 4u * q;
+        const float scale = alone ? 1.0f / sum[c] : 1.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            f4 v = o[c][dt];
+            if (any_odd) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool up = odd[0][16 * dt + 4 * q + e] <= last[c], down = odd[1][16 * dt + 4 * q + e] <= last[c];
+                    v[e] = up ? down ? __builtin_nanf("") : INFINITY : down ? -INFINITY : v[e];
+                }
+            }
+            v = alone && sum[c] < 0.f ? f4{0.f, 0.f, 0.f, 0.f} : v * scale;
+            if (!alone || p.a.ovec) {
+                *reinterpret_cast<f4 *>(to + 16 * dt) = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) to[16 * dt + e] = v[e];
+            }
+        }
+    };
+    if (kg & 1u)
+        finish(std::true_type{});
+    else
+        finish(std::false_type{});
+}
+
 // The parts of a tile's row, joined: a workgroup a row, its lanes HD / 4 columns by as many parts at
 // once as fit.
 template <int HD>
@@ -644,8 +951,14 @@ void run(hipStream_t s, const AttnArgs &p, uint64_t grid) {
         k_paged_attn<HD, 1, 4, true><<<g, 256, 0, s>>>(p);
     else if (p.a.s.tile_rows == 16u)
         k_paged_attn<HD, 1, 4, false><<<g, 256, 0, s>>>(p);
-    else if constexpr (HD < 256)
-        k_paged_attn<HD, 2, 8, false><<<g, 512, 0, s>>>(p);
+    else if constexpr (HD < 256) {
+        if (p.a.s.tile_rows == 32u)
+            k_paged_attn<HD, 2, 8, false><<<g, 512, 0, s>>>(p);
+        else if (p.a.s.tile_rows == 64u)
+            k_paged_prompt<HD, 4><<<g, 512, 0, s>>>(p);
+        else
+            k_paged_prompt<HD, 2><<<g, 512, 0, s>>>(p);
+    }
 }
 
 }  // namespace
