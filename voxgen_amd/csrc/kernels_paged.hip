@@ -123,8 +123,10 @@ __global__ __launch_bounds__(T) void k_paged_plan(PagedPlan a) {
     // a wave's chunks are alike in number
     const uint32_t per = max(((uint32_t)fminf(ceilf(todo), 1e9f) + a.s.waves - 1u) >> wave_shift << wave_shift, a.s.least);
     // Chunks of a part, of which there are `splits`; a request's tiles are all divided alike.
+    // Tiles of many rows are divided where twice the share would be exceeded: what they have to join
+    // takes longer then.
     auto divided = [&](uint32_t many, uint32_t &splits) {
-        splits = min((many + per - 1u) / per, kPagedMaxSplits);
+        splits = min(a.s.tile_rows > 16u ? max(many / per, 1u) : (many + per - 1u) / per, kPagedMaxSplits);
         const uint32_t by = splits > 1u ? ((many + splits - 1u) / splits + a.s.waves - 1u) >> wave_shift << wave_shift : max(many, 1u);
         splits = splits > 1u ? (many + by - 1u) / by : splits;
         return by;

@@ -527,15 +527,25 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     }
 }
 
+// 16 bytes a lane from memory to LDS, 1 KB behind one another from `to` on. The compiler does not count
+// this load, and would have every read of LDS wait for it: who reads waits for all loads and a barrier.
+__device__ __forceinline__ void to_lds(const uint8_t *from, const uint8_t *to) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)to);
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0)
+                 : "s"(at), "v"(from)
+                 : "memory");
+}
+
 // Prompts: a tile of 32 RG query rows, RG x KG waves (8). Wave (rg, kg) has 32 rows and every KG-th
 // chunk; the KG chunks of a stage lie in LDS, where RG waves read them, and the next stage's are on
-// their way to registers meanwhile. (A wave with chunks of its own from memory, as above, is bound by
+// their way there meanwhile. (A wave with chunks of its own from memory, as above, is bound by
 // the 64 bytes a clock that reach a CU: 16 KB for 64 products of 32 rows.)
 template <int HD, int KG>
 __global__ __launch_bounds__(512, 1) void k_paged_prompt(AttnArgs p) {
     constexpr int U = HD / 32, DT = HD / 16, NT = 2, RG = 8 / KG, R = 32 * RG, OROW = HD + 4;
     constexpr uint32_t UNIT = 32 * HD, US = 2 * UNIT + 64, STAGE = 2 * KG * US;   // bytes; 64: a chunk's two units in other banks
-    constexpr int PIECES = KG / 2 * UNIT * 2 / 2048;   // 16 bytes a lane: of a wave's unit, K or V (KG 2) or both
     constexpr uint32_t JOIN = 8 * 16 * OROW * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE > JOIN ? 2 * STAGE : JOIN];
     __shared__ uint32_t where_of[2][2 * KG], odd[2][HD], odd_in[8];
@@ -564,19 +574,15 @@ __global__ __launch_bounds__(512, 1) void k_paged_prompt(AttnArgs p) {
         unit = (page * heads + head) * p.units + (at & (p.a.b.geom.page_size - 1u)) / kPagedUnit;
         where = at;
     };
-    h8 piece[PIECES];
-    auto fetch = [&](uint32_t s) {
+    auto fetch = [&](uint32_t s) {   // straight to LDS
         const size_t from = (size_t)(uint32_t)__builtin_amdgcn_readlane(unit, s & 63u) * UNIT + lane * 16u;
+        uint8_t *const to = lds + (s & 1u) * STAGE + mine_u * US;
 #pragma unroll
-        for (int k = 0; k < PIECES; ++k) {
-            const bool v = KG == 2 ? w & 1u : k >= PIECES / 2;
-            piece[k] = *reinterpret_cast<const h8 *>((v ? vc : kc) + from + (KG == 2 ? k : k % (PIECES / 2)) * 1024);
+        for (uint32_t k = 0; k < (KG == 2 ? 1u : 2u); ++k) {
+            const bool v = KG == 2 ? w & 1u : k != 0u;
+#pragma unroll
+            for (uint32_t b = 0; b < UNIT; b += 1024u) to_lds((v ? vc : kc) + from + b, to + (v ? UNIT : 0u) + b);
         }
-    };
-    auto lay = [&](uint32_t s) {
-        uint8_t *const to = lds + (s & 1u) * STAGE + mine_u * US + (KG == 2 && (w & 1u) ? UNIT : 0u) + lane * 16u;
-#pragma unroll
-        for (int k = 0; k < PIECES; ++k) *reinterpret_cast<h8 *>(to + k * 1024) = piece[k];   // KG 4: V lies behind K
         if (lane == 0 && (KG == 4 || !(w & 1u))) where_of[s & 1u][mine_u] = __builtin_amdgcn_readlane(where, s & 63u);
     };
     const uint32_t stages = (t.n + KG - 1u) / KG;
@@ -611,24 +617,26 @@ __global__ __launch_bounds__(512, 1) void k_paged_prompt(AttnArgs p) {
     uint32_t found = 0;
 
     bool whole = false;
-    auto step = [&](const uint8_t *chunk, uint32_t w0, uint32_t w1, uint32_t next, bool edge) {
+    auto step = [&](const uint8_t *chunk, uint32_t w0, uint32_t w1, bool edge) {
         const uint8_t *const kat = chunk + (i >= 8u ? US : 0u) + (8u * (i / 4u % 2u) + i % 4u) * 16u + q * 256u;
         const uint8_t *const vat = chunk + (q >= 2u ? US : 0u) + UNIT + (q % 2u) * (HD * 16u) + i * 16u;
         f4 x[NT][2];
 #pragma unroll
         for (int c = 0; c < NT; ++c) x[c][0] = x[c][1] = f4{0.f, 0.f, 0.f, 0.f};
+        h8 k[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt) {
-                const h8 k = *reinterpret_cast<const h8 *>(kat + tt * 64 + u * 1024);
-#pragma unroll
-                for (int c = 0; c < NT; ++c) x[c][tt] = mfma16(k, qh[c][u], x[c][tt]);
-#pragma unroll
-                for (int c = 0; c < NT; ++c) x[c][tt] = mfma16(k, ql[c][u], x[c][tt]);
-            }
+            for (int tt = 0; tt < 2; ++tt) k[u][tt] = *reinterpret_cast<const h8 *>(kat + tt * 64 + u * 1024);
         __builtin_amdgcn_sched_barrier(0);
-        fetch(next);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int c = 0; c < 2 * NT; ++c) x[c / 2][c % 2] = mfma16(k[u][c % 2], qh[c / 2][u], x[c / 2][c % 2]);
+#pragma unroll
+            for (int c = 0; c < 2 * NT; ++c) x[c / 2][c % 2] = mfma16(k[u][c % 2], ql[c / 2][u], x[c / 2][c % 2]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         const uint32_t slot0 = (q < 2u ? w0 : w1) + 8u * (q % 2u);
         if (edge) {
 #pragma unroll
@@ -695,15 +703,16 @@ __global__ __launch_bounds__(512, 1) void k_paged_prompt(AttnArgs p) {
             for (int c = 0; c < NT; ++c) o[c][dt] = mfma16(v[dt], pl[c], o[c][dt]);
         }
     };
-    lay(0);
     for (uint32_t s = 0; s < stages; ++s) {
+        __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();   // stage s lies in LDS, the other buffer has been read
-        const uint32_t next = min(s + 1u, stages - 1u);
-        if ((next & 63u) == 0 && next != s) look_up(next);
+        if (s + 1u < stages) {
+            if (((s + 1u) & 63u) == 0) look_up(s + 1u);
+            fetch(s + 1u);
+        }
         const uint8_t *const chunk = lds + (s & 1u) * STAGE + 2u * kg * US;
         const uint32_t w0 = __builtin_amdgcn_readfirstlane(where_of[s & 1u][2u * kg]), w1 = __builtin_amdgcn_readfirstlane(where_of[s & 1u][2u * kg + 1u]);
-        step(chunk, w0, w1, next, max(w0, w1) + kPagedUnit - 1u > sees_all);   // of a chunk behind the last nothing counts
-        if (s + 1u < stages) lay(s + 1u);
+        step(chunk, w0, w1, max(w0, w1) + kPagedUnit - 1u > sees_all);   // of a chunk behind the last nothing counts
     }
     float zero = found ? __builtin_nanf("") : 0.f;
 #pragma unroll
