@@ -527,404 +527,83 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     }
 }
 
-// 16 bytes a lane from memory to LDS, 1 KB behind one another from `to` on. The compiler does not count
-// this load, and would have every read of LDS wait for it: who reads waits for all loads and a barrier.
-__device__ __forceinline__ void to_lds(const uint8_t *from, const uint8_t *to) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)to);
-    uint32_t m0;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(m0)
-                 : "s"(at), "v"(from)
-                 : "memory");
-}
-
-// Prompts: a tile of 32 RG query rows, RG x KG waves (8). Wave (rg, kg) has 32 rows and every KG-th
-// chunk; the KG chunks of a stage lie in LDS, where RG waves read them, and the next stage's are on
-// their way there meanwhile. (A wave with chunks of its own from memory, as above, is bound by
-// the 64 bytes a clock that reach a CU: 16 KB for 64 products of 32 rows.)
-template <int HD, int KG>
-__global__ __launch_bounds__(512, 1) void k_paged_prompt(AttnArgs p) {
-    constexpr int U = HD / 32, DT = HD / 16, NT = 2, RG = 8 / KG, R = 32 * RG, OROW = HD + 4;
-    constexpr uint32_t UNIT = 32 * HD, US = 2 * UNIT + 64, STAGE = 2 * KG * US;   // bytes; 64: a chunk's two units in other banks
-    constexpr uint32_t JOIN = 8 * 16 * OROW * 4;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE > JOIN ? 2 * STAGE : JOIN];
-    __shared__ uint32_t where_of[2][2 * KG], odd[2][HD], odd_in[8];
-    __shared__ float ms[8][32], ls[8][32];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
-    const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6), rg = w / KG, kg = w % KG;
-    const uint32_t heads = p.a.b.geom.kv_heads, head = blockIdx.x % heads;
-    const Tile t = uniform(tile_of(p, blockIdx.x / heads));
-    if (!t.ok || t.n == 0) return;
-    const uint32_t rows = t.count * p.group, r0 = t.tile + 32u * rg;
-    const uint32_t sees_all = t.base + token_of(p, min(r0, rows - 1u));                    // last position that every row of the wave attends to
-    const uint32_t last_pos = t.base + token_of(p, min(t.tile + R, rows) - 1u);            // and that some row of the tile does
-    const uint8_t *const kc = p.a.kc + p.layer_at, *const vc = p.a.vc + p.layer_at;
-
-    // The wave fetches unit mine_u of every stage: lane s has stage s0 + s's.
-    const uint32_t mine_u = KG == 2 ? w >> 1 : w;
-    uint32_t unit = 0, where = kFar;
-    auto look_up = [&](uint32_t s0) {
-        const uint32_t c = (s0 + lane) * KG + mine_u / 2u, at = (t.first + c) * 32u + kPagedUnit * (mine_u & 1u);
-        unit = 0;
-        where = kFar;
-        const uint32_t index = at >> p.shift;
-        if (c >= t.n || at > last_pos || index >= p.a.b.table_width) return;
-        const uint32_t page = p.a.tables[(size_t)t.request * p.a.b.table_width + index];
-        if (page >= p.a.b.geom.pages) return;
-        unit = (page * heads + head) * p.units + (at & (p.a.b.geom.page_size - 1u)) / kPagedUnit;
-        where = at;
-    };
-    auto fetch = [&](uint32_t s) {   // straight to LDS
-        const size_t from = (size_t)(uint32_t)__builtin_amdgcn_readlane(unit, s & 63u) * UNIT + lane * 16u;
-        uint8_t *const to = lds + (s & 1u) * STAGE + mine_u * US;
-#pragma unroll
-        for (uint32_t k = 0; k < (KG == 2 ? 1u : 2u); ++k) {
-            const bool v = KG == 2 ? w & 1u : k != 0u;
-#pragma unroll
-            for (uint32_t b = 0; b < UNIT; b += 1024u) to_lds((v ? vc : kc) + from + b, to + (v ? UNIT : 0u) + b);
-        }
-        if (lane == 0 && (KG == 4 || !(w & 1u))) where_of[s & 1u][mine_u] = __builtin_amdgcn_readlane(where, s & 63u);
-    };
-    const uint32_t stages = (t.n + KG - 1u) / KG;
-    look_up(0);
-    fetch(0);
-
-    for (uint32_t d = tid; d < 2u * HD; d += 512u) odd[d / HD][d % HD] = ~0u;
-    h8 qh[NT][U], ql[NT][U];
-    float factor[NT];
-#pragma unroll
-    for (int c = 0; c < NT; ++c) {
-        const uint32_t row = r0 + 16u * c + i;
-        QRow<HD> qr;
-        qr.load(p, t, head, min(row, rows - 1u), row < rows, q);
-        factor[c] = qr.split(qh[c], ql[c]);
-    }
-    uint32_t last[NT];   // last position that the lane's row of a column tile attends to
-    float m[NT], l[NT];
-    bool saw[NT];
-    f4 o[NT][DT];
-#pragma unroll
-    for (int c = 0; c < NT; ++c) {
-        last[c] = t.base + token_of(p, min(r0 + 16u * c + i, rows - 1u));
-        m[c] = -INFINITY;
-        l[c] = 0.f;
-        saw[c] = false;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[c][dt] = f4{0.f, 0.f, 0.f, 0.f};
-    }
-    float minus = -1.0f;
-    asm("" : "+v"(minus));
-    uint32_t found = 0;
-
-    bool whole = false;
-    auto step = [&](const uint8_t *chunk, uint32_t w0, uint32_t w1, bool edge) {
-        const uint8_t *const kat = chunk + (i >= 8u ? US : 0u) + (8u * (i / 4u % 2u) + i % 4u) * 16u + q * 256u;
-        const uint8_t *const vat = chunk + (q >= 2u ? US : 0u) + UNIT + (q % 2u) * (HD * 16u) + i * 16u;
-        f4 x[NT][2];
-#pragma unroll
-        for (int c = 0; c < NT; ++c) x[c][0] = x[c][1] = f4{0.f, 0.f, 0.f, 0.f};
-        h8 k[U][2];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt) k[u][tt] = *reinterpret_cast<const h8 *>(kat + tt * 64 + u * 1024);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int c = 0; c < 2 * NT; ++c) x[c / 2][c % 2] = mfma16(k[u][c % 2], qh[c / 2][u], x[c / 2][c % 2]);
-#pragma unroll
-            for (int c = 0; c < 2 * NT; ++c) x[c / 2][c % 2] = mfma16(k[u][c % 2], ql[c / 2][u], x[c / 2][c % 2]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        const uint32_t slot0 = (q < 2u ? w0 : w1) + 8u * (q % 2u);
-        if (edge) {
-#pragma unroll
-            for (int c = 0; c < NT; ++c) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[c][e / 4][e % 4] = slot0 + e > last[c] ? -INFINITY : x[c][e / 4][e % 4];
-                saw[c] = saw[c] || slot0 <= last[c];
-            }
-        }
-        whole = whole || !edge;
-        float top[NT];
-        bool moves = false;
-#pragma unroll
-        for (int c = 0; c < NT; ++c) {
-            top[c] = x[c][0][0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) top[c] = fmaxf(top[c], x[c][e / 4][e % 4]);
-            top[c] *= factor[c];
-            moves = moves || top[c] - m[c] > kMost;
-        }
-        if (__builtin_expect(__any(moves), 0)) {
-#pragma unroll
-            for (int c = 0; c < NT; ++c) {
-                const float s = row_max(top[c]), mn = s - m[c] > kMost ? s - kRaise : m[c];
-                const float alpha = mn == m[c] ? 1.f : __builtin_amdgcn_exp2f(m[c] - mn);
-                m[c] = mn;
-                l[c] *= alpha;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) o[c][dt] *= alpha;
-            }
-        }
-        h8 ph[NT], pl[NT];
-#pragma unroll
-        for (int c = 0; c < NT; ++c) {
-            const float ref = m[c] == -INFINITY ? 0.f : m[c];   // as in k_paged_attn
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[c][e / 4][e % 4], factor[c], -ref));
-                l[c] += v[e];
-            }
-            two_terms(v, minus, ph[c], pl[c]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        h8 v[DT];
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) v[dt] = *reinterpret_cast<const h8 *>(vat + dt * 256);
-        if (edge) {   // as in k_paged_attn
-            const U4 keep = halves_below(last_pos + 1u > slot0 ? last_pos + 1u - slot0 : 0u);
-            const U4 own = ~halves_below(sees_all + 1u > slot0 ? sees_all + 1u - slot0 : 0u);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const U4 y = __builtin_bit_cast(U4, v[dt]) & keep, up = ((y & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-                const U4 bad = (up | (up - (up >> 15))) & own;
-                found |= (bad[0] | bad[1]) | (bad[2] | bad[3]);
-                v[dt] = __builtin_bit_cast(h8, y & ~bad);
-            }
-        }
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-#pragma unroll
-            for (int c = 0; c < NT; ++c) o[c][dt] = mfma16(v[dt], ph[c], o[c][dt]);
-#pragma unroll
-            for (int c = 0; c < NT; ++c) o[c][dt] = mfma16(v[dt], pl[c], o[c][dt]);
-        }
-    };
-    for (uint32_t s = 0; s < stages; ++s) {
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();   // stage s lies in LDS, the other buffer has been read
-        if (s + 1u < stages) {
-            if (((s + 1u) & 63u) == 0) look_up(s + 1u);
-            fetch(s + 1u);
-        }
-        const uint8_t *const chunk = lds + (s & 1u) * STAGE + 2u * kg * US;
-        const uint32_t w0 = __builtin_amdgcn_readfirstlane(where_of[s & 1u][2u * kg]), w1 = __builtin_amdgcn_readfirstlane(where_of[s & 1u][2u * kg + 1u]);
-        step(chunk, w0, w1, max(w0, w1) + kPagedUnit - 1u > sees_all);   // of a chunk behind the last nothing counts
-    }
-    float zero = found ? __builtin_nanf("") : 0.f;
-#pragma unroll
-    for (int c = 0; c < NT; ++c) {
-        l[c] = row_sum(l[c]);
-        if (!whole && row_max(saw[c] ? 1.f : 0.f) == 0.f) l[c] = -1.f;   // nothing to add
-        if (q == 0) ms[w][16 * c + i] = m[c], ls[w][16 * c + i] = l[c];
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) zero = __builtin_fmaf(o[c][dt][e], 0.f, zero);
-    }
-    const bool finite_here = __all(zero == 0.f);
-    if (lane == 0) odd_in[w] = !finite_here;
-    __syncthreads();   // the chunks in LDS have been read, every wave's m and l are there
-    bool any_odd = false;
-#pragma unroll
-    for (int v = 0; v < 8; ++v) any_odd = any_odd || odd_in[v] != 0;
-    if (__builtin_expect(any_odd, 0)) {   // rare: V again, a unit a wave, for where its infinities and NaN are
-        for (uint32_t n = w; n < 2u * t.n; n += 8u) {
-            const uint32_t at = t.first * 32u + n * kPagedUnit, index = at >> p.shift;
-            if (at > last_pos || index >= p.a.b.table_width) break;
-            const uint32_t page = p.a.tables[(size_t)t.request * p.a.b.table_width + index];
-            if (page >= p.a.b.geom.pages) continue;
-            const size_t from = (size_t)((page * heads + head) * p.units + (at & (p.a.b.geom.page_size - 1u)) / kPagedUnit) * UNIT;
-            for (uint32_t x = lane; x < 2u * HD; x += 64u) {   // octet x / HD, dimension x % HD
-                const h8 v = *reinterpret_cast<const h8 *>(vc + from + x * 16u);
-                uint32_t up = ~0u, down = ~0u;
-#pragma unroll
-                for (int e = 7; e >= 0; --e) {
-                    const uint32_t slot = at + x / HD * 8u + e;
-                    const bool counts = !finite(v[e]) && slot <= last_pos;
-                    up = counts && !(v[e] < 0.f16) ? slot : up;
-                    down = counts && !(v[e] > 0.f16) ? slot : down;
-                }
-                if (up != ~0u) atomicMin(&odd[0][x % HD], up);
-                if (down != ~0u) atomicMin(&odd[1][x % HD], down);
-            }
-        }
-    }
-    // The KG waves of a row group are joined: their sums to the rows' largest references, then added.
-    float sum[NT], top[NT];
-#pragma unroll
-    for (int c = 0; c < NT; ++c) {
-        float mv[KG], lv[KG];
-        top[c] = -INFINITY;
-        sum[c] = -1.f;
-#pragma unroll
-        for (int v = 0; v < KG; ++v) {
-            mv[v] = ms[rg * KG + v][16 * c + i], lv[v] = ls[rg * KG + v][16 * c + i];
-            top[c] = fmaxf(top[c], mv[v]);
-        }
-#pragma unroll
-        for (int v = 0; v < KG; ++v)
-            if (!(lv[v] < 0.f))
-                sum[c] = (sum[c] < 0.f ? 0.f : sum[c]) + (mv[v] == -INFINITY ? lv[v] : lv[v] * __builtin_amdgcn_exp2f(mv[v] - top[c]));
-        const float share = m[c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[c] - top[c]);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[c][dt] *= share;
-    }
-    auto *const os = reinterpret_cast<float (*)[16][OROW]>(lds);
-    // a wave keeps column tile kg % 2 and gives the other to its partner
-    auto give = [&](auto keeps) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-            *reinterpret_cast<f4 *>(&os[w][i][16 * dt + 4 * q]) = o[decltype(keeps)::value ? 0 : 1][dt];
-    };
-    auto take = [&](auto keeps, uint32_t from) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-            o[decltype(keeps)::value ? 1 : 0][dt] += *reinterpret_cast<const f4 *>(&os[from][i][16 * dt + 4 * q]);
-    };
-    if (kg & 1u)
-        give(std::true_type{});
-    else
-        give(std::false_type{});
-    __syncthreads();
-    if (kg & 1u)
-        take(std::true_type{}, w ^ 1u);
-    else
-        take(std::false_type{}, w ^ 1u);
-    if constexpr (KG == 4) {
-        __syncthreads();
-        if (kg >= 2u) {
-            if (kg & 1u)
-                give(std::false_type{});
-            else
-                give(std::true_type{});
-        }
-        __syncthreads();
-        if (kg >= 2u) return;
-        if (kg & 1u)
-            take(std::true_type{}, w + 2u);
-        else
-            take(std::false_type{}, w + 2u);
-    }
-    const bool alone = t.part == VX_PAGED_NONE;
-    const size_t part = (size_t)head * p.parts + (alone ? 0u : t.part);
-    auto finish = [&](auto keeps) {
-        constexpr int c = decltype(keeps)::value ? 1 : 0;
-        const uint32_t row = r0 + 16u * c + i, in_tile = 32u * rg + 16u * c + i;
-        if (row >= rows) return;
-        if (!alone && q == 0) {
-            p.ml[(part * R + in_tile) * 2u] = top[c];
-            p.ml[(part * R + in_tile) * 2u + 1u] = sum[c];
-        }
-        const uint32_t k0 = token_of(p, row), j = row - k0 * p.group;
-        float *const to = alone ? p.a.out + (size_t)(t.row + k0) * p.a.out_stride + (size_t)(head * p.group + j) * HD + 4u * q
-                                : p.acc + (part * R + in_tile) * HD + 4u * q;
-        const float scale = alone ? 1.0f / sum[c] : 1.f;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            f4 v = o[c][dt];
-            if (any_odd) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const bool up = odd[0][16 * dt + 4 * q + e] <= last[c], down = odd[1][16 * dt + 4 * q + e] <= last[c];
-                    v[e] = up ? down ? __builtin_nanf("") : INFINITY : down ? -INFINITY : v[e];
-                }
-            }
-            v = alone && sum[c] < 0.f ? f4{0.f, 0.f, 0.f, 0.f} : v * scale;
-            if (!alone || p.a.ovec) {
-                *reinterpret_cast<f4 *>(to + 16 * dt) = v;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) to[16 * dt + e] = v[e];
-            }
-        }
-    };
-    if (kg & 1u)
-        finish(std::true_type{});
-    else
-        finish(std::false_type{});
-}
-
-// The parts of a tile's row, joined: a workgroup a row, its lanes HD / 4 columns by as many parts at
-// once as fit.
+// The parts of tiles' rows, joined: a workgroup takes every gridDim-th row, its lanes HD / 4 columns by
+// as many parts at once as fit. What a row's parts hold is asked for as soon as it is known
+// where they are. Bound by three loads that need each other.
 template <int HD>
-__global__ __launch_bounds__(256) void k_paged_join(AttnArgs p) {
-    constexpr int V = HD / 4, Y = 256 / V;
+__global__ __launch_bounds__(256) void k_paged_join(AttnArgs p, uint32_t most) {
+    constexpr int V = HD / 4, Y = 256 / V, E = 8;
     __shared__ float sc[kPagedMaxSplits], red[3][4];
     __shared__ __attribute__((aligned(16))) float os[Y][HD];
     const PagedAttn &a = p.a;
-    const uint32_t tid = threadIdx.x, heads = a.b.geom.kv_heads, head = blockIdx.x % heads, tile_rows = a.s.tile_rows;
-    const uint32_t r = blockIdx.x / heads % tile_rows, index = blockIdx.x / heads / tile_rows;
-    uint32_t step_row, base, first, n, row;   // the tile's request's first row, position of that; the parts; the query row
-    if (a.selected) {
-        step_row = index / p.tiles;
-        row = index % p.tiles * tile_rows + r;
-        base = a.plan[a.s.positions + step_row];
-        first = index * p.splits;
-        if (a.plan[a.s.requests + step_row] >= a.b.requests || row >= p.group || base >= a.b.table_width << p.shift) return;
-        const uint32_t pages = min(a.budget, (base >> p.shift) + 1u), chunks = ((pages << p.shift) + 31u) / 32u;
-        n = (chunks + p.per - 1u) / p.per;
-    } else {
-        if (index >= a.plan[6]) return;
-        const PagedJoin j = reinterpret_cast<const PagedJoin *>(a.plan + a.s.join_at)[index];
-        const uint32_t cap = a.b.table_width << p.shift;
-        if (j.row >= a.b.max_rows || j.count > a.b.max_rows - j.row || j.base > cap || j.count > cap - j.base ||
-            j.tile >= j.count * p.group || j.per == 0u || j.part >= p.parts)
-            return;
-        step_row = j.row;
-        base = j.base;
-        row = j.tile + r;
-        first = j.part;
-        if (row >= j.count * p.group) return;
-        const uint32_t last = base + token_of(p, min(j.tile + tile_rows, j.count * p.group) - 1u);
-        n = min((last / 32u + j.per) / j.per, p.parts - first);   // of the tile's chunks
-    }
-    if (n <= 1u || n > kPagedMaxSplits) return;
-    const size_t at = ((size_t)head * p.parts + first) * tile_rows + r;   // the row's record in the first part
-    const uint32_t c = 4u * (tid % V), y = tid / V;
-    constexpr int E = 8;
-    f4 early[E];   // on their way while the parts' weights are worked out
+    const uint32_t tid = threadIdx.x, heads = a.b.geom.kv_heads, tile_rows = a.s.tile_rows, c = 4u * (tid % V), y = tid / V;
+    const uint32_t all = a.selected ? most : min(a.plan[6] * tile_rows * heads, most);
+    for (uint32_t k = blockIdx.x; k < all; k += gridDim.x) {
+        const uint32_t head = k % heads, r = k / heads % tile_rows, index = k / heads / tile_rows;
+        uint32_t step_row, row, first, n;   // the request's first row, its query row; the parts
+        if (a.selected) {
+            step_row = index / p.tiles;
+            row = index % p.tiles * tile_rows + r;
+            first = index * p.splits;
+            const uint32_t base = a.plan[a.s.positions + step_row];
+            if (a.plan[a.s.requests + step_row] >= a.b.requests || base >= a.b.table_width << p.shift || row >= p.group) continue;
+            const uint32_t pages = min(a.budget, (base >> p.shift) + 1u), chunks = ((pages << p.shift) + 31u) / 32u;
+            n = (chunks + p.per - 1u) / p.per;
+        } else {
+            const PagedJoin j = reinterpret_cast<const PagedJoin *>(a.plan + a.s.join_at)[index];
+            const uint32_t cap = a.b.table_width << p.shift, rows = j.count * p.group;
+            if (j.row >= a.b.max_rows || j.count > a.b.max_rows - j.row || j.base > cap || j.count > cap - j.base ||
+                j.tile >= rows || j.tile + r >= rows || j.per == 0u || j.part >= p.parts)
+                continue;
+            step_row = j.row;
+            row = j.tile + r;
+            first = j.part;
+            const uint32_t last = j.base + token_of(p, min(j.tile + tile_rows, rows) - 1u);
+            n = min((last / 32u + j.per) / j.per, p.parts - first);   // of the tile's chunks
+        }
+        if (n <= 1u || n > kPagedMaxSplits) continue;
+        const size_t at = ((size_t)head * p.parts + first) * tile_rows + r;   // the row's record in the first part
+        f4 early[E];
 #pragma unroll
-    for (int k = 0; k < E; ++k)
-        early[k] = *reinterpret_cast<const f4 *>(p.acc + (at + (size_t)min(y + k * Y, n - 1u) * tile_rows) * HD + c);
-    float m = -INFINITY, l = -1.f;
-    if (tid < n) {
-        m = p.ml[(at + (size_t)tid * tile_rows) * 2u];
-        l = p.ml[(at + (size_t)tid * tile_rows) * 2u + 1u];
-    }
-    float top = m, some = l < 0.f ? 0.f : 1.f;
+        for (int e = 0; e < E; ++e)
+            early[e] = *reinterpret_cast<const f4 *>(p.acc + (at + (size_t)min(y + e * Y, n - 1u) * tile_rows) * HD + c);
+        float m = -INFINITY, l = -1.f;
+        if (tid < n) {
+            m = p.ml[(at + (size_t)tid * tile_rows) * 2u];
+            l = p.ml[(at + (size_t)tid * tile_rows) * 2u + 1u];
+        }
+        float top = m, some = l < 0.f ? 0.f : 1.f;
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64)), some = fmaxf(some, __shfl_xor(some, d, 64));
-    if ((tid & 63u) == 0) red[0][tid >> 6] = top, red[1][tid >> 6] = some;
-    __syncthreads();
-    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    some = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
-    const float mine = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
-    if (tid < n) sc[tid] = mine;
-    float sum = l < 0.f ? 0.f : l * mine;
+        for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64)), some = fmaxf(some, __shfl_xor(some, d, 64));
+        if ((tid & 63u) == 0) red[0][tid >> 6] = top, red[1][tid >> 6] = some;
+        __syncthreads();
+        top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+        some = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+        const float mine = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+        if (tid < n) sc[tid] = mine;
+        float sum = l < 0.f ? 0.f : l * mine;
 #pragma unroll
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
-    if ((tid & 63u) == 0) red[2][tid >> 6] = sum;
-    __syncthreads();
-    sum = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
-    f4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+        if ((tid & 63u) == 0) red[2][tid >> 6] = sum;
+        __syncthreads();
+        sum = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+        f4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < E; ++k)
-        if (y + k * Y < n) o += early[k] * sc[y + k * Y];
+        for (int e = 0; e < E; ++e)
+            if (y + e * Y < n) o += early[e] * sc[y + e * Y];
 #pragma unroll 8
-    for (uint32_t v = y + E * Y; v < n; v += Y)
-        o += *reinterpret_cast<const f4 *>(p.acc + (at + (size_t)v * tile_rows) * HD + c) * sc[v];
-    *reinterpret_cast<f4 *>(&os[y][c]) = o;
-    __syncthreads();
-    if (tid < (uint32_t)HD) {
-        float x = os[0][tid];
+        for (uint32_t v = y + E * Y; v < n; v += Y)
+            o += *reinterpret_cast<const f4 *>(p.acc + (at + (size_t)v * tile_rows) * HD + c) * sc[v];
+        *reinterpret_cast<f4 *>(&os[y][c]) = o;
+        __syncthreads();
+        if (tid < (uint32_t)HD) {
+            float x = os[0][tid];
 #pragma unroll
-        for (int u = 1; u < Y; ++u) x += os[u][tid];
-        const uint32_t k = token_of(p, row), j = row - k * p.group;
-        a.out[(size_t)(step_row + k) * a.out_stride + (size_t)(head * p.group + j) * HD + tid] = some == 0.f ? 0.f : x / sum;
+            for (int u = 1; u < Y; ++u) x += os[u][tid];
+            const uint32_t token = token_of(p, row), j = row - token * p.group;
+            a.out[(size_t)(step_row + token) * a.out_stride + (size_t)(head * p.group + j) * HD + tid] = some == 0.f ? 0.f : x / sum;
+        }
+        __syncthreads();
     }
 }
 
@@ -960,14 +639,8 @@ void run(hipStream_t s, const AttnArgs &p, uint64_t grid) {
         k_paged_attn<HD, 1, 4, true><<<g, 256, 0, s>>>(p);
     else if (p.a.s.tile_rows == 16u)
         k_paged_attn<HD, 1, 4, false><<<g, 256, 0, s>>>(p);
-    else if constexpr (HD < 256) {
-        if (p.a.s.tile_rows == 32u)
-            k_paged_attn<HD, 2, 8, false><<<g, 512, 0, s>>>(p);
-        else if (p.a.s.tile_rows == 64u)
-            k_paged_prompt<HD, 4><<<g, 512, 0, s>>>(p);
-        else
-            k_paged_prompt<HD, 2><<<g, 512, 0, s>>>(p);
-    }
+    else if constexpr (HD < 256)
+        k_paged_attn<HD, 2, 8, false><<<g, 512, 0, s>>>(p);
 }
 
 }  // namespace
@@ -1008,12 +681,12 @@ int launch_paged_attention(hipStream_t s, const PagedAttn &a) {
 #undef CALL
     VX_LAUNCHED("k_paged_attn");
     if (a.selected ? p.splits == 1u : a.s.joins == 0u) return VX_OK;   // nothing is divided
-    const uint64_t joins = (a.selected ? (uint64_t)a.b.max_rows * p.tiles : a.s.joins) * p.a.s.tile_rows * g.kv_heads;
-    const dim3 grid((uint32_t)joins);
+    const uint32_t most = (uint32_t)((a.selected ? (uint64_t)a.b.max_rows * p.tiles : a.s.joins) * p.a.s.tile_rows * g.kv_heads);
+    const dim3 grid(std::min(most, 1024u));
     switch (g.head_dim) {
-        case 64: k_paged_join<64><<<grid, 256, 0, s>>>(p); break;
-        case 128: k_paged_join<128><<<grid, 256, 0, s>>>(p); break;
-        default: k_paged_join<256><<<grid, 256, 0, s>>>(p); break;
+        case 64: k_paged_join<64><<<grid, 256, 0, s>>>(p, most); break;
+        case 128: k_paged_join<128><<<grid, 256, 0, s>>>(p, most); break;
+        default: k_paged_join<256><<<grid, 256, 0, s>>>(p, most); break;
     }
     VX_LAUNCHED("k_paged_join");
     return VX_OK;

@@ -13,10 +13,9 @@ PagedShape paged_shape(const vx_paged_batch &b) {
     PagedShape s{};
     const uint32_t group = b.q_heads / b.geom.kv_heads, rows = b.max_count * group;
     s.packed = rows <= 8u;
-    const uint64_t all = (uint64_t)b.max_rows * group * b.geom.kv_heads;   // query rows of the step
-    s.tile_rows = s.packed ? 8u : rows <= 16u || b.geom.head_dim == 256u ? 16u : rows <= 64u ? 32u : all < 128u * 256u ? 64u : 128u;
+    s.tile_rows = s.packed ? 8u : rows <= 16u || b.geom.head_dim == 256u ? 16u : 32u;
     s.waves = s.tile_rows > 16u ? 8u : 4u;
-    s.workgroups = s.tile_rows > 32u ? 8u : 9u;
+    s.workgroups = 9u;
     // Keys that 32 chunks hold are not worth a second launch to join their parts (576 slots: 10.3 us for two
     // launches, 7.1 for one); else a wave has two chunks at least, so that one is fetched while it works.
     s.least = (uint64_t)b.table_width * b.geom.page_size <= 1024u ? 32u : 2u * s.waves;
