@@ -164,7 +164,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     constexpr int LDS = B * R * OROW > QLDS ? B * R * OROW : QLDS;
     constexpr size_t UNIT = 32 * HD;            // bytes
     __shared__ __attribute__((aligned(16))) float lds[LDS];
-    static_assert((!PK || NT == 1) && (W == 4 || (W == 8 && NT > 1)), "one column tile of both terms; a wave or two a SIMD");
+    static_assert((!PK || NT == 1) && (W == 4 || W == 8), "one column tile of both terms; a wave or two a SIMD");
     __shared__ float ms[W][R], ls[W][R], fs[R];
     // by dimension the first position of a +inf or NaN in V, and of a -inf or NaN
     __shared__ uint32_t odd[2][HD], odd_in[W];
@@ -615,7 +615,7 @@ void divide(const vx_paged_batch &b, const PagedShape &s, uint32_t budget, uint3
     const uint64_t chunks = ((uint64_t)std::min(budget, b.table_width) * b.geom.page_size + 31u) / 32u;
     const uint64_t units = (uint64_t)b.max_rows * b.geom.kv_heads * *tiles;
     uint64_t n = std::min<uint64_t>(std::max<uint64_t>((1u << s.workgroups) / units, 1u), kPagedMaxSplits);
-    *per = (uint32_t)std::max<uint64_t>((chunks + n - 1u) / n, s.least);
+    *per = (uint32_t)std::max<uint64_t>((chunks + n - 1u) / n, chunks <= kPagedWhole ? kPagedWhole : 2u * s.waves);
     *splits = (uint32_t)((chunks + *per - 1u) / *per);
 }
 
@@ -639,8 +639,8 @@ void run(hipStream_t s, const AttnArgs &p, uint64_t grid) {
         k_paged_attn<HD, 1, 4, true><<<g, 256, 0, s>>>(p);
     else if (p.a.s.tile_rows == 16u)
         k_paged_attn<HD, 1, 4, false><<<g, 256, 0, s>>>(p);
-    else if constexpr (HD < 256)
-        k_paged_attn<HD, 2, 8, false><<<g, 512, 0, s>>>(p);
+    else
+        k_paged_attn<HD, 2, HD < 256 ? 8 : 4, false><<<g, HD < 256 ? 512 : 256, 0, s>>>(p);
 }
 
 }  // namespace

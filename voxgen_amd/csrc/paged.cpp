@@ -13,12 +13,12 @@ PagedShape paged_shape(const vx_paged_batch &b) {
     PagedShape s{};
     const uint32_t group = b.q_heads / b.geom.kv_heads, rows = b.max_count * group;
     s.packed = rows <= 8u;
-    s.tile_rows = s.packed ? 8u : rows <= 16u || b.geom.head_dim == 256u ? 16u : 32u;
-    s.waves = s.tile_rows > 16u ? 8u : 4u;
-    s.workgroups = 9u;
-    // Keys that 32 chunks hold are not worth a second launch to join their parts (576 slots: 10.3 us for two
-    // launches, 7.1 for one); else a wave has two chunks at least, so that one is fetched while it works.
-    s.least = (uint64_t)b.table_width * b.geom.page_size <= 1024u ? 32u : 2u * s.waves;
+    s.tile_rows = s.packed ? 8u : rows <= 16u ? 16u : 32u;
+    s.waves = s.tile_rows > 16u && b.geom.head_dim < 256u ? 8u : 4u;
+    s.workgroups = s.tile_rows > 16u ? 8u : 9u;
+    // A part has two chunks a wave at least, so that one is fetched while it works; what kPagedWhole chunks
+    // hold is not divided.
+    s.least = (uint64_t)b.table_width * b.geom.page_size <= 32u * kPagedWhole ? kPagedWhole : 2u * s.waves;
     // Tiles: at most one for each request of so few rows, else a request's last may be part of one. Parts
     // of a tile: what its keys divide into, of which in all a KV head's share of the workgroups comes on top.
     const uint32_t requests = std::min(b.requests, b.max_rows);
