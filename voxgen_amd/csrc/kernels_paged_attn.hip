@@ -112,6 +112,13 @@ struct QRow {
     }
 };
 
+// Eight values; ONCE: not kept in the caches behind them.
+template <bool ONCE>
+__device__ __forceinline__ h8 load_once(const uint8_t *from) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const h8 *>(from));
+    return *reinterpret_cast<const h8 *>(from);
+}
+
 // A lane's share of a chunk of K: for both of the product's row tiles tt, slot 8 (i / 4) + 4 tt +
 // i % 4. Lane (i, q) of the product S^T then holds the scores of query row i and slots 8 q + 4 tt + r:
 // eight consecutive ones.
@@ -119,12 +126,13 @@ template <int HD>
 struct KFrag {
     static constexpr int U = HD / 32;
     h8 x[2][U];
+    template <bool ONCE>
     __device__ __forceinline__ void load(const uint8_t *unit, uint32_t i, uint32_t q) {
         const uint8_t *const at = unit + (8u * (i / 4u % 2u) + i % 4u) * 16u + q * 256u;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-            for (int u = 0; u < U; ++u) x[tt][u] = *reinterpret_cast<const h8 *>(at + tt * 64 + u * 1024);
+            for (int u = 0; u < U; ++u) x[tt][u] = load_once<ONCE>(at + tt * 64 + u * 1024);
     }
 };
 // Of V^T: octet q of the chunk's slots, dimensions 16 dt + i.
@@ -132,10 +140,11 @@ template <int HD>
 struct VFrag {
     static constexpr int DT = HD / 16;
     h8 x[DT];
+    template <bool ONCE>
     __device__ __forceinline__ void load(const uint8_t *unit, uint32_t i, uint32_t q) {
         const uint8_t *const at = unit + (q % 2u) * (HD * 16u) + i * 16u;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) x[dt] = *reinterpret_cast<const h8 *>(at + dt * 256);
+        for (int dt = 0; dt < DT; ++dt) x[dt] = load_once<ONCE>(at + dt * 256);
     }
 };
 
@@ -157,7 +166,7 @@ __device__ __forceinline__ bool finite(_Float16 x) {
 // PK, of at most eight rows: columns 0..7 of the products take the high terms of the rows,
 // columns 8..15 the low ones, so that one product does for both; the scores of the two
 // columns of a row are added, and so are its sums at the end.
-template <int HD, int NT, int W, bool PK>
+template <int HD, int NT, int W, bool PK, bool ONCE>
 __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_attn(AttnArgs p) {
     constexpr int U = HD / 32, DT = HD / 16, OROW = HD + 4, R = 16 * NT, RT = PK ? 8 : R, B = W > 4 ? W / 2 : W;
     constexpr int QLDS = NT > 1 ? R * HD : 0;   // floats: two f16 planes
@@ -213,8 +222,8 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     // K and V of a chunk are fetched when the one ahead is done with them, where registers allow.
     constexpr bool AHEAD = NT == 1;
     if (AHEAD && mine) {
-        kf.load(kc + unit_of(0, i >= 8u), i, q);
-        vf.load(vc + unit_of(0, q >= 2u), i, q);
+        kf.template load<ONCE>(kc + unit_of(0, i >= 8u), i, q);
+        vf.template load<ONCE>(vc + unit_of(0, q >= 2u), i, q);
     }
 
     for (uint32_t d = tid; d < 2u * HD; d += 64u * W) odd[d / HD][d % HD] = ~0u;
@@ -269,7 +278,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     bool whole = false;   // some chunk was none at an edge
     auto step = [&](uint32_t j, uint32_t w0, uint32_t w1, bool edge) {
         const uint8_t *const vu = vc + unit_of(j, q >= 2u);
-        if constexpr (!AHEAD) kf.load(kc + unit_of(j, i >= 8u), i, q);
+        if constexpr (!AHEAD) kf.template load<ONCE>(kc + unit_of(j, i >= 8u), i, q);
         // Behind the last chunk it is fetched once more, without a branch: with one between the products
         // and what reads them, this compiler lost count of the wait that that needs.
         const uint32_t next = min(j + 1u, mine - 1u);
@@ -293,9 +302,9 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
             }
         }
         if constexpr (AHEAD)
-            kf.load(ku, i, q);
+            kf.template load<ONCE>(ku, i, q);
         else
-            vf.load(vu, i, q);
+            vf.template load<ONCE>(vu, i, q);
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (PK) {
 #pragma unroll
@@ -374,7 +383,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
                 for (int c = 0; c < NT; ++c) o[c][dt] = mfma16(vf.x[dt], pl[c], o[c][dt]);
             }
         }
-        if constexpr (AHEAD) vf.load(vnext, i, q);
+        if constexpr (AHEAD) vf.template load<ONCE>(vnext, i, q);
     };
     for (uint32_t j = 0; j < mine; ++j) {
         const uint32_t w0 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u), w1 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u + 1u);
@@ -635,12 +644,22 @@ uint64_t parts_of(const vx_paged_batch &b, const PagedShape &s, uint32_t budget)
 template <int HD>
 void run(hipStream_t s, const AttnArgs &p, uint64_t grid) {
     const dim3 g((uint32_t)grid);
-    if (p.a.s.packed)
-        k_paged_attn<HD, 1, 4, true><<<g, 256, 0, s>>>(p);
+    // K and V of a layer that the last-level cache (256 MB) cannot hold until the next step are read past
+    // the caches, where each is read once (64 requests over up to 24000, 1.06 GB: 194 us, so 182; but 16
+    // over 8000, 86 MB, which lie there still when they are read again: 16.6, so 18.5).
+    const vx_paged_geom &m = p.a.b.geom;
+    const bool once = !p.a.selected && p.a.b.max_count * p.group <= p.a.s.tile_rows &&
+                      (uint64_t)m.pages * m.page_size * m.kv_heads * m.head_dim * 4u > 256u << 20;
+    if (p.a.s.packed && once)
+        k_paged_attn<HD, 1, 4, true, true><<<g, 256, 0, s>>>(p);
+    else if (p.a.s.packed)
+        k_paged_attn<HD, 1, 4, true, false><<<g, 256, 0, s>>>(p);
+    else if (p.a.s.tile_rows == 16u && once)
+        k_paged_attn<HD, 1, 4, false, true><<<g, 256, 0, s>>>(p);
     else if (p.a.s.tile_rows == 16u)
-        k_paged_attn<HD, 1, 4, false><<<g, 256, 0, s>>>(p);
+        k_paged_attn<HD, 1, 4, false, false><<<g, 256, 0, s>>>(p);
     else
-        k_paged_attn<HD, 2, HD < 256 ? 8 : 4, false><<<g, HD < 256 ? 512 : 256, 0, s>>>(p);
+        k_paged_attn<HD, 2, HD < 256 ? 8 : 4, false, false><<<g, HD < 256 ? 512 : 256, 0, s>>>(p);
 }
 
 }  // namespace

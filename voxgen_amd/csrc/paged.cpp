@@ -15,7 +15,7 @@ PagedShape paged_shape(const vx_paged_batch &b) {
     s.packed = rows <= 8u;
     s.tile_rows = s.packed ? 8u : rows <= 16u ? 16u : 32u;
     s.waves = s.tile_rows > 16u && b.geom.head_dim < 256u ? 8u : 4u;
-    s.workgroups = s.tile_rows > 16u ? 8u : 9u;
+    s.workgroups = s.tile_rows > 16u ? 8u : 10u;
     // A part has two chunks a wave at least, so that one is fetched while it works; what kPagedWhole chunks
     // hold is not divided.
     s.least = (uint64_t)b.table_width * b.geom.page_size <= 32u * kPagedWhole ? kPagedWhole : 2u * s.waves;
