@@ -221,6 +221,15 @@ __global__ __launch_bounds__(T) void k_paged_plan(PagedPlan a) {
                               many > by ? begin(part_end, i) + tile * s + split : VX_PAGED_NONE};
         reinterpret_cast<PagedItem *>(a.plan + a.s.item_at)[g] = it;
     }
+    if (a.s.tile_rows <= 16u) {   // a tile is few rows: the pages of its part's first units
+        for (uint32_t g = g0; g < all_items * kPagedListed; g += step) {
+            const uint32_t item = g / kPagedListed, i = owner_of(item_end, n, item), length = length_of[i], cnt = count_of[i];
+            uint32_t s;
+            const uint32_t by = divided((length + cnt + 31u) / 32u, s);
+            const uint32_t at = (item - begin(item_end, i)) % s * by * 32u + g % kPagedListed * kPagedUnit;
+            a.plan[a.s.page_at + g] = at < length + cnt ? page_of(i, length, at) : VX_PAGED_NONE;
+        }
+    }
     for (uint32_t g = g0; g < all_joins; g += step) {
         const uint32_t i = owner_of(join_end, n, g), length = length_of[i], cnt = count_of[i], tile = g - begin(join_end, i);
         uint32_t s;
@@ -627,7 +636,7 @@ int launch_paged_reset(hipStream_t s, const vx_paged_batch &b, uint32_t *lengths
 
 int launch_paged_plan(hipStream_t s, const PagedPlan &a) {
     // one workgroup for so many rows, items or requests as it has threads; 64 for more
-    const uint32_t most = std::max(std::max(a.b.max_rows, a.b.requests), a.s.items);
+    const uint32_t most = std::max(std::max(a.b.max_rows, a.b.requests), a.s.items * (a.s.tile_rows <= 16u ? kPagedListed : 1u));
     auto blocks = [&](uint32_t threads) { return std::min((most + threads - 1u) / threads, 64u); };
     if (a.b.requests <= 256u)
         k_paged_plan<256, 1><<<blocks(256), 256, 0, s>>>(a);

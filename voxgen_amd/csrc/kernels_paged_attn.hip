@@ -19,15 +19,28 @@ namespace {
 
 constexpr uint32_t kFar = 1u << 30;   // the position of a unit that holds no slots: above every row's
 
+// Flat and with what a workgroup asks for first in front: its arguments are memory too, line by line.
 struct AttnArgs {
-    PagedAttn a;
+    const PagedItem *items;          // of the plan
+    const uint32_t *lists;           // of the plan: pages of items; of a selection: [row][KV head][budget] pages
+    const uint32_t *header;          // of the plan
+    const uint32_t *tables;
+    const float *q;
+    uint32_t budget, shift;          // log2 of the page size
+    uint32_t table_width, requests, max_rows, pages;
     uint32_t group, by_group;        // query heads a KV head; 2^32 / group, rounded up (0 where group is 1)
-    uint32_t shift, units;           // log2 of the page size, units of a page
-    size_t layer_at;                 // bytes of the layers before
-    uint32_t tiles, splits, per;     // of a selection: tiles of a row, splits of its list, chunks of one
-    float *ml, *acc;                 // [KV head][part][tile rows][2], [..][tile rows][HD]
+    uint32_t q_stride, out_stride;
+    uint32_t tile_rows, tiles, by_tiles, splits, per;   // tiles of a row, splits of its list, chunks of one (of a selection)
     uint32_t parts;                  // of one KV head
+    const uint8_t *kc, *vc;          // of the layer
+    float *out;
+    float *ml, *acc;                 // [KV head][part][tile rows][2], [..][tile rows][HD]
+    const uint32_t *row_requests, *row_positions;       // of the plan
+    const PagedJoin *joins;          // of the plan
 };
+
+// What a kernel attends to: all pages; all, each read once; those of a selection.
+enum Mode { kDense, kOnce, kSelected };
 
 // The token of a row. The product with 2^32 / group rounded up is exact for rows below 2^22
 // and groups up to 2^10: it is over by less than 2^22 2^10 / 2^32 / group.
@@ -41,29 +54,28 @@ struct Tile {
     uint32_t request, row, base, count, tile, first, n, part;
     bool ok;
 };
-__device__ __forceinline__ Tile tile_of(const AttnArgs &p, uint32_t index) {
-    const PagedAttn &a = p.a;
+template <Mode MODE>
+__device__ __forceinline__ Tile tile_of(const AttnArgs &p) {
     Tile t;
-    if (a.selected) {
-        const uint32_t split = index % p.splits, rest = index / p.splits;
-        t.row = rest / p.tiles;
-        t.tile = rest % p.tiles * a.s.tile_rows;
-        t.request = a.plan[a.s.requests + t.row];
-        t.base = a.plan[a.s.positions + t.row];
+    const uint32_t index = blockIdx.x, cap = p.table_width << p.shift;
+    if constexpr (MODE == kSelected) {
+        t.row = p.by_tiles ? __umulhi(index, p.by_tiles) : index;   // exact: an index is below 2^22, tiles at most 2^10
+        t.tile = (index - t.row * p.tiles) * p.tile_rows;
+        t.request = p.row_requests[t.row];
+        t.base = p.row_positions[t.row];
         t.count = 1;
-        t.ok = t.request < a.b.requests && t.base < a.b.table_width << p.shift;
-        const uint32_t pages = min(a.budget, (t.base >> p.shift) + 1u), chunks = ((pages << p.shift) + 31u) / 32u;
-        t.first = split * p.per;
+        t.ok = t.request < p.requests && t.base < cap;
+        const uint32_t chunks = ((min(p.budget, (t.base >> p.shift) + 1u) << p.shift) + 31u) / 32u;
+        t.first = blockIdx.z * p.per;
         t.n = t.first < chunks ? min(p.per, chunks - t.first) : 0u;
-        t.part = chunks > p.per ? index : VX_PAGED_NONE;
-        return t;
+        t.part = chunks > p.per ? index * p.splits + blockIdx.z : VX_PAGED_NONE;
+    } else {
+        const PagedItem it = p.items[index];
+        t = {it.request, it.row, it.base, it.count, it.tile, it.first, it.n, it.part, false};
+        t.ok = index < p.header[5] && it.request < p.requests && it.row < p.max_rows && it.count <= p.max_rows - it.row &&
+               it.base <= cap && it.count <= cap - it.base && it.tile < it.count * p.group &&
+               (it.part < p.parts || it.part == VX_PAGED_NONE) && it.first <= cap && it.n <= cap;
     }
-    const PagedItem it = reinterpret_cast<const PagedItem *>(a.plan + a.s.item_at)[index];
-    t = {it.request, it.row, it.base, it.count, it.tile, it.first, it.n, it.part, false};
-    const uint32_t cap = a.b.table_width << p.shift;
-    t.ok = index < a.plan[5] && it.request < a.b.requests && it.row < a.b.max_rows && it.count <= a.b.max_rows - it.row &&
-           it.base <= cap && it.count <= cap - it.base && it.tile < it.count * p.group &&
-           (it.part < p.parts || it.part == VX_PAGED_NONE) && it.first <= cap && it.n <= cap;
     return t;
 }
 
@@ -84,18 +96,13 @@ template <int HD>
 struct QRow {
     static constexpr int U = HD / 32;
     float x[U][8];
-    __device__ __forceinline__ void load(const AttnArgs &p, const Tile &t, uint32_t head, uint32_t row, bool valid, uint32_t q) {
+    // Rows lie at any multiple of four bytes, which loads of sixteen take: a branch for those at sixteen would
+    // make what is loaded wait at its end.
+    __device__ __forceinline__ void load(const AttnArgs &p, const Tile &t, uint32_t head, uint32_t row, uint32_t q) {
         const uint32_t k = token_of(p, row), j = row - k * p.group;
-        const float *src = p.a.q + (size_t)(t.row + k) * p.a.q_stride + (size_t)(head * p.group + j) * HD + q * 8u;
+        const float *src = p.q + (size_t)(t.row + k) * p.q_stride + (size_t)(head * p.group + j) * HD + q * 8u;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (valid) {
-                load8(src + 32 * u, p.a.qvec, x[u]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
-            }
-        }
+        for (int u = 0; u < U; ++u) __builtin_memcpy(x[u], src + 32 * u, 32);
     }
     __device__ __forceinline__ float split(h8 *qh, h8 *ql) const {
         float top = 0.f;
@@ -166,7 +173,7 @@ __device__ __forceinline__ bool finite(_Float16 x) {
 // PK, of at most eight rows: columns 0..7 of the products take the high terms of the rows,
 // columns 8..15 the low ones, so that one product does for both; the scores of the two
 // columns of a row are added, and so are its sums at the end.
-template <int HD, int NT, int W, bool PK, bool ONCE>
+template <int HD, int NT, int W, bool PK, Mode MODE>
 __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_attn(AttnArgs p) {
     constexpr int U = HD / 32, DT = HD / 16, OROW = HD + 4, R = 16 * NT, RT = PK ? 8 : R, B = W > 4 ? W / 2 : W;
     constexpr int QLDS = NT > 1 ? R * HD : 0;   // floats: two f16 planes
@@ -179,49 +186,71 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     __shared__ uint32_t odd[2][HD], odd_in[W];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
     const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t heads = p.a.b.geom.kv_heads, head = blockIdx.x % heads;
-    const Tile t = uniform(tile_of(p, blockIdx.x / heads));
+    const uint32_t heads = gridDim.y, head = blockIdx.y;
+    // What the first chunks' pages are is asked for together with what the tile is: the plan's list of the
+    // item's pages, or the row's list of a selection.
+    constexpr bool ONCE = MODE == kOnce;
+    uint32_t early = VX_PAGED_NONE;
+    if constexpr (NT == 1) {
+        const uint32_t k = 2u * (w + W * (lane / 2u)) + (lane & 1u);   // unit of the part
+        if constexpr (MODE == kSelected) {
+            const uint32_t entry = (blockIdx.z * p.per * 32u + kPagedUnit * k) >> p.shift;
+            const uint32_t row = p.by_tiles ? __umulhi(blockIdx.x, p.by_tiles) : blockIdx.x;
+            early = p.lists[((size_t)row * heads + head) * p.budget + min(entry, p.budget - 1u)];
+        } else {
+            early = p.lists[(size_t)blockIdx.x * kPagedListed + min(k, kPagedListed - 1u)];
+        }
+    }
+    const Tile t = uniform(tile_of<MODE>(p));
     if (!t.ok || t.n == 0) return;
     const uint32_t rows = t.count * p.group, r0 = t.tile, ri = PK ? i & 7u : i;
     const uint32_t sees_all = t.base + token_of(p, r0);                               // last position that every row attends to
     const uint32_t last_pos = t.base + token_of(p, min(r0 + RT, rows) - 1u);          // and that some row does
-    const uint8_t *const kc = p.a.kc + p.layer_at, *const vc = p.a.vc + p.layer_at;
+    const uint8_t *const kc = p.kc, *const vc = p.vc;
 
-    // The wave's chunks t.first + w + W j: lane 2 j + h holds unit h of the j-th, 32 chunks at once.
-    uint32_t unit = 0, where = kFar;
-    auto look_up = [&](uint32_t j0) {
+    // The wave's chunks t.first + w + W j: lane 2 (j - start) + h holds unit h of the j-th, up to 32 chunks
+    // at once, in the first place as many as `early` has.
+    uint32_t unit = 0, where = kFar, start = 0;
+    uint32_t stop = NT > 1 || MODE == kSelected ? 32u : kPagedListed / 2u / W;
+    const uint32_t mask = (1u << p.shift) - 1u, units = (mask + 1u) / kPagedUnit;
+    auto look_up = [&](uint32_t j0, auto is_early) {
+        constexpr bool first = decltype(is_early)::value;
         const uint32_t c = w + W * (j0 + lane / 2u), at = (t.first + c) * 32u + kPagedUnit * (lane & 1u);
-        unit = 0;
-        where = kFar;
-        if (c >= t.n) return;
         uint32_t index = at >> p.shift;
-        if (p.a.selected) {
-            index = index < min(p.a.budget, (t.base >> p.shift) + 1u)
-                        ? p.a.selected[((size_t)t.row * heads + head) * p.a.budget + index] : VX_PAGED_NONE;
-            if (index > t.base >> p.shift) return;
+        bool there = c < t.n;
+        if constexpr (MODE == kSelected) {
+            there = there && index < min(p.budget, (t.base >> p.shift) + 1u);
+            if constexpr (first)
+                index = early;
+            else
+                index = there ? p.lists[((size_t)t.row * heads + head) * p.budget + index] : 0u;
+            there = there && index <= t.base >> p.shift;
         }
-        if (index >= p.a.b.table_width) return;
-        const uint32_t off = at & (p.a.b.geom.page_size - 1u), pos = (index << p.shift) + off;
-        if (pos > last_pos) return;
-        const uint32_t page = p.a.tables[(size_t)t.request * p.a.b.table_width + index];
-        if (page >= p.a.b.geom.pages) return;
-        unit = (page * heads + head) * p.units + off / kPagedUnit;
-        where = pos;
+        there = there && index < p.table_width;
+        const uint32_t off = at & mask, pos = (index << p.shift) + off;
+        there = there && pos <= last_pos;
+        uint32_t page = early;
+        if constexpr (MODE == kSelected || !first)
+            page = p.tables[(size_t)t.request * p.table_width + (there ? index : 0u)];
+        there = there && page < p.pages;
+        unit = there ? (page * heads + head) * units + off / kPagedUnit : 0u;
+        where = there ? pos : kFar;
     };
     auto unit_of = [&](uint32_t j, bool second) {   // bytes
-        const uint32_t u0 = __builtin_amdgcn_readlane(unit, (j & 31u) * 2u), u1 = __builtin_amdgcn_readlane(unit, (j & 31u) * 2u + 1u);
+        const uint32_t at = (j - start) * 2u, u0 = __builtin_amdgcn_readlane(unit, at), u1 = __builtin_amdgcn_readlane(unit, at + 1u);
         return (size_t)(second ? u1 : u0) * UNIT;
     };
+    auto where_is = [&](uint32_t j, uint32_t h) { return (uint32_t)__builtin_amdgcn_readlane(where, (j - start) * 2u + h); };
     // Loads come back in order: the queries first, which are worked on while the first chunk is on its way.
     QRow<HD> qr;
-    if constexpr (NT == 1) qr.load(p, t, head, min(r0 + ri, rows - 1u), r0 + ri < rows, q);
-    look_up(0);
+    if constexpr (NT == 1) qr.load(p, t, head, min(r0 + ri, rows - 1u), q);   // rows behind the last are it once more
+    look_up(0, std::bool_constant<NT == 1>{});
     const uint32_t mine = t.n > w ? (t.n - w + W - 1u) / W : 0u;   // the wave's chunks
     KFrag<HD> kf;
     VFrag<HD> vf;
     // K and V of a chunk are fetched when the one ahead is done with them, where registers allow.
     constexpr bool AHEAD = NT == 1;
-    if (AHEAD && mine) {
+    if constexpr (AHEAD) {   // a wave without chunks fetches unit 0: a branch here would have the queries wait for what is in it
         kf.template load<ONCE>(kc + unit_of(0, i >= 8u), i, q);
         vf.template load<ONCE>(vc + unit_of(0, q >= 2u), i, q);
     }
@@ -240,7 +269,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     } else {
         for (uint32_t c = w; c < NT; c += W) {
             const uint32_t row = r0 + 16u * c + i;
-            qr.load(p, t, head, min(row, rows - 1u), row < rows, q);
+            qr.load(p, t, head, min(row, rows - 1u), q);
             const float f = qr.split(qh, ql);
             if (q == 0) fs[16u * c + i] = f;
 #pragma unroll
@@ -282,7 +311,11 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
         // Behind the last chunk it is fetched once more, without a branch: with one between the products
         // and what reads them, this compiler lost count of the wait that that needs.
         const uint32_t next = min(j + 1u, mine - 1u);
-        if ((next & 31u) == 0 && next != j) look_up(next);
+        if (next == stop && next != j) {
+            look_up(next, std::false_type{});
+            start = next;
+            stop = next + 32u;
+        }
         const uint8_t *const ku = kc + unit_of(next, i >= 8u), *const vnext = vc + unit_of(next, q >= 2u);
         f4 x[NT][2];
 #pragma unroll
@@ -386,7 +419,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
         if constexpr (AHEAD) vf.template load<ONCE>(vnext, i, q);
     };
     for (uint32_t j = 0; j < mine; ++j) {
-        const uint32_t w0 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u), w1 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u + 1u);
+        const uint32_t w0 = where_is(j, 0), w1 = where_is(j, 1);
         step(j, w0, w1, max(w0, w1) + kPagedUnit - 1u > sees_all);
     }
 #pragma unroll
@@ -412,8 +445,11 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     for (int v = 0; v < W; ++v) any_odd = any_odd || odd_in[v] != 0;
     if (__builtin_expect(any_odd, 0)) {
         for (uint32_t j = 0; j < mine; ++j) {
-            if ((j & 31u) == 0) look_up(j);
-            const uint32_t w0 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u), w1 = __builtin_amdgcn_readlane(where, (j & 31u) * 2u + 1u);
+            if ((j & 31u) == 0) {
+                look_up(j, std::false_type{});
+                start = j;
+            }
+            const uint32_t w0 = where_is(j, 0), w1 = where_is(j, 1);
             const uint32_t slot0 = (q < 2u ? w0 : w1) + 8u * (q % 2u);
             const uint8_t *const at = vc + unit_of(j, q >= 2u) + (q % 2u) * (HD * 16u) + i * 16u;
 #pragma unroll 1
@@ -526,42 +562,36 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
             continue;
         }
         v = fs[r] < 0.f ? f4{0.f, 0.f, 0.f, 0.f} : v * (1.0f / fs[r]);   // attends to nothing: 0
-        float *const to = p.a.out + (size_t)(t.row + k0) * p.a.out_stride + (size_t)(head * p.group + j) * HD + c;
-        if (p.a.ovec) {
-            *reinterpret_cast<f4 *>(to) = v;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) to[e] = v[e];
-        }
+        float *const to = p.out + (size_t)(t.row + k0) * p.out_stride + (size_t)(head * p.group + j) * HD + c;
+        __builtin_memcpy(to, &v, 16);   // at any multiple of four bytes
     }
 }
 
 // The parts of tiles' rows, joined: a workgroup takes every gridDim-th row, its lanes HD / 4 columns by
 // as many parts at once as fit. What a row's parts hold is asked for as soon as it is known
 // where they are. Bound by three loads that need each other.
-template <int HD>
-__global__ __launch_bounds__(256) void k_paged_join(AttnArgs p, uint32_t most) {
+template <int HD, bool SELECTED>
+__global__ __launch_bounds__(256) void k_paged_join(AttnArgs p, uint32_t most, uint32_t heads) {
     constexpr int V = HD / 4, Y = 256 / V, E = 8;
     __shared__ float sc[kPagedMaxSplits], red[3][4];
     __shared__ __attribute__((aligned(16))) float os[Y][HD];
-    const PagedAttn &a = p.a;
-    const uint32_t tid = threadIdx.x, heads = a.b.geom.kv_heads, tile_rows = a.s.tile_rows, c = 4u * (tid % V), y = tid / V;
-    const uint32_t all = a.selected ? most : min(a.plan[6] * tile_rows * heads, most);
+    const uint32_t tid = threadIdx.x, tile_rows = p.tile_rows, c = 4u * (tid % V), y = tid / V;
+    const uint32_t all = SELECTED ? most : min(p.header[6] * tile_rows * heads, most), cap = p.table_width << p.shift;
     for (uint32_t k = blockIdx.x; k < all; k += gridDim.x) {
         const uint32_t head = k % heads, r = k / heads % tile_rows, index = k / heads / tile_rows;
         uint32_t step_row, row, first, n;   // the request's first row, its query row; the parts
-        if (a.selected) {
+        if constexpr (SELECTED) {
             step_row = index / p.tiles;
             row = index % p.tiles * tile_rows + r;
             first = index * p.splits;
-            const uint32_t base = a.plan[a.s.positions + step_row];
-            if (a.plan[a.s.requests + step_row] >= a.b.requests || base >= a.b.table_width << p.shift || row >= p.group) continue;
-            const uint32_t pages = min(a.budget, (base >> p.shift) + 1u), chunks = ((pages << p.shift) + 31u) / 32u;
+            const uint32_t base = p.row_positions[step_row];
+            if (p.row_requests[step_row] >= p.requests || base >= cap || row >= p.group) continue;
+            const uint32_t chunks = ((min(p.budget, (base >> p.shift) + 1u) << p.shift) + 31u) / 32u;
             n = (chunks + p.per - 1u) / p.per;
         } else {
-            const PagedJoin j = reinterpret_cast<const PagedJoin *>(a.plan + a.s.join_at)[index];
-            const uint32_t cap = a.b.table_width << p.shift, rows = j.count * p.group;
-            if (j.row >= a.b.max_rows || j.count > a.b.max_rows - j.row || j.base > cap || j.count > cap - j.base ||
+            const PagedJoin j = p.joins[index];
+            const uint32_t rows = j.count * p.group;
+            if (j.row >= p.max_rows || j.count > p.max_rows - j.row || j.base > cap || j.count > cap - j.base ||
                 j.tile >= rows || j.tile + r >= rows || j.per == 0u || j.part >= p.parts)
                 continue;
             step_row = j.row;
@@ -610,7 +640,7 @@ __global__ __launch_bounds__(256) void k_paged_join(AttnArgs p, uint32_t most) {
 #pragma unroll
             for (int u = 1; u < Y; ++u) x += os[u][tid];
             const uint32_t token = token_of(p, row), j = row - token * p.group;
-            a.out[(size_t)(step_row + token) * a.out_stride + (size_t)(head * p.group + j) * HD + tid] = some == 0.f ? 0.f : x / sum;
+            p.out[(size_t)(step_row + token) * p.out_stride + (size_t)(head * p.group + j) * HD + tid] = some == 0.f ? 0.f : x / sum;
         }
         __syncthreads();
     }
@@ -628,10 +658,12 @@ void divide(const vx_paged_batch &b, const PagedShape &s, uint32_t budget, uint3
     *splits = (uint32_t)((chunks + *per - 1u) / *per);
 }
 
-// A selection is each row's own: its tiles are a row's query heads.
-vx_paged_batch of_rows(vx_paged_batch b, uint32_t budget) {
+// A selection is each row's own: its tiles are of a row's query heads, 16 at most.
+PagedShape shape_of(vx_paged_batch b, uint32_t budget) {
     if (budget) b.max_count = 1;
-    return b;
+    PagedShape s = paged_shape(b);
+    if (budget && s.tile_rows > 16u) s.tile_rows = 16u, s.waves = 4u, s.workgroups = 10u;
+    return s;
 }
 
 uint64_t parts_of(const vx_paged_batch &b, const PagedShape &s, uint32_t budget) {
@@ -642,70 +674,93 @@ uint64_t parts_of(const vx_paged_batch &b, const PagedShape &s, uint32_t budget)
 }
 
 template <int HD>
-void run(hipStream_t s, const AttnArgs &p, uint64_t grid) {
-    const dim3 g((uint32_t)grid);
+void run(hipStream_t s, const AttnArgs &p, const PagedAttn &a, bool packed, dim3 g) {
     // K and V of a layer that the last-level cache (256 MB) cannot hold until the next step are read past
     // the caches, where each is read once (64 requests over up to 24000, 1.06 GB: 194 us, so 182; but 16
     // over 8000, 86 MB, which lie there still when they are read again: 16.6, so 18.5).
-    const vx_paged_geom &m = p.a.b.geom;
-    const bool once = !p.a.selected && p.a.b.max_count * p.group <= p.a.s.tile_rows &&
+    const vx_paged_geom &m = a.b.geom;
+    const bool once = a.b.max_count * p.group <= p.tile_rows &&
                       (uint64_t)m.pages * m.page_size * m.kv_heads * m.head_dim * 4u > 256u << 20;
-    if (p.a.s.packed && once)
-        k_paged_attn<HD, 1, 4, true, true><<<g, 256, 0, s>>>(p);
-    else if (p.a.s.packed)
-        k_paged_attn<HD, 1, 4, true, false><<<g, 256, 0, s>>>(p);
-    else if (p.a.s.tile_rows == 16u && once)
-        k_paged_attn<HD, 1, 4, false, true><<<g, 256, 0, s>>>(p);
-    else if (p.a.s.tile_rows == 16u)
-        k_paged_attn<HD, 1, 4, false, false><<<g, 256, 0, s>>>(p);
+    constexpr int WIDE = HD < 256 ? 8 : 4;
+    if (a.selected && packed)
+        k_paged_attn<HD, 1, 4, true, kSelected><<<g, 256, 0, s>>>(p);
+    else if (a.selected)
+        k_paged_attn<HD, 1, 4, false, kSelected><<<g, 256, 0, s>>>(p);
+    else if (packed && once)
+        k_paged_attn<HD, 1, 4, true, kOnce><<<g, 256, 0, s>>>(p);
+    else if (packed)
+        k_paged_attn<HD, 1, 4, true, kDense><<<g, 256, 0, s>>>(p);
+    else if (p.tile_rows == 16u && once)
+        k_paged_attn<HD, 1, 4, false, kOnce><<<g, 256, 0, s>>>(p);
+    else if (p.tile_rows == 16u)
+        k_paged_attn<HD, 1, 4, false, kDense><<<g, 256, 0, s>>>(p);
     else
-        k_paged_attn<HD, 2, HD < 256 ? 8 : 4, false, false><<<g, HD < 256 ? 512 : 256, 0, s>>>(p);
+        k_paged_attn<HD, 2, WIDE, false, kDense><<<g, 64 * WIDE, 0, s>>>(p);
+}
+
+template <int HD>
+void join(hipStream_t s, const AttnArgs &p, const PagedAttn &a) {
+    const uint32_t heads = a.b.geom.kv_heads;
+    const uint32_t most = (uint32_t)((a.selected ? (uint64_t)a.b.max_rows * p.tiles : a.s.joins) * p.tile_rows * heads);
+    const dim3 grid(std::min(most, 1024u));
+    if (a.selected)
+        k_paged_join<HD, true><<<grid, 256, 0, s>>>(p, most, heads);
+    else
+        k_paged_join<HD, false><<<grid, 256, 0, s>>>(p, most, heads);
 }
 
 }  // namespace
 
-uint64_t paged_attn_scratch_bytes(const vx_paged_batch &batch, uint32_t budget) {
-    const vx_paged_batch b = of_rows(batch, budget);
-    const PagedShape s = paged_shape(b);
+uint64_t paged_attn_scratch_bytes(const vx_paged_batch &b, uint32_t budget) {
+    const PagedShape s = shape_of(b, budget);
     return parts_of(b, s, budget) * b.geom.kv_heads * s.tile_rows * (b.geom.head_dim + 2u) * 4u;
 }
 
 int launch_paged_attention(hipStream_t s, const PagedAttn &a) {
     AttnArgs p{};
-    p.a = a;
-    const vx_paged_batch rows = of_rows(a.b, a.budget);
     const vx_paged_geom &g = a.b.geom;
-    if (a.selected) {   // the plan stays where it is
-        const PagedShape own = paged_shape(rows);
-        p.a.s.tile_rows = own.tile_rows;
-        p.a.s.packed = own.packed;
-        divide(rows, own, a.budget, &p.tiles, &p.splits, &p.per);
-    }
-    p.group = a.b.q_heads / g.kv_heads;
-    p.by_group = p.group > 1u ? (uint32_t)(((1ull << 32) + p.group - 1u) / p.group) : 0u;
+    const PagedShape shape = shape_of(a.b, a.budget);   // what lies where in the plan is in a.s
+    if (a.selected) divide(a.b, shape, a.budget, &p.tiles, &p.splits, &p.per);
+    p.items = reinterpret_cast<const PagedItem *>(a.plan + a.s.item_at);
+    p.lists = a.selected ? a.selected : a.plan + a.s.page_at;
+    p.header = a.plan;
+    p.tables = a.tables;
+    p.q = a.q;
+    p.budget = a.budget;
     p.shift = paged_shift(g.page_size);
-    p.units = g.page_size / kPagedUnit;
-    p.layer_at = (size_t)a.layer * g.pages * g.kv_heads * g.page_size * g.head_dim * 2u;
-    p.parts = (uint32_t)parts_of(rows, a.selected ? paged_shape(rows) : a.s, a.budget);
-    const uint64_t records = (uint64_t)p.parts * g.kv_heads * p.a.s.tile_rows;
+    p.table_width = a.b.table_width;
+    p.requests = a.b.requests;
+    p.max_rows = a.b.max_rows;
+    p.pages = g.pages;
+    auto inverse = [](uint32_t n) { return n > 1u ? (uint32_t)(((1ull << 32) + n - 1u) / n) : 0u; };
+    p.group = a.b.q_heads / g.kv_heads;
+    p.by_group = inverse(p.group);
+    p.by_tiles = inverse(p.tiles);
+    p.q_stride = a.q_stride;
+    p.out_stride = a.out_stride;
+    p.tile_rows = shape.tile_rows;
+    p.parts = (uint32_t)parts_of(a.b, shape, a.budget);
+    const size_t layer_at = (size_t)a.layer * g.pages * g.kv_heads * g.page_size * g.head_dim * 2u;
+    p.kc = a.kc + layer_at;
+    p.vc = a.vc + layer_at;
+    p.out = a.out;
     p.acc = a.scratch;
-    p.ml = a.scratch + records * g.head_dim;
-    const uint64_t items = a.selected ? (uint64_t)a.b.max_rows * p.tiles * p.splits : a.s.items;
-#define CALL(HD) run<HD>(s, p, items * g.kv_heads)
+    p.ml = a.scratch + (uint64_t)p.parts * g.kv_heads * p.tile_rows * g.head_dim;
+    p.row_requests = a.plan + a.s.requests;
+    p.row_positions = a.plan + a.s.positions;
+    p.joins = reinterpret_cast<const PagedJoin *>(a.plan + a.s.join_at);
+    const dim3 grid(a.selected ? a.b.max_rows * p.tiles : a.s.items, g.kv_heads, a.selected ? p.splits : 1u);
     switch (g.head_dim) {
-        case 64: CALL(64); break;
-        case 128: CALL(128); break;
-        default: CALL(256); break;
+        case 64: run<64>(s, p, a, shape.packed, grid); break;
+        case 128: run<128>(s, p, a, shape.packed, grid); break;
+        default: run<256>(s, p, a, shape.packed, grid); break;
     }
-#undef CALL
     VX_LAUNCHED("k_paged_attn");
     if (a.selected ? p.splits == 1u : a.s.joins == 0u) return VX_OK;   // nothing is divided
-    const uint32_t most = (uint32_t)((a.selected ? (uint64_t)a.b.max_rows * p.tiles : a.s.joins) * p.a.s.tile_rows * g.kv_heads);
-    const dim3 grid(std::min(most, 1024u));
     switch (g.head_dim) {
-        case 64: k_paged_join<64><<<grid, 256, 0, s>>>(p, most); break;
-        case 128: k_paged_join<128><<<grid, 256, 0, s>>>(p, most); break;
-        default: k_paged_join<256><<<grid, 256, 0, s>>>(p, most); break;
+        case 64: join<64>(s, p, a); break;
+        case 128: join<128>(s, p, a); break;
+        default: join<256>(s, p, a); break;
     }
     VX_LAUNCHED("k_paged_join");
     return VX_OK;

@@ -36,7 +36,8 @@ PagedShape paged_shape(const vx_paged_batch &b) {
     s.run_at = (s.granted + b.requests + 3u) / 4u * 4u;
     s.item_at = s.run_at + (uint64_t)s.runs * (sizeof(PagedRun) / 4u);
     s.join_at = s.item_at + (uint64_t)s.items * (sizeof(PagedItem) / 4u);
-    s.words = s.join_at + (uint64_t)s.joins * (sizeof(PagedJoin) / 4u);
+    s.page_at = s.join_at + (uint64_t)s.joins * (sizeof(PagedJoin) / 4u);
+    s.words = s.page_at + (s.tile_rows <= 16u ? (uint64_t)s.items * kPagedListed : 0u);
     return s;
 }
 
@@ -283,8 +284,6 @@ int vx_paged_attention(vx_ctx *ctx, const vx_buf *q, const vx_buf *k_cache, cons
     l.tables = at<uint32_t>(tables);
     l.plan = at<uint32_t>(plan);
     l.selected = selected ? at<uint32_t>(selected) : nullptr;
-    l.qvec = aligned(pc->q_stride, pc->q_base);
-    l.ovec = aligned(pc->out_stride, pc->out_base);
     OnDevice on(ctx->device);
     ProfSpan span(ctx, "paged.attention");
     return launch_paged_attention(ctx->stream, l);
@@ -323,7 +322,6 @@ int vx_paged_select(vx_ctx *ctx, const vx_buf *q, const vx_buf *bounds, const vx
     l.plan = at<uint32_t>(plan);
     l.selected = at<uint32_t>(selected);
     l.scratch = at<uint64_t>(scratch);
-    l.qvec = aligned(pc->q_stride, pc->q_base);
     OnDevice on(ctx->device);
     ProfSpan span(ctx, "paged.select");
     return launch_paged_select(ctx->stream, l);

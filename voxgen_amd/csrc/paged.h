@@ -11,6 +11,7 @@ constexpr uint32_t kPagedMaxTokens = 1u << 28;   // positions of a request
 constexpr uint32_t kPagedMaxRowHeads = 1u << 22; // rows of a step times query heads: bounds every grid
 constexpr uint32_t kPagedUnit = 16;              // slots of a unit: 32 * head_dim bytes of K, and of V
 constexpr uint32_t kPagedMaxSplits = 256;        // of a tile of query rows
+constexpr uint32_t kPagedListed = 64;            // units of an item whose pages the plan lists, for tiles of 16 rows or fewer
 
 // Chunks that are not divided: a CU takes 0.117 us for one (16 KB of heads of 128, 64 bytes a clock), the
 // launch that joins parts 4 (48 chunks: 10.2 us whole, 10.6 divided).
@@ -27,7 +28,7 @@ struct PagedShape {
     uint32_t workgroups, least;      // 2^workgroups
     uint32_t runs, items, joins, parts;              // most of each; items, joins and parts of one KV head
     // words of the plan
-    uint64_t slots, requests, positions, granted, run_at, item_at, join_at, words;
+    uint64_t slots, requests, positions, granted, run_at, item_at, join_at, page_at, words;
 };
 PagedShape paged_shape(const vx_paged_batch &b);
 
@@ -76,7 +77,6 @@ struct PagedAttn {
     const uint8_t *kc = nullptr, *vc = nullptr;
     float *out = nullptr, *scratch = nullptr;
     const uint32_t *tables = nullptr, *plan = nullptr, *selected = nullptr;
-    bool qvec = false, ovec = false;            // rows 16-byte aligned
 };
 uint64_t paged_attn_scratch_bytes(const vx_paged_batch &b, uint32_t budget);
 int launch_paged_attention(hipStream_t s, const PagedAttn &a);
@@ -90,7 +90,6 @@ struct PagedSelect {
     const uint32_t *tables = nullptr, *plan = nullptr;
     uint32_t *selected = nullptr;
     uint64_t *scratch = nullptr;
-    bool qvec = false;
 };
 uint64_t paged_select_scratch_bytes(const vx_paged_batch &b);
 int launch_paged_select(hipStream_t s, const PagedSelect &a);
