@@ -602,10 +602,14 @@ __global__ __launch_bounds__(256) void k_paged_join(AttnArgs p, uint32_t most, u
         }
         if (n <= 1u || n > kPagedMaxSplits) continue;
         const size_t at = ((size_t)head * p.parts + first) * tile_rows + r;   // the row's record in the first part
-        f4 early[E];
+        f4 early[2 * E] = {};
+        auto ask = [&](int e) { early[e] = *reinterpret_cast<const f4 *>(p.acc + (at + (size_t)min(y + e * Y, n - 1u) * tile_rows) * HD + c); };
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            early[e] = *reinterpret_cast<const f4 *>(p.acc + (at + (size_t)min(y + e * Y, n - 1u) * tile_rows) * HD + c);
+        for (int e = 0; e < E; ++e) ask(e);
+        if (n > (uint32_t)(E * Y)) {
+#pragma unroll
+            for (int e = E; e < 2 * E; ++e) ask(e);
+        }
         float m = -INFINITY, l = -1.f;
         if (tid < n) {
             m = p.ml[(at + (size_t)tid * tile_rows) * 2u];
@@ -628,10 +632,10 @@ __global__ __launch_bounds__(256) void k_paged_join(AttnArgs p, uint32_t most, u
         sum = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
         f4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < E; ++e)
+        for (int e = 0; e < 2 * E; ++e)
             if (y + e * Y < n) o += early[e] * sc[y + e * Y];
 #pragma unroll 8
-        for (uint32_t v = y + E * Y; v < n; v += Y)
+        for (uint32_t v = y + 2 * E * Y; v < n; v += Y)
             o += *reinterpret_cast<const f4 *>(p.acc + (at + (size_t)v * tile_rows) * HD + c) * sc[v];
         *reinterpret_cast<f4 *>(&os[y][c]) = o;
         __syncthreads();
