@@ -343,7 +343,7 @@ def test_single_tokens(ctx, heads, page_size):
 
 @pytest.mark.parametrize("heads,page_size,lengths", [
     ((16, 2, 128), 64, [5000]), ((16, 2, 128), 16, [2047, 9000, 3]), ((16, 1, 256), 32, [3001]), ((8, 8, 64), 256, [7000, 640]),
-    ((1, 1, 128), 32, [12345])])
+    ((1, 1, 128), 32, [12345]), ((16, 1, 64), 32, [6000, 50])])
 def test_single_tokens_over_long_caches(ctx, heads, page_size, lengths):
     side = Side(ctx, heads, page_size, lengths, [1] * len(lengths), 22)
     side.plan()
@@ -367,6 +367,32 @@ def test_several_tokens(ctx, heads, page_size, lengths, counts):
 def test_prompts(ctx, heads, page_size, lengths, counts):
     side = Side(ctx, heads, page_size, lengths, counts, 24)
     side.plan()
+    side.store()
+    side.check_attention()
+
+
+@pytest.mark.parametrize("heads,page_size,lengths,counts,pages", [
+    ((16, 2, 128), 256, [700, 3], [1, 1], 1030), ((32, 2, 128), 64, [3000, 90, 31], [1, 1, 1], 4100), ((8, 2, 64), 64, [400, 30], [2, 1], 8200),
+    ((16, 1, 64), 32, [1700], [1], 33000), ((16, 2, 256), 16, [100, 40], [1, 1], 8200), ((12, 1, 256), 128, [2000], [1], 2050)])
+def test_layers_beyond_the_caches(ctx, heads, page_size, lengths, counts, pages):
+    """A layer of more than 256 MB, its pages anywhere."""
+    side = Side(ctx, heads, page_size, lengths, counts, 28, spare=pages - sum(-(-(a + c) // page_size) for a, c in zip(lengths, counts)))
+    assert side.k.nbytes + side.v.nbytes > 256 << 20
+    side.plan()
+    side.store()
+    side.check_attention()
+
+
+@pytest.mark.parametrize("heads,n,count", [((8, 4, 64), 128, 1), ((8, 2, 128), 300, 2), ((4, 4, 64), 40, 40)])
+def test_parts_of_many_pages(ctx, heads, n, count):
+    """So many requests that a part has more chunks than the plan lists pages of (32) and than a wave's share of a few:
+    all of them over the same 4096 slots, each with a page of its own behind them."""
+    side = Side(ctx, heads, 128, [4096] + [0] * (n - 1), [count] * n, 29, spare=0)
+    side.tables[:, :32] = side.tables[0, :32]
+    side.lengths[:] = 4096
+    side.send()
+    side.plan()
+    assert (side.want["granted"] == count).all()
     side.store()
     side.check_attention()
 
@@ -592,7 +618,8 @@ def check_selection(side, budget, sinks, recent, q=None, layer=0):
     ((16, 2, 128), 32, [0, 31, 32, 700, 2000], [1] * 5, 8, 1, 2), ((16, 2, 128), 16, [1000, 40], [1, 3], 20, 0, 1),
     ((8, 8, 64), 64, [900, 130], [2, 1], 3, 1, 1), ((16, 1, 256), 16, [600], [1], 9, 2, 3), ((32, 4, 128), 128, [4000, 0], [1, 1], 5, 0, 5),
     ((10, 2, 128), 16, [3000], [1], 1, 0, 1), ((3, 3, 64), 16, [5000, 9], [1, 0], 100, 50, 50), ((64, 2, 64), 32, [800], [1], 7, 1, 1),
-    ((4, 2, 64), 16, [0], [300], 6, 1, 2), ((16, 2, 128), 32, [100, 7], [1, 1], 50, 0, 1)])
+    ((4, 2, 64), 16, [0], [300], 6, 1, 2), ((16, 2, 128), 32, [100, 7], [1, 1], 50, 0, 1), ((16, 2, 128), 32, [5000, 3300], [1, 1], 100, 1, 4),
+    ((40, 2, 128), 64, [6000], [1], 60, 0, 1), ((12, 1, 256), 16, [4000], [1], 200, 3, 5), ((8, 1, 256), 64, [5000, 40], [1, 2], 50, 1, 1)])
 def test_selection(ctx, heads, page_size, lengths, counts, budget, sinks, recent):
     side = Side(ctx, heads, page_size, lengths, counts, 41, layers=2, bounds=True, max_rows=sum(counts) + 1,
                 width=max(-(-(a + c) // page_size) for a, c in zip(lengths, counts)))
@@ -621,6 +648,28 @@ def test_selection_of_many_pages(ctx):
         for i in range(2):
             want = ref.select(ref.scores(q[i], bounds, 0, tables[i], int(lengths[i]), ps, 0), budget, sinks, recent)
             assert np.array_equal(got[i], want), (budget, i)
+
+
+@pytest.mark.parametrize("n,hd", [(512, 128), (513, 64), (1024, 256), (1025, 128), (2048, 64), (5000, 128), (8192, 256), (8193, 64)])
+def test_selection_by_the_width_of_tables(ctx, n, hd):
+    """About the sizes at which a thread holds more orders."""
+    rng = np.random.default_rng(46)
+    c = PagedCache(ctx, 1, n, 16, 2, hd, 2, n, 2, 4, bounds=True)
+    bounds = np.sort(rng.standard_normal((1, n, 2, 2, hd)).astype(np.float16), axis=3)
+    tables = np.stack([rng.permutation(n), rng.permutation(n)]).astype(np.uint32)
+    lengths = np.array([n * 16 - 1, n * 11], np.uint32)
+    for buf, x in ((c.bounds, bounds), (c.tables, tables), (c.lengths, lengths), (c.counts, np.array([1, 1], np.uint32))):
+        buf.upload(x)
+    c.plan()
+    q = rng.standard_normal((2, 2, 2, hd)).astype(np.float32)
+    for budget, sinks, recent in ((2, 0, 1), (n // 8, 1, 4), (n - 1, 2, 1)):
+        sel = c.selection(budget)
+        c.select(0, ctx.array(q), sel, budget, sinks, recent)
+        got = sel.download(np.uint32).reshape(2, 2, budget)
+        for i in range(2):
+            for h in range(2):
+                want = ref.select(ref.scores(q[i, h], bounds, 0, tables[i], int(lengths[i]), 16, h), budget, sinks, recent)
+                assert np.array_equal(got[i, h], want), (budget, i, h)
 
 
 def test_equal_scores_go_to_the_lowest_pages(ctx):

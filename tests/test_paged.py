@@ -68,7 +68,7 @@ lib = abi.load()
 def kernels():
     return launches("k_paged")
 G = dict(layers=2, pages=30, page_size=16, kv_heads=2, head_dim=128)
-B = dict(requests=3, table_width=10, max_rows=6, max_count=4, q_heads=8)
+B = dict(requests=3, table_width=200, max_rows=6, max_count=4, q_heads=8)
 def batch(**kw):
     return abi.PagedBatch(abi.PagedGeom(*[kw.get(n, v) for n, v in G.items()]), *[kw.get(n, v) for n, v in B.items()])
 def store_push(**kw):
@@ -83,7 +83,7 @@ kc, vc, bounds = ctx.alloc(cache), ctx.alloc(cache), ctx.alloc(lib.vx_paged_boun
 k, v = ctx.alloc(6 * 256 * 4), ctx.alloc(6 * 256 * 4)
 q, out = ctx.alloc(6 * 1024 * 4), ctx.alloc(6 * 1024 * 4)
 lengths, counts, keep = ctx.alloc(12), ctx.alloc(12), ctx.alloc(12)
-tables, pool, plan = ctx.alloc(120), ctx.alloc(31 * 4), ctx.alloc(lib.vx_paged_plan_bytes(batch()))
+tables, pool, plan = ctx.alloc(2400), ctx.alloc(31 * 4), ctx.alloc(lib.vx_paged_plan_bytes(batch()))
 selected = ctx.alloc(6 * 2 * 5 * 4)
 scratch = ctx.alloc(1 << 26)
 small = ctx.alloc(4)
@@ -207,7 +207,7 @@ bare = PagedCache(ctx, 1, 30, 16, 2, 128, 3, 10, 6, 8)
 assert bare.bounds is None and refused(bare.select, 0, q, sel, 5) == "VX_ERR_STATE"
 assert refused(c.select, 0, q, sel, 11) == "VX_ERR_BOUNDS" and refused(c.select, 0, q, c.selection(11), 11) == "VX_OK"
 # scratch that is refused leaves the cache as it was
-big = PagedCache(ctx, 1, 30, 16, 2, 128, 3, 10, 1024, 8)
+big = PagedCache(ctx, 1, 30, 16, 2, 128, 3, 200, 1024, 8)
 qs, outs = ctx.alloc(1024 * 1024 * 4), ctx.alloc(1024 * 1024 * 4)
 refuse(4096, 1 << 40)
 assert refused(big.attention, 0, qs, outs) == "VX_ERR_OOM" and big._scratch is None
@@ -222,11 +222,11 @@ def test_scratch_is_what_the_kernels_reach(fake):  # noqa: F811
     rng = np.random.default_rng(5)
     for _ in range(300):
         kv = int(rng.choice([1, 2, 3, 8]))
-        log2 = int(rng.choice([9, 10]))
+        log2 = int(rng.choice([7, 8, 9, 10]))
         share = -(-(1 << log2) // kv)
         n = int(rng.integers(1, 200))
         chunks, tiles = rng.integers(1, 1 << int(rng.integers(1, 14)), n), rng.integers(1, 1 << int(rng.integers(1, 10)), n)
-        per = max(int((int((chunks * tiles).sum()) * kv + (1 << log2) - 1) >> log2), int(rng.choice([4, 8])))
+        per = max(int((int((chunks * tiles).sum()) * kv + (1 << log2) - 1) >> log2), int(rng.choice([4, 8, 16, 48])))
         splits = np.minimum(-(-chunks // per), 256)
         by = -(-chunks // splits)
         splits = -(-chunks // by)
@@ -272,4 +272,54 @@ for kw in (dict(max_rows=1 << 22, max_count=1 << 22, q_heads=1, kv_heads=1, page
     tab = ctx.alloc(4 * b.requests * b.table_width)
     assert attn(pc, q=ctx.alloc(rows), out=ctx.alloc(rows), kc=big[0], vc=big[1], tables=tab, plan=plan,
                 scratch=ctx.alloc(lib.vx_paged_attention_scratch_bytes(pc))) == "VX_OK"
+""")
+
+
+def test_every_kernel_has_a_case_whose_values_are_compared(roomy):  # noqa: F811
+    """The kernels of a call go by sizes. Each that the library holds is launched by a case of the GPU tests that compares
+    values with the restatement, so that no change of a rule leaves a kernel untested, or one that no call reaches."""
+    child(roomy, CALLS + """
+import re
+sys.path[:0] = ["tests", "oracle"]
+import test_gpu_paged as gpu
+from pathlib import Path
+held = set(n.decode() for n in re.findall(rb"_ZN2vx[0-9A-Z_]*k_paged_[A-Za-z0-9_]+", Path(abi.LIB_PATH).read_bytes()) if b"device_stub" not in n)
+names = set(re.search("k_paged_.*", n).group() for n in held)
+names = set(n for n in names if not re.match("k_paged_(advance|cut|reset)", n))          # one each
+assert len(names) > 40, names
+def params(test):
+    sets = [{}]
+    for m in [m for m in test.pytestmark if m.name == "parametrize"]:
+        keys = m.args[0].split(",")
+        rows = [dict(zip(keys, v if len(keys) > 1 else (v,))) for v in m.args[1]]
+        sets = [dict(s, **r) for s in sets for r in rows]
+    return sets
+big = {n: ctx.alloc(1 << 36) for n in ("a", "b", "c", "d", "e", "f", "g")}
+def step(heads, page_size, lengths, counts, pages=None, budget=0, bounds=False, width=None):
+    need = [-(-(a + c) // page_size) for a, c in zip(lengths, counts)]
+    b = abi.PagedBatch(abi.PagedGeom(1, pages or sum(need) + 3, page_size, heads[1], heads[2]), len(lengths), width or max(need) + 2,
+                       sum(counts), max(counts), heads[0])
+    row, qrow = heads[1] * heads[2], heads[0] * heads[2]
+    assert make(b, big["a"], big["b"], big["c"], big["d"], big["e"]) == "VX_OK"
+    assert store(abi.PagedStorePush(b, 0, row, row, 0, 0), big["a"], big["b"], big["c"], big["d"], big["e"] if bounds else None, big["f"]) == "VX_OK"
+    assert attn(abi.PagedAttentionPush(b, 0, qrow, qrow, 0, 0, budget), big["a"], big["b"], big["c"], big["d"], big["e"], big["f"],
+                big["g"] if budget else None, ctx.alloc(1 << 36)) == "VX_OK"
+    if budget:
+        pc = abi.PagedSelectPush(b, 0, qrow, 0, budget, 0, 1)
+        assert select(pc, big["a"], big["b"], big["c"], big["d"], big["e"], big["f"]) == "VX_OK"
+for p in params(gpu.test_single_tokens):
+    step(p["heads"], p["page_size"], [511, 300], [1, 1])
+for p in params(gpu.test_single_tokens_over_long_caches):
+    step(p["heads"], p["page_size"], p["lengths"], [1] * len(p["lengths"]))
+for test in (gpu.test_several_tokens, gpu.test_prompts, gpu.test_layers_beyond_the_caches, gpu.test_store):
+    for p in params(test):
+        step(**p)
+for p in params(gpu.test_selection):
+    step(*[p[n] for n in ("heads", "page_size", "lengths", "counts")], budget=p["budget"], bounds=True)
+for p in params(gpu.test_selection_by_the_width_of_tables):
+    step((4, 2, p["hd"]), 16, [5, 5], [1, 1], pages=p["n"], budget=p["n"] // 8, width=p["n"])
+for p in params(gpu.test_plan):
+    step((4, 2, 64), p["page_size"], [5] * p["n"], [1] * p["n"])
+missing = [n for n in names if not launches(n)]
+assert not missing, missing
 """)
