@@ -71,7 +71,7 @@ __device__ __forceinline__ uint32_t owner_of(const uint32_t *end, uint32_t n, ui
 // request that it is of, and its page.
 template <uint32_t T, uint32_t E>
 __global__ __launch_bounds__(T) void k_paged_plan(PagedPlan a) {
-    constexpr uint32_t N = T * E;
+    constexpr uint32_t N = T * E, kPagedLists = 7;
     __shared__ uint32_t length_of[N], count_of[N], row_end[N], page_end[N], run_end[N], item_end[N], join_end[N], part_end[N];
     __shared__ uint32_t between[T / 64][6];
     __shared__ float work[T / 64];
@@ -173,7 +173,10 @@ __global__ __launch_bounds__(T) void k_paged_plan(PagedPlan a) {
 
     const uint32_t all_runs = min(sum[0], a.s.runs), all_items = min(sum[1], a.s.items), all_joins = min(sum[2], a.s.joins);
     const uint32_t taken = min(sum[4], free);
-    const uint32_t g0 = blockIdx.x * T + tid, step = gridDim.x * T;
+    // What is left is lists whose entries stand for themselves; each begins at another workgroup, so that
+    // short ones are made at the same time.
+    const uint32_t step = gridDim.x * T;
+    auto turn = [&](uint32_t list) { return (blockIdx.x >= list ? blockIdx.x - list : blockIdx.x + gridDim.x - list) * T + tid; };
     auto begin = [&](const uint32_t *end, uint32_t i) { return i ? end[i - 1u] : 0u; };
     auto part_of = [&](uint32_t i) { return run_end[i] != begin(run_end, i); };
     // the page of position p of request i that takes part: one in use, or one from the top of the pool
@@ -184,7 +187,7 @@ __global__ __launch_bounds__(T) void k_paged_plan(PagedPlan a) {
         const uint32_t page = *from;
         return k < have || nth < free ? page : VX_PAGED_NONE;
     };
-    for (uint32_t r = g0; r < rows; r += step) {
+    for (uint32_t r = turn(0); r < rows; r += step) {
         uint32_t slot = VX_PAGED_NONE, request = VX_PAGED_NONE, position = VX_PAGED_NONE;
         if (r < all_rows) {
             const uint32_t i = owner_of(row_end, n, r);
@@ -199,7 +202,7 @@ __global__ __launch_bounds__(T) void k_paged_plan(PagedPlan a) {
         a.plan[a.s.requests + r] = request;
         a.plan[a.s.positions + r] = position;
     }
-    for (uint32_t g = g0; g < all_runs; g += step) {
+    for (uint32_t g = turn(1); g < all_runs; g += step) {
         const uint32_t i = owner_of(run_end, n, g), length = length_of[i], k = g - begin(run_end, i);
         const uint32_t first = k ? ((length >> shift) + k) << shift : length;       // position of the run's first row
         const uint32_t last = min(((first >> shift) + 1u) << shift, length + count_of[i]);
@@ -208,7 +211,7 @@ __global__ __launch_bounds__(T) void k_paged_plan(PagedPlan a) {
                               page < pages ? (page << shift) + (first & (ps - 1u)) : VX_PAGED_NONE, 0u};
         reinterpret_cast<PagedRun *>(a.plan + a.s.run_at)[g] = run;
     }
-    for (uint32_t g = g0; g < all_items; g += step) {
+    for (uint32_t g = turn(2); g < all_items; g += step) {
         const uint32_t i = owner_of(item_end, n, g), length = length_of[i], cnt = count_of[i], k = g - begin(item_end, i);
         uint32_t s;
         const uint32_t by = divided((length + cnt + 31u) / 32u, s);
@@ -222,7 +225,7 @@ __global__ __launch_bounds__(T) void k_paged_plan(PagedPlan a) {
         reinterpret_cast<PagedItem *>(a.plan + a.s.item_at)[g] = it;
     }
     if (a.s.tile_rows <= 16u) {   // a tile is few rows: the pages of its part's first units
-        for (uint32_t g = g0; g < all_items * kPagedListed; g += step) {
+        for (uint32_t g = turn(3); g < all_items * kPagedListed; g += step) {
             const uint32_t item = g / kPagedListed, i = owner_of(item_end, n, item), length = length_of[i], cnt = count_of[i];
             uint32_t s;
             const uint32_t by = divided((length + cnt + 31u) / 32u, s);
@@ -230,19 +233,19 @@ __global__ __launch_bounds__(T) void k_paged_plan(PagedPlan a) {
             a.plan[a.s.page_at + g] = at < length + cnt ? page_of(i, length, at) : VX_PAGED_NONE;
         }
     }
-    for (uint32_t g = g0; g < all_joins; g += step) {
+    for (uint32_t g = turn(4); g < all_joins; g += step) {
         const uint32_t i = owner_of(join_end, n, g), length = length_of[i], cnt = count_of[i], tile = g - begin(join_end, i);
         uint32_t s;
         const uint32_t by = divided((length + cnt + 31u) / 32u, s);
         const PagedJoin j = {begin(row_end, i), length, cnt, tile << tile_shift, begin(part_end, i) + tile * s, by, {0, 0}};
         reinterpret_cast<PagedJoin *>(a.plan + a.s.join_at)[g] = j;
     }
-    for (uint32_t i = g0; i < n; i += step) a.plan[a.s.granted + i] = part_of(i) ? count_of[i] : 0u;
-    for (uint32_t g = g0; g < taken; g += step) {   // pages that requests that take part want: they are the first of all wanted
+    for (uint32_t i = turn(5); i < n; i += step) a.plan[a.s.granted + i] = part_of(i) ? count_of[i] : 0u;
+    for (uint32_t g = turn(6); g < taken; g += step) {   // pages that requests that take part want: they are the first of all wanted
         const uint32_t i = owner_of(page_end, n, g), have = (length_of[i] + ps - 1u) >> shift;
         a.tables[(size_t)i * width + have + g - begin(page_end, i)] = a.pool[free - g];
     }
-    if (blockIdx.x == 0) {
+    if (blockIdx.x == kPagedLists) {
         uint32_t some = most_taking;
         if constexpr (E > 1) {
             some = taking;
@@ -635,9 +638,10 @@ int launch_paged_reset(hipStream_t s, const vx_paged_batch &b, uint32_t *lengths
 }
 
 int launch_paged_plan(hipStream_t s, const PagedPlan &a) {
-    // one workgroup for so many rows, items or requests as it has threads; 64 for more
+    // a workgroup for so many rows, entries of a list or requests as it has threads; 64 for more, and one for
+    // each of the lists and the header (16 requests of a token: 5.8 us, by one workgroup 7.1)
     const uint32_t most = std::max(std::max(a.b.max_rows, a.b.requests), a.s.items * (a.s.tile_rows <= 16u ? kPagedListed : 1u));
-    auto blocks = [&](uint32_t threads) { return std::min((most + threads - 1u) / threads, 64u); };
+    auto blocks = [&](uint32_t threads) { return std::min(std::max((most + threads - 1u) / threads, 8u), 64u); };
     if (a.b.requests <= 256u)
         k_paged_plan<256, 1><<<blocks(256), 256, 0, s>>>(a);
     else if (a.b.requests <= 1024u)
