@@ -539,6 +539,23 @@ def test_plan_of_any_content_stays_in_bounds(ctx):
         assert np.array_equal(got[31:], guard[31:])
 
 
+def test_lists_of_any_content_stay_in_bounds(ctx):
+    """The same of plans of single tokens over tables that are divided: pages of items and joins are anything too."""
+    side = Side(ctx, (16, 2, 128), 16, [2000, 20, 900], [1, 1, 1], 34, width=200)
+    side.plan()
+    side.store()
+    rng = np.random.default_rng(2)
+    words = side.dev.plan_buffer.nbytes // 4
+    for most in (2, 8, 64, 200, 2400, 1 << 32):
+        side.dev.plan_buffer.upload(rng.integers(0, most, words, dtype=np.uint64).astype(np.uint32))
+        guard = side.rng.standard_normal((3 + 64, 2048)).astype(np.float32)
+        out, q = ctx.array(guard), ctx.array(side.queries())
+        side.dev.attention(0, q, out)
+        assert np.array_equal(out.download(np.float32).reshape(guard.shape)[3:], guard[3:])
+    side.plan()
+    side.check_attention()                                          # nothing of it is left
+
+
 def test_offsets_beyond_32_bits(ctx):
     """Caches of more than 4 GiB each, their last layer and pages; a selection too."""
     layers, pages, ps = 3, 24000, 256

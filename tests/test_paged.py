@@ -216,6 +216,21 @@ assert refused(big.attention, 0, qs, outs) == "VX_OK"
 """)
 
 
+def test_scratch_of_calls_that_divide_nothing(fake):  # noqa: F811
+    """Tables of a few chunks: no partial sums, but a size that tells such a call from one that is not valid."""
+    child(fake, CALLS + """
+for kw in (dict(table_width=1), dict(table_width=96), dict(table_width=200, budget=5)):
+    need = lib.vx_paged_attention_scratch_bytes(attn_push(**kw))
+    assert need == 16, (kw, need)
+few = dict(table_width=10)
+p = ctx.alloc(lib.vx_paged_plan_bytes(batch(**few)))
+assert attn(attn_push(**few), plan=p, scratch=small) == "VX_ERR_BOUNDS"
+assert attn(attn_push(**few), plan=p, scratch=None) == "VX_ERR_INVALID_ARG"
+assert attn(attn_push(**few), plan=p, scratch=ctx.alloc(16)) == "VX_OK"
+assert lib.vx_paged_attention_scratch_bytes(attn_push()) > 16
+""")
+
+
 def test_scratch_is_what_the_kernels_reach(fake):  # noqa: F811
     """Parts of a step: never more than its share of workgroups makes, whatever lengths the plan finds (the kernel's
     arithmetic, here with the sizes that a batch fixes)."""

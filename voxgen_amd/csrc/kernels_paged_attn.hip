@@ -717,7 +717,8 @@ void join(hipStream_t s, const AttnArgs &p, const PagedAttn &a) {
 
 uint64_t paged_attn_scratch_bytes(const vx_paged_batch &b, uint32_t budget) {
     const PagedShape s = shape_of(b, budget);
-    return parts_of(b, s, budget) * b.geom.kv_heads * s.tile_rows * (b.geom.head_dim + 2u) * 4u;
+    // never 0, which is what a batch that is not valid has
+    return std::max<uint64_t>(parts_of(b, s, budget) * b.geom.kv_heads * s.tile_rows * (b.geom.head_dim + 2u) * 4u, 16u);
 }
 
 int launch_paged_attention(hipStream_t s, const PagedAttn &a) {
