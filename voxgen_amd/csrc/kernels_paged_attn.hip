@@ -262,25 +262,29 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
 
     for (uint32_t d = tid; d < 2u * HD; d += 64u * W) odd[d / HD][d % HD] = ~0u;
     uint32_t found = 0;
-    h8 qh[U], ql[U];
+    // The two terms of the queries, in registers where these do; the tiles of 32 rows get them through LDS, which the other
+    // heads' read again each chunk (heads of 128: 919 tokens 60.3 us, read each time 62.4; 2000 at 6000 267 and 288;
+    // but heads of 64, of which a CU then holds one workgroup and not two, 160 and 137).
+    constexpr bool HELD = NT == 1 || HD == 128;
+    h8 qh[HELD ? NT : 1][U], ql[HELD ? NT : 1][U];
     float factor[NT];
     h8 *const qs = reinterpret_cast<h8 *>(lds);   // [NT][U][hi, lo][64]
     if constexpr (NT == 1) {
-        factor[0] = qr.split(qh, ql);
+        factor[0] = qr.split(qh[0], ql[0]);
         if constexpr (PK) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) qh[u] = i < 8u ? qh[u] : ql[u];
+            for (int u = 0; u < U; ++u) qh[0][u] = i < 8u ? qh[0][u] : ql[0][u];
         }
     } else {
         for (uint32_t c = w; c < NT; c += W) {
             const uint32_t row = r0 + 16u * c + i;
             qr.load(p, t, head, min(row, rows - 1u), q);
-            const float f = qr.split(qh, ql);
+            const float f = qr.split(qh[0], ql[0]);
             if (q == 0) fs[16u * c + i] = f;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                qs[((c * U + u) * 2u) * 64u + lane] = qh[u];
-                qs[((c * U + u) * 2u + 1u) * 64u + lane] = ql[u];
+                qs[((c * U + u) * 2u) * 64u + lane] = qh[0][u];
+                qs[((c * U + u) * 2u + 1u) * 64u + lane] = ql[0][u];
             }
         }
     }
@@ -288,6 +292,15 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
         __syncthreads();
 #pragma unroll
         for (int c = 0; c < NT; ++c) factor[c] = fs[16 * c + i];
+        if constexpr (HELD) {
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    qh[c][u] = qs[((c * U + u) * 2u) * 64u + lane];
+                    ql[c][u] = qs[((c * U + u) * 2u + 1u) * 64u + lane];
+                }
+        }
     }
     // last position that the lane's row of a column tile attends to
     auto limit = [&](int c) { return t.base + token_of(p, min(r0 + 16u * c + ri, rows - 1u)); };
@@ -329,8 +342,8 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
         for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int c = 0; c < NT; ++c) {
-                const h8 hi = NT == 1 ? qh[u] : qs[((c * U + u) * 2u) * 64u + lane];
-                const h8 lo = NT == 1 ? ql[u] : qs[((c * U + u) * 2u + 1u) * 64u + lane];
+                const h8 hi = HELD ? qh[HELD ? c : 0][u] : qs[((c * U + u) * 2u) * 64u + lane];
+                const h8 lo = HELD ? ql[HELD ? c : 0][u] : qs[((c * U + u) * 2u + 1u) * 64u + lane];
                 x[c][0] = mfma16(kf.x[0][u], hi, x[c][0]);
                 x[c][1] = mfma16(kf.x[1][u], hi, x[c][1]);
                 if constexpr (!PK) {
