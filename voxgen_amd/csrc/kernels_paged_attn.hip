@@ -685,7 +685,7 @@ void divide(const vx_paged_batch &b, const PagedShape &s, uint32_t budget, uint3
 PagedShape shape_of(vx_paged_batch b, uint32_t budget) {
     if (budget) b.max_count = 1;
     PagedShape s = paged_shape(b);
-    if (budget && s.tile_rows > 16u) s.tile_rows = 16u, s.waves = 4u, s.workgroups = 10u;
+    if (budget && s.tile_rows > 16u) s.tile_rows = 16u, s.waves = 4u, s.workgroups = b.geom.head_dim < 256u ? 10u : 9u;
     return s;
 }
 
