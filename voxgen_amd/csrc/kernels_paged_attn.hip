@@ -176,8 +176,8 @@ __device__ __forceinline__ bool finite(_Float16 x) {
 //
 // Bound, with heads of 128: one token over 511, 6.0 us, by what needs each other, the part, its pages, q and K,
 // four chunks a wave and the join in LDS; 64 requests over up to 24000, 184, by reading 1.06 GB (5.75 TB/s; a kernel
-// that only reads: 6.25); 919 tokens of two requests, 62, by the issue of products (0.42 of the CUs' busy time) and other
-// vector instructions (0.31), and by 460 tiles on 256 CUs (busy 0.70 of it): 740 TFLOP/s of two-term products.
+// that only reads: 6.25); 919 tokens of two requests, 60, by the issue of products (0.45 of the CUs' busy time) and other
+// vector instructions (0.33), and by 460 tiles on 256 CUs (busy 0.69 of it): 770 TFLOP/s of two-term products.
 template <int HD, int NT, int W, bool PK, Mode MODE>
 __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_attn(AttnArgs p) {
     constexpr int U = HD / 32, DT = HD / 16, OROW = HD + 4, R = 16 * NT, RT = PK ? 8 : R, B = W > 4 ? W / 2 : W;
