@@ -180,9 +180,9 @@ __device__ __forceinline__ bool finite(_Float16 x) {
 // vector instructions (0.33), and by 460 tiles on 256 CUs (busy 0.69 of it): 770 TFLOP/s of two-term products.
 template <int HD, int NT, int W, bool PK, Mode MODE>
 __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_attn(AttnArgs p) {
-    constexpr int U = HD / 32, DT = HD / 16, OROW = HD + 4, R = 16 * NT, RT = PK ? 8 : R, B = W > 4 ? W / 2 : W;
+    constexpr int U = HD / 32, DT = HD / 16, OROW = HD + 4, R = 16 * NT, RT = PK ? 8 : R;
     constexpr int QLDS = NT > 1 ? R * HD : 0;   // floats: two f16 planes
-    constexpr int LDS = B * R * OROW > QLDS ? B * R * OROW : QLDS;
+    constexpr int LDS = W * R * OROW > QLDS ? W * R * OROW : QLDS;
     constexpr size_t UNIT = 32 * HD;            // bytes
     __shared__ __attribute__((aligned(16))) float lds[LDS];
     static_assert((!PK || NT == 1) && (W == 4 || W == 8), "one column tile of both terms; a wave or two a SIMD");
@@ -488,8 +488,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
 
     // A wave's sums are taken to the row's largest reference. One without keys has nothing
     // to give; one whose every score is NaN has no reference but a NaN sum.
-    constexpr int PART = W > B ? R / 2 : R;   // rows of a wave's part
-    auto *const os = reinterpret_cast<float (*)[PART][OROW]>(lds);
+    auto *const os = reinterpret_cast<float (*)[R][OROW]>(lds);
     float sum[NT], top[NT];
 #pragma unroll
     for (int c = 0; c < NT; ++c) {
@@ -508,41 +507,10 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[c][dt] *= share;
     }
-    if constexpr (W > B) {
-        // Waves w and w + 4 exchange halves of their tiles, so that all write and read: each adds
-        // the partner's half to its own, in the partner's part of LDS.
-        constexpr int H = NT / 2;
-        auto give = [&](auto upper) {
 #pragma unroll
-            for (int c = 0; c < H; ++c)
+    for (int c = 0; c < NT; ++c)
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-                    *reinterpret_cast<f4 *>(&os[w][16 * c + i][16 * dt + 4 * q]) = o[decltype(upper)::value ? c : H + c][dt];
-        };
-        auto take = [&](auto upper) {
-#pragma unroll
-            for (int c = 0; c < H; ++c)
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    f4 *const at = reinterpret_cast<f4 *>(&os[w ^ B][16 * c + i][16 * dt + 4 * q]);
-                    *at = *at + o[decltype(upper)::value ? H + c : c][dt];
-                }
-        };
-        if (w < B)
-            give(std::false_type{});
-        else
-            give(std::true_type{});
-        __syncthreads();
-        if (w < B)
-            take(std::false_type{});
-        else
-            take(std::true_type{});
-    } else {
-#pragma unroll
-        for (int c = 0; c < NT; ++c)
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f4 *>(&os[w][16 * c + i][16 * dt + 4 * q]) = o[c][dt];
-    }
+        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f4 *>(&os[w][16 * c + i][16 * dt + 4 * q]) = o[c][dt];
     const bool alone = t.part == VX_PAGED_NONE;
     const size_t part = (size_t)head * p.parts + (alone ? 0u : t.part);
     if (w == 0 && q == 0) {   // the factors of the scores have been read, a barrier ago and more
@@ -559,13 +527,12 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     for (uint32_t k = tid; k < (uint32_t)RT * V; k += 64u * W) {
         const uint32_t r = k / V, c = 4u * (k % V), row = r0 + r;
         if (row >= rows) break;
-        const uint32_t u0 = W > B && r < (uint32_t)PART ? B : 0u, at = r % (uint32_t)PART;   // a half's sums: in the other's parts
-        f4 v = *reinterpret_cast<const f4 *>(&os[u0][at][c]);
+        f4 v = *reinterpret_cast<const f4 *>(&os[0][r][c]);
 #pragma unroll
-        for (int u = 1; u < B; ++u) v += *reinterpret_cast<const f4 *>(&os[u0 + u][at][c]);
+        for (int u = 1; u < W; ++u) v += *reinterpret_cast<const f4 *>(&os[u][r][c]);
         if constexpr (PK) {
 #pragma unroll
-            for (int u = 0; u < B; ++u) v += *reinterpret_cast<const f4 *>(&os[u][r + 8u][c]);
+            for (int u = 0; u < W; ++u) v += *reinterpret_cast<const f4 *>(&os[u][r + 8u][c]);
         }
         const uint32_t k0 = token_of(p, row), j = row - k0 * p.group;
         if (any_odd) {
