@@ -175,9 +175,9 @@ __device__ __forceinline__ bool finite(_Float16 x) {
 // columns of a row are added, and so are its sums at the end.
 //
 // Bound, with heads of 128: one token over 511, 6.0 us, by what needs each other, the part, its pages, q and K,
-// four chunks a wave and the join in LDS; 64 requests over up to 24000, 184, by reading 1.06 GB (5.75 TB/s; a kernel
-// that only reads: 6.25); 919 tokens of two requests, 60, by the issue of products (0.45 of the CUs' busy time) and other
-// vector instructions (0.33), and by 460 tiles on 256 CUs (busy 0.69 of it): 770 TFLOP/s of two-term products.
+// four chunks a wave and the join in LDS; 64 requests over up to 24000, 183, by reading 1.06 GB (5.8 TB/s; a kernel
+// that only reads: 6.25); 919 tokens of two requests, 58, by the issue of products (0.46 of the CUs' busy time) and other
+// vector instructions (0.33), and by 460 tiles on 256 CUs (busy 0.69 of it): 790 TFLOP/s of two-term products.
 template <int HD, int NT, int W, bool PK, Mode MODE>
 __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_attn(AttnArgs p) {
     constexpr int U = HD / 32, DT = HD / 16, OROW = HD + 4, R = 16 * NT, RT = PK ? 8 : R;

@@ -15,7 +15,7 @@ PagedShape paged_shape(const vx_paged_batch &b) {
     // Of eight rows both f16 terms go through the products side by side, not one behind the other, and scratch
     // has eight rows, not sixteen (one token over 32700: 8.6 us and 4.7 to join, else 9.0 and 4.5; 64 requests over
     // up to 24000, which wait for memory: 184 and 5.2, else 181 and 8.0). Tiles of 32 rows ask for K and V half
-    // as often as those of 16 (919 tokens: 60 us, with 16 rows 77 and 34 to join; 5 tokens of 64 requests over
+    // as often as those of 16 (919 tokens: 58 us, with 16 rows 77 and 34 to join; 5 tokens of 64 requests over
     // 8000: 111, 129 and 21; but 60 tokens at 1000 13.6, 11.7). They have eight waves, and of heads of 256 four,
     // for which there are registers (400 tokens at 2000 of those: 54).
     s.packed = rows <= 8u;
