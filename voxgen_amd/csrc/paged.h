@@ -16,6 +16,9 @@ constexpr uint32_t kPagedListed = 64;            // units of an item whose pages
 // Chunks that are not divided: a CU takes 0.117 us for one (16 KB of heads of 128, 64 bytes a clock), the
 // launch that joins parts 4 (one token: 47 chunks whole 9.9 us, 63 divided 6.0 and 4.1).
 constexpr uint32_t kPagedWhole = 48;
+// Of tiles of 32 rows with four waves, each of which takes 3 us for a chunk (heads of 256: 20 tokens of two requests at
+// 1300 whole 32 us, divided 16.7 and 4.6; 100 at 1000 29, 17.9 and 7.5; but 600 at 600 50, 49.6 and 4.6).
+constexpr uint32_t kPagedWholeWide = 32;
 
 inline uint32_t paged_shift(uint32_t page_size) { return 31u - (uint32_t)__builtin_clz(page_size); }
 
