@@ -697,7 +697,8 @@ uint64_t vx_paged_attention_scratch_bytes(const vx_paged_attention_push *pc);
  * pages of its list: indices into the request's table, each once; of the first
  * min(budget, position / page_size + 1) entries those that are such pages count, and a
  * row with none of them has an output of 0. A NaN or an infinity that is stored reaches the rows
- * that attend to its slot and no other; slots that hold no token may hold anything. */
+ * that attend to its slot and no other, as IEEE arithmetic on the formula has it (a key with a score of -inf has
+ * a weight of 0); slots that hold no token may hold anything. Calls with infinite keys take some 20 times as long. */
 int vx_paged_attention(vx_ctx *ctx, const vx_buf *q, const vx_buf *k_cache, const vx_buf *v_cache, vx_buf *out,
                        const vx_buf *tables, const vx_buf *plan, const vx_buf *selected, vx_buf *scratch,
                        const vx_paged_attention_push *pc);

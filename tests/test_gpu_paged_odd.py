@@ -1,0 +1,135 @@
+"""The paged KV cache's attention where values or tables are out of the ordinary, on tiles of 8, 16 and 32
+query rows of each head size: against the formula in 64 bits, element by element (a library's matrix product need not
+keep to IEEE arithmetic where factors are infinite).
+
+Finite outputs are compared by relative 2-norm with the bound that test_gpu_paged.py derives; a score of the path for
+infinite keys is a sum of head_dim products in f32, off by sqrt(head_dim) 2^-24 of its terms' size, which is below
+what that bound has for products of two terms.
+"""
+import numpy as np
+import pytest
+
+import pagedref as ref
+from conftest import rel_l2
+from test_gpu_paged import NONE, TOL, Side, rows_of
+
+pytestmark = pytest.mark.gpu
+
+# (heads, rows of a request): tokens x group is what a tile is chosen by
+TILES = [((16, 2, 128), 1), ((8, 4, 64), 4), ((4, 1, 256), 2),            # 8 rows
+         ((32, 2, 128), 1), ((16, 4, 64), 3), ((16, 1, 256), 1),          # 16
+         ((16, 2, 128), 5), ((8, 1, 64), 9), ((6, 1, 256), 7)]            # 32
+
+
+def by_formula(side, q, layer=0, pages=None, tables=None):
+    """softmax(q . K / sqrt(head_dim)) . V of every row that takes part, NaN in the others."""
+    out = np.full(q.shape, np.nan)
+    tables = side.tables if tables is None else tables
+    row = 0
+    with np.errstate(all="ignore"):
+        for i, count in enumerate(side.counts.tolist()):
+            n = int(side.lengths[i]) + count
+            for h in range(side.kv_heads):
+                k, there = ref.rows(side.k, layer, tables[i], h, n, False)
+                v, _ = ref.rows(side.v, layer, tables[i], h, n, True)
+                for t in range(count if side.want["granted"][i] else 0):
+                    sees = there & (np.arange(n) <= n - count + t)
+                    if pages is not None:
+                        sees &= np.isin(np.arange(n) // side.ps, pages[row + t][h])
+                    for j in range(q.shape[2]):
+                        s = (q[row + t, h, j].astype(np.float64) * k[sees]).sum(-1) / np.sqrt(side.hd)
+                        e = np.exp(s - s.max()) if len(s) else s
+                        out[row + t, h, j] = (e[:, None] / e.sum() * v[sees]).sum(0) if len(s) else 0
+            row += count
+    return out
+
+
+def check(got, want):
+    assert np.array_equal(np.isnan(got), np.isnan(want)), np.argwhere(np.isnan(got) != np.isnan(want))[:4]
+    assert np.array_equal(np.isinf(got), np.isinf(want)) and np.array_equal(got[np.isinf(got)], want[np.isinf(want)])
+    for r in np.ndindex(*got.shape[:3]):
+        ok = np.isfinite(want[r])
+        off = rel_l2(got[r][ok], want[r][ok])
+        assert off < TOL, r
+
+
+def mixed_signs(q, dim, sign):
+    """Queries whose product with an infinity of that sign in dimension `dim` is -inf; of some rows, however small they
+    are there; of some +inf or, where they are 0, NaN."""
+    rows = q.reshape(-1, q.shape[-1])
+    rows[:, dim] = -sign * (np.abs(rows[:, dim]) + np.float32(0.01))
+    rows[1::5, dim] *= np.float32(1e-14)
+    rows[3::11, dim] *= -1
+    rows[7::11, dim] = 0
+    return q
+
+
+# ------------------------------------------------------------ infinite keys
+@pytest.mark.parametrize("heads,count", TILES)
+@pytest.mark.parametrize("sign", [1, -1])
+def test_infinite_keys(ctx, heads, count, sign):
+    """A key that is infinite (what is stored of 65520 or more is) has a score of -inf for queries of the other sign: a
+    weight of 0, and the row is what its other slots make it. Cached ones, and the step's own, which its earlier rows do not
+    attend to; one whose value is infinite too, for 0 times that is NaN."""
+    side = Side(ctx, heads, 16, [90, 40, 33], [count] * 3, 61)
+    side.plan()
+    ref_k = np.full(side.hd, np.float32(0.5))
+    ref_k[3] = sign * np.inf
+    ref.put(side.k, 0, side.tables[0, 1], 0, 1, ref_k, False)
+    ref.put(side.k, 0, side.tables[1, 0], 0, 11, ref_k, False)
+    for slot, dim, x in ((11, 2, np.inf), (12, 6, -np.inf)):
+        v = np.ones(side.hd, np.float32)
+        v[dim] = x
+        ref.put(side.v, 0, side.tables[1, 0], 0, slot, v, True)
+    side.send()
+    side.plan()
+    k, v = (rows_of(side.rng, side.max_rows, side.kv_heads, side.hd) for _ in range(2))
+    k[-1, -1, 3] = sign * 70000                                     # of the third request's last row
+    side.store(0, k, v)
+    assert np.isinf(side.k[0, side.tables[2, (33 + count - 1) // 16]]).any()
+    q = mixed_signs(side.queries(), 3, sign)
+    want = by_formula(side, q)
+    assert np.isfinite(want[0, 0]).all(-1).any() and np.isnan(want).any()
+    got, _ = side.attend(q)
+    check(got, want)
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 128), (32, 2, 64), (8, 1, 256)])
+def test_infinite_keys_of_divided_requests(ctx, heads):
+    """Among parts that have none, and a part of which every slot has one."""
+    side = Side(ctx, heads, 32, [3000, 2500, 0], [1] * 3, 62, width=100)
+    side.plan()
+    side.store()
+    for i, slots in ((0, list(range(300)) + [2999]), (1, [1700])):
+        for s in slots:
+            for h in range(side.kv_heads):
+                x = rows_of(side.rng, side.hd)
+                x[9] = -np.inf
+                ref.put(side.k, 0, side.tables[i, s // 32], h, s % 32, x, False)
+    x = rows_of(side.rng, side.hd)
+    x[9] = -np.inf
+    ref.put(side.k, 0, side.tables[2, 0], 0, 0, x, False)           # all that a request has: -inf less -inf is NaN
+    side.send()
+    q = mixed_signs(side.queries(), 9, -1)
+    want = by_formula(side, q)
+    assert np.isfinite(want[:2]).all(-1).sum() > 5 and np.isnan(want[2, 0]).all()
+    check(side.attend(q)[0], want)
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 128), (32, 2, 64), (24, 1, 256)])
+def test_infinite_keys_of_selected_pages(ctx, heads):
+    side = Side(ctx, heads, 16, [1500, 200], [1, 1], 63, width=120)
+    side.plan()
+    side.store()
+    for i, s in ((0, 37), (0, 1490), (1, 60)):
+        x = rows_of(side.rng, side.hd)
+        x[9] = np.inf
+        ref.put(side.k, 0, side.tables[i, s // 16], 0, s % 16, x, False)
+    side.send()
+    lists = np.full((2, side.kv_heads, 90), NONE, np.uint32)
+    lists[0], lists[1, :, :6] = np.arange(2, 92), [3, 0, 9, 2, 1, 12]
+    lists[0, :, -1] = 1490 // 16
+    q = mixed_signs(side.queries(), 9, 1)
+    want = by_formula(side, q, pages=lists)
+    assert np.isfinite(want[:, 0]).all(-1).any() and np.isnan(want).any()
+    check(side.attend(q, 0, ctx.array(lists), 90)[0], want)

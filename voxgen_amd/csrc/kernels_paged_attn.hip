@@ -88,6 +88,10 @@ __device__ __forceinline__ Tile uniform(Tile t) {
     return t;
 }
 
+// log2(e) / sqrt(HD): weights are powers of two.
+template <int HD>
+constexpr float kScale = kLog2e / (HD == 64 ? 8.0f : HD == 128 ? 11.3137085f : 16.0f);
+
 // Sixteen query rows as the B operand: lane (i, q) holds row i, dimensions 32 u + 8 q + 0..7 in
 // step u; split() makes two f16 terms of the row, with log2(e) / sqrt(HD) in it and scaled, and
 // returns the scale that is left to the scores. It is a power of two: products with it are exact,
@@ -110,7 +114,7 @@ struct QRow {
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[u][i]));
-        constexpr float c = kLog2e / (HD == 64 ? 8.0f : HD == 128 ? 11.3137085f : 16.0f);
+        constexpr float c = kScale<HD>;
         const int e = scale_of(row_max(top) * c);
         const float up = ldexpf(c, 10 - e);
 #pragma unroll
@@ -166,6 +170,167 @@ __device__ __forceinline__ U4 halves_below(uint32_t n) {
 __device__ __forceinline__ bool finite(_Float16 x) {
     return (__builtin_bit_cast(uint16_t, x) & 0x7c00u) != 0x7c00u;
 }
+__device__ __forceinline__ bool infinite(_Float16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7fffu) == 0x7c00u; }
+
+// Over the 16 lanes of a row of lanes, in each of them (row_ror 8, 4, 2, 1).
+__device__ __forceinline__ float max16(float v) {
+    v = fmaxf(v, dpp<0x128>(v));
+    v = fmaxf(v, dpp<0x124>(v));
+    v = fmaxf(v, dpp<0x122>(v));
+    return fmaxf(v, dpp<0x121>(v));
+}
+__device__ __forceinline__ float sum16(float v) {
+    v += dpp<0x128>(v);
+    v += dpp<0x124>(v);
+    v += dpp<0x122>(v);
+    return v + dpp<0x121>(v);
+}
+
+// A kernel's arguments once more, from where they lie: the compiler need not keep them in registers for a rare path, nor
+// from one turn of its loops to the next.
+typedef decltype(__builtin_amdgcn_kernarg_segment_ptr()) Arguments;
+__device__ __forceinline__ const AttnArgs &again(Arguments args) {
+    asm("" : "+s"(args));
+    return *(const AttnArgs *)args;
+}
+
+// The first position of unit h of chunk c of a tile's part, and where it lies in the caches (bytes); kFar where there is
+// no such unit, or no slot that some row of the tile attends to. Uniform.
+template <Mode MODE>
+__device__ __forceinline__ uint32_t unit_at(Arguments args, const Tile &t, uint32_t head, uint32_t last_pos, uint32_t c,
+                                            uint32_t h, size_t unit_bytes, size_t *at) {
+    const AttnArgs &p = again(args);
+    const uint32_t first = (t.first + c) * 32u + kPagedUnit * h, mask = (1u << p.shift) - 1u;
+    uint32_t index = first >> p.shift;
+    if constexpr (MODE == kSelected) {
+        const uint32_t own = t.base >> p.shift;
+        if (index >= min(p.budget, own + 1u)) return kFar;
+        index = p.lists[((size_t)t.row * gridDim.y + head) * p.budget + index];
+        if (index > own) return kFar;
+    }
+    if (index >= p.table_width) return kFar;
+    const uint32_t pos = (index << p.shift) + (first & mask), page = p.tables[(size_t)t.request * p.table_width + index];
+    if (page >= p.pages || pos > last_pos) return kFar;
+    *at = (size_t)((page * gridDim.y + head) * ((mask + 1u) / kPagedUnit) + (first & mask) / kPagedUnit) * unit_bytes;
+    return pos;
+}
+
+// The rare path of a part in whose keys there are infinities. Times the two terms of a query these are infinities of
+// both signs, or NaN, where the key's product with the query is one infinity: -inf, say, whose slot has a weight of 0. So the
+// tile's rows are made by the formula in f32, as IEEE arithmetic has it: a wave takes some rows through 16 slots at a time,
+// without matrix products (2000 tokens at 6000, one infinite key: 6.3 ms in place of 0.25; one token over 1000: 0.14). False,
+// and nothing is done, where K has none. Its arguments and a lane's numbers are made anew, so that what comes before has the
+// registers and the time that it has without it.
+template <int HD, int RT, int W, Mode MODE>
+__device__ __forceinline__ bool by_formula(uint32_t *endless) {
+    constexpr int U = HD / 32, D = HD / 64;   // D dimensions of a lane: lane + 64 d
+    constexpr size_t UNIT = 32 * HD;
+    uint32_t tid = threadIdx.x;
+    asm("" : "+v"(tid));   // nor are a lane's numbers kept
+    const uint32_t lane = tid & 63u, i = lane & 15u, q = lane >> 4, head = blockIdx.y, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Arguments args = __builtin_amdgcn_kernarg_segment_ptr();
+    const Tile t = uniform(tile_of<MODE>(again(args)));
+    const uint32_t rows = t.count * again(args).group, last_pos = t.base + token_of(again(args), min(t.tile + RT, rows) - 1u);
+    size_t at = 0;
+    for (uint32_t c = w; c < 2u * t.n; c += W) {
+        const uint32_t pos = unit_at<MODE>(args, t, head, last_pos, c / 2u, c & 1u, UNIT, &at);
+        if (pos == kFar) continue;
+        uint32_t some = 0;
+        for (uint32_t e = lane; e < 2u * HD; e += 64u) {   // eighths [head_dim / 8][slot]
+            const h8 x = *reinterpret_cast<const h8 *>(again(args).kc + at + e * 16u);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) some |= infinite(x[k]) && pos + e % 16u <= last_pos;
+        }
+        if (some) *endless = 1u;
+    }
+    __syncthreads();
+    if (*endless == 0u) return false;
+    constexpr int N = HD < 256 ? RT / W : 2;   // rows of a wave at once, as many as registers hold: r + W n
+    for (uint32_t r = w; r < (uint32_t)RT && t.tile + r < rows; r += W * N) {
+        float top[N], sum[N], o[N][D];
+        bool any[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            top[n] = -INFINITY, sum[n] = 0.f, any[n] = false;
+#pragma unroll
+            for (int d = 0; d < D; ++d) o[n][d] = 0.f;
+        }
+        for (uint32_t c = 0; c < 2u * t.n; ++c) {
+            const uint32_t pos = unit_at<MODE>(args, t, head, last_pos, c / 2u, c & 1u, UNIT, &at);
+            if (pos == kFar) continue;
+            const AttnArgs &p = again(args);
+            h8 k[U], x[2][D];
+#pragma unroll
+            for (int u = 0; u < U; ++u) k[u] = *reinterpret_cast<const h8 *>(p.kc + at + (4u * u + q) * 256u + i * 16u);
+            bool wild = false;                    // some value is not finite
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int d = 0; d < D; ++d) {
+                    x[h][d] = *reinterpret_cast<const h8 *>(p.vc + at + (h * HD + lane + 64u * d) * 16u);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) wild = wild || !finite(x[h][d][e]);
+                }
+            wild = __any(wild);
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const uint32_t row = t.tile + r + W * n, token = token_of(p, row), last = t.base + token;
+                if (row >= rows || pos > last) continue;
+                any[n] = true;
+                const float *const src = p.q + (size_t)(t.row + token) * p.q_stride + (size_t)(head * p.group + row - token * p.group) * HD + 8u * q;
+                float s = 0.f;                    // of slot i
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s = __builtin_fmaf((float)k[u][e], src[32 * u + e], s);
+                s = row_sum(s) * kScale<HD>;
+                const bool sees = pos + i <= last;
+                const float most = fmaxf(top[n], max16(sees ? s : -INFINITY)), ref = most == -INFINITY ? 0.f : most;
+                const float alpha = most == top[n] ? 1.f : __builtin_amdgcn_exp2f(top[n] - most);
+                const float weight = sees ? __builtin_amdgcn_exp2f(s - ref) : 0.f;
+                auto of = [&](uint32_t e) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(uint32_t, weight), e)); };
+                top[n] = most;
+                sum[n] = sum[n] * alpha + sum16(weight);
+#pragma unroll
+                for (int d = 0; d < D; ++d) o[n][d] = __builtin_isfinite(o[n][d]) ? o[n][d] * alpha : o[n][d];
+                if (!wild) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+#pragma unroll
+                        for (int d = 0; d < D; ++d) o[n][d] = __builtin_fmaf(of(e), (float)x[e / 8][d][e % 8], o[n][d]);
+                    continue;
+                }
+                const uint32_t seen = (uint32_t)__ballot(sees), none = (uint32_t)__ballot(s == -INFINITY);
+#pragma unroll 1
+                for (uint32_t e = 0; e < 16u; ++e) {
+                    if (!(seen >> e & 1u)) continue;
+#pragma unroll
+                    for (int d = 0; d < D; ++d) {   // an infinity is itself by any weight but that of -inf, the one that is 0
+                        const _Float16 v = reinterpret_cast<const _Float16 *>(p.vc + at)[(e / 8u * HD + lane + 64u * d) * 8u + e % 8u];
+                        o[n][d] += finite(v) || (none >> e & 1u) ? of(e) * (float)v : (float)v;
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const AttnArgs &p = again(args);
+            const uint32_t row = t.tile + r + W * n, token = token_of(p, row);
+            if (row >= rows) continue;
+            if (t.part == VX_PAGED_NONE) {
+                float *const to = p.out + (size_t)(t.row + token) * p.out_stride + (size_t)(head * p.group + row - token * p.group) * HD + lane;
+#pragma unroll
+                for (int d = 0; d < D; ++d) to[64 * d] = any[n] ? o[n][d] * (1.0f / sum[n]) : 0.f;
+            } else {
+                const size_t record = ((size_t)head * p.parts + t.part) * RT + r + W * n;
+#pragma unroll
+                for (int d = 0; d < D; ++d) p.acc[record * HD + lane + 64u * d] = o[n][d];
+                if (lane == 0) p.ml[record * 2u] = top[n], p.ml[record * 2u + 1u] = any[n] ? sum[n] : -1.f;
+            }
+        }
+    }
+    return true;
+}
 
 // One workgroup: a tile of 16 NT query rows (tokens x the KV head's query heads) of a request over
 // a part of its chunks, which the waves take in turn, each with its own running maximum and sum;
@@ -188,7 +353,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     static_assert((!PK || NT == 1) && (W == 4 || W == 8), "one column tile of both terms; a wave or two a SIMD");
     __shared__ float ms[W][R], ls[W][R], fs[R];
     // by dimension the first position of a +inf or NaN in V, and of a -inf or NaN
-    __shared__ uint32_t odd[2][HD], odd_in[W];
+    __shared__ uint32_t odd[2][HD], odd_in[W], endless;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, i = lane & 15u, q = lane >> 4;
     const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t heads = gridDim.y, head = blockIdx.y;
@@ -261,6 +426,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     }
 
     for (uint32_t d = tid; d < 2u * HD; d += 64u * W) odd[d / HD][d % HD] = ~0u;
+    if (tid == 0) endless = 0u;
     uint32_t found = 0;
     // The two terms of the queries, in registers where these do; the tiles of 32 rows get them through LDS, which the other
     // heads' read again each chunk (heads of 128: 919 tokens 60.3 us, read each time 62.4; 2000 at 6000 267 and 288;
@@ -446,7 +612,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
         if (!whole && row_max(saw[c] ? 1.f : 0.f) == 0.f) l[c] = -1.f;   // nothing to add
         if (q == 0) ms[w][16 * c + i] = m[c], ls[w][16 * c + i] = l[c];
     }
-    // Infinities in V have no two terms to be multiplied by, and some were taken as zero: where a sum
+    // Infinities in K and V have no two terms to be multiplied by, and some of V were taken as zero: where a sum
     // is not finite or such a value was found, the chunks are gone through again (rare).
     float zero = found ? __builtin_nanf("") : 0.f;
 #pragma unroll
@@ -462,6 +628,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
 #pragma unroll
     for (int v = 0; v < W; ++v) any_odd = any_odd || odd_in[v] != 0;
     if (__builtin_expect(any_odd, 0)) {
+        if (by_formula<HD, RT, W, MODE>(&endless)) return;
         for (uint32_t j = 0; j < mine; ++j) {
             if ((j & 31u) == 0) {
                 look_up(j, std::false_type{});
