@@ -133,3 +133,30 @@ def test_infinite_keys_of_selected_pages(ctx, heads):
     want = by_formula(side, q, pages=lists)
     assert np.isfinite(want[:, 0]).all(-1).any() and np.isnan(want).any()
     check(side.attend(q, 0, ctx.array(lists), 90)[0], want)
+
+
+# ------------------------------------------------------------ infinite values in parts that hardly count
+@pytest.mark.parametrize("selected", [False, True])
+def test_infinite_values_in_parts_of_little_weight(ctx, selected):
+    """An infinite value reaches the rows that attend to it, whatever its weight, if all its part's are far below the
+    others': 300 less in the exponent here, which 64 bits hold and 32 do not."""
+    side = Side(ctx, (8, 1, 128), 32, [3000], [1], 64, width=100)
+    side.plan()
+    u = np.where(side.rng.random(128) < 0.5, -1, 1).astype(np.float32)
+    for s in range(3000):
+        x = u * (3 if s >= 1500 else -3) + 0.01 * side.rng.standard_normal(128).astype(np.float32)
+        ref.put(side.k, 0, side.tables[0, s // 32], 0, s % 32, x, False)
+    v = np.ones(128, np.float32)
+    v[[4, 5]] = np.inf, -np.inf
+    ref.put(side.v, 0, side.tables[0, 1], 0, 7, v, True)
+    side.send()
+    side.plan()
+    side.store(0, u[None, None] * 3, rows_of(side.rng, 1, 1, 128))
+    q = (np.ones((1, 1, 8, 128), np.float32) * u * 4.4).astype(np.float32)
+    if selected:
+        lists = np.arange(94, dtype=np.uint32).reshape(1, 1, 94)
+        got, want = side.attend(q, 0, ctx.array(lists), 94)[0], by_formula(side, q, pages=lists)
+    else:
+        got, want = side.attend(q)[0], by_formula(side, q)
+    assert np.isinf(want).sum() == 16 and not np.isnan(want).any()
+    check(got, want)

@@ -775,7 +775,9 @@ __global__ __launch_bounds__(256) void k_paged_join(AttnArgs p, uint32_t most, u
         __syncthreads();
         top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
         some = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
-        const float mine = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+        // Not 0, which an infinite sum times would be NaN: a part's sums are below 2^59 (2^28 slots of weights up to 2^15 and
+        // values below 2^16), so that with 2^-126 they are below 2^-67 where the row's own weights reach 1 and more.
+        const float part = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top), mine = part == 0.f ? 0x1p-126f : part;
         if (tid < n) sc[tid] = mine;
         float sum = l < 0.f ? 0.f : l * mine;
 #pragma unroll
