@@ -692,7 +692,8 @@ typedef struct vx_paged_attention_push {
 uint64_t vx_paged_attention_scratch_bytes(const vx_paged_attention_push *pc);
 /* out = softmax(q . K / sqrt(head_dim)) . V over the positions each row attends to, in f32
  * (products on the matrix cores, q and the weights as two f16 terms each, sums in f32).
- * Rows that take no part are left as they were. With selected (nullable; u32
+ * Rows that take no part are left as they were. Pages are those that the tables have at the time of the call (of
+ * entries that changed since the plan it takes some 20 times as long). With selected (nullable; u32
  * [max_rows][kv_heads][budget]) a row attends to those positions only that lie in the
  * pages of its list: indices into the request's table, each once; of the first
  * min(budget, position / page_size + 1) entries those that are such pages count, and a

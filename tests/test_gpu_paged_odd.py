@@ -160,3 +160,47 @@ def test_infinite_values_in_parts_of_little_weight(ctx, selected):
         got, want = side.attend(q)[0], by_formula(side, q)
     assert np.isinf(want).sum() == 16 and not np.isnan(want).any()
     check(got, want)
+
+
+# ------------------------------------------------------------ tables that change behind a plan
+def edit(side, tables, i, gone, swapped):
+    """Entries of request i that are no page, and two whose pages change places."""
+    tables[i, gone] = [side.pages, 0xFFFFFFFE, NONE][:len(gone)]
+    tables[i, swapped] = tables[i, swapped[::-1]]
+
+
+@pytest.mark.parametrize("heads,count", TILES)
+@pytest.mark.parametrize("before", [True, False])
+def test_tables_of_the_call(ctx, heads, count, before):
+    """Pages are those of the tables at the time of the attention, whether the plan was made of the same or not: the first
+    ones of a part, those further on, and a request without any."""
+    side = Side(ctx, heads, 16, [1400, 150, 20], [count] * 3, 65, max_rows=3 * count + 1, width=95)
+    side.plan()
+    side.store()
+    tables = side.tables.copy()
+    edit(side, tables, 0, [0, 3, 70], [1, 80])
+    edit(side, tables, 1, [2], [4, 5])
+    tables[2, :] = NONE
+    side.dev.tables.upload(tables)
+    if before:
+        side.dev.plan()
+    q = side.queries()
+    want = by_formula(side, q, tables=tables)
+    got, old = side.attend(q)
+    assert not want[2 * count:3 * count].any()
+    assert np.array_equal(got[3 * count:], old[3 * count:])
+    check(got[:3 * count], want[:3 * count])
+
+
+@pytest.mark.parametrize("heads", [(8, 4, 64), (16, 1, 128), (4, 1, 256)])
+def test_tables_of_the_call_in_divided_requests(ctx, heads):
+    side = Side(ctx, heads, 32, [6000, 2100], [1, 1], 66, width=200)
+    side.plan()
+    side.store()
+    tables = side.tables.copy()
+    edit(side, tables, 0, [0, 8, 101], [7, 150])
+    edit(side, tables, 1, list(range(3)), [40, 60])
+    tables[1, 8:16] = NONE                                          # a part's whole
+    side.dev.tables.upload(tables)
+    q = side.queries()
+    check(side.attend(q)[0], by_formula(side, q, tables=tables))

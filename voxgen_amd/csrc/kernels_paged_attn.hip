@@ -218,11 +218,11 @@ __device__ __forceinline__ uint32_t unit_at(Arguments args, const Tile &t, uint3
 // The rare path of a part in whose keys there are infinities. Times the two terms of a query these are infinities of
 // both signs, or NaN, where the key's product with the query is one infinity: -inf, say, whose slot has a weight of 0. So the
 // tile's rows are made by the formula in f32, as IEEE arithmetic has it: a wave takes some rows through 16 slots at a time,
-// without matrix products (2000 tokens at 6000, one infinite key: 6.3 ms in place of 0.25; one token over 1000: 0.14). False,
-// and nothing is done, where K has none. Its arguments and a lane's numbers are made anew, so that what comes before has the
-// registers and the time that it has without it.
+// without matrix products (2000 tokens at 6000, one infinite key: 6.3 ms in place of 0.25; one token over 1000: 0.14). And of a
+// part whose pages are not those that the plan has listed (`must`). False, and nothing is done, where there is no need. Its
+// arguments and a lane's numbers are made anew, so that what comes before has the registers and the time that it has without it.
 template <int HD, int RT, int W, Mode MODE>
-__device__ __forceinline__ bool by_formula(uint32_t *endless) {
+__device__ __forceinline__ bool by_formula(bool must, uint32_t *endless) {
     constexpr int U = HD / 32, D = HD / 64;   // D dimensions of a lane: lane + 64 d
     constexpr size_t UNIT = 32 * HD;
     uint32_t tid = threadIdx.x;
@@ -232,7 +232,7 @@ __device__ __forceinline__ bool by_formula(uint32_t *endless) {
     const Tile t = uniform(tile_of<MODE>(again(args)));
     const uint32_t rows = t.count * again(args).group, last_pos = t.base + token_of(again(args), min(t.tile + RT, rows) - 1u);
     size_t at = 0;
-    for (uint32_t c = w; c < 2u * t.n; c += W) {
+    for (uint32_t c = w; c < 2u * t.n && !must; c += W) {
         const uint32_t pos = unit_at<MODE>(args, t, head, last_pos, c / 2u, c & 1u, UNIT, &at);
         if (pos == kFar) continue;
         uint32_t some = 0;
@@ -244,7 +244,7 @@ __device__ __forceinline__ bool by_formula(uint32_t *endless) {
         if (some) *endless = 1u;
     }
     __syncthreads();
-    if (*endless == 0u) return false;
+    if (!must && *endless == 0u) return false;
     constexpr int N = HD < 256 ? RT / W : 2;   // rows of a wave at once, as many as registers hold: r + W n
     for (uint32_t r = w; r < (uint32_t)RT && t.tile + r < rows; r += W * N) {
         float top[N], sum[N], o[N][D];
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     const uint32_t heads = gridDim.y, head = blockIdx.y;
     // What the first chunks' pages are is asked for together with what the tile is: the plan's list of the
     // item's pages, or the row's list of a selection.
-    constexpr bool ONCE = MODE == kOnce;
+    constexpr bool ONCE = MODE == kOnce, LISTED = NT == 1 && MODE != kSelected;
     uint32_t early = VX_PAGED_NONE;
     if constexpr (NT == 1) {
         const uint32_t k = 2u * (w + W * (lane / 2u)) + (lane & 1u);   // unit of the part
@@ -380,7 +380,10 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
 
     // The wave's chunks t.first + w + W j: lane 2 (j - start) + h holds unit h of the j-th, up to 32 chunks
     // at once, in the first place as many as `early` has.
-    uint32_t unit = 0, where = kFar, start = 0;
+    // The table has the last word on pages: what it says of those that the plan has listed is asked for with the first
+    // chunk, and compared with the list at the end.
+    uint32_t unit = 0, where = kFar, start = 0, tabled = 0;
+    uint64_t pages_in = 0;   // lanes with a unit that some row attends to
     uint32_t stop = NT > 1 || MODE == kSelected ? 32u : kPagedListed / 2u / W;
     const uint32_t mask = (1u << p.shift) - 1u, units = (mask + 1u) / kPagedUnit;
     auto look_up = [&](uint32_t j0, auto is_early) {
@@ -399,9 +402,8 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
         there = there && index < p.table_width;
         const uint32_t off = at & mask, pos = (index << p.shift) + off;
         there = there && pos <= last_pos;
-        uint32_t page = early;
-        if constexpr (MODE == kSelected || !first)
-            page = p.tables[(size_t)t.request * p.table_width + (there ? index : 0u)];
+        uint32_t page = p.tables[(size_t)t.request * p.table_width + (there ? index : 0u)];
+        if constexpr (first && MODE != kSelected) tabled = page, pages_in = __ballot(there), page = early;
         there = there && page < p.pages;
         unit = there ? (page * heads + head) * units + off / kPagedUnit : 0u;
         where = there ? pos : kFar;
@@ -418,7 +420,9 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
     const uint32_t mine = t.n > w ? (t.n - w + W - 1u) / W : 0u;   // the wave's chunks
     KFrag<HD> kf;
     VFrag<HD> vf;
-    // K and V of a chunk are fetched when the one ahead is done with them, where registers allow.
+    // K and V of a chunk are fetched when the one ahead is done with them; not of tiles of 32 rows: heads of 128 and 256
+    // have no registers for it, and heads of 64 take 138, with which a CU has one workgroup and not two (2000 tokens at 6000
+    // 158 us in place of 128, but 5 drafted tokens of 64 requests 60 in place of 73).
     constexpr bool AHEAD = NT == 1;
     if constexpr (AHEAD) {   // a wave without chunks fetches unit 0: a branch here would have the queries wait for what is in it
         kf.template load<ONCE>(kc + unit_of(0, i >= 8u), i, q);
@@ -621,14 +625,15 @@ __global__ __launch_bounds__(64 * W, NT > 1 || HD > 128 ? 1 : 2) void k_paged_at
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) zero = __builtin_fmaf(o[c][dt][e], 0.f, zero);
-    const bool finite_here = __all(zero == 0.f);
-    if (lane == 0) odd_in[w] = !finite_here;
+    const bool finite_here = __all(zero == 0.f), as_listed = !LISTED || (__ballot(tabled != early) & pages_in & ((1ull << kPagedListed / W) - 1ull)) == 0u;
+    if (lane == 0) odd_in[w] = (finite_here ? 0u : 1u) | (as_listed ? 0u : 2u);
     __syncthreads();   // the queries in LDS have been read, every wave's m and l are there
-    bool any_odd = false;
+    uint32_t odds = 0;
 #pragma unroll
-    for (int v = 0; v < W; ++v) any_odd = any_odd || odd_in[v] != 0;
+    for (int v = 0; v < W; ++v) odds |= odd_in[v];
+    const bool any_odd = odds != 0u;
     if (__builtin_expect(any_odd, 0)) {
-        if (by_formula<HD, RT, W, MODE>(&endless)) return;
+        if (by_formula<HD, RT, W, MODE>(odds & 2u, &endless)) return;
         for (uint32_t j = 0; j < mine; ++j) {
             if ((j & 31u) == 0) {
                 look_up(j, std::false_type{});

@@ -11,7 +11,8 @@ constexpr uint32_t kPagedMaxTokens = 1u << 28;   // positions of a request
 constexpr uint32_t kPagedMaxRowHeads = 1u << 22; // rows of a step times query heads: bounds every grid
 constexpr uint32_t kPagedUnit = 16;              // slots of a unit: 32 * head_dim bytes of K, and of V
 constexpr uint32_t kPagedMaxSplits = 256;        // of a tile of query rows
-constexpr uint32_t kPagedListed = 64;            // units of an item whose pages the plan lists, for tiles of 16 rows or fewer
+constexpr uint32_t kPagedListed = 64;            // units of an item whose pages the plan lists, for tiles of 16 rows or fewer:
+                                                 // the attention need not wait for the table, which has the last word
 
 // Chunks that are not divided: a CU takes 0.117 us for one (16 KB of heads of 128, 64 bytes a clock), the
 // launch that joins parts 4 (one token: 47 chunks whole 9.9 us, 63 divided 6.0 and 4.1).
