@@ -72,9 +72,7 @@ __device__ __forceinline__ Tile tile_of(const AttnArgs &p) {
     } else {
         const PagedItem it = p.items[index];
         t = {it.request, it.row, it.base, it.count, it.tile, it.first, it.n, it.part, false};
-        t.ok = index < p.header[5] && it.request < p.requests && it.row < p.max_rows && it.count <= p.max_rows - it.row &&
-               it.base <= cap && it.count <= cap - it.base && it.tile < it.count * p.group &&
-               (it.part < p.parts || it.part == VX_PAGED_NONE) && it.first <= cap && it.n <= cap;
+        t.ok = index < p.header[5] && paged_is_item(it, p.requests, p.max_rows, p.group, cap, p.parts);
     }
     return t;
 }

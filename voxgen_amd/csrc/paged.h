@@ -45,6 +45,16 @@ struct PagedItem {
     uint32_t request, row, base, count;   // the request, its first row, tokens cached before it, its rows
     uint32_t tile, first, n, part;        // the tile's first query row; where its partial sums go (VX_PAGED_NONE: none)
 };
+// Whether an item is one: its rows are rows of the step, their positions (below cap) within the table, its chunks such as
+// they attend to, its part one of `parts`. What else a plan's buffer may hold is no work, however long, and reaches nothing.
+__host__ __device__ inline bool paged_is_item(const PagedItem &it, uint32_t requests, uint32_t max_rows, uint32_t group, uint32_t cap,
+                                              uint32_t parts) {
+    if (it.request >= requests || it.row >= max_rows || it.count > max_rows - it.row || it.base > cap || it.count > cap - it.base ||
+        it.tile >= it.count * group || (it.part >= parts && it.part != VX_PAGED_NONE))
+        return false;
+    const uint32_t chunks = (it.base + it.count + 31u) / 32u;
+    return it.first <= chunks && it.n <= chunks - it.first;
+}
 // A tile whose keys are divided: partial sums first_part.. + parts.
 struct PagedJoin {
     uint32_t row, base, count, tile, part, per, unused[2];   // per: chunks of a part
