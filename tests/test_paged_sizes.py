@@ -70,3 +70,75 @@ int main() {
         }
 }
 """)
+
+
+def test_lists_and_scratch_hold_what_the_plan_makes(run):
+    """The plan's lists and the attention's parts, sized by a batch, hold what the kernel's division makes of any step of it,
+    with any of its requests refused for want of pages. For parts of tiles of every size, tables that are divided and that
+    are not, and steps of which nothing is spare."""
+    run("plans", """
+int main() {
+    std::mt19937_64 rng(2);
+    auto pick = [&](uint64_t lo, uint64_t hi) { return (uint32_t)(lo + rng() % (hi - lo + 1)); };
+    auto log = [&](uint32_t lo, uint32_t hi) { return (uint32_t)std::exp(std::log(lo) + (std::log(hi + 0.99) - std::log(lo)) * (rng() % 10000) / 10000.0); };
+    uint64_t full[4] = {}, kinds[6] = {};
+    for (int n = 0; n < 20000; ++n) {
+        const uint32_t heads[] = {1, 2, 3, 8, 32}, dims[] = {64, 128, 256};
+        vx_paged_batch b{};
+        b.geom = {1, 1u << 20, 16u << pick(0, 4), heads[rng() % 5], dims[rng() % 3]};
+        b.requests = log(1, 300);
+        b.table_width = std::max(1u, log(1, 100000) / b.geom.page_size);
+        b.max_rows = log(1, 2000);
+        b.max_count = rng() % 2 ? 1u : std::min(b.max_rows, log(1, 500));
+        b.q_heads = b.geom.kv_heads * log(1, 40);
+        if (!vx_paged_plan_bytes(&b)) continue;
+        const PagedShape s = paged_shape(b);
+        const uint32_t group = b.q_heads / b.geom.kv_heads, ps = b.geom.page_size, cap = b.table_width * ps;
+        kinds[s.tile_rows == 8 ? 0 : s.tile_rows == 16 ? 1 : s.waves == 8 ? 2 : 3]++;
+        kinds[s.joins ? 4 : 5]++;
+        for (int step = 0; step < 20; ++step) {
+            // lengths: any, all alike, one long, all full, about some multiple of a part
+            const int kind = rng() % 5;
+            const uint32_t alike = pick(0, cap - 1);
+            std::vector<uint32_t> length, count;
+            uint32_t rows = 0;
+            float work = 0.f;
+            for (uint32_t i = 0; i < b.requests; ++i) {
+                uint32_t c = rng() % 8 == 0 ? 0u : kind == 3 || rng() % 2 ? b.max_count : pick(1, b.max_count);
+                c = std::min(std::min(c, b.max_rows - rows), cap);
+                rows += c;
+                const uint32_t most = cap - c;
+                const uint32_t l = kind == 0 ? pick(0, most) : kind == 1 ? alike : kind == 2 ? (i == 0 ? most : pick(0, 40)) : kind == 3 ? most
+                                   : pick(1, 4) * 32u * s.least + pick(0, 64);
+                length.push_back(std::min(l, most));
+                count.push_back(c);
+                if (c) work += (float)((c * group + s.tile_rows - 1) / s.tile_rows) * (float)((length.back() + c + 31) / 32);
+            }
+            const uint32_t per = paged_per(s, b.geom.kv_heads, work);
+            const bool refuse = rng() % 4 == 0;
+            uint64_t runs = 0, items = 0, joins = 0, parts = 0;
+            for (uint32_t i = 0; i < b.requests; ++i) {
+                const uint32_t c = count[i], l = length[i];
+                if (c == 0 || (refuse && rng() % 3 == 0)) continue;
+                uint32_t splits;
+                const uint32_t chunks = (l + c + 31) / 32, by = paged_divide(s, per, chunks, splits), tiles = (c * group + s.tile_rows - 1) / s.tile_rows;
+                CHECK(splits >= 1 && splits <= kPagedMaxSplits && (uint64_t)by * splits >= chunks && (uint64_t)by * (splits - 1) < chunks);
+                CHECK(splits == 1 || by % s.waves == 0);
+                runs += (l + c - 1) / ps - l / ps + 1;
+                items += (uint64_t)tiles * splits;
+                joins += splits > 1 ? tiles : 0;
+                parts += splits > 1 ? (uint64_t)tiles * splits : 0;
+            }
+            CHECK(runs <= s.runs && items <= s.items && joins <= s.joins && parts <= s.parts);
+            full[0] += runs * 10 > s.runs * 9ull, full[1] += items * 2 > s.items, full[2] += s.joins && joins * 2 > s.joins;
+            full[3] += s.parts && parts * 3 > s.parts;
+            // what the attention allocates for the parts
+            vx_paged_attention_push pc{};
+            pc.batch = b;
+            CHECK(vx_paged_attention_scratch_bytes(&pc) >= parts * b.geom.kv_heads * s.tile_rows * (b.geom.head_dim + 2) * 4);
+        }
+    }
+    for (uint64_t x : full) CHECK(x > 100);      // sizes are not far above what is needed
+    for (uint64_t x : kinds) CHECK(x > 100);
+}
+""")

@@ -78,8 +78,7 @@ __global__ __launch_bounds__(T) void k_paged_plan(PagedPlan a) {
     const uint32_t tid = threadIdx.x, n = a.b.requests, r0 = tid * E;
     const uint32_t pages = a.b.geom.pages, shift = 31u - __clz(a.b.geom.page_size), ps = a.b.geom.page_size;
     const uint32_t width = a.b.table_width, cap = width << shift, rows = a.b.max_rows;
-    const uint32_t group = a.b.q_heads / a.b.geom.kv_heads, heads = a.b.geom.kv_heads;
-    const uint32_t tile_shift = 31u - __clz(a.s.tile_rows), wave_shift = 31u - __clz(a.s.waves);
+    const uint32_t group = a.b.q_heads / a.b.geom.kv_heads, tile_shift = 31u - __clz(a.s.tile_rows);
     const uint32_t free = min(a.pool[0], pages);
     uint32_t len[E], count[E], need[E], v[1] = {0}, before[1], all[1];
     bool takes[E];
@@ -96,8 +95,7 @@ __global__ __launch_bounds__(T) void k_paged_plan(PagedPlan a) {
     }
     scan<1, T>(v, before, all, rows + 1u, reinterpret_cast<uint32_t (*)[1]>(between));
     const uint32_t all_rows = min(all[0], rows);
-    // What the attention has to do, chunks of 32 keys by tiles of query rows, of requests that may take
-    // part; rounded up enough for the sums' order not to matter.
+    // What the attention has to do, chunks of 32 keys by tiles of query rows, of requests that may take part.
     uint32_t at = before[0], tiles[E], chunks[E];
     float todo = 0.f;
     v[0] = 0;
@@ -119,21 +117,8 @@ __global__ __launch_bounds__(T) void k_paged_plan(PagedPlan a) {
     todo = 0.f;
 #pragma unroll
     for (uint32_t u = 0; u < T / 64u; ++u) todo += work[u];
-    todo = todo * 1.0001f * (float)heads / (float)(1u << a.s.workgroups);
-    // Of little work half the workgroups, all of which run at once, make fewer parts to join (16 requests over
-    // up to 8000: 16.6 us, with twice as many 20.2); of much twice as many end together (64 over 24000: 200, 194).
-    if (a.s.tile_rows <= 16u && todo < 16.f) todo *= 2.f;
-    // a wave's chunks are alike in number
-    const uint32_t per = max(((uint32_t)fminf(ceilf(todo), 1e9f) + a.s.waves - 1u) >> wave_shift << wave_shift, a.s.least);
-    // Chunks of a part, of which there are `splits`; a request's tiles are all divided alike.
-    // Tiles of many rows are divided where twice the share would be exceeded: what they have to join
-    // takes longer then.
-    auto divided = [&](uint32_t many, uint32_t &splits) {
-        splits = min(a.s.tile_rows > 16u ? max(many / per, 1u) : (many + per - 1u) / per, kPagedMaxSplits);
-        const uint32_t by = splits > 1u ? ((many + splits - 1u) / splits + a.s.waves - 1u) >> wave_shift << wave_shift : max(many, 1u);
-        splits = splits > 1u ? (many + by - 1u) / by : splits;
-        return by;
-    };
+    const uint32_t per = paged_per(a.s, a.b.geom.kv_heads, todo);
+    auto divided = [&](uint32_t many, uint32_t &splits) { return paged_divide(a.s, per, many, splits); };
     // runs, items, joins and parts of each request, and pages, rows and requests that take part
     uint32_t splits[E], w[6] = {0, 0, 0, 0, 0, 0}, done[6], sum[6], taking = 0;
     at = before[0];

@@ -2,6 +2,8 @@
 // descriptions shared by the C ABI checks (paged.cpp) and the kernels (kernels_paged*.hip).
 #pragma once
 
+#include <cmath>
+
 #include "vx_internal.h"
 
 namespace vx {
@@ -35,6 +37,30 @@ struct PagedShape {
     uint64_t slots, requests, positions, granted, run_at, item_at, join_at, page_at, words;
 };
 PagedShape paged_shape(const vx_paged_batch &b);
+
+// Chunks of a part in a step whose tiles have so many in all (a sum in f32, rounded up enough for its order not to matter).
+__host__ __device__ inline uint32_t paged_per(const PagedShape &s, uint32_t kv_heads, float chunks) {
+    float share = chunks * 1.0001f * (float)kv_heads / (float)(1u << s.workgroups);
+    // Of little work half the workgroups, all of which run at once, make fewer parts to join (16 requests over
+    // up to 8000: 16.6 us, with twice as many 20.2); of much twice as many end together (64 over 24000: 200, 194).
+    if (s.tile_rows <= 16u && share < 16.f) share *= 2.f;
+    // a wave's chunks are alike in number
+    const uint32_t shift = 31u - (uint32_t)__builtin_clz(s.waves), per = ((uint32_t)fminf(ceilf(share), 1e9f) + s.waves - 1u) >> shift << shift;
+    return per > s.least ? per : s.least;
+}
+// Chunks of a part of a tile that has `chunks`, and the number of its parts; a request's tiles are all divided alike.
+// Tiles of many rows are divided where twice the share would be exceeded: what they have to join
+// takes longer then.
+__host__ __device__ inline uint32_t paged_divide(const PagedShape &s, uint32_t per, uint32_t chunks, uint32_t &splits) {
+    const uint32_t shift = 31u - (uint32_t)__builtin_clz(s.waves);
+    splits = s.tile_rows > 16u ? chunks / per : (chunks + per - 1u) / per;
+    if (s.tile_rows > 16u && splits == 0u) splits = 1u;
+    if (splits > kPagedMaxSplits) splits = kPagedMaxSplits;
+    if (splits <= 1u) return chunks ? chunks : 1u;
+    const uint32_t by = ((chunks + splits - 1u) / splits + s.waves - 1u) >> shift << shift;
+    splits = (chunks + by - 1u) / by;
+    return by;
+}
 
 // Records of a plan. Rows of a request that lie in one page.
 struct PagedRun {
