@@ -1,11 +1,13 @@
 """The paged KV cache's sizes on the CPU, from the library's own arithmetic: small C++ programs over csrc/paged.h, linked
-with the library."""
+with the library, and the grids that its calls launch."""
 import subprocess
 from pathlib import Path
 
 import pytest
 
-from test_refused_memory import HIP_INCLUDE
+from test_kv4 import roomy  # noqa: F401  (fixture)
+from test_paged import CALLS
+from test_refused_memory import HIP_INCLUDE, child, fake  # noqa: F401  (fixture)
 from voxgen_amd import abi
 
 ROOT = Path(__file__).resolve().parents[1]
@@ -141,4 +143,67 @@ int main() {
     for (uint64_t x : full) CHECK(x > 100);      // sizes are not far above what is needed
     for (uint64_t x : kinds) CHECK(x > 100);
 }
+""")
+
+
+GRIDS = """
+#define __HIP_PLATFORM_AMD__ 1
+#include <hip/hip_runtime_api.h>
+static int seen, bad;
+int grids_seen(void) { return seen; }
+int grids_bad(void) { int n = bad; bad = 0; return n; }
+hipError_t hipLaunchKernel(const void *fn, dim3 g, dim3 b, void **a, size_t s, hipStream_t st) {
+    unsigned long long x = (unsigned long long)g.x * b.x;
+    ++seen;
+    bad += !g.x || !g.y || !g.z || x >= 1ull << 32 || g.y > 65535 || g.z > 65535 || b.x * b.y * b.z > 1024 || b.x % 64 || b.y * b.z != 1;
+    return hipSuccess;
+}
+"""
+
+
+def test_grids_of_every_call(roomy, tmp_path):  # noqa: F811
+    """Launch grids at the largest sizes that a batch may have, and the least: some workgroups, fewer than 2^32 threads,
+    in the other dimensions at most 65535."""
+    source, library = tmp_path / "grids.c", tmp_path / "libgrids.so"
+    source.write_text(GRIDS)
+    subprocess.run(["gcc", "-std=gnu11", "-O1", "-w", "-shared", "-fPIC", "-I", str(HIP_INCLUDE), str(source), "-Wl,--no-as-needed", str(roomy),
+                    f"-Wl,-rpath,{roomy.parent}", "-o", str(library)], check=True)
+    child(library, CALLS + """
+def one(**kw):
+    b = batch(**kw)
+    g = b.geom
+    need = lib.vx_paged_plan_bytes(b)
+    assert need, (kw, lib.vx_last_error())
+    row, wide, budget = g.kv_heads * g.head_dim, b.q_heads * g.head_dim, min(b.table_width, 200)
+    apc = attn_push(q_stride=wide, out_stride=wide, **kw)
+    spc, pick = attn_push(q_stride=wide, out_stride=wide, budget=budget, **kw), select_push(q_stride=wide, budget=budget, sinks=0, recent=1, **kw)
+    state = dict(lengths=ctx.alloc(4 * b.requests), tables=ctx.alloc(4 * b.requests * b.table_width), pool=ctx.alloc(4 * (g.pages + 1)))
+    plan, other = ctx.alloc(need), ctx.alloc(4 * b.requests)
+    caches = dict(kc=ctx.alloc(lib.vx_paged_cache_bytes(g)), vc=ctx.alloc(lib.vx_paged_cache_bytes(g)))
+    lo_hi, rows = ctx.alloc(lib.vx_paged_bounds_bytes(g)), {n: ctx.alloc(4 * b.max_rows * row) for n in "kv"}
+    qo = dict(q=ctx.alloc(4 * b.max_rows * wide), out=ctx.alloc(4 * b.max_rows * wide))
+    sel = ctx.alloc(4 * b.max_rows * g.kv_heads * budget)
+    room = lambda n: ctx.alloc(n)
+    for call in (lambda: reset(b, **state), lambda: make(b, counts=other, plan=plan, **state),
+                 lambda: advance(b, plan=plan, lengths=state["lengths"], pool=state["pool"]), lambda: cut(b, keep=other, **state),
+                 lambda: store(store_push(k_stride=row, v_stride=row, **kw), bounds=lo_hi, plan=plan, **rows, **caches),
+                 lambda: store(store_push(k_stride=row, v_stride=row, **kw), bounds=None, plan=plan, **rows, **caches),
+                 lambda: attn(apc, tables=state["tables"], plan=plan, scratch=room(lib.vx_paged_attention_scratch_bytes(apc)), **qo, **caches),
+                 lambda: attn(spc, tables=state["tables"], plan=plan, selected=sel, scratch=room(lib.vx_paged_attention_scratch_bytes(spc)), **qo, **caches),
+                 lambda: select(pick, q=qo["q"], bounds=lo_hi, tables=state["tables"], plan=plan, selected=sel,
+                                scratch=room(lib.vx_paged_select_scratch_bytes(pick)))):
+        n, got = fake.grids_seen(), call()
+        assert got == "VX_OK", (kw, got, lib.vx_last_error())
+        assert fake.grids_seen() > n and fake.grids_bad() == 0, kw
+many = dict(layers=1, head_dim=64)
+one(max_rows=1 << 22, max_count=1 << 22, q_heads=1, kv_heads=1, pages=1 << 20, table_width=1 << 18, requests=1, **many)
+one(max_rows=1 << 22, max_count=1, q_heads=1, kv_heads=1, pages=1 << 20, table_width=1 << 16, requests=4096, **many)
+one(max_rows=1 << 19, max_count=1, q_heads=8, kv_heads=8, pages=1 << 16, table_width=1 << 12, requests=4096, **many)
+one(max_rows=1 << 12, max_count=1 << 12, q_heads=1024, kv_heads=1, pages=1 << 16, table_width=1 << 12, requests=4096, **many)
+one(max_rows=240, max_count=240, q_heads=17408, kv_heads=17, pages=64, table_width=64, requests=64, **many)
+one(max_rows=64, max_count=64, q_heads=65535, kv_heads=65535, pages=64, table_width=64, requests=64, **many)
+one(max_rows=64, max_count=1, q_heads=65535, kv_heads=65535, pages=64, table_width=64, requests=64, **many)
+one(max_rows=64, max_count=1, q_heads=65535, kv_heads=65535, pages=1 << 12, table_width=1 << 18, requests=1, **many)
+one(max_rows=1, max_count=1, q_heads=1, kv_heads=1, pages=1, table_width=1, requests=1, **many)
+one(max_rows=1, max_count=1, q_heads=1024, kv_heads=1, pages=1, table_width=1 << 24, requests=1, layers=1, head_dim=256)
 """)
