@@ -6,12 +6,15 @@ Finite outputs are compared by relative 2-norm with the bound that test_gpu_page
 infinite keys is a sum of head_dim products in f32, off by sqrt(head_dim) 2^-24 of its terms' size, which is below
 what that bound has for products of two terms.
 """
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import pagedref as ref
 from conftest import rel_l2
 from test_gpu_paged import NONE, TOL, Side, rows_of
+from voxgen_amd import abi
 
 pytestmark = pytest.mark.gpu
 
@@ -204,3 +207,60 @@ def test_tables_of_the_call_in_divided_requests(ctx, heads):
     side.dev.tables.upload(tables)
     q = side.queries()
     check(side.attend(q)[0], by_formula(side, q, tables=tables))
+
+
+# ------------------------------------------------------------ what a call does not write
+class Guarded:
+    """Buffers of chosen sizes with words behind them that no call may change."""
+
+    def __init__(self, ctx, rng):
+        self.ctx, self.rng, self.all = ctx, rng, []
+
+    def buffer(self, words):
+        x = self.rng.integers(0, 1 << 32, words + 256, dtype=np.uint64).astype(np.uint32)
+        b = self.ctx.array(x)
+        self.all.append((b, words, x[words:]))
+        return b
+
+    def check(self):
+        for b, words, x in self.all:
+            assert np.array_equal(b.download(np.uint32, 256, 4 * words), x), words
+
+
+@pytest.mark.parametrize("heads,max_count", [((16, 2, 128), 1), ((32, 2, 64), 1), ((8, 1, 256), 20), ((16, 2, 128), 20)])
+def test_no_content_makes_a_call_write_behind_a_buffer(ctx, heads, max_count):
+    """Plans, tables, lengths, pools and selections of any content, in buffers of just the sizes that a call asks for."""
+    q_heads, kv_heads, hd = heads
+    rng = np.random.default_rng(67)
+    requests, width, rows, pages, ps, budget, layers = 3, 120, 21, 70, 16, 9, 2
+    batch = abi.PagedBatch(abi.PagedGeom(layers, pages, ps, kv_heads, hd), requests, width, rows, max_count, q_heads)
+    lib, wide, row = abi.load(), q_heads * hd, kv_heads * hd
+    store = abi.PagedStorePush(batch, 1, row, row, 0, 0)
+    attn, sparse = (abi.PagedAttentionPush(batch, 1, wide, wide, 0, 0, n) for n in (0, budget))
+    pick = abi.PagedSelectPush(batch, 1, wide, 0, budget, 1, 2)
+    g = Guarded(ctx, rng)
+    nbytes = lib.vx_paged_cache_bytes(C.byref(batch.geom))
+    need = lib.vx_paged_plan_bytes(C.byref(batch))
+    kc, vc, bounds = (g.buffer(n // 4) for n in (nbytes, nbytes, lib.vx_paged_bounds_bytes(C.byref(batch.geom))))
+    lengths, counts, keep, tables, pool = (g.buffer(n) for n in (requests, requests, requests, requests * width, pages + 1))
+    plan, k, v, q, out, sel = (g.buffer(n) for n in (need // 4, rows * row, rows * row, rows * wide, rows * wide, rows * kv_heads * budget))
+    scratch = [g.buffer(n // 4) for n in (lib.vx_paged_attention_scratch_bytes(C.byref(attn)), lib.vx_paged_attention_scratch_bytes(C.byref(sparse)),
+                                          lib.vx_paged_select_scratch_bytes(C.byref(pick)))]
+    h = lambda *x: [b.handle for b in x]  # noqa: E731
+    for most in (3, 8, 70, 1900, 1 << 12, 1 << 32):
+        fill = lambda b, words, top=most: b.upload(rng.integers(0, top, words, dtype=np.uint64).astype(np.uint32))  # noqa: E731
+        for made in (False, True):
+            fill(lengths, requests), fill(counts, requests, min(most, 30)), fill(keep, requests)
+            fill(tables, requests * width), fill(pool, pages + 1), fill(plan, need // 4), fill(sel, rows * kv_heads * budget)
+            if made:
+                abi.call("vx_paged_plan", ctx.handle, *h(lengths, counts, tables, pool, plan), batch)
+            abi.call("vx_paged_store", ctx.handle, *h(k, v, kc, vc, bounds, plan), store)
+            abi.call("vx_paged_attention", ctx.handle, *h(q, kc, vc, out, tables, plan), None, scratch[0].handle, attn)
+            abi.call("vx_paged_attention", ctx.handle, *h(q, kc, vc, out, tables, plan, sel, scratch[1]), sparse)
+            abi.call("vx_paged_select", ctx.handle, *h(q, bounds, tables, plan, sel, scratch[2]), pick)
+            abi.call("vx_paged_attention", ctx.handle, *h(q, kc, vc, out, tables, plan, sel, scratch[1]), sparse)
+            abi.call("vx_paged_advance", ctx.handle, *h(plan, lengths, pool), batch)
+            abi.call("vx_paged_cut", ctx.handle, *h(keep, lengths, tables, pool), batch)
+            g.check()
+    abi.call("vx_paged_reset", ctx.handle, *h(lengths, tables, pool), batch)
+    g.check()
