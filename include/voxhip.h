@@ -614,8 +614,11 @@ int vx_kv4_compact(vx_ctx *ctx, const vx_buf *plan, vx_buf *k_cache, vx_buf *v_c
 /*   vx_paged_store, vx_paged_attention   in every layer;                      */
 /*   vx_paged_advance   after the last: lengths and pool as the plan left them.*/
 /* vx_paged_cut takes tokens back (all of them when a request ends, rejected   */
-/* drafts) and returns their pages. Everything is read from device memory, so  */
-/* a step captures into a graph; sizes of vx_paged_batch are fixed by it.      */
+/* drafts) and returns their pages. Between a plan and its advance nothing     */
+/* else may change lengths or pool: a cut comes before the one or behind the   */
+/* other (a plan that is not advanced may be dropped). Everything is read from  */
+/* device memory, so a step captures into a graph; sizes of vx_paged_batch are */
+/* fixed by it.                                                                */
 /*                                                                            */
 /* No content of a device buffer makes a call read or write outside of the     */
 /* buffers: a table entry that is no page holds no slots (nothing is stored     */

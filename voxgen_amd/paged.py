@@ -19,8 +19,8 @@ With bounds=True, in place of the attention over everything:
         cache.select(layer, q, selected, budget, sinks=1, recent=4)
         cache.attention(layer, q, out, selected=selected, budget=budget)
 
-cache.cut(keep) takes tokens back and returns their pages. Lengths, counts, tables and pool
-live on the device, so a step captures into a graph.
+cache.cut(keep) takes tokens back and returns their pages; not between a plan and its advance.
+Lengths, counts, tables and pool live on the device, so a step captures into a graph.
 """
 from __future__ import annotations
 
@@ -95,12 +95,13 @@ class PagedCache:
         return got
 
     def advance(self) -> None:
-        """Lengths and pool as the plan left them: once a plan, after the last layer."""
+        """Lengths and pool as the plan left them: once a plan, after the last layer, with no cut or reset since the plan."""
         abi.call("vx_paged_advance", self.ctx.handle, self.plan_buffer.handle, self.lengths.handle, self.pool.handle,
                  self._batch)
 
     def cut(self, keep: Buffer) -> None:
-        """Requests down to keep (u32[requests]) tokens at most; their pages return to the pool."""
+        """Requests down to keep (u32[requests]) tokens at most; their pages return to the pool. Before a plan or behind its
+        advance: both go by the lengths and the pool that the plan found."""
         abi.call("vx_paged_cut", self.ctx.handle, keep.handle, self.lengths.handle, self.tables.handle, self.pool.handle,
                  self._batch)
 
