@@ -8,8 +8,6 @@
 namespace vx {
 namespace {
 
-typedef double d2 __attribute__((ext_vector_type(2)));
-
 __device__ __forceinline__ uint32_t add_up_to(uint32_t a, uint32_t b, uint32_t most) { return min(a + b, most); }
 
 // v of another lane of the wave by a DPP control, 0 where there is none or ROWS does not have the lane's row.
