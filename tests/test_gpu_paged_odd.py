@@ -15,6 +15,7 @@ import pagedref as ref
 from conftest import rel_l2
 from test_gpu_paged import NONE, TOL, Side, rows_of
 from voxgen_amd import abi
+from voxgen_amd.paged import PagedCache
 
 pytestmark = pytest.mark.gpu
 
@@ -207,6 +208,32 @@ def test_tables_of_the_call_in_divided_requests(ctx, heads):
     side.dev.tables.upload(tables)
     q = side.queries()
     check(side.attend(q)[0], by_formula(side, q, tables=tables))
+
+
+# ------------------------------------------------------------ two batches over one state
+@pytest.mark.parametrize("heads", [(16, 2, 128), (16, 1, 256)])
+def test_steps_of_two_batches_over_the_same_requests(ctx, heads):
+    """Prompts by a batch that has room for them, single tokens by one of a row a request: lengths, tables, pool and pages are
+    the same, plans and scratch each batch's own."""
+    q_heads, kv_heads, hd = heads
+    side = Side(ctx, heads, 16, [0, 700, 33], [40, 3, 0], 68, spare=8, max_rows=60, max_count=40, width=50)
+    wide, state = side.dev, "k v lengths counts tables pool".split()
+    narrow = PagedCache(ctx, 1, side.pages, 16, kv_heads, hd, 3, side.width, 3, q_heads)
+    for name in state:
+        setattr(narrow, name, getattr(wide, name))
+    for dev, counts in ((wide, [40, 3, 0]), (narrow, [1, 0, 1]), (narrow, [1, 1, 1]), (wide, [0, 37, 5]), (narrow, [1, 1, 1])):
+        side.dev, side.max_rows, side.counts = dev, dev.max_rows, np.array(counts, np.uint32)
+        dev.counts.upload(side.counts)
+        side.plan()
+        side.check_plan()
+        assert list(side.want["granted"]) == counts
+        side.store()
+        side.check_bytes()
+        side.check_attention()
+        dev.advance()
+        side.lengths = side.lengths + side.want["granted"]
+        side.pool[0] -= side.want["pages"]
+        assert np.array_equal(wide.lengths.download(np.uint32), side.lengths) and wide.pool.download(np.uint32, 1)[0] == side.pool[0]
 
 
 # ------------------------------------------------------------ what a call does not write

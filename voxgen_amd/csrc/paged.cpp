@@ -24,8 +24,8 @@ PagedShape paged_shape(const vx_paged_batch &b) {
     // A CU holds four of the workgroups of 16 rows at most, or one of heads of 256, whose are half as many (16
     // requests over up to 8000, of one KV head: 19.6 us, with 1024 25.4), and one of 32 rows.
     s.workgroups = s.tile_rows > 16u ? 8u : b.geom.head_dim < 256u ? 10u : 9u;
-    // A part has two chunks a wave at least, so that one is fetched while it works; what `whole` chunks
-    // hold is not divided.
+    // A part has two chunks a wave at least, so that one is fetched while it works; of tables of `whole` chunks
+    // or fewer no request is divided.
     const uint32_t whole = s.tile_rows > 16u && s.waves == 4u ? kPagedWholeWide : kPagedWhole;
     s.least = (uint64_t)b.table_width * b.geom.page_size <= 32u * whole ? whole : 2u * s.waves;
     // Tiles: at most one for each request of so few rows, else a request's last may be part of one. Parts
