@@ -210,6 +210,30 @@ def test_tables_of_the_call_in_divided_requests(ctx, heads):
     check(side.attend(q)[0], by_formula(side, q, tables=tables))
 
 
+@pytest.mark.parametrize("heads,page_size,lengths,count,pages", [
+    ((16, 2, 128), 256, [900, 3], 1, 1030), ((32, 2, 64), 256, [600, 30], 1, 2060), ((16, 1, 256), 128, [500, 40], 1, 2060)])
+def test_layers_beyond_the_caches(ctx, heads, page_size, lengths, count, pages):
+    """Of more than 256 MB, which are read past the caches: infinite keys, and tables that change behind the plan."""
+    need = [-(-(a + count) // page_size) for a in lengths]
+    side = Side(ctx, heads, page_size, lengths, [count] * 2, 69, spare=pages - sum(need), width=12)
+    assert side.k.nbytes + side.v.nbytes > 256 << 20
+    side.plan()
+    side.store()
+    q = mixed_signs(side.queries(), 5, 1)
+    x = rows_of(side.rng, side.hd)
+    x[5] = np.inf
+    ref.put(side.k, 0, side.tables[0, 0], 0, 7, x, False)
+    side.dev.k.upload(side.k)
+    want = by_formula(side, q)
+    assert np.isfinite(want[0, 0]).all(-1).any() and np.isnan(want).any()
+    check(side.attend(q)[0], want)
+    tables = side.tables.copy()
+    tables[0, [0, 1]] = tables[0, [1, 0]]
+    tables[1, 0] = side.pages
+    side.dev.tables.upload(tables)
+    check(side.attend(q)[0], by_formula(side, q, tables=tables))
+
+
 # ------------------------------------------------------------ two batches over one state
 @pytest.mark.parametrize("heads", [(16, 2, 128), (16, 1, 256)])
 def test_steps_of_two_batches_over_the_same_requests(ctx, heads):
